@@ -103,6 +103,24 @@ VKWR_EXPORT int vkwr_wkv7_fp32_step_rows_slots(int B, int C, int H, float* pool,
                                                const uint16_t* k, const uint16_t* v, const uint16_t* a,
                                                const uint16_t* b, uint16_t* y, void* stream);
 
+/* WKV-7 over drafted tokens (speculative decoding), on a slot pool, the state written one step
+ * late: sequence i first takes the kept[i] (0..P) tokens of row pending_rows[i] (NULL: i) of the
+ * pending vectors pw, pk, pv, pa, pb [n_pending, P, C] fp16 -- the w, k, v, a, b that an earlier
+ * step ran as drafts -- then pool[slots[i]] is written (where kept[i] > 0), then T further tokens
+ * r..b [B, T, C] run on from it with y [B, T, C] as in vkwr_wkv7_fp32_forward_slots, their state
+ * not written.  T = 0 only writes the kept tokens; P = 0 (kept NULL) only runs the drafts.  The dot
+ * products are in the order of vkwr_wkv7_fp32_step_rows_slots: P + T tokens give the bits of that
+ * many of its steps.  slots distinct; a slot outside [0, n_slots), a kept count outside [0, P] or,
+ * where kept[i] > 0, a pending row outside [0, n_pending) makes the sequence's y rows NaN and leaves
+ * its pool entry untouched.  pool and token vectors 16-byte aligned.  No counterpart in the reference. */
+VKWR_EXPORT int vkwr_wkv7_fp32_drafts_slots(int B, int P, int T, int C, int H, float* pool, int n_slots,
+                                            const int32_t* slots, const int32_t* kept, int n_pending,
+                                            const int32_t* pending_rows, const uint16_t* pw,
+                                            const uint16_t* pk, const uint16_t* pv, const uint16_t* pa,
+                                            const uint16_t* pb, const uint16_t* r, const uint16_t* w,
+                                            const uint16_t* k, const uint16_t* v, const uint16_t* a,
+                                            const uint16_t* b, uint16_t* y, void* stream);
+
 /* Layouts of an fp32 64x64 WKV state block (16 KiB) in a pool.
  *   VKWR_WKV_STATE_STD: row-major S[i][j] at float 64 i + j (the reference's
  *     [.., H, 64, 64] layout; every other entry point uses it).
@@ -488,6 +506,45 @@ VKWR_EXPORT int vkwr_tmix_groupnorm_bonus_gate_frag_f16(int B, int T, int C, int
                                                         const uint16_t* weight, const uint16_t* bias,
                                                         const uint16_t* g, uint16_t* out, void* stream);
 
+/* --------------------------------------------- adapters of many requests
+ *
+ * y[i] = epilogue(base[i] + scale[g] * (x[i] A_g^T) B_g^T), g = adapters[i], for the rows i of a step
+ * whose requests use different low-rank adapters beside one shared projection (base = its output).
+ * g < 0: no adapter, y[i] = epilogue(base[i]); g >= n_adapters: y[i] = NaN.  fp32 sums; x A^T enters
+ * the second product with 22 bits; one rounding to fp16.  No counterpart in the reference. */
+
+/* The plan of a step: its rows ordered by adapter, made on the device from adapters [m] int32 (device)
+ * once for all projections of the step.  plan: device memory of vkwr_lora_plan_bytes(m, n_adapters)
+ * bytes (-1 on invalid arguments; it grows with m), 16-byte aligned.  1 <= n_adapters <= 8192. */
+VKWR_EXPORT int64_t vkwr_lora_plan_bytes(int64_t m, int n_adapters);
+VKWR_EXPORT int vkwr_lora_plan(int64_t m, int n_adapters, const int32_t* adapters, void* plan,
+                               int64_t plan_bytes, void* stream);
+
+/* One projection: x [m, k], a [n_adapters, rank, k], b [n_adapters, n, rank], base (NULL: y) and
+ * y [m, n] fp16, contiguous.  epilogue: VKWR_GEMM_EPI_NONE or VKWR_GEMM_EPI_RELU_SQUARE. */
+typedef struct vkwr_lora_target {
+  const uint16_t* x;
+  const uint16_t* a;
+  const uint16_t* b;
+  const uint16_t* base;
+  uint16_t* y;
+  int64_t n, k;
+  int epilogue;
+} vkwr_lora_target;
+
+/* Device workspace that vkwr_lora_f16 needs for these targets at any row count up to m (only n, k and
+ * epilogue of the targets are read), or -1 on invalid arguments. */
+VKWR_EXPORT int64_t vkwr_lora_workspace_bytes(int64_t m, int n_adapters, int rank, int n_targets,
+                                              const vkwr_lora_target* targets);
+
+/* 1..8 projections in two launches, on a plan made for the same m and n_adapters (with another one
+ * nothing is written).  scale [n_adapters] fp32 (device) or NULL (1).  rank a multiple of 8 up to 128
+ * (zero rows and columns pad an adapter of lower rank exactly), n and k multiples of 8; all pointers 16-byte aligned.  y must not
+ * overlap any x, another y or base, nor its own base unless they are equal (rejected). */
+VKWR_EXPORT int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* scale, const void* plan,
+                              int n_targets, const vkwr_lora_target* targets, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------- fragment-layout GEMM
  *
  * Decode-step GEMMs (m <= a few hundred rows) are bound by streaming the
@@ -620,6 +677,28 @@ VKWR_EXPORT int vkwr_sampling_repetition_topk_topp(int B, int T, int V, const fl
                                                    double presence_penalty, double repetition_penalty,
                                                    double penalty_decay, double temperature, int top_k,
                                                    double top_p, void* stream);
+
+/* Verification of drafted tokens.  Sequence b has K + 1 rows of logits [B, K+1, V] (fp16 where
+ * logits_f16, else fp32; row i: after i drafts) and n_draft[b] <= K (NULL: K) drafts [B, K] int32.
+ * Per row p is the distribution that the ops above draw from (same filter; probabilities, masses and
+ * sums in 64 bits, ties by logit).  Draft i, in order, is accepted while
+ *   uniforms[b, i] * q(d_i) < p_i(d_i),
+ * q = draft_probs [B, K, V] fp32 (finite, >= 0), or 1 where draft_probs is NULL (a drafter that
+ * proposes single tokens).  At the first rejected draft the new token is drawn from max(p_i - q_i, 0)
+ * normalised (p_i without the draft; p_i itself where nothing is left), with all accepted from p_n:
+ * the first x in vocabulary order whose inclusive sum exceeds uniforms[b, K] * total.  uniforms
+ * [B, K+1] fp32 in [0, 1).  tokens [B, K+1] int32: the accepted drafts, the new token, -1 behind it;
+ * accepted [B] int32: the number of accepted drafts.  n_draft outside [0, K]: accepted -1 and every
+ * token -1.  A draft outside [0, V) has p = 0.  Deterministic, and independent of the batch.
+ * V, temperature, top_k, top_p as above; logits 16-byte (fp16: 8-byte) and draft_probs 16-byte
+ * aligned; workspace: vkwr_sampling_verify_workspace_bytes(B, K, V) bytes, 16-byte aligned.
+ * No counterpart in the reference. */
+VKWR_EXPORT int64_t vkwr_sampling_verify_workspace_bytes(int B, int K, int V);
+VKWR_EXPORT int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logits, int logits_f16,
+                                            const int32_t* drafts, const int32_t* n_draft,
+                                            const float* draft_probs, const float* uniforms, int32_t* tokens,
+                                            int32_t* accepted, double temperature, int top_k, double top_p,
+                                            void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Host-side Philox4x32-10 block (the generator the sampling kernels run), for
  * checking it against published known-answer vectors.  No counterpart in the

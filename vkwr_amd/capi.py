@@ -67,6 +67,10 @@ class LnShiftGroup(ctypes.Structure):
     _fields_ = [("row0", _i64), ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("slots", _p)]
 
 
+class LoraTarget(ctypes.Structure):
+    _fields_ = [("x", _p), ("a", _p), ("b", _p), ("base", _p), ("y", _p), ("n", _i64), ("k", _i64), ("epilogue", _i)]
+
+
 def _sig(name, args, res=_i):
     fn = getattr(_LIB, name)
     fn.argtypes = args
@@ -124,6 +128,14 @@ _samp_setup = _sig("vkwr_sampling_setup_rand", [_i64, _i, _p, _p])
 _samp_temp = _sig("vkwr_sampling_temperature_topk_topp", [_i, _i, _i, _p, _p, _p, _p, _d, _i, _d, _p])
 _samp_rep = _sig("vkwr_sampling_repetition_topk_topp",
                  [_i, _i, _i, _p, _p, _p, _p, _p, _d, _d, _d, _d, _i, _d, _p])
+_verify = _sig("vkwr_sampling_verify_drafts",
+               [_i, _i, _i, _p, _i, _p, _p, _p, _p, _p, _p, _d, _i, _d, _p, _i64, _p])
+_verify_ws = _sig("vkwr_sampling_verify_workspace_bytes", [_i, _i, _i], _i64)
+_wkv_drafts = _sig("vkwr_wkv7_fp32_drafts_slots", [_i] * 5 + [_p, _i, _p, _p, _i] + [_p] * 14)
+_lora_plan_bytes = _sig("vkwr_lora_plan_bytes", [_i64, _i], _i64)
+_lora_plan = _sig("vkwr_lora_plan", [_i64, _i, _p, _p, _i64, _p])
+_lora_ws = _sig("vkwr_lora_workspace_bytes", [_i64, _i, _i, _i, ctypes.POINTER(LoraTarget)], _i64)
+_lora = _sig("vkwr_lora_f16", [_i64, _i, _i, _p, _p, _i, ctypes.POINTER(LoraTarget), _p, _i64, _p])
 SAMPLING_STATE_BYTES = 32
 SAMPLING_REGISTER_VOCAB = 65536  # larger vocabularies need a B*V fp32 scratch buffer
 
@@ -445,3 +457,138 @@ def sample(logits, states, out, temperature=1.0, top_k=-1, top_p=1.0, penalties=
         st = _samp_rep(B, T, V, _ptr(logits), _ptr(penalties), _ptr(states), _ptr(out), _ptr(scratch), presence,
                        repetition, decay, temperature, top_k, top_p, _stream())
         _check(st, "vkwr_sampling_repetition_topk_topp")
+
+
+def _dev(t, dtype, n, what):
+    """Pointer of a tensor that a kernel reads or writes as n values of dtype: contiguous, on the
+    current device, with exactly n entries."""
+    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.numel() != n:
+        raise TypeError(f"{what}: expected a contiguous {dtype} CUDA tensor of {n} entries, got "
+                        f"{t.dtype} {t.device} shape {tuple(t.shape)} contiguous={t.is_contiguous()}")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def wkv_drafts_slots(B, T, C, H, pool, slots, r, w, k, v, a, b, y, kept=None, pending=None, pending_rows=None):
+    """WKV-7 over drafted tokens on a slot pool [n_slots, H, 64, 64] (vkwr_wkv7_fp32_drafts_slots):
+    sequence i takes kept[i] tokens of the pending vectors (w, k, v, a, b), each [n, P, C] -- row
+    pending_rows[i], or i -- its state is written, and r..b [B, T, C] run on from it into y [B, T, C]
+    without being written.  T = 0 (r..y may be None): only the kept tokens; no pending: only drafts."""
+    h = torch.float16
+    n_slots = pool.shape[0]
+    P = n_pending = 0
+    pv = [None] * 5
+    if (kept is None) != (pending is None):
+        raise ValueError("wkv_drafts_slots: kept and pending go together")
+    if pending is not None:
+        n_pending, P = pending[0].shape[:2]
+        pv = [_dev(t, h, n_pending * P * C, "pending") for t in pending]
+    n = B * T * C
+    ins = [_dev(t, h, n, "r, w, k, v, a, b, y") for t in (r, w, k, v, a, b, y)] if T else [None] * 7
+    _check(_wkv_drafts(B, P, T, C, H, _dev(pool, torch.float32, n_slots * H * 4096, "pool"), n_slots,
+                       _dev(slots, torch.int32, B, "slots"), _dev(kept, torch.int32, B, "kept") if P else None,
+                       n_pending, None if pending_rows is None else _dev(pending_rows, torch.int32, B, "pending_rows"),
+                       *pv, *ins, _stream()), "vkwr_wkv7_fp32_drafts_slots")
+
+
+def verify_workspace_bytes(B, K, V):
+    """Workspace of verify_drafts for up to B sequences of up to K drafts (V is the vocabulary)."""
+    return _verify_ws(B, K, V)
+
+
+def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_draft=None, draft_probs=None, temperature=1.0,
+                  top_k=-1, top_p=1.0, workspace=None):
+    """Accept or reject drafted tokens (vkwr_sampling_verify_drafts): logits [B, K+1, V] fp16 or fp32,
+    drafts [B, K] int32, uniforms [B, K+1] fp32 in [0, 1), n_draft [B] int32 (None: K each),
+    draft_probs [B, K, V] fp32 (None: single proposals).  Writes tokens [B, K+1] (accepted drafts, the
+    new token, then -1) and accepted [B], both int32.  workspace: uint8, verify_workspace_bytes."""
+    B, T, V = logits.shape
+    K = T - 1
+    if logits.dtype not in (torch.float16, torch.float32):
+        raise TypeError(f"logits: fp16 or fp32, got {logits.dtype}")
+    i32, f32 = torch.int32, torch.float32
+    if workspace is None:
+        workspace = torch.empty(_verify_ws(B, K, V), dtype=torch.uint8, device=logits.device)
+    _check(_verify(B, K, V, _dev(logits, logits.dtype, B * T * V, "logits"), int(logits.dtype == torch.float16),
+                   _dev(drafts, i32, B * K, "drafts"), None if n_draft is None else _dev(n_draft, i32, B, "n_draft"),
+                   None if draft_probs is None else _dev(draft_probs, f32, B * K * V, "draft_probs"),
+                   _dev(uniforms, f32, B * T, "uniforms"), _dev(tokens, i32, B * T, "tokens"),
+                   _dev(accepted, i32, B, "accepted"), temperature, top_k, top_p,
+                   _dev(workspace, torch.uint8, workspace.numel(), "workspace"), workspace.numel(), _stream()),
+           "vkwr_sampling_verify_drafts")
+
+
+LORA_MAX_TARGETS = 8
+
+
+class LoraPlan:
+    """Device buffer of a step's plan (rows ordered by adapter) for up to max_rows rows."""
+
+    def __init__(self, max_rows, n_adapters, device):
+        nbytes = _lora_plan_bytes(max_rows, n_adapters)
+        if nbytes < 0:
+            raise ValueError(f"lora plan: bad size ({max_rows} rows, {n_adapters} adapters)")
+        self.max_rows, self.n_adapters, self.m = max_rows, n_adapters, None
+        self.buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def lora_plan_empty(max_rows, n_adapters, device):
+    """A plan buffer to be filled by lora_plan."""
+    return LoraPlan(max_rows, n_adapters, device)
+
+
+def lora_plan(adapters, plan):
+    """Fills `plan` for rows with these adapters (int32 [m]; negative: none): once per step, for every
+    projection of it."""
+    m = adapters.numel()
+    if m > plan.max_rows:
+        raise ValueError(f"lora plan of {plan.max_rows} rows, got {m}")
+    _check(_lora_plan(m, plan.n_adapters, _dev(adapters, torch.int32, m, "adapters"),
+                      _dev(plan.buf, torch.uint8, plan.buf.numel(), "plan"), plan.buf.numel(), _stream()),
+           "vkwr_lora_plan")
+    plan.m = m
+
+
+def lora_target(x, a, b, y, base=None, epilogue=EPI_NONE):
+    """One projection: y[i] = epilogue(base[i] + scale[g] (x[i] a[g]^T) b[g]^T), x [m, k],
+    a [G, rank, k], b [G, n, rank], y and base [m, n] fp16 (base None: y, in place)."""
+    G, rank, k = a.shape
+    n = b.shape[1]
+    m = x.numel() // k
+    h = torch.float16
+    if tuple(b.shape) != (G, n, rank):
+        raise ValueError(f"lora_target: a {tuple(a.shape)} and b {tuple(b.shape)} do not match")
+    t = LoraTarget(_dev(x, h, m * k, "x"), _dev(a, h, G * rank * k, "a"), _dev(b, h, G * n * rank, "b"),
+                   None if base is None else _dev(base, h, m * n, "base"), _dev(y, h, m * n, "y"), n, k, epilogue)
+    t.sizes = (m, G, rank)
+    t.tensors = (x, a, b, y, base)  # what the pointers point to
+    return t
+
+
+def _lora_targets(targets):
+    if not 1 <= len(targets) <= LORA_MAX_TARGETS or len({t.sizes for t in targets}) != 1:
+        raise ValueError("lora: 1 to 8 targets with the same rows, adapters and rank")
+    return targets[0].sizes, (LoraTarget * len(targets))(*targets)
+
+
+def lora_workspace_bytes(max_rows, n_adapters, targets):
+    """Workspace of `lora` for these targets at any row count up to max_rows."""
+    (_, G, rank), arr = _lora_targets(targets)
+    n = _lora_ws(max_rows, n_adapters, rank, len(targets), arr)
+    if n < 0:
+        raise RuntimeError(f"vkwr_lora_workspace_bytes: {_LIB.vkwr_last_error().decode()}")
+    return n
+
+
+def lora(plan, targets, scale=None, workspace=None):
+    """Adds each row's adapter to 1..8 projections that the rows of `plan` go through (vkwr_lora_f16).
+    scale: fp32 [G] (None: 1).  workspace: uint8, lora_workspace_bytes (None: allocated)."""
+    (m, G, rank), arr = _lora_targets(targets)
+    if plan.m != m or plan.n_adapters != G:
+        raise ValueError(f"lora: plan of {plan.m} rows and {plan.n_adapters} adapters, targets of {m} and {G}")
+    if workspace is None:
+        workspace = torch.empty(lora_workspace_bytes(m, G, targets), dtype=torch.uint8, device=plan.buf.device)
+    _check(_lora(m, G, rank, None if scale is None else _dev(scale, torch.float32, G, "scale"), _ptr(plan.buf),
+                 len(targets), arr, _dev(workspace, torch.uint8, workspace.numel(), "workspace"), workspace.numel(),
+                 _stream()), "vkwr_lora_f16")

@@ -1,0 +1,500 @@
+// Low-rank adapters of many requests beside a shared projection.
+//
+//   y_i = epi(base_i + scale[g] (x_i A_g^T) B_g^T),  g = adapters[i]; no adapter (g < 0): y_i = epi(base_i)
+//
+// x [m, K], A [G, R, K], B [G, N, R], base and y [m, N] fp16; sums in fp32.
+//
+// Plan: the rows ordered by adapter and cut into tiles of at most kTileM rows of one adapter, made
+// on the device from the step's adapter indices, once for every projection of the step.
+// Two launches per set of projections:
+//   shrink  h = x A^T for each tile, K cut into parts that fill the chip when there are few tiles
+//           (a decode batch); fp32 parts go to scratch
+//   expand  the parts added in order, y = epi(base + scale h B^T)
+// Both run on the matrix cores with 16 rows of x (or h) as the columns of v_mfma_f32_16x16x32_f16,
+// the adapter's rows as its rows.  h is not rounded to fp16: it enters the second product as a sum
+// of two halves (fp16(h) and fp16(h - fp16(h)), 22 bits), 16 ranks filling the 32-deep product, after
+// a power of two per row has brought its largest value to [1, 2) so that neither half leaves
+// fp16's range.
+
+#include <algorithm>
+
+#include "vk_capi.h"
+#include "vk_common.cuh"
+
+namespace vk {
+namespace {
+
+typedef _Float16 hv8 __attribute__((ext_vector_type(8)));
+typedef float fv4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTileM = 64;         // rows of a tile: up to 4 columns blocks of 16
+constexpr int kSub = kTileM / 16;
+constexpr int kMaxTargets = 8;
+constexpr int kMaxRank = 128;
+constexpr int kMaxAdapters = 8192;
+constexpr int kRankBlock = 64;     // ranks per shrink workgroup
+constexpr int kColBlock = 256;     // output columns per expand workgroup (64 per wave)
+constexpr int kNone = -1, kBad = -2;
+
+struct Tile {
+  int adapter, row0, rows, pad;
+};
+struct PlanHead {
+  int n_tiles;     // all tiles
+  int n_adapter;   // those with an adapter (they come first)
+  int m, G;        // what it was made for
+};
+
+__host__ __device__ inline int64_t max_tiles(int64_t m, int64_t G) { return (m < G + 2 ? m : G + 2) + m / kTileM; }
+
+__device__ __forceinline__ const Tile* plan_tiles(const void* plan) {
+  return reinterpret_cast<const Tile*>(reinterpret_cast<const char*>(plan) + sizeof(PlanHead));
+}
+__device__ __forceinline__ const int32_t* plan_order(const void* plan, int64_t tiles) {
+  return reinterpret_cast<const int32_t*>(plan_tiles(plan) + tiles);
+}
+
+// One workgroup: counts per bin (adapters, then rows without one, then indices out of range), prefix
+// sums of counts and tiles, tiles, and the rows' places.  Rows of one bin are placed in the order
+// in which their waves get there; what is computed for a row does not depend on its place.
+__global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const int32_t* adapters, void* plan,
+                                                         int64_t tiles_cap) {
+  extern __shared__ int lds[];
+  int* const cnt = lds;          // [G + 2] counts, then next free place
+  int* const red = lds + G + 2;  // [32]
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, nb = G + 2;
+  Tile* const tiles = const_cast<Tile*>(plan_tiles(plan));
+  int32_t* const order = const_cast<int32_t*>(plan_order(plan, tiles_cap));
+  auto bin_of = [&](int64_t i) {
+    const int g = adapters[i];
+    return g < 0 ? G : g < G ? g : G + 1;
+  };
+  // this lane's place among `take` consecutive ones of its bin; one atomic where a wave agrees
+  auto place = [&](bool live, int bin) {
+    const int first = __builtin_amdgcn_readfirstlane(bin);
+    if (__ballot(live && bin == first) == ~0ull) {
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&cnt[bin], 64);
+      return __builtin_amdgcn_readfirstlane(at) + lane;
+    }
+    return live ? atomicAdd(&cnt[bin], 1) : 0;
+  };
+  for (int k = t; k < nb; k += 1024) cnt[k] = 0;
+  __syncthreads();
+  for (int64_t i0 = 0; i0 < m; i0 += 1024) {
+    const bool live = i0 + t < m;
+    place(live, live ? bin_of(i0 + t) : 0);
+  }
+  __syncthreads();
+  const int per = (nb + 1023) / 1024, k0 = min(t * per, nb), k1 = min(k0 + per, nb);
+  int rows = 0, tl = 0;
+  for (int k = k0; k < k1; ++k) {
+    rows += cnt[k];
+    tl += (cnt[k] + kTileM - 1) / kTileM;
+  }
+  int ri = rows, ti = tl;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int a = __shfl_up(ri, d, 64), b = __shfl_up(ti, d, 64);
+    if (lane >= d) {
+      ri += a;
+      ti += b;
+    }
+  }
+  if (lane == 63) {
+    red[wv] = ri;
+    red[16 + wv] = ti;
+  }
+  __syncthreads();
+  int row = ri - rows, tile = ti - tl;
+  for (int w = 0; w < wv; ++w) {
+    row += red[w];
+    tile += red[16 + w];
+  }
+  PlanHead* const head = reinterpret_cast<PlanHead*>(plan);
+  if (t == 0) {
+    head->m = (int)m;
+    head->G = G;
+  }
+  for (int k = k0; k < k1; ++k) {
+    const int c = cnt[k];
+    if (k == G) head->n_adapter = tile;
+    for (int r = 0; r < c; r += kTileM)
+      tiles[tile++] = Tile{k < G ? k : k == G ? kNone : kBad, row + r, min(kTileM, c - r), 0};
+    if (k == nb - 1) head->n_tiles = tile;
+    cnt[k] = row;
+    row += c;
+  }
+  __syncthreads();
+  for (int64_t i0 = 0; i0 < m; i0 += 1024) {
+    const bool live = i0 + t < m;
+    const int at = place(live, live ? bin_of(i0 + t) : 0);
+    if (live) order[at] = (int32_t)(i0 + t);
+  }
+}
+
+struct Target {
+  const _Float16 *x, *a, *b, *base;
+  _Float16* y;
+  int n, k;
+  int relu2;
+  int col_block0;  // expand: this target's first column block
+};
+struct LoraArgs {
+  const void* plan;
+  int64_t tiles_cap, m;
+  int G;
+  const float* scale;
+  float* h;        // [parts][target][m][rank_pad]
+  int rank, rank_pad, n_targets, parts, rank_blocks;
+  Target t[kMaxTargets];
+};
+
+__device__ __forceinline__ fv4 mfma(hv8 a, hv8 b, fv4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Grid: x = part, y = tile, z = target * rank_blocks + rank block.  Four waves cut the part's K
+// between them; their sums are added in wave order through LDS.
+template <int RT>
+__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
+  __shared__ fv4 lds[4][kSub][RT][64];
+  const PlanHead* head = reinterpret_cast<const PlanHead*>(p.plan);
+  if ((int)blockIdx.y >= head->n_adapter || head->m != p.m || head->G != p.G) return;
+  const Tile tile = plan_tiles(p.plan)[blockIdx.y];
+  const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
+  const int ti = blockIdx.z / p.rank_blocks, rb = blockIdx.z - ti * p.rank_blocks;
+  const Target& tg = p.t[ti];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int K = tg.k, ns = (tile.rows + 15) >> 4;
+  const int li = lane & 15, kg = 8 * (lane >> 4);
+  const _Float16* xr[kSub];
+#pragma unroll
+  for (int s = 0; s < kSub; ++s)
+    xr[s] = tg.x + (int64_t)order[min(16 * s + li, tile.rows - 1)] * K;
+  const int r0 = rb * kRankBlock;
+  const _Float16* ar[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+    ar[j] = tg.a + ((int64_t)tile.adapter * p.rank + min(r0 + 16 * j + li, p.rank - 1)) * K;
+  // this wave's 32-deep steps of the part
+  const int steps = (K + 31) >> 5, chunks = 4 * p.parts, c = 4 * blockIdx.x + wv;
+  const int s0 = (int)((int64_t)steps * c / chunks), s1 = (int)((int64_t)steps * (c + 1) / chunks);
+  fv4 acc[kSub][RT];
+#pragma unroll
+  for (int s = 0; s < kSub; ++s)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[s][j] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
+  const hv8 zero = {};
+  for (int st = s0; st < s1; ++st) {
+    const int k = 32 * st + kg;
+    const bool in = k < K;
+    hv8 fa[RT];
+#pragma unroll
+    for (int j = 0; j < RT; ++j) fa[j] = in ? *reinterpret_cast<const hv8*>(ar[j] + k) : zero;
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      if (s >= ns) break;
+      const hv8 fb = in ? *reinterpret_cast<const hv8*>(xr[s] + k) : zero;
+#pragma unroll
+      for (int j = 0; j < RT; ++j) acc[s][j] = mfma(fa[j], fb, acc[s][j]);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kSub; ++s) {
+    if (s >= ns) break;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) lds[wv][s][j][lane] = acc[s][j];
+  }
+  __syncthreads();
+  // lane (row li, ranks 16 j + 4 (lane / 16) ..): four consecutive ranks
+  float* h = p.h + ((int64_t)(blockIdx.x * p.n_targets + ti) * p.m + tile.row0) * p.rank_pad + r0;
+  for (int i = tid; i < ns * RT * 64; i += 256) {
+    const int l = i & 63, j = (i >> 6) % RT, s = (i >> 6) / RT;
+    const int r = 16 * s + (l & 15);
+    if (r >= tile.rows || r0 + 16 * j >= p.rank_pad) continue;
+    const fv4 v = ((lds[0][s][j][l] + lds[1][s][j][l]) + lds[2][s][j][l]) + lds[3][s][j][l];
+    *reinterpret_cast<fv4*>(h + (int64_t)r * p.rank_pad + 16 * j + 4 * (l >> 4)) = v;
+  }
+}
+
+// Grid: x = column block over all targets, y = tile.
+__global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
+  extern __shared__ char dyn[];
+  const PlanHead* head = reinterpret_cast<const PlanHead*>(p.plan);
+  if ((int)blockIdx.y >= head->n_tiles || head->m != p.m || head->G != p.G) return;
+  const Tile tile = plan_tiles(p.plan)[blockIdx.y];
+  const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
+  int ti = 0;
+  while (ti + 1 < p.n_targets && (int)blockIdx.x >= p.t[ti + 1].col_block0) ++ti;
+  const Target& tg = p.t[ti];
+  const int N = tg.n, c0 = ((int)blockIdx.x - tg.col_block0) * kColBlock;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  if (tile.adapter < 0) {
+    // no adapter: the epilogue alone; an index out of range: NaN
+    if (tile.adapter == kNone && !tg.relu2 && tg.base == tg.y) return;
+    for (int i = tid; i < tile.rows * (kColBlock / 8); i += 256) {
+      const int c = c0 + 8 * (i % (kColBlock / 8));
+      if (c >= N) continue;
+      const int64_t at = (int64_t)order[i / (kColBlock / 8)] * N + c;
+      h8 v = ld8(tg.base + at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (tile.adapter == kBad) v.v[e] = (_Float16)__builtin_nanf("");
+        else if (tg.relu2) {
+          const float f = (float)v.v[e], z = f > 0.0f ? f : (f != f ? f : 0.0f);
+          v.v[e] = f16_of(z * z);
+        }
+      }
+      st8(tg.y + at, v);
+    }
+    return;
+  }
+  const int ns = (tile.rows + 15) >> 4, chunks = p.rank_pad >> 4;
+  hv8* const hf = reinterpret_cast<hv8*>(dyn);                                   // [chunk][sub][lane]
+  uint32_t* const rmax = reinterpret_cast<uint32_t*>(hf + chunks * kSub * 64);   // [kTileM] largest |h| of a row
+  if (tid < kTileM) rmax[tid] = 0;
+  __syncthreads();
+  // h = scale * (sum of the parts, in order), 8 ranks of a row per item; at most 4 items a lane
+  const float sc = p.scale ? p.scale[tile.adapter] : 1.0f;
+  const int groups = p.rank_pad >> 3, items = tile.rows * groups;
+  constexpr int kItems = kTileM * (kMaxRank / 8) / 256;
+  float hv[kItems][8];
+  const float* h0 = p.h + ((int64_t)ti * p.m + tile.row0) * p.rank_pad;
+  const int64_t plane = (int64_t)p.n_targets * p.m * p.rank_pad;
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    const int i = tid + 256 * u;
+    if (i >= items) break;
+    const int r = i / groups, gr = i - r * groups;
+    const float* src = h0 + (int64_t)r * p.rank_pad + 8 * gr;
+    fv4 lo = *reinterpret_cast<const fv4*>(src), hi = *reinterpret_cast<const fv4*>(src + 4);
+    for (int q = 1; q < p.parts; ++q) {
+      lo += *reinterpret_cast<const fv4*>(src + q * plane);
+      hi += *reinterpret_cast<const fv4*>(src + q * plane + 4);
+    }
+    uint32_t mx = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hv[u][e] = 8 * gr < p.rank ? (e < 4 ? lo[e & 3] : hi[e & 3]) * sc : 0.0f;  // ranks of the padding: 0
+      mx = max(mx, __builtin_bit_cast(uint32_t, hv[u][e]) & 0x7fffffffu);
+    }
+    atomicMax(&rmax[r], mx);  // a maximum does not depend on the order
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    const int i = tid + 256 * u;
+    if (i >= items) break;
+    const int r = i / groups, gr = i - r * groups;
+    const int ex = (int)(rmax[r] >> 23);                  // biased exponent of the row's largest value
+    const int sh = ex == 0 || ex == 255 ? 0 : 127 - ex;   // zeros (and denormals), infinities, NaN: as they are
+    hv8 vh, vl;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = __builtin_ldexpf(hv[u][e], sh);
+      vh[e] = (_Float16)f;
+      // an infinity has no second half
+      vl[e] = __builtin_isinf((float)vh[e]) ? (_Float16)0.0f : (_Float16)(f - (float)vh[e]);
+    }
+    // k groups 0, 1 of the product: ranks 0-7, 8-15 of the chunk's first half; 2, 3: second half
+    hv8* d = hf + ((gr >> 1) * kSub + (r >> 4)) * 64 + (r & 15);
+    d[16 * (gr & 1)] = vh;
+    d[16 * (2 + (gr & 1))] = vl;
+  }
+  __syncthreads();
+  const int cw = c0 + 64 * wv;
+  if (cw >= N) return;
+  const int li = lane & 15, grp = lane >> 4;
+  // product row li of column tile t is output column cw + 16 (li / 4) + 4 t + li % 4, so that a lane
+  // of group grp ends up with the 16 consecutive columns cw + 16 grp ..
+  fv4 acc[kSub][4];
+#pragma unroll
+  for (int s = 0; s < kSub; ++s)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[s][t] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
+  const hv8 zero = {};
+  for (int ch = 0; ch < chunks; ++ch) {
+    const int rk = 16 * ch + 8 * (grp & 1);
+    hv8 fa[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int col = cw + 16 * (li >> 2) + 4 * t + (li & 3);
+      fa[t] = rk < p.rank && col < N
+                  ? *reinterpret_cast<const hv8*>(tg.b + ((int64_t)tile.adapter * N + col) * p.rank + rk)
+                  : zero;
+    }
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      if (s >= ns) break;
+      const hv8 fb = hf[(ch * kSub + s) * 64 + lane];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], fb, acc[s][t]);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kSub; ++s) {
+    if (s >= ns) break;
+    const int r = 16 * s + li;
+    if (r >= tile.rows) continue;
+    const int ex = (int)(rmax[r] >> 23);
+    const int back = ex == 0 || ex == 255 ? 0 : ex - 127;
+    const int64_t at = (int64_t)order[r] * N + cw + 16 * grp;
+#pragma unroll
+    for (int hf2 = 0; hf2 < 2; ++hf2) {
+      if (cw + 16 * grp + 8 * hf2 >= N) continue;
+      h8 v = ld8(tg.base + at + 8 * hf2);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float f = (float)v.v[e] + __builtin_ldexpf(acc[s][2 * hf2 + (e >> 2)][e & 3], back);
+        if (tg.relu2) {
+          f = f > 0.0f ? f : (f != f ? f : 0.0f);
+          f = f * f;
+        }
+        v.v[e] = f16_of(f);
+      }
+      st8(tg.y + at + 8 * hf2, v);
+    }
+  }
+}
+
+struct LoraPlan {
+  int parts, rank_pad, rank_blocks;
+  int64_t bytes;
+};
+
+// K parts: enough workgroups for the chip where the rows make few tiles, each wave's share of a part
+// at least 64 deep.
+LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min) {
+  LoraPlan s{};
+  s.rank_pad = (rank + 15) / 16 * 16;
+  s.rank_blocks = (rank + kRankBlock - 1) / kRankBlock;
+  const int64_t tiles = (m < G ? m : G) + m / kTileM;
+  int64_t parts = 1;
+  while (parts < 8 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 256) parts *= 2;
+  s.parts = (int)parts;
+  s.bytes = parts * n_targets * m * s.rank_pad * 4;
+  return s;
+}
+
+int check_lora(const char* fn, int64_t m, int G, int rank, int n_targets, const vkwr_lora_target* t) {
+  VK_REQUIRE(m >= 0 && m <= 0x7fffffff - 64, "%s: bad row count %lld", fn, (long long)m);
+  VK_REQUIRE(G >= 1 && G <= kMaxAdapters, "%s: 1 to %d adapters, got %d", fn, kMaxAdapters, G);
+  VK_REQUIRE(rank >= 8 && rank <= kMaxRank && rank % 8 == 0, "%s: rank must be a multiple of 8 up to %d, got %d", fn,
+             kMaxRank, rank);
+  VK_REQUIRE(n_targets >= 1 && n_targets <= kMaxTargets && t, "%s: 1 to %d targets, got %d", fn, kMaxTargets,
+             n_targets);
+  for (int i = 0; i < n_targets; ++i) {
+    VK_REQUIRE(t[i].n >= 8 && t[i].n % 8 == 0 && t[i].n <= (1 << 20) && t[i].k >= 8 && t[i].k % 8 == 0 &&
+                   t[i].k <= (1 << 20),
+               "%s: target %d: n and k must be multiples of 8 up to 2^20, got n=%lld k=%lld", fn, i,
+               (long long)t[i].n, (long long)t[i].k);
+    VK_REQUIRE(t[i].epilogue == VKWR_GEMM_EPI_NONE || t[i].epilogue == VKWR_GEMM_EPI_RELU_SQUARE,
+               "%s: target %d: unsupported epilogue %d", fn, i, t[i].epilogue);
+  }
+  return VKWR_OK;
+}
+
+int64_t least_k(int n_targets, const vkwr_lora_target* t) {
+  int64_t k = t[0].k;
+  for (int i = 1; i < n_targets; ++i) k = t[i].k < k ? t[i].k : k;
+  return k;
+}
+
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+}  // namespace
+}  // namespace vk
+
+using namespace vk;
+
+extern "C" int64_t vkwr_lora_plan_bytes(int64_t m, int n_adapters) {
+  if (m < 0 || m > 0x7fffffff - 64 || n_adapters < 1 || n_adapters > kMaxAdapters) return -1;
+  return (int64_t)sizeof(PlanHead) + max_tiles(m, n_adapters) * (int64_t)sizeof(Tile) + 4 * m;
+}
+
+extern "C" int vkwr_lora_plan(int64_t m, int n_adapters, const int32_t* adapters, void* plan, int64_t plan_bytes,
+                              void* stream) {
+  clear_error();
+  const char* fn = "vkwr_lora_plan";
+  const int64_t need = vkwr_lora_plan_bytes(m, n_adapters);
+  VK_REQUIRE(need >= 0, "%s: bad size (m=%lld, %d adapters; at most %d adapters)", fn, (long long)m, n_adapters,
+             kMaxAdapters);
+  VK_REQUIRE(m == 0 || adapters, "%s: null pointer", fn);
+  VK_REQUIRE(plan && plan_bytes >= need && (uintptr_t)plan % 16 == 0,
+             "%s: needs a 16-byte aligned plan of %lld bytes, got %lld", fn, (long long)need, (long long)plan_bytes);
+  hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (n_adapters + 2 + 32) * sizeof(int), (hipStream_t)stream, m,
+                     n_adapters, adapters, plan, max_tiles(m, n_adapters));
+  return check_launch(fn);
+}
+
+extern "C" int64_t vkwr_lora_workspace_bytes(int64_t m, int n_adapters, int rank, int n_targets,
+                                             const vkwr_lora_target* targets) {
+  clear_error();
+  if (check_lora("vkwr_lora_workspace_bytes", m, n_adapters, rank, n_targets, targets)) return -1;
+  const int64_t k = least_k(n_targets, targets);
+  int64_t most = lora_split(m, n_adapters, rank, n_targets, k).bytes;
+  // fewer rows can be cut into more parts; from 512 row tiles on there is one part
+  for (int64_t r = 1; r < m && r < 512 * kTileM; ++r)
+    most = std::max(most, lora_split(r, n_adapters, rank, n_targets, k).bytes);
+  return most;
+}
+
+extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* scale, const void* plan,
+                             int n_targets, const vkwr_lora_target* targets, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* fn = "vkwr_lora_f16";
+  if (int e = check_lora(fn, m, n_adapters, rank, n_targets, targets)) return e;
+  if (m == 0) return VKWR_OK;
+  const LoraPlan sp = lora_split(m, n_adapters, rank, n_targets, least_k(n_targets, targets));
+  VK_REQUIRE(plan && (uintptr_t)plan % 16 == 0, "%s: null or misaligned plan", fn);
+  VK_REQUIRE(workspace && workspace_bytes >= sp.bytes && (uintptr_t)workspace % 16 == 0,
+             "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn, (long long)sp.bytes,
+             (long long)workspace_bytes);
+  LoraArgs a{};
+  a.plan = plan;
+  a.tiles_cap = max_tiles(m, n_adapters);
+  a.m = m;
+  a.G = n_adapters;
+  a.scale = scale;
+  a.h = reinterpret_cast<float*>(workspace);
+  a.rank = rank;
+  a.rank_pad = sp.rank_pad;
+  a.n_targets = n_targets;
+  a.parts = sp.parts;
+  a.rank_blocks = sp.rank_blocks;
+  int cols = 0;
+  for (int i = 0; i < n_targets; ++i) {
+    const vkwr_lora_target& t = targets[i];
+    const uint16_t* base = t.base ? t.base : t.y;
+    VK_REQUIRE(t.x && t.a && t.b && t.y, "%s: target %d: null pointer", fn, i);
+    VK_REQUIRE(((uintptr_t)t.x | (uintptr_t)t.a | (uintptr_t)t.b | (uintptr_t)t.y | (uintptr_t)base) % 16 == 0,
+               "%s: target %d: pointers must be 16-byte aligned", fn, i);
+    VK_REQUIRE(base == t.y || !overlap(base, 2 * m * t.n, t.y, 2 * m * t.n), "%s: target %d: base overlaps y", fn, i);
+    for (int j = 0; j < n_targets; ++j) {
+      VK_REQUIRE(!overlap(targets[j].x, 2 * m * targets[j].k, t.y, 2 * m * t.n), "%s: y of target %d overlaps x of %d",
+                 fn, i, j);
+      VK_REQUIRE(j == i || (!overlap(targets[j].y, 2 * m * targets[j].n, t.y, 2 * m * t.n) &&
+                            !(targets[j].base && overlap(targets[j].base, 2 * m * targets[j].n, t.y, 2 * m * t.n))),
+                 "%s: y of target %d overlaps y or base of %d", fn, i, j);
+    }
+    a.t[i] = Target{reinterpret_cast<const _Float16*>(t.x), reinterpret_cast<const _Float16*>(t.a),
+                    reinterpret_cast<const _Float16*>(t.b), reinterpret_cast<const _Float16*>(base),
+                    reinterpret_cast<_Float16*>(t.y), (int)t.n, (int)t.k,
+                    t.epilogue == VKWR_GEMM_EPI_RELU_SQUARE, cols};
+    cols += (int)((t.n + kColBlock - 1) / kColBlock);
+  }
+  VK_REQUIRE(a.tiles_cap <= 65535, "%s: %lld row tiles, at most 65535", fn, (long long)a.tiles_cap);
+  const hipStream_t s = (hipStream_t)stream;
+  const dim3 grid(sp.parts, (unsigned)a.tiles_cap, n_targets * sp.rank_blocks);
+  const int rt = (rank < kRankBlock ? sp.rank_pad : kRankBlock) / 16;
+  if (rt == 1) hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(256), 0, s, a);
+  else if (rt == 2) hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL(lora_expand_kernel, dim3(cols, (unsigned)a.tiles_cap), dim3(256),
+                     sp.rank_pad / 16 * kSub * 1024 + kTileM * 4, s, a);
+  return check_launch(fn);
+}
