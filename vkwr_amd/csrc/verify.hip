@@ -14,7 +14,7 @@
 // sum_{j' <= j} w > u_K sum w, in vocabulary order.
 //
 // Numbers are whole-token decisions next to borders of sums over the vocabulary, so they are held in
-// 64 bits: weights by a polynomial of relative error 3e-13, masses as integers in units of 2^-43
+// 64 bits: weights by a polynomial of relative error 1.1e-12, masses as integers in units of 2^-43
 // (sums of up to 2^20 weights <= 1 do not overflow, and integer sums do not depend on their order),
 // the draw's prefix sums in fp64.  A token differs from that of exact arithmetic only where a
 // uniform lies within ~1e-11 of a border.
@@ -33,7 +33,7 @@ namespace {
 constexpr int kVerThreads = 1024;
 constexpr int kVerWaves = kVerThreads / 64;
 constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
-constexpr int kVerCand = 1024;   // entries of one bin that are ranked directly
+constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
 constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a workgroup reads at once
 constexpr int kVerMaxV = 1 << 20;
 constexpr int kVerMaxTiles = kVerMaxV / kVerTile;
@@ -42,7 +42,15 @@ constexpr double kMassUnit = 1.0 / 8796093022208.0;  // 2^-43
 struct RowStat {
   double z, comp;
   float max, tau;
-  int ok, pad;
+  int ok, mode;
+};
+// How a row's logits are read so that only finite values and -inf (weight 0) remain:
+enum {
+  kPlain = 0,   // as they are: no NaN and no +inf
+  kNanZero = 1, // NaN -> 0
+  kInfOnly = 2, // +inf present (it stands for the largest float, beside which every finite value
+                // weighs nothing): +inf -> 0, anything else -> -inf
+  kAllLow = 3   // -inf everywhere: all entries tied
 };
 static_assert(sizeof(RowStat) == 32, "row stat size");
 
@@ -52,37 +60,37 @@ struct VerifyArgs {
   const int32_t *drafts, *n_draft;
   const float *q, *u;
   int32_t *tokens, *accepted;
-  RowStat* stat;
-  double scale;  // log2(e) / temperature
+  RowStat* stat;   // [B, K+1]
+  double* sums;    // [B, K+1, tiles * kVerWaves] wave sums of the weights, without a filter
+  double scale, d_min;  // log2(e) / temperature; -1023 / scale (weight 0)
   float bin_scale;
   int top_k;
   double top_p;
   int use_mass, truncate;
 };
 
-__device__ __forceinline__ float sf(float x) {
-  const float y = __builtin_isnan(x) ? 0.0f : x;
-  return fminf(fmaxf(y, -FLT_MAX), FLT_MAX);
-}
-
-// 2^x for x <= 0: x = n + f with |f| <= 1/2, the degree-10 Taylor polynomial of e^{f ln 2} (remainder
-// (0.3466)^11 / 11! = 2.2e-13), an exact power of two.
-__device__ __forceinline__ double exp2_neg(double x) {
-  x = fmax(x, -2000.0);  // -inf (padding) too; the result is 0
-  const double n = __builtin_rint(x);
-  const double f = x - n;
-  double p = 7.054911620801123e-09;
-  p = __builtin_fma(p, f, 1.0178086009239701e-07);
-  p = __builtin_fma(p, f, 1.3215486790144309e-06);
-  p = __builtin_fma(p, f, 1.5252733804059841e-05);
-  p = __builtin_fma(p, f, 1.5403530393381609e-04);
-  p = __builtin_fma(p, f, 1.3333558146428443e-03);
-  p = __builtin_fma(p, f, 9.6181291076284771e-03);
-  p = __builtin_fma(p, f, 5.5504108664821580e-02);
-  p = __builtin_fma(p, f, 2.4022650695910071e-01);
-  p = __builtin_fma(p, f, 6.9314718055994531e-01);
+// 2^(d scale) for d <= 0: d scale = n + f with |f| <= 1/2, n from the sum with 1.5 2^52, whose low word
+// it is; 2^f by the degree-8 polynomial through 2^f at the Chebyshev points of [-1/2, 1/2] (relative
+// error 1.1e-12, exactly 1 at 0); 2^n from its exponent bits.  d_min = -1023 / scale is where those
+// are all zero: from there down (masks too) the weight is exactly 0.  16 instructions at the rate of an
+// fp32 FMA (ldexp and the conversion of n took four times that each).
+__device__ __forceinline__ double exp2_neg(double d, double scale, double d_min) {
+  constexpr double kMagic = 6755399441055744.0;
+  d = fmax(d, d_min);
+  const double t = __builtin_fma(d, scale, kMagic);
+  const double f = __builtin_fma(d, scale, kMagic - t);
+  double p = 1.3255224884799127e-06;
+  p = __builtin_fma(p, f, 1.5310079402383103e-05);
+  p = __builtin_fma(p, f, 1.5403455852419016e-04);
+  p = __builtin_fma(p, f, 1.3333450568000008e-03);
+  p = __builtin_fma(p, f, 9.61812915940262e-03);
+  p = __builtin_fma(p, f, 5.550410941205934e-02);
+  p = __builtin_fma(p, f, 2.402265069581299e-01);
+  p = __builtin_fma(p, f, 6.931471805459335e-01);
   p = __builtin_fma(p, f, 1.0);
-  return __builtin_ldexp(p, (int)n);
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+  return p * __builtin_bit_cast(double, u2{0u, (n << 20) + (1023u << 20)});
 }
 
 // A weight in [0, 1] as a whole number of 2^-43: 512 + x has that spacing.
@@ -90,25 +98,64 @@ __device__ __forceinline__ uint64_t mass_of(double x) {
   return __builtin_bit_cast(uint64_t, 512.0 + x) - __builtin_bit_cast(uint64_t, 512.0);
 }
 
-template <class X>
-__device__ __forceinline__ X wave_add(X v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
+// ---- wave reductions: DPP inside rows of 16 lanes, readlane across the four rows.  Fixed order; the
+// result is wave-uniform.
+template <int CTRL, class X>
+__device__ __forceinline__ X dpp(X x) {
+  static_assert(sizeof(X) == 4 || sizeof(X) == 8, "one or two registers");
+  if constexpr (sizeof(X) == 4) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+  } else {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    const i2 v = __builtin_bit_cast(i2, x);
+    return __builtin_bit_cast(X, i2{__builtin_amdgcn_update_dpp(0, v[0], CTRL, 0xF, 0xF, true),
+                                    __builtin_amdgcn_update_dpp(0, v[1], CTRL, 0xF, 0xF, true)});
+  }
 }
-__device__ __forceinline__ float wave_fmax(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-  return v;
+template <class X>
+__device__ __forceinline__ X lane_read(X x, int l) {
+  if constexpr (sizeof(X) == 4) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+  } else {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    const i2 v = __builtin_bit_cast(i2, x);
+    return __builtin_bit_cast(X, i2{__builtin_amdgcn_readlane(v[0], l), __builtin_amdgcn_readlane(v[1], l)});
+  }
+}
+template <class X>
+__device__ __forceinline__ X wave_add(X x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  x += dpp<0x140>(x);
+  return (lane_read(x, 0) + lane_read(x, 16)) + (lane_read(x, 32) + lane_read(x, 48));
+}
+__device__ __forceinline__ float wave_fmax(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));
+  x = fmaxf(x, dpp<0x4E>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  x = fmaxf(x, dpp<0x140>(x));
+  return fmaxf(fmaxf(lane_read(x, 0), lane_read(x, 16)), fmaxf(lane_read(x, 32), lane_read(x, 48)));
+}
+// Inclusive sum in lane order: row_shr 1, 2, 4, 8 with zero fill, then the rows before.
+template <class X>
+__device__ __forceinline__ X wave_scan(X x, int lane) {
+  x += dpp<0x111>(x);
+  x += dpp<0x112>(x);
+  x += dpp<0x114>(x);
+  x += dpp<0x118>(x);
+  const X r0 = lane_read(x, 15), r1 = lane_read(x, 31), r2 = lane_read(x, 47);
+  const X r01 = r0 + r1;
+  return x + (lane < 16 ? X(0) : lane < 32 ? r0 : lane < 48 ? r01 : r01 + r2);
 }
 
 struct StatShared {
   uint64_t mass[kVerBins];
   uint32_t cnt[kVerBins];
-  uint64_t red64[kVerWaves];
-  uint64_t redm[kVerWaves];
-  uint32_t redc[kVerWaves], redd[kVerWaves];
-  float redf[kVerWaves];
+  uint64_t redm[2][kVerWaves];
+  double redd[2][kVerWaves];
+  uint32_t redc[2][kVerWaves], rede[2][kVerWaves];
+  float redf[2][kVerWaves], redg[2][kVerWaves];
   float cand[kVerCand];
   uint64_t candm[kVerCand];
   int n_cand, bin;
@@ -116,37 +163,75 @@ struct StatShared {
   uint64_t before_m;
 };
 
-// Block reductions: every lane gets the result; two barriers.
-__device__ __forceinline__ float block_fmax(StatShared& sh, float v) {
-  v = wave_fmax(v);
-  if ((threadIdx.x & 63) == 0) sh.redf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = sh.redf[0];
-#pragma unroll
-  for (int w = 1; w < kVerWaves; ++w) r = fmaxf(r, sh.redf[w]);
-  __syncthreads();
-  return r;
+// Sum (maximum) of the 16 values that the lanes of a row hold, in every lane.
+template <class X>
+__device__ __forceinline__ X row_add(X x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  return x + dpp<0x140>(x);
 }
-__device__ __forceinline__ void block_add(StatShared& sh, uint32_t& a, uint32_t& b, uint64_t& m) {
+__device__ __forceinline__ float row_fmax(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));
+  x = fmaxf(x, dpp<0x4E>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  return fmaxf(x, dpp<0x140>(x));
+}
+
+// Block reductions with one barrier: consecutive ones alternate between two buffers (par), so a wave
+// overwrites a buffer only behind the barrier that every wave reaches after reading it.  Each row of 16
+// lanes adds the 16 wave values.
+static_assert(kVerWaves == 16, "a row of lanes holds the wave values");
+__device__ __forceinline__ void block_max2(StatShared& sh, int& par, float& a, float& b) {
+  a = wave_fmax(a);
+  b = wave_fmax(b);
+  if ((threadIdx.x & 63) == 0) {
+    sh.redf[par][threadIdx.x >> 6] = a;
+    sh.redg[par][threadIdx.x >> 6] = b;
+  }
+  __syncthreads();
+  a = row_fmax(sh.redf[par][threadIdx.x & 15]);
+  b = row_fmax(sh.redg[par][threadIdx.x & 15]);
+  par ^= 1;
+}
+__device__ __forceinline__ float block_max(StatShared& sh, int& par, float a) {
+  a = wave_fmax(a);
+  if ((threadIdx.x & 63) == 0) sh.redf[par][threadIdx.x >> 6] = a;
+  __syncthreads();
+  a = row_fmax(sh.redf[par][threadIdx.x & 15]);
+  par ^= 1;
+  return a;
+}
+__device__ __forceinline__ double block_sum(StatShared& sh, int& par, double a) {
+  a = wave_add(a);
+  if ((threadIdx.x & 63) == 0) sh.redd[par][threadIdx.x >> 6] = a;
+  __syncthreads();
+  a = row_add(sh.redd[par][threadIdx.x & 15]);
+  par ^= 1;
+  return a;
+}
+__device__ __forceinline__ void block_add(StatShared& sh, int& par, uint32_t& a, uint32_t& b, uint64_t& m) {
   a = wave_add(a);
   b = wave_add(b);
   m = wave_add(m);
   if ((threadIdx.x & 63) == 0) {
     const int w = threadIdx.x >> 6;
-    sh.redc[w] = a;
-    sh.redd[w] = b;
-    sh.redm[w] = m;
+    sh.redc[par][w] = a;
+    sh.rede[par][w] = b;
+    sh.redm[par][w] = m;
   }
   __syncthreads();
-  a = b = 0;
-  m = 0;
-#pragma unroll
-  for (int w = 0; w < kVerWaves; ++w) {
-    a += sh.redc[w];
-    b += sh.redd[w];
-    m += sh.redm[w];
-  }
-  __syncthreads();
+  const int w = threadIdx.x & 15;
+  a = row_add(sh.redc[par][w]);
+  b = row_add(sh.rede[par][w]);
+  m = row_add(sh.redm[par][w]);
+  par ^= 1;
+}
+
+__device__ __forceinline__ float read_as(float l, int mode) {
+  if (mode == kInfOnly) return l == INFINITY ? 0.0f : -INFINITY;
+  if (mode == kAllLow) return 0.0f;
+  return __builtin_isnan(l) ? 0.0f : l;
 }
 
 // Order-preserving key of a finite float.
@@ -158,39 +243,51 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __builtin_bit_cast(float, (k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// Four consecutive entries of a row.
+// Four consecutive entries of a row, as stored and as finite fp32 values.
+typedef _Float16 hv4 __attribute__((ext_vector_type(4)));
 template <bool kHalf>
-__device__ __forceinline__ f4 load4(const void* row, int i) {
-  if constexpr (kHalf) {
-    typedef _Float16 hv4 __attribute__((ext_vector_type(4)));
-    const hv4 x = *reinterpret_cast<const hv4*>(reinterpret_cast<const _Float16*>(row) + i);
-    return f4{sf((float)x[0]), sf((float)x[1]), sf((float)x[2]), sf((float)x[3])};
-  } else {
-    const f4 x = *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(row) + i);
-    return f4{sf(x[0]), sf(x[1]), sf(x[2]), sf(x[3])};
-  }
+struct Raw {
+  typedef hv4 type;
+};
+template <>
+struct Raw<false> {
+  typedef f4 type;
+};
+template <bool kHalf>
+struct Elem {
+  typedef _Float16 type;
+};
+template <>
+struct Elem<false> {
+  typedef float type;
+};
+template <bool kHalf>
+__device__ __forceinline__ typename Raw<kHalf>::type load_raw(const void* row, int i) {
+  typedef typename Raw<kHalf>::type R;
+  return *reinterpret_cast<const R*>(reinterpret_cast<const char*>(row) + (size_t)i * (kHalf ? 2 : 4));
+}
+template <class R>
+__device__ __forceinline__ f4 to_f4(R x) {
+  return f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
 }
 template <bool kHalf>
 __device__ __forceinline__ const void* row_at(const VerifyArgs& p, int64_t row) {
   return reinterpret_cast<const char*>(p.logits) + row * p.V * (kHalf ? 2 : 4);
 }
-template <bool kHalf>
-__device__ __forceinline__ float load1(const void* row, int i) {
-  if constexpr (kHalf) return sf((float)reinterpret_cast<const _Float16*>(row)[i]);
-  else return sf(reinterpret_cast<const float*>(row)[i]);
-}
 
 // The kept weight of logit l in units of its row's largest weight.
-__device__ __forceinline__ double kept_of(double scale, const RowStat& st, float l) {
-  if (!(l >= st.tau)) return 0.0;
-  const double x = exp2_neg(((double)l - (double)st.max) * scale);
-  return l > st.tau ? x : x * st.comp;
+__device__ __forceinline__ double kept_of(const VerifyArgs& p, const RowStat& st, float l) {
+  const double x = exp2_neg((double)l - (double)st.max, p.scale, p.d_min);
+  return l > st.tau ? x : l == st.tau ? x * st.comp : 0.0;
 }
 
-// J > 0: the row's J tiles stay in registers (V <= J * kVerTile); J == 0: re-read in every pass.
-template <bool kHalf, int J>
+// kTiles > 0: the row (V <= kTiles * kVerTile) stays in LDS as stored; 0: it is re-read from memory in
+// every pass.
+template <bool kHalf, int kTiles>
 __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) {
+  typedef typename Raw<kHalf>::type R;
   __shared__ StatShared sh;
+  __shared__ R lrow[kTiles > 0 ? kTiles * kVerThreads : 1];
   const int T = p.K + 1;
   const int b = blockIdx.x / T, i = blockIdx.x - b * T;
   const int n = p.n_draft ? p.n_draft[b] : p.K;
@@ -198,169 +295,267 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = p.V;
   const void* row = row_at<kHalf>(p, (int64_t)b * T + i);
   const int tiles = (V + kVerTile - 1) / kVerTile;
-  f4 reg[J > 0 ? J : 1];
-  const f4 kNone = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  if constexpr (J > 0) {
+  int par = 0, mode = kPlain;
+  typedef typename Elem<kHalf>::type E;
+  const E kLow = (E)(-INFINITY);
+  const R kPad = R{kLow, kLow, kLow, kLow};
+
+  // Largest value, and whether any is NaN or infinite (x * 0 is NaN exactly then); from the first tile
+  // the smallest that is not a mask's, a guess at the histogram's range.  Every lane reads back only
+  // what it stored.
+  float mx = -INFINITY, mn = INFINITY;
+  bool odd = false;
+  {
+    R big = kPad, acc = R{};
+    constexpr int kB = 8;  // tiles whose loads are in flight together
+    for (int j0 = 0; j0 < tiles; j0 += kB) {
+      R x[kB];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int at = j * kVerTile + 4 * t;
-      reg[j] = at < V ? load4<kHalf>(row, at) : kNone;
-    }
-  }
-  // f(entry) over this lane's entries; padding entries are -inf
-  auto each = [&](auto&& f) __attribute__((always_inline)) {
-    if constexpr (J > 0) {
+      for (int u = 0; u < kB; ++u) x[u] = load_raw<kHalf>(row, min((j0 + u) * kVerTile + 4 * t, V - 4));
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f(reg[j][e]);
-    } else {
-      for (int j = 0; j < tiles; ++j) {
-        const int at = j * kVerTile + 4 * t;
-        const f4 x = at < V ? load4<kHalf>(row, at) : kNone;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f(x[e]);
+      for (int u = 0; u < kB; ++u) {
+        if (j0 + u >= tiles) break;
+        acc = __builtin_elementwise_fma(x[u], R{}, acc);  // past the end: the row's last entries again
+        if ((j0 + u + 1) * kVerTile > V) x[u] = (j0 + u) * kVerTile + 4 * t < V ? x[u] : kPad;
+        big = __builtin_elementwise_max(big, x[u]);
+        if (j0 + u == 0)
+          for (int e = 0; e < 4; ++e) mn = fminf(mn, (float)x[0][e] > -30000.0f ? (float)x[0][e] : INFINITY);
+        if constexpr (kTiles > 0) lrow[(j0 + u) * kVerThreads + t] = x[u];
       }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mx = fmaxf(mx, (float)big[e]);
+      odd = odd || __builtin_isnan((float)acc[e]);
+    }
+  }
+  auto tile_of = [&](int j) __attribute__((always_inline)) -> f4 {
+    if constexpr (kTiles > 0) {
+      return to_f4(lrow[j * kVerThreads + t]);
+    } else {
+      const int at = j * kVerTile + 4 * t;
+      f4 x = at < V ? to_f4(load_raw<kHalf>(row, at)) : f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (mode != kPlain && at < V)
+        for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], mode);
+      return x;
+    }
   };
-
-  float mx = -INFINITY;
-  each([&](float l) { mx = fmaxf(mx, l); });
-  mx = block_fmax(sh, mx);
+  // f(four entries) over this lane's entries; entries of the padding are -inf
+  auto each4 = [&](auto&& f) __attribute__((always_inline)) {
+    int j = 0;
+    for (; j + 2 <= tiles; j += 2) {
+      const f4 x = tile_of(j), y = tile_of(j + 1);
+      f(x);
+      f(y);
+    }
+    if (j < tiles) f(tile_of(j));
+  };
+  auto each = [&](auto&& f) __attribute__((always_inline)) {
+    each4([&](f4 x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(x[e]);
+    });
+  };
+  float lane_max = mx, oddf = odd ? 1.0f : 0.0f;
+  block_max2(sh, par, mx, oddf);
+  if (oddf > 0.0f) {
+    // NaN or an infinity somewhere (masked entries, often): read the row another way
+    bool nan = false;
+    each([&](float l) { nan = nan || __builtin_isnan(l); });
+    nan = block_max(sh, par, nan ? 1.0f : 0.0f) > 0.0f;
+    mode = mx == INFINITY ? kInfOnly : nan ? kNanZero : mx == -INFINITY ? kAllLow : kPlain;
+    if (mode != kPlain) {
+      if constexpr (kTiles > 0) {
+        for (int j = 0; j < tiles; ++j) {
+          const int at = j * kVerTile + 4 * t;
+          if (at >= V) continue;
+          R x = lrow[j * kVerThreads + t];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = (E)read_as((float)x[e], mode);
+          lrow[j * kVerThreads + t] = x;
+        }
+      }
+      mx = -INFINITY;
+      each([&](float l) { mx = fmaxf(mx, l); });
+      lane_max = mx;
+      mx = block_max(sh, par, mx);
+      mn = fminf(mn, 0.0f);
+    }
+  }
   const double mxd = (double)mx;
-  auto weight = [&](float l) { return exp2_neg(((double)l - mxd) * p.scale); };
+  auto weight = [&](float l) __attribute__((always_inline)) { return exp2_neg((double)l - mxd, p.scale, p.d_min); };
 
   RowStat st;
   st.max = mx;
   st.tau = -INFINITY;
   st.comp = 1.0;
-  st.ok = st.pad = 0;
+  st.ok = 0;
+  st.mode = mode;
+  uint32_t none = 0, none2 = 0;
   if (!p.truncate) {
-    uint64_t m = 0;
-    uint32_t u0 = 0, u1 = 0;
-    each([&](float l) { m += mass_of(weight(l)); });
-    block_add(sh, u0, u1, m);
-    st.z = (double)m * kMassUnit;
+    // the sums of each wave's 256 consecutive entries are kept for the draw
+    double m = 0.0;
+    double* const sums = p.sums + ((int64_t)b * T + i) * tiles * kVerWaves + wv;
+    for (int j = 0; j < tiles; ++j) {
+      const f4 x = tile_of(j);
+      const double s = wave_add((weight(x[0]) + weight(x[1])) + (weight(x[2]) + weight(x[3])));
+      if (lane == 0) sums[j * kVerWaves] = s;
+      m += s;
+    }
+    if (lane != 0) m = 0.0;
+    st.z = block_sum(sh, par, m);
   } else {
-    // Histogram of (max - l) in kVerBins equal steps: 32 per octave of the weight, or finer where
-    // the entries of weight 2^-64 and more span less than that.  Larger l never falls in a later bin.
-    float far = 0.0f;
-    each([&](float l) {
-      const float d = mx - l;
-      far = fmaxf(far, d * p.bin_scale <= (float)kVerBins ? d : 0.0f);
-    });
-    far = block_fmax(sh, far);
+    // floor: a value that tau cannot lie below; entries under it are left out of the search.  In each
+    // wave the q-th largest of its lanes' maxima, q = ceil(top_k / 16), is at or below q of its
+    // entries, so the smallest of the 16 waves' has top_k entries at or above it.
+    float floor = -INFINITY;
+    if (p.top_k <= kVerThreads) {
+      const int q = (p.top_k + kVerWaves - 1) / kVerWaves;
+      float lm = lane_max, at = -INFINITY;
+      for (int k = 0; k < q; ++k) {
+        at = wave_fmax(lm);
+        const uint64_t hit = __ballot(lm == at);
+        if (lane == (int)__builtin_ctzll(hit)) lm = -INFINITY;
+      }
+      floor = -at;
+    }
+    mn = -mn;
+    block_max2(sh, par, floor, mn);
+    floor = p.top_k <= kVerThreads ? -floor : -INFINITY;
+    mn = -mn;
+    // Histogram of (mx - l) in kVerBins equal steps: 32 per octave of the weight, or finer where the
+    // entries from floor up span less.  Larger l never falls in a later bin.  The same pass adds up
+    // the mass of the whole row, top_p's measure.
+    const float far = mx - fmaxf(mn, floor);
     const float s = far > 0.0f ? fminf(fmaxf(p.bin_scale, (float)(kVerBins - 1) / far), FLT_MAX) : p.bin_scale;
-    auto bin_of = [&](float l) { return (int)fminf((mx - l) * s, (float)(kVerBins - 1)); };
+    auto bin_at = [&](float l) __attribute__((always_inline)) { return fminf((mx - l) * s, (float)(kVerBins - 1)); };
     for (int k = t; k < kVerBins; k += kVerThreads) {
       sh.cnt[k] = 0;
       sh.mass[k] = 0;
     }
-    if (t == 0) sh.n_cand = 0;
+    if (t == 0) {
+      sh.n_cand = 0;
+      sh.bin = kVerBins;
+    }
     __syncthreads();
-    each([&](float l) {
-      if (l > -INFINITY) {
-        const int k = bin_of(l);
-        atomicAdd(&sh.cnt[k], 1u);
-        atomicAdd((unsigned long long*)&sh.mass[k], (unsigned long long)mass_of(weight(l)));
+    const bool by_count = p.top_k < V;
+    double all = 0.0;
+    floor = fmaxf(floor, -FLT_MAX);  // masked entries have no weight
+    each4([&](f4 x) __attribute__((always_inline)) {
+      double w[4];
+      if (p.use_mass) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = weight(x[e]);
+        all += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      if (__ballot(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor) == 0) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (x[e] >= floor) {
+          const int k = (int)bin_at(x[e]);
+          if (by_count) atomicAdd(&sh.cnt[k], 1u);
+          if (p.use_mass) atomicAdd((unsigned long long*)&sh.mass[k], (unsigned long long)mass_of(w[e]));
+        }
       }
     });
-    __syncthreads();
+    all = block_sum(sh, par, all);  // its barrier also ends the histogram
+    const double goal = p.top_p * all;  // in units of the largest weight
+    auto enough = [&](uint32_t c, uint64_t m) {
+      return c >= (uint32_t)p.top_k || (p.use_mass && (double)m * kMassUnit >= goal);
+    };
     // inclusive prefix over the bins (two per lane) and the first bin that reaches the budget
     const uint32_t c0 = sh.cnt[2 * t], c1 = sh.cnt[2 * t + 1];
     const uint64_t m0 = sh.mass[2 * t], m1 = sh.mass[2 * t + 1];
-    uint32_t ci = c0 + c1;
-    uint64_t mi = m0 + m1;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t co = __shfl_up(ci, d, 64);
-      const uint64_t mo = __shfl_up(mi, d, 64);
-      if (lane >= d) {
-        ci += co;
-        mi += mo;
-      }
-    }
+    uint32_t ci = wave_scan(c0 + c1, lane);
+    uint64_t mi = wave_scan(m0 + m1, lane);
     if (lane == 63) {
-      sh.redc[wv] = ci;
-      sh.redm[wv] = mi;
+      sh.redc[par][wv] = ci;
+      sh.redm[par][wv] = mi;
     }
-    if (t == 0) sh.bin = kVerBins;
     __syncthreads();
-    uint64_t all = 0;
-    for (int w = 0; w < kVerWaves; ++w) {
-      if (w < wv) {
-        ci += sh.redc[w];
-        mi += sh.redm[w];
+    ci += row_add((lane & 15) < wv ? sh.redc[par][lane & 15] : 0u);
+    mi += row_add((lane & 15) < wv ? sh.redm[par][lane & 15] : (uint64_t)0);
+    par ^= 1;
+    if (enough(ci - c1, mi - m1)) {
+      if (!enough(ci - c1 - c0, mi - m1 - m0)) {
+        sh.bin = 2 * t;
+        sh.before_c = ci - c1 - c0;
+        sh.before_m = mi - m1 - m0;
       }
-      all += sh.redm[w];
-    }
-    const double goal = p.top_p * (double)all;
-    auto enough = [&](uint32_t c, uint64_t m) { return c >= (uint32_t)p.top_k || (p.use_mass && (double)m >= goal); };
-    if (enough(ci - c1, mi - m1)) atomicMin(&sh.bin, 2 * t);
-    else if (enough(ci, mi)) atomicMin(&sh.bin, 2 * t + 1);
-    __syncthreads();
-    const int bin = sh.bin;  // exists: the count over all bins is V >= top_k
-    if (bin == 2 * t) {
-      sh.before_c = ci - c1 - c0;
-      sh.before_m = mi - m1 - m0;
-    } else if (bin == 2 * t + 1) {
+    } else if (enough(ci, mi)) {
+      sh.bin = 2 * t + 1;
       sh.before_c = ci - c1;
       sh.before_m = mi - m1;
     }
     __syncthreads();
-    const uint32_t before_c = sh.before_c;
-    const uint64_t before_m = sh.before_m;
-    const int in_bin = (int)sh.cnt[bin];
-    if (in_bin <= kVerCand) {
-      each([&](float l) {
-        if (l > -INFINITY && bin_of(l) == bin) {
-          const int at = atomicAdd(&sh.n_cand, 1);  // any order: only sums and a maximum follow
-          sh.cand[at] = l;
-          sh.candm[at] = mass_of(weight(l));
+    // None: fewer entries than top_k have a weight at all (the others are masked); all of those are kept.
+    const bool found = sh.bin < kVerBins;
+    const int bin = found ? sh.bin : kVerBins - 1;
+    const uint32_t before_c = found ? sh.before_c : 0;
+    const uint64_t before_m = found ? sh.before_m : 0;
+    if (found) {
+      const float bf = (float)bin;
+      // the bin's span in logits with room for rounding, so that most groups are passed over quickly
+      const float room = 1.0e-5f * (fabsf(mx) + (float)kVerBins / s);
+      const float top = bin == 0 ? mx : mx - bf / s + room;
+      const float low = bin == kVerBins - 1 ? floor : fmaxf(floor, mx - (bf + 1.0f) / s - room);
+      each4([&](f4 x) __attribute__((always_inline)) {
+        bool in[4], any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any = any || (x[e] >= low && x[e] <= top);
+        if (__ballot(any) == 0) return;
+        any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float at = bin_at(x[e]);
+          in[e] = at >= bf && at < bf + 1.0f && x[e] >= floor;
+          any = any || in[e];
+        }
+        if (__ballot(any) == 0) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (in[e]) {
+            const int at = atomicAdd(&sh.n_cand, 1);  // any order: only sums and a maximum follow
+            if (at < kVerCand) {
+              sh.cand[at] = x[e];
+              sh.candm[at] = p.use_mass ? mass_of(weight(x[e])) : 0;
+            }
+          }
         }
       });
-      __syncthreads();
-      float best = -INFINITY;
+    }
+    __syncthreads();
+    const int in_bin = found ? sh.n_cand : kVerCand + 1;
+    if (!found) floor = -FLT_MAX;
+    uint32_t ngt = 0, neq = 0;
+    uint64_t mgt = 0;
+    if (in_bin <= kVerCand) {
+      uint32_t c = before_c;
+      uint64_t m = before_m;
+      float v = -INFINITY;
       if (t < in_bin) {
-        const float v = sh.cand[t];
-        uint32_t c = before_c;
-        uint64_t m = before_m;
+        v = sh.cand[t];
         for (int k = 0; k < in_bin; ++k) {
           const bool ge = sh.cand[k] >= v;
           c += ge ? 1u : 0u;
           m += ge ? sh.candm[k] : 0;
         }
-        if (enough(c, m)) best = v;
       }
-      st.tau = block_fmax(sh, best);
+      st.tau = block_max(sh, par, t < in_bin && enough(c, m) ? v : -INFINITY);
+      ngt = t < in_bin && v > st.tau ? 1 : 0;
+      neq = t < in_bin && v == st.tau ? 1 : 0;
+      mgt = ngt ? sh.candm[t] : 0;
+      block_add(sh, par, ngt, neq, mgt);
+      ngt += before_c;
+      mgt += before_m;
     } else {
-      // many entries in one bin (ties, or a spread that outliers stretch): bisection over keys
-      uint32_t lo = 0xffffffffu, hi = 0;
-      each([&](float l) {
-        if (l > -INFINITY && bin_of(l) == bin) {
-          lo = min(lo, key_of(l));
-          hi = max(hi, key_of(l));
-        }
-      });
-#pragma unroll
-      for (int m = 32; m >= 1; m >>= 1) {
-        lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
-        hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
-      }
-      if (lane == 0) {
-        sh.redc[wv] = lo;
-        sh.redd[wv] = hi;
-      }
-      __syncthreads();
-      for (int w = 0; w < kVerWaves; ++w) {
-        lo = min(lo, sh.redc[w]);
-        hi = max(hi, sh.redd[w]);
-      }
-      __syncthreads();
-      while (lo < hi) {  // the largest key with enough entries at or above it: at most 32 rounds
+      // many entries in one bin (ties, or a spread that outliers stretch): bisection over the keys of
+      // every entry, at most 32 rounds, for the largest value with enough entries at or above it
+      uint32_t lo = key_of(floor), hi = found ? key_of(mx) : lo;
+      while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2u + 1u;
         const float v = of_key(mid);
-        uint32_t c = 0, unused = 0;
+        uint32_t c = 0;
         uint64_t m = 0;
         each([&](float l) {
           if (l >= v) {
@@ -368,36 +563,46 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
             m += p.use_mass ? mass_of(weight(l)) : 0;
           }
         });
-        block_add(sh, c, unused, m);
+        block_add(sh, par, c, none, m);
         if (enough(c, m)) lo = mid;
         else hi = mid - 1u;
       }
-      st.tau = of_key(lo);
+      // lo may lie below every entry: then tau is the smallest of them
+      float least = -INFINITY;
+      const float lov = of_key(lo);
+      each([&](float l) { least = l >= lov ? fmaxf(least, -l) : least; });
+      st.tau = -block_max(sh, par, least);
+      each([&](float l) {
+        ngt += l > st.tau ? 1 : 0;
+        neq += l == st.tau ? 1 : 0;
+        mgt += l > st.tau && p.use_mass ? mass_of(weight(l)) : 0;
+      });
+      block_add(sh, par, ngt, neq, mgt);
     }
-    // entries above and at tau
-    uint32_t ngt = 0, neq = 0;
-    uint64_t mgt = 0;
-    each([&](float l) {
-      if (l > st.tau) {
-        ngt += 1;
-        mgt += mass_of(weight(l));
-      }
-      neq += l == st.tau ? 1 : 0;
-    });
-    block_add(sh, ngt, neq, mgt);
+    if (!p.use_mass) {  // the mass above tau was not needed so far
+      mgt = 0;
+      each4([&](f4 x) __attribute__((always_inline)) {
+        if (__ballot(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > st.tau) == 0) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mgt += x[e] > st.tau ? mass_of(weight(x[e])) : 0;
+      });
+      block_add(sh, par, none, none2, mgt);
+    }
     const double x = weight(st.tau);
-    double comp = (double)((int64_t)p.top_k - (int64_t)ngt) / (double)neq;
-    if (p.use_mass) comp = fmin(comp, (goal - (double)mgt) * kMassUnit / (x * (double)neq));
+    double comp = by_count ? (double)((int64_t)p.top_k - (int64_t)ngt) / (double)neq : 1.0;
+    if (p.use_mass) comp = fmin(comp, (goal - (double)mgt * kMassUnit) / (x * (double)neq));
     comp = fmax(fmin(comp, 1.0), 0.0);
     // no entry above tau: the kept ones are ties, whose common share does not matter
-    st.comp = ngt == 0 ? 1.0 : comp;
+    st.comp = mgt == 0 ? 1.0 : comp;
     st.z = (double)mgt * kMassUnit + st.comp * x * (double)neq;
   }
   if (t == 0) {
     if (i < n) {
       const int d = p.drafts[(int64_t)b * p.K + i];
       const bool in = d >= 0 && d < V;
-      const double pd = in ? kept_of(p.scale, st, load1<kHalf>(row, d)) / st.z : 0.0;
+      const float l = in ? read_as(kHalf ? (float)reinterpret_cast<const _Float16*>(row)[d]
+                                         : reinterpret_cast<const float*>(row)[d], mode) : 0.0f;
+      const double pd = in ? kept_of(p, st, l) / st.z : 0.0;
       const double qd = p.q ? (in ? (double)p.q[((int64_t)b * p.K + i) * V + d] : 0.0) : 1.0;
       st.ok = (double)p.u[(int64_t)b * T + i] * qd < pd ? 1 : 0;
     }
@@ -422,8 +627,16 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs p) 
     if (t == 0) p.accepted[b] = -1;
     return;
   }
-  int j = 0;
-  while (j < n && p.stat[(int64_t)b * T + j].ok) ++j;
+  // the first rejected row, 64 at a time
+  int j = n;
+  for (int k0 = 0; k0 < n; k0 += 64) {
+    const bool no = k0 + lane < n && !p.stat[(int64_t)b * T + k0 + lane].ok;
+    const uint64_t hit = __ballot(no);
+    if (hit) {
+      j = k0 + __builtin_ctzll(hit);
+      break;
+    }
+  }
   const RowStat st = p.stat[(int64_t)b * T + j];
   const void* row = row_at<kHalf>(p, (int64_t)b * T + j);
   const float* q = p.q && j < n ? p.q + ((int64_t)b * p.K + j) * V : nullptr;
@@ -431,123 +644,145 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs p) 
   const int tiles = (V + kVerTile - 1) / kVerTile, n_sum = tiles * kVerWaves;
   const double inv_z = 1.0 / st.z;
   bool beyond = j < n;  // draw from what p has beyond q
-  // weights of the four entries at `at`
-  auto weights = [&](int at, double* w) {
-    const f4 l = load4<kHalf>(row, at);
-    f4 qv = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (q && beyond) qv = *reinterpret_cast<const f4*>(q + at);
+  // weights of four entries at `at`
+  auto weights = [&](f4 l, f4 qv, int at, double* w) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      double x = kept_of(p.scale, st, l[e]) * inv_z;
-      if (beyond) x = p.q ? fmax(x - (double)qv[e], 0.0) : (at + e == draft ? 0.0 : x);
-      w[e] = x;
-    }
+    for (int e = 0; e < 4; ++e) w[e] = 0.0;
+    if (p.truncate && __ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= st.tau) == 0) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = kept_of(p, st, l[e]) * inv_z;
+    if (!beyond) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = p.q ? fmax(w[e] - (double)qv[e], 0.0) : at + e == draft ? 0.0 : w[e];
   };
+  const f4 kZero = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  const f4 kPad = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  auto load_l = [&](int at) {
+    f4 x = at < V ? to_f4(load_raw<kHalf>(row, at)) : kPad;
+    if (st.mode != kPlain && at < V)
+      for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], st.mode);
+    return x;
+  };
+  auto load_q = [&](int at) { return q && beyond && at < V ? *reinterpret_cast<const f4*>(q + at) : kZero; };
+  const int per = (n_sum + kVerThreads - 1) / kVerThreads;  // wave sums per lane in the scan: at most 4
   double total, lane_total;
+  // Without a filter the row's sums are there; a lookup's rejected draft changes one of them.
+  const bool kept_sums = !p.truncate && !q;
+  const int64_t row_id = (int64_t)b * T + j;
   for (;;) {
-    for (int k = 0; k < tiles; ++k) {
-      const int at = k * kVerTile + 4 * t;
-      double w[4] = {0.0, 0.0, 0.0, 0.0};
-      if (at < V) weights(at, w);
-      const double s = wave_add((w[0] + w[1]) + (w[2] + w[3]));
-      if (lane == 0) sh.sum[k * kVerWaves + wv] = s;
-    }
-    __syncthreads();
-    // prefix over the wave sums, ceil(n_sum / 1024) <= 4 consecutive ones per lane
-    const int per = (n_sum + kVerThreads - 1) / kVerThreads;
-    double s = 0.0;
-    for (int k = t * per; k < min((t + 1) * per, n_sum); ++k) s += sh.sum[k];
-    double incl = s;
+    if (kept_sums) {
+      const double* src = p.sums + row_id * n_sum;
+      const int ds = beyond && draft >= 0 && draft < V ? draft / kVerTile * kVerWaves + (draft % kVerTile) / 256 : -1;
+      for (int k = t; k < n_sum; k += kVerThreads)
+        if (k != ds) sh.sum[k] = src[k] * inv_z;
+      if (ds >= 0 && wv == ds % kVerWaves) {
+        double w[4];
+        const int at = ds / kVerWaves * kVerTile + 4 * t;
+        weights(load_l(at), kZero, at, w);
+        const double s = wave_add((w[0] + w[1]) + (w[2] + w[3]));
+        if (lane == 0) sh.sum[ds] = s;
+      }
+    } else {
+    // kB tiles at a time: their loads are issued together, then their sums
+    constexpr int kB = 4;
+    for (int k0 = 0; k0 < tiles; k0 += kB) {
+      f4 l[kB], qv[kB];
+      double s[kB];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double o = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += o;
+      for (int k = 0; k < kB; ++k) {
+        const int at = (k0 + k) * kVerTile + 4 * t;
+        l[k] = load_l(at);
+        qv[k] = load_q(at);
+      }
+#pragma unroll
+      for (int k = 0; k < kB; ++k) {
+        double w[4];
+        weights(l[k], qv[k], (k0 + k) * kVerTile + 4 * t, w);
+        s[k] = (w[0] + w[1]) + (w[2] + w[3]);
+      }
+#pragma unroll
+      for (int k = 0; k < kB; ++k) s[k] = wave_add(s[k]);
+#pragma unroll
+      for (int k = 0; k < kB; ++k)
+        if (lane == 0 && k0 + k < tiles) sh.sum[(k0 + k) * kVerWaves + wv] = s[k];
     }
-    if (lane == 63) sh.red[wv] = incl;
+    }
     if (t == 0) {
       sh.first = n_sum;
       sh.last = -1;
     }
     __syncthreads();
-    total = 0.0;
-    double pre = 0.0;
-    for (int w = 0; w < kVerWaves; ++w) {
-      if (w == wv) pre = total;
-      total += sh.red[w];
-    }
-    lane_total = pre + incl - s;
+    double s = 0.0;
+    for (int k = t * per; k < min((t + 1) * per, n_sum); ++k) s += sh.sum[k];
+    const double incl = wave_scan(s, lane);
+    if (lane == 63) sh.red[wv] = incl;
+    __syncthreads();
+    const double of_wave = sh.red[lane & 15];
+    total = row_add(of_wave);
+    lane_total = row_add((lane & 15) < wv ? of_wave : 0.0) + incl - s;
     if (total > 0.0 || !beyond) break;
     beyond = false;
     __syncthreads();
   }
   const double target = (double)p.u[(int64_t)b * T + p.K] * total;
-  {
-    const int per = (n_sum + kVerThreads - 1) / kVerThreads;
-    double run = lane_total;
-    int first = n_sum, last = -1;
-    for (int k = t * per; k < min((t + 1) * per, n_sum); ++k) {
-      const double s = sh.sum[k];
-      if (s > 0.0) {
-        last = k;
-        if (run + s > target && first == n_sum) first = k;
-      }
-      run += s;
+  double run = lane_total;
+  int first = n_sum, last = -1;
+  for (int k = t * per; k < min((t + 1) * per, n_sum); ++k) {
+    const double s = sh.sum[k];
+    if (s > 0.0) {
+      last = k;
+      if (run + s > target && first == n_sum) first = k;
     }
-    if (first < n_sum) atomicMin(&sh.first, first);
-    if (last >= 0) atomicMax(&sh.last, last);
+    run += s;
   }
+  if (first < n_sum) atomicMin(&sh.first, first);
+  if (last >= 0) atomicMax(&sh.last, last);
   __syncthreads();
   for (int k = t; k < T; k += kVerThreads)
     if (k != j) out[k] = k < j ? p.drafts[(int64_t)b * p.K + k] : -1;
   if (t == 0) p.accepted[b] = j;
   // the 256 entries that hold the target (rounding short of the end: the last with weight), by one wave
   const int seg = sh.first < n_sum ? sh.first : sh.last;
-  if (wv != 0 || seg < 0) {
-    if (seg < 0 && t == 0) out[j] = -1;
+  if (wv != 0) return;
+  if (seg < 0) {
+    if (lane == 0) out[j] = -1;
     return;
   }
   double before = 0.0;
-  // the prefix before the segment again, in the order that found it
-  {
-    const int per = (n_sum + kVerThreads - 1) / kVerThreads;
-    (void)per;
-    for (int k = lane; k < seg; k += 64) before += sh.sum[k];
-    before = wave_add(before);
-  }
+  for (int k = lane; k < seg; k += 64) before += sh.sum[k];
+  before = wave_add(before);
   const int at = (seg / kVerWaves) * kVerTile + (seg % kVerWaves) * 256 + 4 * lane;
-  double w[4] = {0.0, 0.0, 0.0, 0.0};
-  if (at < V) weights(at, w);
-  double incl = (w[0] + w[1]) + (w[2] + w[3]);
-  const double mine = incl;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += o;
-  }
-  double run = before + incl - mine;
-  int pick = -1, last = -1;
+  double w[4];
+  weights(load_l(at), load_q(at), at, w);
+  const double mine = (w[0] + w[1]) + (w[2] + w[3]);
+  run = before + wave_scan(mine, lane) - mine;
+  int pick = -1, end = -1;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     run += w[e];
     if (w[e] > 0.0) {
-      last = at + e;
+      end = at + e;
       if (pick < 0 && run > target) pick = at + e;
     }
   }
-  const uint64_t hit = __ballot(pick >= 0), any = __ballot(last >= 0);
+  const uint64_t hit = __ballot(pick >= 0), any = __ballot(end >= 0);
   if (hit) {
     if (lane == __builtin_ctzll(hit)) out[j] = pick;
   } else if (any) {
-    if (lane == 63 - __builtin_clzll(any)) out[j] = last;
+    if (lane == 63 - __builtin_clzll(any)) out[j] = end;
   }
 }
 
+// Rows of up to 128 KiB stay in LDS (one workgroup per CU then; up to 32 KiB two), longer ones are
+// re-read from memory.
 template <bool kHalf>
 void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
+  constexpr int kTileBytes = kVerTile * (kHalf ? 2 : 4);
+  constexpr int kSmall = (32 << 10) / kTileBytes, kLarge = (128 << 10) / kTileBytes;
   const dim3 grid(B * (a.K + 1)), block(kVerThreads);
   const int tiles = (a.V + kVerTile - 1) / kVerTile;
-  if (tiles <= 4) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 4>), grid, block, 0, s, a);
-  else if (tiles <= 16) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 16>), grid, block, 0, s, a);
+  if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall>), grid, block, 0, s, a);
+  else if (tiles <= kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0>), grid, block, 0, s, a);
   hipLaunchKernelGGL(verify_draw_kernel<kHalf>, dim3(B), block, 0, s, a);
 }
@@ -558,8 +793,9 @@ void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
 using namespace vk;
 
 extern "C" int64_t vkwr_sampling_verify_workspace_bytes(int B, int K, int V) {
-  (void)V;
-  return B > 0 && K >= 0 ? (int64_t)B * ((int64_t)K + 1) * (int64_t)sizeof(RowStat) : 0;
+  if (B <= 0 || K < 0 || V <= 0) return 0;
+  const int64_t rows = (int64_t)B * ((int64_t)K + 1), tiles = (V + kVerTile - 1) / kVerTile;
+  return rows * ((int64_t)sizeof(RowStat) + tiles * kVerWaves * (int64_t)sizeof(double));
 }
 
 extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logits, int logits_f16,
@@ -599,7 +835,9 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.tokens = tokens;
   a.accepted = accepted;
   a.stat = reinterpret_cast<RowStat*>(workspace);
+  a.sums = reinterpret_cast<double*>(a.stat + (int64_t)B * ((int64_t)K + 1));
   a.scale = 1.4426950408889634 / temperature;
+  a.d_min = -1023.0 / a.scale;
   a.bin_scale = (float)(32.0 * a.scale);
   a.top_k = top_k;
   a.top_p = top_p;
