@@ -19,8 +19,10 @@
 // the draw's prefix sums in fp64.  A token differs from that of exact arithmetic only where a
 // uniform lies within ~1e-11 of a border.
 //
-// Two launches: one workgroup per row finds max, tau, comp and Z and tests the row's draft; one
-// workgroup per sequence finds its first rejected row and draws.
+// Launches: one workgroup per row finds max, tau, comp and Z and tests the row's draft; the row that a
+// sequence stops at is added up in segments of 256 entries, by several workgroups (without a filter and
+// without a drafter's distribution the rows' workgroups have done that already: no launch); one
+// workgroup per sequence finds the segment and the entry that the uniform falls on.
 
 #include <cfloat>
 
@@ -36,7 +38,8 @@ constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
 constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
 constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a workgroup reads at once
 constexpr int kVerMaxV = 1 << 20;
-constexpr int kVerMaxTiles = kVerMaxV / kVerTile;
+constexpr int kSeg = 256;        // consecutive entries whose weights are added up for the draw (one wave's 64 x 4)
+constexpr int kMaxSegs = kVerMaxV / kSeg;
 constexpr double kMassUnit = 1.0 / 8796093022208.0;  // 2^-43
 
 struct RowStat {
@@ -61,7 +64,8 @@ struct VerifyArgs {
   const float *q, *u;
   int32_t *tokens, *accepted;
   RowStat* stat;   // [B, K+1]
-  double* sums;    // [B, K+1, tiles * kVerWaves] wave sums of the weights, without a filter
+  double* sums;    // [B, K+1, segments] what the segments of a row hold
+  int segs;
   double scale, d_min;  // log2(e) / temperature; -1023 / scale (weight 0)
   float bin_scale;
   int top_k;
@@ -130,6 +134,18 @@ __device__ __forceinline__ X wave_add(X x) {
   x += dpp<0x140>(x);
   return (lane_read(x, 0) + lane_read(x, 16)) + (lane_read(x, 32) + lane_read(x, 48));
 }
+// Sums of four values over the wave, x[l & 3] in lane l: each step on lane bits 0 and 1 halves the number
+// of values a lane carries; then the 16 quads.  A third of four separate sums' instructions.
+__device__ __forceinline__ double wave_add4(const double* x, int lane) {
+  const bool b0 = lane & 1, b1 = lane & 2;
+  const double p = (b0 ? x[1] : x[0]) + dpp<0xB1>(b0 ? x[0] : x[1]);
+  const double q = (b0 ? x[3] : x[2]) + dpp<0xB1>(b0 ? x[2] : x[3]);
+  double r = (b1 ? q : p) + dpp<0x4E>(b1 ? p : q);
+  r += dpp<0x124>(r);  // rotations by 4 and 8 inside the row
+  r += dpp<0x128>(r);
+  r += __shfl_xor(r, 16, 64);
+  return r + __shfl_xor(r, 32, 64);
+}
 __device__ __forceinline__ float wave_fmax(float x) {
   x = fmaxf(x, dpp<0xB1>(x));
   x = fmaxf(x, dpp<0x4E>(x));
@@ -156,7 +172,7 @@ struct StatShared {
   double redd[2][kVerWaves];
   uint32_t redc[2][kVerWaves], rede[2][kVerWaves];
   float redf[2][kVerWaves], redg[2][kVerWaves];
-  float cand[kVerCand];
+  alignas(16) float cand[kVerCand];
   uint64_t candm[kVerCand];
   int n_cand, bin;
   uint32_t before_c;
@@ -329,26 +345,30 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
       odd = odd || __builtin_isnan((float)acc[e]);
     }
   }
-  auto tile_of = [&](int j) __attribute__((always_inline)) -> f4 {
-    if constexpr (kTiles > 0) {
-      return to_f4(lrow[j * kVerThreads + t]);
-    } else {
-      const int at = j * kVerTile + 4 * t;
-      f4 x = at < V ? to_f4(load_raw<kHalf>(row, at)) : f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (mode != kPlain && at < V)
-        for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], mode);
-      return x;
-    }
+  auto raw_of = [&](int j) __attribute__((always_inline)) -> R {
+    if constexpr (kTiles > 0) return lrow[j * kVerThreads + t];
+    else return load_raw<kHalf>(row, min(j * kVerTile + 4 * t, V - 4));
   };
-  // f(four entries) over this lane's entries; entries of the padding are -inf
+  auto entries = [&](int j, R x) __attribute__((always_inline)) -> f4 {
+    f4 l = to_f4(x);
+    if constexpr (kTiles == 0) {
+      if (mode != kPlain)
+        for (int e = 0; e < 4; ++e) l[e] = read_as(l[e], mode);
+      if ((j + 1) * kVerTile > V && j * kVerTile + 4 * t >= V) l = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    }
+    return l;
+  };
+  // f(four entries) over this lane's entries, four tiles' loads at a time; entries of the padding are -inf
   auto each4 = [&](auto&& f) __attribute__((always_inline)) {
     int j = 0;
-    for (; j + 2 <= tiles; j += 2) {
-      const f4 x = tile_of(j), y = tile_of(j + 1);
-      f(x);
-      f(y);
+    for (; j + 4 <= tiles; j += 4) {
+      const R x0 = raw_of(j), x1 = raw_of(j + 1), x2 = raw_of(j + 2), x3 = raw_of(j + 3);
+      f(entries(j, x0));
+      f(entries(j + 1, x1));
+      f(entries(j + 2, x2));
+      f(entries(j + 3, x3));
     }
-    if (j < tiles) f(tile_of(j));
+    for (; j < tiles; ++j) f(entries(j, raw_of(j)));
   };
   auto each = [&](auto&& f) __attribute__((always_inline)) {
     each4([&](f4 x) __attribute__((always_inline)) {
@@ -393,16 +413,24 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   st.mode = mode;
   uint32_t none = 0, none2 = 0;
   if (!p.truncate) {
-    // the sums of each wave's 256 consecutive entries are kept for the draw
+    // the sums of the segments are kept for the draw
     double m = 0.0;
-    double* const sums = p.sums + ((int64_t)b * T + i) * tiles * kVerWaves + wv;
-    for (int j = 0; j < tiles; ++j) {
-      const f4 x = tile_of(j);
-      const double s = wave_add((weight(x[0]) + weight(x[1])) + (weight(x[2]) + weight(x[3])));
-      if (lane == 0) sums[j * kVerWaves] = s;
-      m += s;
+    double* const sums = p.sums + ((int64_t)b * T + i) * p.segs + wv;
+    for (int j = 0; j < tiles; j += 4) {
+      double s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        s[u] = 0.0;
+        if (j + u < tiles) {
+          const f4 x = entries(j + u, raw_of(j + u));
+          s[u] = (weight(x[0]) + weight(x[1])) + (weight(x[2]) + weight(x[3]));
+        }
+      }
+      m += (s[0] + s[1]) + (s[2] + s[3]);
+      const double w = wave_add4(s, lane);
+      const int seg = (j + lane) * kVerWaves;
+      if (lane < 4 && seg + wv < p.segs) sums[seg] = w;
     }
-    if (lane != 0) m = 0.0;
     st.z = block_sum(sh, par, m);
   } else {
     // floor: a value that tau cannot lie below; entries under it are left out of the search.  In each
@@ -533,12 +561,20 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
       uint32_t c = before_c;
       uint64_t m = before_m;
       float v = -INFINITY;
+      if (t < 4 && in_bin + t < kVerCand) sh.cand[in_bin + t] = -INFINITY;  // fills the last group of four
+      __syncthreads();
       if (t < in_bin) {
         v = sh.cand[t];
-        for (int k = 0; k < in_bin; ++k) {
-          const bool ge = sh.cand[k] >= v;
-          c += ge ? 1u : 0u;
-          m += ge ? sh.candm[k] : 0;
+        for (int k = 0; k < in_bin; k += 4) {
+          const f4 o = *reinterpret_cast<const f4*>(&sh.cand[k]);
+          uint64_t om[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) om[e] = sh.candm[k + e];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            c += o[e] >= v ? 1u : 0u;
+            m += o[e] >= v ? om[e] : 0;
+          }
         }
       }
       st.tau = block_max(sh, par, t < in_bin && enough(c, m) ? v : -INFINITY);
@@ -610,152 +646,201 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   }
 }
 
-struct DrawShared {
-  double sum[kVerMaxTiles * kVerWaves];  // mass of each tile's 256 entries per wave
-  double red[kVerWaves];
-  int first, last;
-};
-
+// What the two kernels behind the rows' share: the row a sequence stops at and the weights it draws from.
 template <bool kHalf>
-__global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs p) {
-  __shared__ DrawShared sh;
-  const int T = p.K + 1, b = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6, V = p.V;
-  const int n = p.n_draft ? p.n_draft[b] : p.K;
-  int32_t* out = p.tokens + (int64_t)b * T;
-  if (n < 0 || n > p.K) {
-    for (int k = t; k < T; k += kVerThreads) out[k] = -1;
-    if (t == 0) p.accepted[b] = -1;
-    return;
-  }
-  // the first rejected row, 64 at a time
-  int j = n;
-  for (int k0 = 0; k0 < n; k0 += 64) {
-    const bool no = k0 + lane < n && !p.stat[(int64_t)b * T + k0 + lane].ok;
-    const uint64_t hit = __ballot(no);
-    if (hit) {
-      j = k0 + __builtin_ctzll(hit);
-      break;
+struct Stop {
+  const VerifyArgs& p;
+  int64_t id;      // row b (K + 1) + j
+  int j, n, draft;
+  const float* q;  // the drafter's row, where j is a rejected draft's and there is one
+  bool beyond;     // draw from what p has beyond q
+  RowStat st;
+  double unit, unit_tau;  // of a weight above tau, and at it
+  const void* row;
+
+  __device__ __forceinline__ Stop(const VerifyArgs& a, int b, int n_, int lane) : p(a), n(n_) {
+    const int T = p.K + 1;
+    j = n;
+    for (int k0 = 0; k0 < n; k0 += 64) {
+      const uint64_t hit = __ballot(k0 + lane < n && !p.stat[(int64_t)b * T + k0 + lane].ok);
+      if (hit) {
+        j = k0 + __builtin_ctzll(hit);
+        break;
+      }
     }
+    id = (int64_t)b * T + j;
+    st = p.stat[id];
+    row = row_at<kHalf>(p, id);
+    beyond = j < n;
+    q = p.q && beyond ? p.q + ((int64_t)b * p.K + j) * p.V : nullptr;
+    draft = beyond && !p.q ? p.drafts[(int64_t)b * p.K + j] : -1;
+    unit = 1.0 / st.z;
+    unit_tau = unit * st.comp;
   }
-  const RowStat st = p.stat[(int64_t)b * T + j];
-  const void* row = row_at<kHalf>(p, (int64_t)b * T + j);
-  const float* q = p.q && j < n ? p.q + ((int64_t)b * p.K + j) * V : nullptr;
-  const int draft = j < n && !p.q ? p.drafts[(int64_t)b * p.K + j] : -1;
-  const int tiles = (V + kVerTile - 1) / kVerTile, n_sum = tiles * kVerWaves;
-  const double inv_z = 1.0 / st.z;
-  bool beyond = j < n;  // draw from what p has beyond q
-  // weights of four entries at `at`
-  auto weights = [&](f4 l, f4 qv, int at, double* w) __attribute__((always_inline)) {
+  __device__ __forceinline__ f4 load_l(int at) const {
+    f4 x = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (at < p.V) {
+      x = to_f4(load_raw<kHalf>(row, at));
+      if (st.mode != kPlain)
+        for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], st.mode);
+    }
+    return x;
+  }
+  __device__ __forceinline__ f4 load_q(int at) const {
+    return q && beyond && at < p.V ? *reinterpret_cast<const f4*>(q + at) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // weights of the four entries at `at`
+  __device__ __forceinline__ void weights(f4 l, f4 qv, int at, double* w) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = 0.0;
     if (p.truncate && __ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= st.tau) == 0) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = kept_of(p, st, l[e]) * inv_z;
+    for (int e = 0; e < 4; ++e) {
+      const double x = exp2_neg((double)l[e] - (double)st.max, p.scale, p.d_min);
+      w[e] = x * (l[e] > st.tau ? unit : l[e] == st.tau ? unit_tau : 0.0);
+    }
     if (!beyond) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = p.q ? fmax(w[e] - (double)qv[e], 0.0) : at + e == draft ? 0.0 : w[e];
+  }
+};
+
+// The segments' sums of the row each sequence stops at (not where the rows' kernel left them: without
+// a filter, all drafts accepted).  A workgroup takes 8 segments for each of its 4 waves.
+constexpr int kPartSegs = 8;
+template <bool kHalf>
+__global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
+  const int parts = (p.segs + 4 * kPartSegs - 1) / (4 * kPartSegs);
+  const int b = blockIdx.x / parts, part = blockIdx.x - b * parts, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int n = p.n_draft ? p.n_draft[b] : p.K;
+  if (n < 0 || n > p.K) return;
+  const Stop<kHalf> stop(p, b, n, lane);
+  if (!p.truncate && !stop.beyond) return;
+  const int seg0 = (part * 4 + wv) * kPartSegs;
+  f4 l[kPartSegs], qv[kPartSegs];
+#pragma unroll
+  for (int k = 0; k < kPartSegs; ++k) {
+    const int at = (seg0 + k) * kSeg + 4 * lane;
+    l[k] = stop.load_l(at);
+    qv[k] = stop.load_q(at);
+  }
+  double* const sums = p.sums + stop.id * p.segs + seg0;
+#pragma unroll
+  for (int k0 = 0; k0 < kPartSegs; k0 += 4) {
+    double s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      double w[4];
+      stop.weights(l[k0 + u], qv[k0 + u], (seg0 + k0 + u) * kSeg + 4 * lane, w);
+      s[u] = (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    const double w = wave_add4(s, lane);
+    if (lane < 4 && seg0 + k0 + lane < p.segs) sums[k0 + lane] = w;
+  }
+}
+
+constexpr int kDrawThreads = 256;
+struct DrawShared {
+  double sum[kMaxSegs];
+  double red[4];
+  int first, last;
+};
+
+// One workgroup per sequence: the segment that holds the target, then the entry.
+template <bool kHalf>
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p) {
+  __shared__ DrawShared sh;
+  const int T = p.K + 1, b = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6, segs = p.segs;
+  const int n = p.n_draft ? p.n_draft[b] : p.K;
+  const double u = (double)p.u[(int64_t)b * T + p.K];
+  int32_t* out = p.tokens + (int64_t)b * T;
+  if (n < 0 || n > p.K) {
+    for (int k = t; k < T; k += kDrawThreads) out[k] = -1;
+    if (t == 0) p.accepted[b] = -1;
+    return;
+  }
+  Stop<kHalf> stop(p, b, n, lane);
+  const int j = stop.j;
+  for (int k = t; k < T; k += kDrawThreads)
+    if (k != j) out[k] = k < j ? p.drafts[(int64_t)b * p.K + k] : -1;
+  if (t == 0) p.accepted[b] = j;
+  // the sum of segment k by one wave (the rows' and parts' kernels' order of additions aside)
+  auto segment = [&](int k) {
+    double w[4];
+    const int at = k * kSeg + 4 * lane;
+    stop.weights(stop.load_l(at), stop.load_q(at), at, w);
+    return wave_add((w[0] + w[1]) + (w[2] + w[3]));
   };
-  const f4 kZero = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  const f4 kPad = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  auto load_l = [&](int at) {
-    f4 x = at < V ? to_f4(load_raw<kHalf>(row, at)) : kPad;
-    if (st.mode != kPlain && at < V)
-      for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], st.mode);
-    return x;
-  };
-  auto load_q = [&](int at) { return q && beyond && at < V ? *reinterpret_cast<const f4*>(q + at) : kZero; };
-  const int per = (n_sum + kVerThreads - 1) / kVerThreads;  // wave sums per lane in the scan: at most 4
-  double total, lane_total;
-  // Without a filter the row's sums are there; a lookup's rejected draft changes one of them.
-  const bool kept_sums = !p.truncate && !q;
-  const int64_t row_id = (int64_t)b * T + j;
-  for (;;) {
-    if (kept_sums) {
-      const double* src = p.sums + row_id * n_sum;
-      const int ds = beyond && draft >= 0 && draft < V ? draft / kVerTile * kVerWaves + (draft % kVerTile) / 256 : -1;
-      for (int k = t; k < n_sum; k += kVerThreads)
-        if (k != ds) sh.sum[k] = src[k] * inv_z;
-      if (ds >= 0 && wv == ds % kVerWaves) {
-        double w[4];
-        const int at = ds / kVerWaves * kVerTile + 4 * t;
-        weights(load_l(at), kZero, at, w);
-        const double s = wave_add((w[0] + w[1]) + (w[2] + w[3]));
-        if (lane == 0) sh.sum[ds] = s;
+  const int per = (segs + kDrawThreads - 1) / kDrawThreads;  // segments per lane of the scan: at most 16
+  const int k0 = min(t * per, segs), k1 = min(k0 + per, segs);
+  double total, run0;
+  for (bool again = false;; again = true) {
+    if (again) {  // nothing beyond the drafter's probabilities: p itself, whose sums nobody has
+      for (int k = wv; k < segs; k += 4) {
+        const double s = segment(k);
+        if (lane == 0) sh.sum[k] = s;
       }
     } else {
-    // kB tiles at a time: their loads are issued together, then their sums
-    constexpr int kB = 4;
-    for (int k0 = 0; k0 < tiles; k0 += kB) {
-      f4 l[kB], qv[kB];
-      double s[kB];
-#pragma unroll
-      for (int k = 0; k < kB; ++k) {
-        const int at = (k0 + k) * kVerTile + 4 * t;
-        l[k] = load_l(at);
-        qv[k] = load_q(at);
+      // sums of the rows' kernel are in units of the largest weight and hold the rejected draft of a lookup
+      const double unit = !p.truncate && !stop.q ? stop.unit : 1.0;
+      const int own = !p.truncate && stop.draft >= 0 && stop.draft < p.V ? stop.draft / kSeg : -1;
+      const double* src = p.sums + stop.id * segs;
+      for (int k = t; k < segs; k += kDrawThreads)
+        if (k != own) sh.sum[k] = src[k] * unit;
+      if (own >= 0 && wv == 0) {
+        const double s = segment(own);
+        if (lane == 0) sh.sum[own] = s;
       }
-#pragma unroll
-      for (int k = 0; k < kB; ++k) {
-        double w[4];
-        weights(l[k], qv[k], (k0 + k) * kVerTile + 4 * t, w);
-        s[k] = (w[0] + w[1]) + (w[2] + w[3]);
-      }
-#pragma unroll
-      for (int k = 0; k < kB; ++k) s[k] = wave_add(s[k]);
-#pragma unroll
-      for (int k = 0; k < kB; ++k)
-        if (lane == 0 && k0 + k < tiles) sh.sum[(k0 + k) * kVerWaves + wv] = s[k];
-    }
     }
     if (t == 0) {
-      sh.first = n_sum;
+      sh.first = segs;
       sh.last = -1;
     }
     __syncthreads();
     double s = 0.0;
-    for (int k = t * per; k < min((t + 1) * per, n_sum); ++k) s += sh.sum[k];
+    for (int k = k0; k < k1; ++k) s += sh.sum[k];
     const double incl = wave_scan(s, lane);
     if (lane == 63) sh.red[wv] = incl;
     __syncthreads();
-    const double of_wave = sh.red[lane & 15];
-    total = row_add(of_wave);
-    lane_total = row_add((lane & 15) < wv ? of_wave : 0.0) + incl - s;
-    if (total > 0.0 || !beyond) break;
-    beyond = false;
+    const double r0 = sh.red[0], r1 = sh.red[1], r2 = sh.red[2], r3 = sh.red[3];
+    total = (r0 + r1) + (r2 + r3);
+    run0 = (wv == 0 ? 0.0 : wv == 1 ? r0 : wv == 2 ? r0 + r1 : r0 + r1 + r2) + incl - s;
+    if (total > 0.0 || !stop.beyond) break;
+    stop.beyond = false;
     __syncthreads();
   }
-  const double target = (double)p.u[(int64_t)b * T + p.K] * total;
-  double run = lane_total;
-  int first = n_sum, last = -1;
-  for (int k = t * per; k < min((t + 1) * per, n_sum); ++k) {
-    const double s = sh.sum[k];
-    if (s > 0.0) {
-      last = k;
-      if (run + s > target && first == n_sum) first = k;
+  const double target = u * total;
+  {
+    double run = run0;
+    int first = segs, last = -1;
+    for (int k = k0; k < k1; ++k) {
+      const double s = sh.sum[k];
+      if (s > 0.0) {
+        last = k;
+        if (run + s > target && first == segs) first = k;
+      }
+      run += s;
     }
-    run += s;
+    if (first < segs) atomicMin(&sh.first, first);
+    if (last >= 0) atomicMax(&sh.last, last);
   }
-  if (first < n_sum) atomicMin(&sh.first, first);
-  if (last >= 0) atomicMax(&sh.last, last);
   __syncthreads();
-  for (int k = t; k < T; k += kVerThreads)
-    if (k != j) out[k] = k < j ? p.drafts[(int64_t)b * p.K + k] : -1;
-  if (t == 0) p.accepted[b] = j;
-  // the 256 entries that hold the target (rounding short of the end: the last with weight), by one wave
-  const int seg = sh.first < n_sum ? sh.first : sh.last;
+  // the segment that holds the target (rounding short of the end: the last with weight), by one wave
+  const int seg = sh.first < segs ? sh.first : sh.last;
   if (wv != 0) return;
   if (seg < 0) {
     if (lane == 0) out[j] = -1;
     return;
   }
+  const int at = seg * kSeg + 4 * lane;
+  const f4 l = stop.load_l(at), qv = stop.load_q(at);
   double before = 0.0;
   for (int k = lane; k < seg; k += 64) before += sh.sum[k];
   before = wave_add(before);
-  const int at = (seg / kVerWaves) * kVerTile + (seg % kVerWaves) * 256 + 4 * lane;
   double w[4];
-  weights(load_l(at), load_q(at), at, w);
+  stop.weights(l, qv, at, w);
   const double mine = (w[0] + w[1]) + (w[2] + w[3]);
-  run = before + wave_scan(mine, lane) - mine;
+  double run = before + wave_scan(mine, lane) - mine;
   int pick = -1, end = -1;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -784,7 +869,10 @@ void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
   if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall>), grid, block, 0, s, a);
   else if (tiles <= kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0>), grid, block, 0, s, a);
-  hipLaunchKernelGGL(verify_draw_kernel<kHalf>, dim3(B), block, 0, s, a);
+  if (a.truncate || a.q)
+    hipLaunchKernelGGL(verify_parts_kernel<kHalf>, dim3(B * ((a.segs + 4 * kPartSegs - 1) / (4 * kPartSegs))), dim3(256), 0,
+                       s, a);
+  hipLaunchKernelGGL(verify_draw_kernel<kHalf>, dim3(B), dim3(kDrawThreads), 0, s, a);
 }
 
 }  // namespace
@@ -794,8 +882,8 @@ using namespace vk;
 
 extern "C" int64_t vkwr_sampling_verify_workspace_bytes(int B, int K, int V) {
   if (B <= 0 || K < 0 || V <= 0) return 0;
-  const int64_t rows = (int64_t)B * ((int64_t)K + 1), tiles = (V + kVerTile - 1) / kVerTile;
-  return rows * ((int64_t)sizeof(RowStat) + tiles * kVerWaves * (int64_t)sizeof(double));
+  const int64_t rows = (int64_t)B * ((int64_t)K + 1);
+  return rows * ((int64_t)sizeof(RowStat) + (V + kSeg - 1) / kSeg * (int64_t)sizeof(double));
 }
 
 extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logits, int logits_f16,
@@ -810,7 +898,7 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
              "%s: vocabulary size must be a multiple of 4 and at most 1048576, got %d", fn, V);
   VK_REQUIRE(temperature >= 0.001 && temperature <= 1000, "%s: temperature %g outside [0.001, 1000]", fn,
              temperature);
-  VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= 0x7fffffff, "%s: B*(K+1) too large", fn);
+  VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= 0x7fffffff && B <= (1 << 24), "%s: B or B*(K+1) too large", fn);
   if (B == 0) return VKWR_OK;
   VK_REQUIRE(logits && uniforms && tokens && accepted && (K == 0 || drafts), "%s: null pointer", fn);
   VK_REQUIRE((uintptr_t)logits % (logits_f16 ? 8 : 16) == 0 && (uintptr_t)draft_probs % 16 == 0,
@@ -835,6 +923,7 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.tokens = tokens;
   a.accepted = accepted;
   a.stat = reinterpret_cast<RowStat*>(workspace);
+  a.segs = (V + kSeg - 1) / kSeg;
   a.sums = reinterpret_cast<double*>(a.stat + (int64_t)B * ((int64_t)K + 1));
   a.scale = 1.4426950408889634 / temperature;
   a.d_min = -1023.0 / a.scale;
