@@ -19,10 +19,14 @@
 // the draw's prefix sums in fp64.  A token differs from that of exact arithmetic only where a
 // uniform lies within ~1e-11 of a border.
 //
-// Launches: one workgroup per row finds max, tau, comp and Z and tests the row's draft; the row that a
-// sequence stops at is added up in segments of 256 entries, by several workgroups (without a filter and
-// without a drafter's distribution the rows' workgroups have done that already: no launch); one
-// workgroup per sequence finds the segment and the entry that the uniform falls on.
+// Launches:
+//   sums   every row in groups of 2048 entries, a wave each: the group's largest logit, its mass relative
+//          to that (without a filter also that of its 8 segments of 256), and a value that the top_k
+//          largest of the row cannot all lie below
+//   rows   (with a filter) one workgroup per row: tau, comp, Z and the test of the row's draft
+//   parts  (with a filter or a drafter's distribution) the segments' sums of w for the row that each
+//          sequence stops at, by several workgroups
+//   draw   one workgroup per sequence: the segment that the uniform falls on, and the entry
 
 #include <cfloat>
 
@@ -36,10 +40,13 @@ constexpr int kVerThreads = 1024;
 constexpr int kVerWaves = kVerThreads / 64;
 constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
 constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
+constexpr int kVerList = kVerThreads;  // entries above the floor that are taken one per lane
 constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a workgroup reads at once
 constexpr int kVerMaxV = 1 << 20;
 constexpr int kSeg = 256;        // consecutive entries whose weights are added up for the draw (one wave's 64 x 4)
 constexpr int kMaxSegs = kVerMaxV / kSeg;
+constexpr int kGroupSegs = 8;    // segments per wave of the sums' kernel
+constexpr int kMaxRank = 32;     // floors: at most this many lane maxima are taken out of a group
 constexpr double kMassUnit = 1.0 / 8796093022208.0;  // 2^-43
 
 struct RowStat {
@@ -47,15 +54,14 @@ struct RowStat {
   float max, tau;
   int ok, mode;
 };
+static_assert(sizeof(RowStat) == 32, "row stat size");
 // How a row's logits are read so that only finite values and -inf (weight 0) remain:
 enum {
-  kPlain = 0,   // as they are: no NaN and no +inf
-  kNanZero = 1, // NaN -> 0
-  kInfOnly = 2, // +inf present (it stands for the largest float, beside which every finite value
+  kNanZero = 0, // NaN -> 0
+  kInfOnly = 1, // +inf present (it stands for the largest float, beside which every finite value
                 // weighs nothing): +inf -> 0, anything else -> -inf
-  kAllLow = 3   // -inf everywhere: all entries tied
+  kAllLow = 2   // -inf everywhere: all entries tied
 };
-static_assert(sizeof(RowStat) == 32, "row stat size");
 
 struct VerifyArgs {
   int K, V;
@@ -63,9 +69,12 @@ struct VerifyArgs {
   const int32_t *drafts, *n_draft;
   const float *q, *u;
   int32_t *tokens, *accepted;
-  RowStat* stat;   // [B, K+1]
-  double* sums;    // [B, K+1, segments] what the segments of a row hold
-  int segs;
+  RowStat* stat;       // [B, K+1] (with a filter)
+  double* seg_sum;     // [B, K+1, segs] (without one)
+  double* group_sum;   // [B, K+1, groups]
+  float *group_max, *group_floor;
+  double* part_sum;    // [B, segs]
+  int segs, groups, rank;  // rank: lane maxima per group that make a floor (0: none)
   double scale, d_min;  // log2(e) / temperature; -1023 / scale (weight 0)
   float bin_scale;
   int top_k;
@@ -166,7 +175,10 @@ __device__ __forceinline__ X wave_scan(X x, int lane) {
 }
 
 struct StatShared {
-  uint64_t mass[kVerBins];
+  union {
+    uint64_t mass[kVerBins];
+    float list[kVerList];  // before the histogram
+  };
   uint32_t cnt[kVerBins];
   uint64_t redm[2][kVerWaves];
   double redd[2][kVerWaves];
@@ -270,14 +282,6 @@ struct Raw<false> {
   typedef f4 type;
 };
 template <bool kHalf>
-struct Elem {
-  typedef _Float16 type;
-};
-template <>
-struct Elem<false> {
-  typedef float type;
-};
-template <bool kHalf>
 __device__ __forceinline__ typename Raw<kHalf>::type load_raw(const void* row, int i) {
   typedef typename Raw<kHalf>::type R;
   return *reinterpret_cast<const R*>(reinterpret_cast<const char*>(row) + (size_t)i * (kHalf ? 2 : 4));
@@ -297,8 +301,108 @@ __device__ __forceinline__ double kept_of(const VerifyArgs& p, const RowStat& st
   return l > st.tau ? x : l == st.tau ? x * st.comp : 0.0;
 }
 
-// kTiles > 0: the row (V <= kTiles * kVerTile) stays in LDS as stored; 0: it is re-read from memory in
-// every pass.
+// One wave per group of kGroupSegs segments, four groups per workgroup.
+template <bool kHalf>
+__global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
+  const int T = p.K + 1, wgs = (p.groups + 3) / 4;
+  const int64_t id = blockIdx.x / wgs;
+  const int b = (int)(id / T), i = (int)(id - (int64_t)b * T);
+  const int n = p.n_draft ? p.n_draft[b] : p.K;
+  if (n < 0 || n > p.K || i > n) return;
+  const int lane = threadIdx.x & 63, group = (int)(blockIdx.x - id * wgs) * 4 + (threadIdx.x >> 6);
+  if (group >= p.groups) return;
+  const void* row = row_at<kHalf>(p, id);
+  const int at0 = group * (kGroupSegs * kSeg) + 4 * lane;
+  typename Raw<kHalf>::type raw[kGroupSegs];
+#pragma unroll
+  for (int k = 0; k < kGroupSegs; ++k) raw[k] = load_raw<kHalf>(row, min(at0 + k * kSeg, p.V - 4));
+  f4 l[kGroupSegs];
+  float lane_max = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kGroupSegs; ++k) {
+    l[k] = to_f4(raw[k]);
+    const bool in = at0 + k * kSeg < p.V;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      l[k][e] = !in ? -INFINITY : __builtin_isnan(l[k][e]) ? 0.0f : l[k][e];
+      lane_max = fmaxf(lane_max, l[k][e]);
+    }
+  }
+  const float mx = wave_fmax(lane_max);
+  if (p.rank > 0) {
+    // the rank-th largest lane maximum: as many entries of the group lie at or above it
+    float lm = lane_max, at = -INFINITY;
+    for (int k = 0; k < p.rank; ++k) {
+      at = wave_fmax(lm);
+      const uint64_t hit = __ballot(lm == at);
+      if (lane == (int)__builtin_ctzll(hit)) lm = -INFINITY;
+    }
+    if (lane == 0) p.group_floor[id * p.groups + group] = at;
+  }
+  if (lane == 0) p.group_max[id * p.groups + group] = mx;
+  if (p.truncate && !p.use_mass) return;
+  double total = 0.0;
+  if (mx > -INFINITY) {
+    const bool inf = mx == INFINITY;
+    const double mxd = inf ? 0.0 : (double)mx;
+#pragma unroll
+    for (int k0 = 0; k0 < kGroupSegs; k0 += 4) {
+      double s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        double w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = exp2_neg((double)(inf ? read_as(l[k0 + u][e], kInfOnly) : l[k0 + u][e]) - mxd, p.scale, p.d_min);
+        s[u] = (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      total += (s[0] + s[1]) + (s[2] + s[3]);
+      if (!p.truncate) {
+        const double w = wave_add4(s, lane);
+        const int seg = group * kGroupSegs + k0 + lane;
+        if (lane < 4 && seg < p.segs) p.seg_sum[id * p.segs + seg] = w;
+      }
+    }
+    total = wave_add(total);
+  }
+  if (lane == 0) p.group_sum[id * p.groups + group] = total;
+}
+
+// What a group's sums, relative to its own largest logit, are in units of the row's largest weight.
+__device__ __forceinline__ double group_factor(const VerifyArgs& p, float group_max, float mx) {
+  return group_max == mx ? 1.0 : exp2_neg((double)group_max - (double)mx, p.scale, p.d_min);
+}
+
+// Largest logit, how to read the row, its mass and its floor, from the groups': one wave.
+struct RowSummary {
+  float max;  // as read
+  int mode;
+  double mass;
+  float floor;
+};
+__device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id, int lane) {
+  RowSummary r;
+  float mx = -INFINITY, below = -INFINITY;
+  for (int g = lane; g < p.groups; g += 64) {
+    mx = fmaxf(mx, p.group_max[id * p.groups + g]);
+    if (p.rank > 0) below = fmaxf(below, -p.group_floor[id * p.groups + g]);
+  }
+  mx = wave_fmax(mx);
+  r.floor = p.rank > 0 ? -wave_fmax(below) : -INFINITY;
+  double m = 0.0;
+  if (!p.truncate || p.use_mass) {
+    for (int g = lane; g < p.groups; g += 64)
+      m += p.group_sum[id * p.groups + g] * group_factor(p, p.group_max[id * p.groups + g], mx);
+    m = wave_add(m);
+  }
+  r.mode = mx == INFINITY ? kInfOnly : mx == -INFINITY ? kAllLow : kNanZero;
+  r.mass = r.mode == kAllLow ? (double)p.V : m;
+  r.max = r.mode == kNanZero ? mx : 0.0f;
+  if (r.mode != kNanZero) r.floor = r.floor == INFINITY || r.mode == kAllLow ? 0.0f : -INFINITY;
+  return r;
+}
+
+// kTiles > 0: a row (V <= kTiles * kVerTile) that is searched as a whole stays in LDS; 0: it is re-read.
 template <bool kHalf, int kTiles>
 __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) {
   typedef typename Raw<kHalf>::type R;
@@ -309,66 +413,95 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   const int n = p.n_draft ? p.n_draft[b] : p.K;
   if (n < 0 || n > p.K || i > n) return;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = p.V;
-  const void* row = row_at<kHalf>(p, (int64_t)b * T + i);
+  const int64_t id = (int64_t)b * T + i;
+  const void* row = row_at<kHalf>(p, id);
   const int tiles = (V + kVerTile - 1) / kVerTile;
-  int par = 0, mode = kPlain;
-  typedef typename Elem<kHalf>::type E;
-  const E kLow = (E)(-INFINITY);
-  const R kPad = R{kLow, kLow, kLow, kLow};
-
-  // Largest value, and whether any is NaN or infinite (x * 0 is NaN exactly then); from the first tile
-  // the smallest that is not a mask's, a guess at the histogram's range.  Every lane reads back only
-  // what it stored.
-  float mx = -INFINITY, mn = INFINITY;
-  bool odd = false;
-  {
-    R big = kPad, acc = R{};
-    constexpr int kB = 8;  // tiles whose loads are in flight together
-    for (int j0 = 0; j0 < tiles; j0 += kB) {
-      R x[kB];
-#pragma unroll
-      for (int u = 0; u < kB; ++u) x[u] = load_raw<kHalf>(row, min((j0 + u) * kVerTile + 4 * t, V - 4));
-#pragma unroll
-      for (int u = 0; u < kB; ++u) {
-        if (j0 + u >= tiles) break;
-        acc = __builtin_elementwise_fma(x[u], R{}, acc);  // past the end: the row's last entries again
-        if ((j0 + u + 1) * kVerTile > V) x[u] = (j0 + u) * kVerTile + 4 * t < V ? x[u] : kPad;
-        big = __builtin_elementwise_max(big, x[u]);
-        if (j0 + u == 0)
-          for (int e = 0; e < 4; ++e) mn = fminf(mn, (float)x[0][e] > -30000.0f ? (float)x[0][e] : INFINITY);
-        if constexpr (kTiles > 0) lrow[(j0 + u) * kVerThreads + t] = x[u];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mx = fmaxf(mx, (float)big[e]);
-      odd = odd || __builtin_isnan((float)acc[e]);
+  int par = 0;
+  // what the draft's test needs, requested early
+  int draft = -1;
+  float draft_l = -INFINITY, draft_q = 1.0f, draft_u = 0.0f;
+  if (t == 0 && i < n) {
+    draft = p.drafts[(int64_t)b * p.K + i];
+    draft_u = p.u[id];
+    if (draft >= 0 && draft < V) {
+      draft_l = kHalf ? (float)reinterpret_cast<const _Float16*>(row)[draft] : reinterpret_cast<const float*>(row)[draft];
+      if (p.q) draft_q = p.q[((int64_t)b * p.K + i) * V + draft];
     }
   }
-  auto raw_of = [&](int j) __attribute__((always_inline)) -> R {
-    if constexpr (kTiles > 0) return lrow[j * kVerThreads + t];
-    else return load_raw<kHalf>(row, min(j * kVerTile + 4 * t, V - 4));
+  const RowSummary sum = summarize(p, id, lane);
+  const float mx = sum.max;
+  const int mode = sum.mode;
+  const double mxd = (double)mx, all = sum.mass;
+  auto weight = [&](float l) __attribute__((always_inline)) { return exp2_neg((double)l - mxd, p.scale, p.d_min); };
+  const double goal = p.top_p * all;  // in units of the largest weight
+  auto enough = [&](uint32_t c, uint64_t m) {
+    return c >= (uint32_t)p.top_k || (p.use_mass && (double)m * kMassUnit >= goal);
   };
+  const bool by_count = p.top_k < V;
+  // floor: a value that tau cannot lie below; entries under it are left out of the search.  By count: the
+  // smallest of the groups' floors has top_k entries at or above it.  By mass: the entries lighter than
+  // (1 - top_p) all / V together hold less than 1 - top_p of it, so the others hold top_p (with room for
+  // the roundings of the logarithm and of the sum).  Masked entries have no weight.
+  float floor = sum.floor;
+  if (p.use_mass) {
+    const float least = (float)((1.0 - p.top_p) * all / (double)V);
+    if (least > 1.0e-30f) floor = fmaxf(floor, (float)(mxd + ((double)__log2f(least) - 0.01) / p.scale));
+  }
+  floor = fmaxf(floor, -FLT_MAX);
+
   auto entries = [&](int j, R x) __attribute__((always_inline)) -> f4 {
     f4 l = to_f4(x);
-    if constexpr (kTiles == 0) {
-      if (mode != kPlain)
-        for (int e = 0; e < 4; ++e) l[e] = read_as(l[e], mode);
-      if ((j + 1) * kVerTile > V && j * kVerTile + 4 * t >= V) l = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l[e] = __builtin_isnan(l[e]) ? 0.0f : l[e];
+    if (mode != kNanZero)
+      for (int e = 0; e < 4; ++e) l[e] = read_as(l[e], mode);
+    if ((j + 1) * kVerTile > V && j * kVerTile + 4 * t >= V) l = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     return l;
   };
-  // f(four entries) over this lane's entries, four tiles' loads at a time; entries of the padding are -inf
-  auto each4 = [&](auto&& f) __attribute__((always_inline)) {
-    int j = 0;
-    for (; j + 4 <= tiles; j += 4) {
-      const R x0 = raw_of(j), x1 = raw_of(j + 1), x2 = raw_of(j + 2), x3 = raw_of(j + 3);
-      f(entries(j, x0));
-      f(entries(j + 1, x1));
-      f(entries(j + 2, x2));
-      f(entries(j + 3, x3));
+  // f(four entries) over this lane's part of the row, four tiles' loads at a time; padding is -inf.
+  // first: from memory, into LDS if the row fits there; then from where it is.
+  auto each_row = [&](bool first, auto&& f) __attribute__((always_inline)) {
+    for (int j = 0; j < tiles; j += 4) {
+      R x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (kTiles == 0 || first) x[u] = load_raw<kHalf>(row, min((j + u) * kVerTile + 4 * t, V - 4));
+        else x[u] = lrow[min(j + u, tiles - 1) * kVerThreads + t];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (j + u >= tiles) break;
+        if (kTiles > 0 && first) lrow[(j + u) * kVerThreads + t] = x[u];
+        f(entries(j + u, x[u]));
+      }
     }
-    for (; j < tiles; ++j) f(entries(j, raw_of(j)));
+  };
+
+  // With a floor by count the entries from it up are few: one per lane from here on.
+  bool listed = false, loaded = false;
+  float mine = -INFINITY;
+  if (p.rank > 0) {
+    if (t == 0) sh.n_cand = 0;
+    __syncthreads();
+    each_row(true, [&](f4 x) __attribute__((always_inline)) {
+      if (__ballot(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor) == 0) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (x[e] >= floor) {
+          const int at = atomicAdd(&sh.n_cand, 1);  // any order: only sums and a maximum follow
+          if (at < kVerList) sh.list[at] = x[e];
+        }
+      }
+    });
+    __syncthreads();
+    listed = sh.n_cand <= kVerList;
+    loaded = true;
+    if (listed && t < sh.n_cand) mine = sh.list[t];
+    __syncthreads();
+  }
+  auto each4 = [&](auto&& f) __attribute__((always_inline)) {
+    if (listed) f(f4{mine, -INFINITY, -INFINITY, -INFINITY});
+    else each_row(!loaded, f);
   };
   auto each = [&](auto&& f) __attribute__((always_inline)) {
     each4([&](f4 x) __attribute__((always_inline)) {
@@ -376,85 +509,16 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
       for (int e = 0; e < 4; ++e) f(x[e]);
     });
   };
-  float lane_max = mx, oddf = odd ? 1.0f : 0.0f;
-  block_max2(sh, par, mx, oddf);
-  if (oddf > 0.0f) {
-    // NaN or an infinity somewhere (masked entries, often): read the row another way
-    bool nan = false;
-    each([&](float l) { nan = nan || __builtin_isnan(l); });
-    nan = block_max(sh, par, nan ? 1.0f : 0.0f) > 0.0f;
-    mode = mx == INFINITY ? kInfOnly : nan ? kNanZero : mx == -INFINITY ? kAllLow : kPlain;
-    if (mode != kPlain) {
-      if constexpr (kTiles > 0) {
-        for (int j = 0; j < tiles; ++j) {
-          const int at = j * kVerTile + 4 * t;
-          if (at >= V) continue;
-          R x = lrow[j * kVerThreads + t];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (E)read_as((float)x[e], mode);
-          lrow[j * kVerThreads + t] = x;
-        }
-      }
-      mx = -INFINITY;
-      each([&](float l) { mx = fmaxf(mx, l); });
-      lane_max = mx;
-      mx = block_max(sh, par, mx);
-      mn = fminf(mn, 0.0f);
-    }
-  }
-  const double mxd = (double)mx;
-  auto weight = [&](float l) __attribute__((always_inline)) { return exp2_neg((double)l - mxd, p.scale, p.d_min); };
 
   RowStat st;
   st.max = mx;
-  st.tau = -INFINITY;
-  st.comp = 1.0;
-  st.ok = 0;
   st.mode = mode;
+  st.ok = 0;
   uint32_t none = 0, none2 = 0;
-  if (!p.truncate) {
-    // the sums of the segments are kept for the draw
-    double m = 0.0;
-    double* const sums = p.sums + ((int64_t)b * T + i) * p.segs + wv;
-    for (int j = 0; j < tiles; j += 4) {
-      double s[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        s[u] = 0.0;
-        if (j + u < tiles) {
-          const f4 x = entries(j + u, raw_of(j + u));
-          s[u] = (weight(x[0]) + weight(x[1])) + (weight(x[2]) + weight(x[3]));
-        }
-      }
-      m += (s[0] + s[1]) + (s[2] + s[3]);
-      const double w = wave_add4(s, lane);
-      const int seg = (j + lane) * kVerWaves;
-      if (lane < 4 && seg + wv < p.segs) sums[seg] = w;
-    }
-    st.z = block_sum(sh, par, m);
-  } else {
-    // floor: a value that tau cannot lie below; entries under it are left out of the search.  In each
-    // wave the q-th largest of its lanes' maxima, q = ceil(top_k / 16), is at or below q of its
-    // entries, so the smallest of the 16 waves' has top_k entries at or above it.
-    float floor = -INFINITY;
-    if (p.top_k <= kVerThreads) {
-      const int q = (p.top_k + kVerWaves - 1) / kVerWaves;
-      float lm = lane_max, at = -INFINITY;
-      for (int k = 0; k < q; ++k) {
-        at = wave_fmax(lm);
-        const uint64_t hit = __ballot(lm == at);
-        if (lane == (int)__builtin_ctzll(hit)) lm = -INFINITY;
-      }
-      floor = -at;
-    }
-    mn = -mn;
-    block_max2(sh, par, floor, mn);
-    floor = p.top_k <= kVerThreads ? -floor : -INFINITY;
-    mn = -mn;
+  {
     // Histogram of (mx - l) in kVerBins equal steps: 32 per octave of the weight, or finer where the
-    // entries from floor up span less.  Larger l never falls in a later bin.  The same pass adds up
-    // the mass of the whole row, top_p's measure.
-    const float far = mx - fmaxf(mn, floor);
+    // entries from floor up span less.  Larger l never falls in a later bin.
+    const float far = mx - floor;
     const float s = far > 0.0f ? fminf(fmaxf(p.bin_scale, (float)(kVerBins - 1) / far), FLT_MAX) : p.bin_scale;
     auto bin_at = [&](float l) __attribute__((always_inline)) { return fminf((mx - l) * s, (float)(kVerBins - 1)); };
     for (int k = t; k < kVerBins; k += kVerThreads) {
@@ -466,31 +530,24 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
       sh.bin = kVerBins;
     }
     __syncthreads();
-    const bool by_count = p.top_k < V;
-    double all = 0.0;
-    floor = fmaxf(floor, -FLT_MAX);  // masked entries have no weight
     each4([&](f4 x) __attribute__((always_inline)) {
-      double w[4];
+      if (__ballot(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor) == 0) return;
+      uint64_t m[4];
       if (p.use_mass) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = weight(x[e]);
-        all += (w[0] + w[1]) + (w[2] + w[3]);
+        for (int e = 0; e < 4; ++e) m[e] = mass_of(weight(x[e]));
       }
-      if (__ballot(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor) == 0) return;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (x[e] >= floor) {
           const int k = (int)bin_at(x[e]);
           if (by_count) atomicAdd(&sh.cnt[k], 1u);
-          if (p.use_mass) atomicAdd((unsigned long long*)&sh.mass[k], (unsigned long long)mass_of(w[e]));
+          if (p.use_mass) atomicAdd((unsigned long long*)&sh.mass[k], (unsigned long long)m[e]);
         }
       }
     });
-    all = block_sum(sh, par, all);  // its barrier also ends the histogram
-    const double goal = p.top_p * all;  // in units of the largest weight
-    auto enough = [&](uint32_t c, uint64_t m) {
-      return c >= (uint32_t)p.top_k || (p.use_mass && (double)m * kMassUnit >= goal);
-    };
+    loaded = true;
+    __syncthreads();
     // inclusive prefix over the bins (two per lane) and the first bin that reaches the budget
     const uint32_t c0 = sh.cnt[2 * t], c1 = sh.cnt[2 * t + 1];
     const uint64_t m0 = sh.mass[2 * t], m1 = sh.mass[2 * t + 1];
@@ -633,43 +690,58 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
     st.z = (double)mgt * kMassUnit + st.comp * x * (double)neq;
   }
   if (t == 0) {
-    if (i < n) {
-      const int d = p.drafts[(int64_t)b * p.K + i];
-      const bool in = d >= 0 && d < V;
-      const float l = in ? read_as(kHalf ? (float)reinterpret_cast<const _Float16*>(row)[d]
-                                         : reinterpret_cast<const float*>(row)[d], mode) : 0.0f;
-      const double pd = in ? kept_of(p, st, l) / st.z : 0.0;
-      const double qd = p.q ? (in ? (double)p.q[((int64_t)b * p.K + i) * V + d] : 0.0) : 1.0;
-      st.ok = (double)p.u[(int64_t)b * T + i] * qd < pd ? 1 : 0;
-    }
-    p.stat[(int64_t)b * T + i] = st;
+    if (draft >= 0 && draft < V)
+      st.ok = (double)draft_u * (double)draft_q < kept_of(p, st, read_as(draft_l, mode)) / st.z ? 1 : 0;
+    p.stat[id] = st;
   }
 }
 
-// What the two kernels behind the rows' share: the row a sequence stops at and the weights it draws from.
+// What the last two kernels share: the row a sequence stops at and the weights it draws from.  Four
+// waves; without a filter they make the rows' statistics from the groups' sums, a row each at a time.
+struct StopShared {
+  RowStat stat[64];
+};
 template <bool kHalf>
 struct Stop {
   const VerifyArgs& p;
   int64_t id;      // row b (K + 1) + j
-  int j, n, draft;
+  int j, draft;
   const float* q;  // the drafter's row, where j is a rejected draft's and there is one
   bool beyond;     // draw from what p has beyond q
   RowStat st;
   double unit, unit_tau;  // of a weight above tau, and at it
   const void* row;
 
-  __device__ __forceinline__ Stop(const VerifyArgs& a, int b, int n_, int lane) : p(a), n(n_) {
+  __device__ __forceinline__ Stop(const VerifyArgs& a, StopShared& sh, int b, int n, int lane, int wv) : p(a) {
     const int T = p.K + 1;
-    j = n;
-    for (int k0 = 0; k0 < n; k0 += 64) {
-      const uint64_t hit = __ballot(k0 + lane < n && !p.stat[(int64_t)b * T + k0 + lane].ok);
-      if (hit) {
-        j = k0 + __builtin_ctzll(hit);
-        break;
+    j = -1;
+    for (int k0 = 0; j < 0; k0 += 64) {  // 64 rows at a time; row n ends the search
+      bool last = k0 + lane >= n;
+      if (p.truncate) {
+        last = last || !p.stat[(int64_t)b * T + k0 + lane].ok;
+      } else {
+        if (k0 > 0) __syncthreads();
+        for (int k = wv; k < 64 && k0 + k <= n; k += 4) {
+          const int64_t r = (int64_t)b * T + k0 + k;
+          const int d = k0 + k < n ? p.drafts[(int64_t)b * p.K + k0 + k] : -1;
+          const bool in = d >= 0 && d < p.V;
+          const float l = !in ? 0.0f : kHalf ? (float)reinterpret_cast<const _Float16*>(row_at<kHalf>(p, r))[d]
+                                             : reinterpret_cast<const float*>(row_at<kHalf>(p, r))[d];
+          const double qd = in && p.q ? (double)p.q[((int64_t)b * p.K + k0 + k) * p.V + d] : 1.0;
+          const double u = (double)p.u[r];
+          const RowSummary sum = summarize(p, r, lane);
+          RowStat s{sum.mass, 1.0, sum.max, -INFINITY, 0, sum.mode};
+          s.ok = in && u * qd < kept_of(p, s, read_as(l, sum.mode)) / s.z ? 1 : 0;
+          if (lane == 0) sh.stat[k] = s;
+        }
+        __syncthreads();
+        last = last || !sh.stat[lane].ok;
       }
+      const uint64_t hit = __ballot(last);
+      if (hit) j = k0 + __builtin_ctzll(hit);
     }
     id = (int64_t)b * T + j;
-    st = p.stat[id];
+    st = p.truncate ? p.stat[id] : sh.stat[j & 63];
     row = row_at<kHalf>(p, id);
     beyond = j < n;
     q = p.q && beyond ? p.q + ((int64_t)b * p.K + j) * p.V : nullptr;
@@ -681,8 +753,8 @@ struct Stop {
     f4 x = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     if (at < p.V) {
       x = to_f4(load_raw<kHalf>(row, at));
-      if (st.mode != kPlain)
-        for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], st.mode);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = read_as(x[e], st.mode);
     }
     return x;
   }
@@ -705,16 +777,17 @@ struct Stop {
   }
 };
 
-// The segments' sums of the row each sequence stops at (not where the rows' kernel left them: without
-// a filter, all drafts accepted).  A workgroup takes 8 segments for each of its 4 waves.
+// The segments' sums of w for the row each sequence stops at (not where the sums' kernel left them:
+// without a filter, all drafts accepted).  A workgroup takes 8 segments for each of its 4 waves.
 constexpr int kPartSegs = 8;
 template <bool kHalf>
 __global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
+  __shared__ StopShared shared;
   const int parts = (p.segs + 4 * kPartSegs - 1) / (4 * kPartSegs);
   const int b = blockIdx.x / parts, part = blockIdx.x - b * parts, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int n = p.n_draft ? p.n_draft[b] : p.K;
   if (n < 0 || n > p.K) return;
-  const Stop<kHalf> stop(p, b, n, lane);
+  const Stop<kHalf> stop(p, shared, b, n, lane, wv);
   if (!p.truncate && !stop.beyond) return;
   const int seg0 = (part * 4 + wv) * kPartSegs;
   f4 l[kPartSegs], qv[kPartSegs];
@@ -724,7 +797,7 @@ __global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
     l[k] = stop.load_l(at);
     qv[k] = stop.load_q(at);
   }
-  double* const sums = p.sums + stop.id * p.segs + seg0;
+  double* const sums = p.part_sum + (int64_t)b * p.segs + seg0;
 #pragma unroll
   for (int k0 = 0; k0 < kPartSegs; k0 += 4) {
     double s[4];
@@ -741,6 +814,7 @@ __global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
 
 constexpr int kDrawThreads = 256;
 struct DrawShared {
+  StopShared stop;
   double sum[kMaxSegs];
   double red[4];
   int first, last;
@@ -759,7 +833,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
     if (t == 0) p.accepted[b] = -1;
     return;
   }
-  Stop<kHalf> stop(p, b, n, lane);
+  Stop<kHalf> stop(p, sh.stop, b, n, lane, wv);
   const int j = stop.j;
   for (int k = t; k < T; k += kDrawThreads)
     if (k != j) out[k] = k < j ? p.drafts[(int64_t)b * p.K + k] : -1;
@@ -781,12 +855,22 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
         if (lane == 0) sh.sum[k] = s;
       }
     } else {
-      // sums of the rows' kernel are in units of the largest weight and hold the rejected draft of a lookup
-      const double unit = !p.truncate && !stop.q ? stop.unit : 1.0;
-      const int own = !p.truncate && stop.draft >= 0 && stop.draft < p.V ? stop.draft / kSeg : -1;
-      const double* src = p.sums + stop.id * segs;
-      for (int k = t; k < segs; k += kDrawThreads)
-        if (k != own) sh.sum[k] = src[k] * unit;
+      const bool parts = p.truncate || stop.q;
+      // the sums' kernel's are relative to their group's largest weight, and hold a lookup's rejected draft
+      const int own = !parts && stop.draft >= 0 && stop.draft < p.V ? stop.draft / kSeg : -1;
+      const double* src = parts ? p.part_sum + (int64_t)b * segs : p.seg_sum + stop.id * segs;
+      const float top = stop.st.mode == kInfOnly ? INFINITY : stop.st.max;
+      for (int k = t; k < segs; k += kDrawThreads) {
+        if (k == own) continue;
+        double s;
+        if (parts) s = src[k];
+        else if (stop.st.mode == kAllLow) s = (double)(min(p.V, (k + 1) * kSeg) - k * kSeg) * stop.unit;
+        else {
+          const float gm = p.group_max[stop.id * p.groups + k / kGroupSegs];
+          s = gm > -INFINITY ? src[k] * group_factor(p, gm, top) * stop.unit : 0.0;
+        }
+        sh.sum[k] = s;
+      }
       if (own >= 0 && wv == 0) {
         const double s = segment(own);
         if (lane == 0) sh.sum[own] = s;
@@ -858,21 +942,41 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
   }
 }
 
-// Rows of up to 128 KiB stay in LDS (one workgroup per CU then; up to 32 KiB two), longer ones are
-// re-read from memory.
+// Rows of up to 128 KiB stay in LDS while they are searched, longer ones are re-read from memory; so is a
+// row whose top_k gives a floor, which is read once (its list then holds what is searched).
 template <bool kHalf>
 void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
   constexpr int kTileBytes = kVerTile * (kHalf ? 2 : 4);
   constexpr int kSmall = (32 << 10) / kTileBytes, kLarge = (128 << 10) / kTileBytes;
-  const dim3 grid(B * (a.K + 1)), block(kVerThreads);
+  const unsigned rows = (unsigned)B * (a.K + 1);
   const int tiles = (a.V + kVerTile - 1) / kVerTile;
-  if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall>), grid, block, 0, s, a);
-  else if (tiles <= kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0>), grid, block, 0, s, a);
+  hipLaunchKernelGGL(verify_sums_kernel<kHalf>, dim3(rows * ((a.groups + 3) / 4)), dim3(256), 0, s, a);
+  if (a.truncate) {
+    const dim3 grid(rows), block(kVerThreads);
+    if (a.rank > 0 || tiles > kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0>), grid, block, 0, s, a);
+    else if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge>), grid, block, 0, s, a);
+  }
   if (a.truncate || a.q)
     hipLaunchKernelGGL(verify_parts_kernel<kHalf>, dim3(B * ((a.segs + 4 * kPartSegs - 1) / (4 * kPartSegs))), dim3(256), 0,
                        s, a);
   hipLaunchKernelGGL(verify_draw_kernel<kHalf>, dim3(B), dim3(kDrawThreads), 0, s, a);
+}
+
+// Workspace: row statistics, segments', groups' and parts' sums, groups' maxima and floors.
+struct VerifySpace {
+  int64_t seg_sum, group_sum, part_sum, group_max, group_floor, bytes;
+};
+VerifySpace verify_space(int64_t B, int64_t K, int64_t V) {
+  const int64_t rows = B * (K + 1), segs = (V + kSeg - 1) / kSeg, groups = (segs + kGroupSegs - 1) / kGroupSegs;
+  VerifySpace w;
+  w.seg_sum = rows * (int64_t)sizeof(RowStat);
+  w.group_sum = w.seg_sum + rows * segs * 8;
+  w.part_sum = w.group_sum + rows * groups * 8;
+  w.group_max = w.part_sum + B * segs * 8;
+  w.group_floor = w.group_max + rows * groups * 4;
+  w.bytes = w.group_floor + rows * groups * 4;
+  return w;
 }
 
 }  // namespace
@@ -882,8 +986,7 @@ using namespace vk;
 
 extern "C" int64_t vkwr_sampling_verify_workspace_bytes(int B, int K, int V) {
   if (B <= 0 || K < 0 || V <= 0) return 0;
-  const int64_t rows = (int64_t)B * ((int64_t)K + 1);
-  return rows * ((int64_t)sizeof(RowStat) + (V + kSeg - 1) / kSeg * (int64_t)sizeof(double));
+  return verify_space(B, K, V).bytes;
 }
 
 extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logits, int logits_f16,
@@ -898,7 +1001,8 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
              "%s: vocabulary size must be a multiple of 4 and at most 1048576, got %d", fn, V);
   VK_REQUIRE(temperature >= 0.001 && temperature <= 1000, "%s: temperature %g outside [0.001, 1000]", fn,
              temperature);
-  VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= 0x7fffffff && B <= (1 << 24), "%s: B or B*(K+1) too large", fn);
+  // (256 threads per 8192 entries of a row, 1024 per row: fewer than 2^32 in a launch)
+  VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= (1 << 21) / ((V + 131071) / 131072), "%s: B*(K+1) too large", fn);
   if (B == 0) return VKWR_OK;
   VK_REQUIRE(logits && uniforms && tokens && accepted && (K == 0 || drafts), "%s: null pointer", fn);
   VK_REQUIRE((uintptr_t)logits % (logits_f16 ? 8 : 16) == 0 && (uintptr_t)draft_probs % 16 == 0,
@@ -922,9 +1026,16 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.u = uniforms;
   a.tokens = tokens;
   a.accepted = accepted;
-  a.stat = reinterpret_cast<RowStat*>(workspace);
+  char* const ws = reinterpret_cast<char*>(workspace);
+  const VerifySpace w = verify_space(B, K, V);
+  a.stat = reinterpret_cast<RowStat*>(ws);
+  a.seg_sum = reinterpret_cast<double*>(ws + w.seg_sum);
+  a.group_sum = reinterpret_cast<double*>(ws + w.group_sum);
+  a.part_sum = reinterpret_cast<double*>(ws + w.part_sum);
+  a.group_max = reinterpret_cast<float*>(ws + w.group_max);
+  a.group_floor = reinterpret_cast<float*>(ws + w.group_floor);
   a.segs = (V + kSeg - 1) / kSeg;
-  a.sums = reinterpret_cast<double*>(a.stat + (int64_t)B * ((int64_t)K + 1));
+  a.groups = (a.segs + kGroupSegs - 1) / kGroupSegs;
   a.scale = 1.4426950408889634 / temperature;
   a.d_min = -1023.0 / a.scale;
   a.bin_scale = (float)(32.0 * a.scale);
@@ -932,6 +1043,8 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.top_p = top_p;
   a.use_mass = top_p < 1.0;
   a.truncate = top_k < V || a.use_mass;
+  const int rank = (top_k + a.groups - 1) / a.groups;
+  a.rank = a.truncate && rank <= kMaxRank ? rank : 0;
   if (logits_f16) launch_verify<true>(a, B, (hipStream_t)stream);
   else launch_verify<false>(a, B, (hipStream_t)stream);
   return check_launch(fn);
