@@ -93,6 +93,37 @@ def test_masked_and_non_finite_logits(gpu, half, filt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("V,k", [(65536, 40), (65536, 64), (20004, 200), (4096, 64), (2000, 64), (131072, 20), (8192, 300)])
+def test_largest_entries_side_by_side(gpu, V, k, probs):
+    """The top_k entries in one stretch of the vocabulary, in a few stretches, and spread: what a part
+    of the row holds of them is anything from none to all."""
+    d = make(6, 3, V, seed=29 + V, probs=probs)
+    l = d["logits"].float()
+    l[0], l[1] = l[0].sort(dim=-1, descending=True)[0], l[1].sort(dim=-1)[0]
+    l[2, :, 100:100 + 2 * k] += 9.0
+    l[3, :, -k:] += 9.0
+    l[4] = torch.floor(l[4])  # and ties
+    d["logits"] = l.half()
+    d["n_draft"][:] = 3
+    for filt in ({"top_k": k}, {"top_k": k, "top_p": 0.9}, {"top_k": k, "top_p": 0.999, "temperature": 4.0}):
+        check(gpu, d, **filt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("left", [1, 3, 50])
+def test_few_entries_left_by_a_mask(gpu, left):
+    """Fewer entries than top_k (and than a list would hold) are not masked."""
+    d = make(4, 2, 65536, seed=37)
+    keep = torch.randperm(65536, generator=torch.Generator().manual_seed(left))[:left]
+    mask = torch.full((65536,), -float("inf"))
+    mask[keep] = 0.0
+    d["logits"] = (d["logits"].float() + mask).half()
+    for filt in ({}, {"top_k": 40}, {"top_k": 40, "top_p": 0.9}, {"top_p": 0.9}):
+        check(gpu, d, **filt)
+
+
+@pytest.mark.gpu
 def test_uniforms_at_their_ends(gpu):
     for u in (0.0, 1.0 - 2.0 ** -24):
         for probs in (True, False):

@@ -21,14 +21,18 @@
 //
 // Launches:
 //   sums   every row in groups of 2048 entries, a wave each: the group's largest logit, its mass relative
-//          to that (without a filter also that of its 8 segments of 256), and a value that the top_k
-//          largest of the row cannot all lie below
-//   rows   (with a filter) one workgroup per row: tau, comp, Z and the test of the row's draft
-//   parts  (with a filter or a drafter's distribution) the segments' sums of w for the row that each
-//          sequence stops at, by several workgroups
+//          to that (without a filter also that of its 8 segments of 256), and for a small top_k a list of
+//          its largest entries
+//   rows   (with a filter) one workgroup per row: tau, comp, Z and the test of the row's draft; from the
+//          lists, where they reach down to tau, also the token if the sequence stops at this row;
+//          otherwise from the whole row
+//   parts  (with a larger top_k or a drafter's distribution) the segments' sums of w for the row that
+//          each sequence stops at, by several workgroups
 //   draw   one workgroup per sequence: the segment that the uniform falls on, and the entry
 
+#include <algorithm>
 #include <cfloat>
+#include <cmath>
 
 #include "vk_capi.h"
 #include "vk_common.cuh"
@@ -40,21 +44,22 @@ constexpr int kVerThreads = 1024;
 constexpr int kVerWaves = kVerThreads / 64;
 constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
 constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
-constexpr int kVerList = kVerThreads;  // entries above the floor that are taken one per lane
+constexpr int kVerList = kVerThreads;  // listed entries of a row: one per lane
+constexpr int kVerDraw = 256;    // kept entries that the rows' kernel draws from directly
 constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a workgroup reads at once
 constexpr int kVerMaxV = 1 << 20;
 constexpr int kSeg = 256;        // consecutive entries whose weights are added up for the draw (one wave's 64 x 4)
 constexpr int kMaxSegs = kVerMaxV / kSeg;
 constexpr int kGroupSegs = 8;    // segments per wave of the sums' kernel
-constexpr int kMaxRank = 32;     // floors: at most this many lane maxima are taken out of a group
 constexpr double kMassUnit = 1.0 / 8796093022208.0;  // 2^-43
 
 struct RowStat {
   double z, comp;
   float max, tau;
   int ok, mode;
+  int token, pad;  // the new token if the sequence stops here; -1: not known yet
 };
-static_assert(sizeof(RowStat) == 32, "row stat size");
+static_assert(sizeof(RowStat) == 40, "row stat size");
 // How a row's logits are read so that only finite values and -inf (weight 0) remain:
 enum {
   kNanZero = 0, // NaN -> 0
@@ -72,9 +77,12 @@ struct VerifyArgs {
   RowStat* stat;       // [B, K+1] (with a filter)
   double* seg_sum;     // [B, K+1, segs] (without one)
   double* group_sum;   // [B, K+1, groups]
-  float *group_max, *group_floor;
+  float *group_max, *group_floor;  // group_floor: all entries of the group from it up are listed
+  int32_t* group_count;
+  float2* list;        // [B, K+1, groups, cap] logit, index
   double* part_sum;    // [B, segs]
-  int segs, groups, rank;  // rank: lane maxima per group that make a floor (0: none)
+  int segs, groups;
+  int cap, rank;       // entries listed per group (0: no lists); maxima that a row of lanes gives
   double scale, d_min;  // log2(e) / temperature; -1023 / scale (weight 0)
   float bin_scale;
   int top_k;
@@ -177,7 +185,10 @@ __device__ __forceinline__ X wave_scan(X x, int lane) {
 struct StatShared {
   union {
     uint64_t mass[kVerBins];
-    float list[kVerList];  // before the histogram
+    struct {  // behind the histogram
+      double w[kVerDraw], sorted_w[kVerDraw];
+      int at[kVerDraw], sorted_at[kVerDraw];
+    } draw;
   };
   uint32_t cnt[kVerBins];
   uint64_t redm[2][kVerWaves];
@@ -329,15 +340,50 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
     }
   }
   const float mx = wave_fmax(lane_max);
-  if (p.rank > 0) {
-    // the rank-th largest lane maximum: as many entries of the group lie at or above it
-    float lm = lane_max, at = -INFINITY;
-    for (int k = 0; k < p.rank; ++k) {
-      at = wave_fmax(lm);
-      const uint64_t hit = __ballot(lm == at);
-      if (lane == (int)__builtin_ctzll(hit)) lm = -INFINITY;
+  if (p.cap > 0) {
+    // The rank-th largest lane maximum of each row of 16 lanes, the smallest of the four: 4 rank entries
+    // or more lie at or above it.  More than cap: fewer maxima.
+    float at = INFINITY;
+    int count = 0;
+    for (int r = p.rank; r > 0; --r) {
+      float lm = lane_max, a = -INFINITY;
+      for (int k = 0; k < r; ++k) {
+        a = row_fmax(lm);
+        lm = lm == a ? -INFINITY : lm;
+      }
+      a = fminf(fminf(lane_read(a, 0), lane_read(a, 16)), fminf(lane_read(a, 32), lane_read(a, 48)));
+      at = fmaxf(a, -FLT_MAX);
+      count = 0;
+#pragma unroll
+      for (int k = 0; k < kGroupSegs; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) count += __builtin_popcountll(__ballot(l[k][e] >= at));
+      if (count <= p.cap) break;
     }
-    if (lane == 0) p.group_floor[id * p.groups + group] = at;
+    if (count > p.cap) {
+      at = INFINITY;
+      count = 0;
+    }
+    float2* out = p.list + (id * p.groups + group) * p.cap;
+    int base = 0;
+    if (count > 0) {
+#pragma unroll
+      for (int k = 0; k < kGroupSegs; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = l[k][e] >= at;
+          const uint64_t m = __ballot(in);
+          if (m == 0) continue;
+          if (in)
+            out[base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] =
+                make_float2(l[k][e], __builtin_bit_cast(float, at0 + k * kSeg + e));
+          base += __builtin_popcountll(m);
+        }
+    }
+    if (lane == 0) {
+      p.group_floor[id * p.groups + group] = at;
+      p.group_count[id * p.groups + group] = count;
+    }
   }
   if (lane == 0) p.group_max[id * p.groups + group] = mx;
   if (p.truncate && !p.use_mass) return;
@@ -373,22 +419,28 @@ __device__ __forceinline__ double group_factor(const VerifyArgs& p, float group_
   return group_max == mx ? 1.0 : exp2_neg((double)group_max - (double)mx, p.scale, p.d_min);
 }
 
-// Largest logit, how to read the row, its mass and its floor, from the groups': one wave.
+// Largest logit, how to read the row, its mass and its lists' reach, from the groups': one wave.
 struct RowSummary {
   float max;  // as read
   int mode;
   double mass;
-  float floor;
+  float floor;  // top_k entries or more lie at or above it (-inf: not known)
+  float reach;  // all entries from it up are listed
 };
 __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id, int lane) {
   RowSummary r;
-  float mx = -INFINITY, below = -INFINITY;
+  float mx = -INFINITY, below = -INFINITY, reach = -INFINITY;
+  int count = 0;
   for (int g = lane; g < p.groups; g += 64) {
     mx = fmaxf(mx, p.group_max[id * p.groups + g]);
-    if (p.rank > 0) below = fmaxf(below, -p.group_floor[id * p.groups + g]);
+    if (p.cap > 0) {
+      const float f = p.group_floor[id * p.groups + g];
+      below = fmaxf(below, -f);
+      reach = fmaxf(reach, f);
+      count += p.group_count[id * p.groups + g];
+    }
   }
   mx = wave_fmax(mx);
-  r.floor = p.rank > 0 ? -wave_fmax(below) : -INFINITY;
   double m = 0.0;
   if (!p.truncate || p.use_mass) {
     for (int g = lane; g < p.groups; g += 64)
@@ -398,12 +450,18 @@ __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id,
   r.mode = mx == INFINITY ? kInfOnly : mx == -INFINITY ? kAllLow : kNanZero;
   r.mass = r.mode == kAllLow ? (double)p.V : m;
   r.max = r.mode == kNanZero ? mx : 0.0f;
-  if (r.mode != kNanZero) r.floor = r.floor == INFINITY || r.mode == kAllLow ? 0.0f : -INFINITY;
+  r.floor = -INFINITY;
+  r.reach = INFINITY;
+  if (p.cap > 0 && r.mode == kNanZero) {
+    r.floor = wave_add(count) >= p.top_k ? -wave_fmax(below) : -INFINITY;
+    r.reach = wave_fmax(reach);
+  }
   return r;
 }
 
 // kTiles > 0: a row (V <= kTiles * kVerTile) that is searched as a whole stays in LDS; 0: it is re-read.
-template <bool kHalf, int kTiles>
+// kLists: the groups' lists are searched first.
+template <bool kHalf, int kTiles, bool kLists>
 __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) {
   typedef typename Raw<kHalf>::type R;
   __shared__ StatShared sh;
@@ -420,6 +478,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   // what the draft's test needs, requested early
   int draft = -1;
   float draft_l = -INFINITY, draft_q = 1.0f, draft_u = 0.0f;
+  const float last_u = p.u[(int64_t)b * T + p.K];
   if (t == 0 && i < n) {
     draft = p.drafts[(int64_t)b * p.K + i];
     draft_u = p.u[id];
@@ -439,15 +498,15 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   };
   const bool by_count = p.top_k < V;
   // floor: a value that tau cannot lie below; entries under it are left out of the search.  By count: the
-  // smallest of the groups' floors has top_k entries at or above it.  By mass: the entries lighter than
+  // smallest of the groups' floors has top_k entries at or above it, listed.  By mass: the entries lighter than
   // (1 - top_p) all / V together hold less than 1 - top_p of it, so the others hold top_p (with room for
   // the roundings of the logarithm and of the sum).  Masked entries have no weight.
-  float floor = sum.floor;
+  float floor0 = sum.floor;
   if (p.use_mass) {
     const float least = (float)((1.0 - p.top_p) * all / (double)V);
-    if (least > 1.0e-30f) floor = fmaxf(floor, (float)(mxd + ((double)__log2f(least) - 0.01) / p.scale));
+    if (least > 1.0e-30f) floor0 = fmaxf(floor0, (float)(mxd + ((double)__log2f(least) - 0.01) / p.scale));
   }
-  floor = fmaxf(floor, -FLT_MAX);
+  floor0 = fmaxf(floor0, -FLT_MAX);
 
   auto entries = [&](int j, R x) __attribute__((always_inline)) -> f4 {
     f4 l = to_f4(x);
@@ -477,30 +536,20 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
     }
   };
 
-  // With a floor by count the entries from it up are few: one per lane from here on.
-  bool listed = false, loaded = false;
+  // The lists: one entry per lane.
+  bool listed = kLists && sum.reach < INFINITY, loaded = false;
   float mine = -INFINITY;
-  if (p.rank > 0) {
-    if (t == 0) sh.n_cand = 0;
-    __syncthreads();
-    each_row(true, [&](f4 x) __attribute__((always_inline)) {
-      if (__ballot(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor) == 0) return;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (x[e] >= floor) {
-          const int at = atomicAdd(&sh.n_cand, 1);  // any order: only sums and a maximum follow
-          if (at < kVerList) sh.list[at] = x[e];
-        }
-      }
-    });
-    __syncthreads();
-    listed = sh.n_cand <= kVerList;
-    loaded = true;
-    if (listed && t < sh.n_cand) mine = sh.list[t];
-    __syncthreads();
+  int mine_at = -1;
+  if (listed) {
+    const int g = t / p.cap, k = t - g * p.cap;
+    if (g < p.groups && k < p.group_count[id * p.groups + g]) {
+      const float2 e = p.list[(id * p.groups + g) * p.cap + k];
+      mine = e.x;
+      mine_at = __builtin_bit_cast(int, e.y);
+    }
   }
   auto each4 = [&](auto&& f) __attribute__((always_inline)) {
-    if (listed) f(f4{mine, -INFINITY, -INFINITY, -INFINITY});
+    if (kLists && listed) f(f4{mine, -INFINITY, -INFINITY, -INFINITY});
     else each_row(!loaded, f);
   };
   auto each = [&](auto&& f) __attribute__((always_inline)) {
@@ -514,8 +563,11 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   st.max = mx;
   st.mode = mode;
   st.ok = 0;
+  st.token = -1;
+  st.pad = 0;
   uint32_t none = 0, none2 = 0;
-  {
+  for (;;) {
+    const float floor = listed ? fmaxf(floor0, sum.reach) : floor0;
     // Histogram of (mx - l) in kVerBins equal steps: 32 per octave of the weight, or finer where the
     // entries from floor up span less.  Larger l never falls in a later bin.
     const float far = mx - floor;
@@ -546,7 +598,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
         }
       }
     });
-    loaded = true;
+    loaded = loaded || !listed;
     __syncthreads();
     // inclusive prefix over the bins (two per lane) and the first bin that reaches the budget
     const uint32_t c0 = sh.cnt[2 * t], c1 = sh.cnt[2 * t + 1];
@@ -573,8 +625,13 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
       sh.before_m = mi - m1;
     }
     __syncthreads();
-    // None: fewer entries than top_k have a weight at all (the others are masked); all of those are kept.
     const bool found = sh.bin < kVerBins;
+    if (kLists && !found && listed && sum.reach > -FLT_MAX) {  // tau lies below the lists' reach: the whole row
+      __syncthreads();
+      listed = false;
+      continue;
+    }
+    // Not found: fewer entries than top_k have a weight at all (the others are masked); all are kept.
     const int bin = found ? sh.bin : kVerBins - 1;
     const uint32_t before_c = found ? sh.before_c : 0;
     const uint64_t before_m = found ? sh.before_m : 0;
@@ -611,7 +668,6 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
     }
     __syncthreads();
     const int in_bin = found ? sh.n_cand : kVerCand + 1;
-    if (!found) floor = -FLT_MAX;
     uint32_t ngt = 0, neq = 0;
     uint64_t mgt = 0;
     if (in_bin <= kVerCand) {
@@ -644,7 +700,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
     } else {
       // many entries in one bin (ties, or a spread that outliers stretch): bisection over the keys of
       // every entry, at most 32 rounds, for the largest value with enough entries at or above it
-      uint32_t lo = key_of(floor), hi = found ? key_of(mx) : lo;
+      uint32_t lo = key_of(found ? floor : -FLT_MAX), hi = found ? key_of(mx) : lo;
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2u + 1u;
         const float v = of_key(mid);
@@ -688,6 +744,62 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
     // no entry above tau: the kept ones are ties, whose common share does not matter
     st.comp = mgt == 0 ? 1.0 : comp;
     st.z = (double)mgt * kMassUnit + st.comp * x * (double)neq;
+    break;
+  }
+
+  // The token if the sequence stops here: all kept entries are listed.  Sorted by index (places counted,
+  // so that the sums' order does not hang on the order of the atomics), then the prefix sums in one wave.
+  if (kLists && listed) {
+    double w = 0.0;
+    if (mine >= st.tau) {
+      w = kept_of(p, st, mine) / st.z;
+      if (i < n) {
+        if (p.q) w = fmax(w - (double)p.q[((int64_t)b * p.K + i) * V + mine_at], 0.0);
+        else if (mine_at == p.drafts[(int64_t)b * p.K + i]) w = 0.0;
+      }
+    }
+    if (t == 0) sh.n_cand = 0;
+    __syncthreads();
+    if (mine >= st.tau && mine > -INFINITY) {
+      const int at = atomicAdd(&sh.n_cand, 1);
+      if (at < kVerDraw) {
+        sh.draw.w[at] = w;
+        sh.draw.at[at] = mine_at;
+      }
+    }
+    __syncthreads();
+    const int kept = sh.n_cand;
+    if (kept <= kVerDraw) {
+      if (t < kept) {
+        const int my = sh.draw.at[t];
+        int place = 0;
+        for (int k = 0; k < kept; ++k) place += sh.draw.at[k] < my ? 1 : 0;
+        sh.draw.sorted_w[place] = sh.draw.w[t];
+        sh.draw.sorted_at[place] = my;
+      }
+      __syncthreads();
+      if (wv == 0) {
+        double x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = 4 * lane + e < kept ? sh.draw.sorted_w[4 * lane + e] : 0.0;
+        const double s = (x[0] + x[1]) + (x[2] + x[3]);
+        const double incl = wave_scan(s, lane);
+        const double total = lane_read(incl, 63), target = (double)last_u * total;
+        double run = incl - s;
+        int pick = -1, end = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          run += x[e];
+          if (x[e] > 0.0) {
+            end = 4 * lane + e;
+            if (pick < 0 && run > target) pick = 4 * lane + e;
+          }
+        }
+        const uint64_t hit = __ballot(pick >= 0), any = __ballot(end >= 0);
+        if (hit) st.token = sh.draw.sorted_at[__builtin_amdgcn_readlane(pick, __builtin_ctzll(hit))];
+        else if (any) st.token = sh.draw.sorted_at[__builtin_amdgcn_readlane(end, 63 - __builtin_clzll(any))];
+      }
+    }
   }
   if (t == 0) {
     if (draft >= 0 && draft < V)
@@ -730,7 +842,7 @@ struct Stop {
           const double qd = in && p.q ? (double)p.q[((int64_t)b * p.K + k0 + k) * p.V + d] : 1.0;
           const double u = (double)p.u[r];
           const RowSummary sum = summarize(p, r, lane);
-          RowStat s{sum.mass, 1.0, sum.max, -INFINITY, 0, sum.mode};
+          RowStat s{sum.mass, 1.0, sum.max, -INFINITY, 0, sum.mode, -1, 0};
           s.ok = in && u * qd < kept_of(p, s, read_as(l, sum.mode)) / s.z ? 1 : 0;
           if (lane == 0) sh.stat[k] = s;
         }
@@ -838,6 +950,11 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
   for (int k = t; k < T; k += kDrawThreads)
     if (k != j) out[k] = k < j ? p.drafts[(int64_t)b * p.K + k] : -1;
   if (t == 0) p.accepted[b] = j;
+  if (stop.st.token >= 0) {
+    if (t == 0) out[j] = stop.st.token;
+    return;
+  }
+  const bool parts = p.truncate ? p.cap == 0 : stop.q != nullptr;  // the parts' kernel has run
   // the sum of segment k by one wave (the rows' and parts' kernels' order of additions aside)
   auto segment = [&](int k) {
     double w[4];
@@ -849,13 +966,13 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
   const int k0 = min(t * per, segs), k1 = min(k0 + per, segs);
   double total, run0;
   for (bool again = false;; again = true) {
-    if (again) {  // nothing beyond the drafter's probabilities: p itself, whose sums nobody has
+    if (again || (p.truncate && !parts)) {
+      // nothing beyond the drafter's probabilities (then p itself), or lists that did not reach down to tau
       for (int k = wv; k < segs; k += 4) {
         const double s = segment(k);
         if (lane == 0) sh.sum[k] = s;
       }
     } else {
-      const bool parts = p.truncate || stop.q;
       // the sums' kernel's are relative to their group's largest weight, and hold a lookup's rejected draft
       const int own = !parts && stop.draft >= 0 && stop.draft < p.V ? stop.draft / kSeg : -1;
       const double* src = parts ? p.part_sum + (int64_t)b * segs : p.seg_sum + stop.id * segs;
@@ -942,8 +1059,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
   }
 }
 
-// Rows of up to 128 KiB stay in LDS while they are searched, longer ones are re-read from memory; so is a
-// row whose top_k gives a floor, which is read once (its list then holds what is searched).
+// Rows of up to 128 KiB stay in LDS while they are searched, longer ones are re-read from memory; with
+// lists the row is read only where they do not reach down to tau.
 template <bool kHalf>
 void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
   constexpr int kTileBytes = kVerTile * (kHalf ? 2 : 4);
@@ -953,19 +1070,23 @@ void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
   hipLaunchKernelGGL(verify_sums_kernel<kHalf>, dim3(rows * ((a.groups + 3) / 4)), dim3(256), 0, s, a);
   if (a.truncate) {
     const dim3 grid(rows), block(kVerThreads);
-    if (a.rank > 0 || tiles > kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0>), grid, block, 0, s, a);
-    else if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge>), grid, block, 0, s, a);
+    if (a.cap > 0) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0, true>), grid, block, 0, s, a);
+    else if (tiles > kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0, false>), grid, block, 0, s, a);
+    else if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge, false>), grid, block, 0, s, a);
   }
-  if (a.truncate || a.q)
+  if (a.truncate ? a.cap == 0 : a.q != nullptr)
     hipLaunchKernelGGL(verify_parts_kernel<kHalf>, dim3(B * ((a.segs + 4 * kPartSegs - 1) / (4 * kPartSegs))), dim3(256), 0,
                        s, a);
   hipLaunchKernelGGL(verify_draw_kernel<kHalf>, dim3(B), dim3(kDrawThreads), 0, s, a);
 }
 
-// Workspace: row statistics, segments', groups' and parts' sums, groups' maxima and floors.
+// Entries listed per group: kVerList per row, at most 128; no lists for rows of more than 64 groups.
+int list_cap(int64_t groups) { return groups <= 64 ? (int)std::min<int64_t>(128, kVerList / groups) : 0; }
+
+// Workspace: row statistics, segments', groups' and parts' sums, groups' maxima, floors and lists.
 struct VerifySpace {
-  int64_t seg_sum, group_sum, part_sum, group_max, group_floor, bytes;
+  int64_t seg_sum, group_sum, part_sum, list, group_max, group_floor, group_count, bytes;
 };
 VerifySpace verify_space(int64_t B, int64_t K, int64_t V) {
   const int64_t rows = B * (K + 1), segs = (V + kSeg - 1) / kSeg, groups = (segs + kGroupSegs - 1) / kGroupSegs;
@@ -973,10 +1094,22 @@ VerifySpace verify_space(int64_t B, int64_t K, int64_t V) {
   w.seg_sum = rows * (int64_t)sizeof(RowStat);
   w.group_sum = w.seg_sum + rows * segs * 8;
   w.part_sum = w.group_sum + rows * groups * 8;
-  w.group_max = w.part_sum + B * segs * 8;
+  w.list = w.part_sum + B * segs * 8;
+  w.group_max = w.list + rows * groups * list_cap(groups) * 8;
   w.group_floor = w.group_max + rows * groups * 4;
-  w.bytes = w.group_floor + rows * groups * 4;
+  w.group_count = w.group_floor + rows * groups * 4;
+  w.bytes = w.group_count + rows * groups * 4;
   return w;
+}
+
+// Lists pay where they nearly always reach down to the top_k-th entry: a group's share of the top_k,
+// m = top_k / groups on average and m + 5 sqrt(m) + 3 hardly ever exceeded if they are spread at random,
+// within the 4 rank entries that a list holds at least.
+void use_lists(VerifyArgs& a) {
+  a.cap = a.truncate && a.top_k < a.V ? list_cap(a.groups) : 0;
+  a.rank = a.cap / 8;
+  const double m = (double)a.top_k / a.groups;
+  if (4.0 * a.rank < (a.groups > 1 ? m + 5.0 * std::sqrt(m) + 3.0 : m)) a.cap = a.rank = 0;
 }
 
 }  // namespace
@@ -1034,6 +1167,8 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.part_sum = reinterpret_cast<double*>(ws + w.part_sum);
   a.group_max = reinterpret_cast<float*>(ws + w.group_max);
   a.group_floor = reinterpret_cast<float*>(ws + w.group_floor);
+  a.group_count = reinterpret_cast<int32_t*>(ws + w.group_count);
+  a.list = reinterpret_cast<float2*>(ws + w.list);
   a.segs = (V + kSeg - 1) / kSeg;
   a.groups = (a.segs + kGroupSegs - 1) / kGroupSegs;
   a.scale = 1.4426950408889634 / temperature;
@@ -1043,8 +1178,7 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.top_p = top_p;
   a.use_mass = top_p < 1.0;
   a.truncate = top_k < V || a.use_mass;
-  const int rank = (top_k + a.groups - 1) / a.groups;
-  a.rank = a.truncate && rank <= kMaxRank ? rank : 0;
+  use_lists(a);
   if (logits_f16) launch_verify<true>(a, B, (hipStream_t)stream);
   else launch_verify<false>(a, B, (hipStream_t)stream);
   return check_launch(fn);
