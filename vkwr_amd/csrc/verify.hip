@@ -40,13 +40,13 @@
 namespace vk {
 namespace {
 
-constexpr int kVerThreads = 1024;
+constexpr int kVerThreads = 512;   // per row: three workgroups fit on a CU, and one's loads cover another's work
 constexpr int kVerWaves = kVerThreads / 64;
 constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
 constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
-constexpr int kVerList = kVerThreads;  // listed entries of a row: one per lane
+constexpr int kVerList = 2 * kVerThreads;  // listed entries of a row: two per lane
 constexpr int kVerDraw = 256;    // kept entries that the rows' kernel draws from directly
-constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a workgroup reads at once
+constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a row's workgroup reads at once
 constexpr int kVerMaxV = 1 << 20;
 constexpr int kSeg = 256;        // consecutive entries whose weights are added up for the draw (one wave's 64 x 4)
 constexpr int kMaxSegs = kVerMaxV / kSeg;
@@ -187,7 +187,8 @@ struct StatShared {
     uint64_t mass[kVerBins];
     struct {  // behind the histogram
       double w[kVerDraw], sorted_w[kVerDraw];
-      int at[kVerDraw], sorted_at[kVerDraw];
+      alignas(16) int at[kVerDraw];
+      int sorted_at[kVerDraw];
     } draw;
   };
   uint32_t cnt[kVerBins];
@@ -202,25 +203,27 @@ struct StatShared {
   uint64_t before_m;
 };
 
-// Sum (maximum) of the 16 values that the lanes of a row hold, in every lane.
+// Sum (maximum) of the values that 8 (16) consecutive lanes hold, in every one of them.
 template <class X>
-__device__ __forceinline__ X row_add(X x) {
+__device__ __forceinline__ X oct_add(X x) {
   x += dpp<0xB1>(x);
   x += dpp<0x4E>(x);
-  x += dpp<0x141>(x);
-  return x + dpp<0x140>(x);
+  return x + dpp<0x141>(x);
 }
-__device__ __forceinline__ float row_fmax(float x) {
+__device__ __forceinline__ float oct_fmax(float x) {
   x = fmaxf(x, dpp<0xB1>(x));
   x = fmaxf(x, dpp<0x4E>(x));
-  x = fmaxf(x, dpp<0x141>(x));
+  return fmaxf(x, dpp<0x141>(x));
+}
+__device__ __forceinline__ float row_fmax(float x) {
+  x = oct_fmax(x);
   return fmaxf(x, dpp<0x140>(x));
 }
 
 // Block reductions with one barrier: consecutive ones alternate between two buffers (par), so a wave
-// overwrites a buffer only behind the barrier that every wave reaches after reading it.  Each row of 16
-// lanes adds the 16 wave values.
-static_assert(kVerWaves == 16, "a row of lanes holds the wave values");
+// overwrites a buffer only behind the barrier that every wave reaches after reading it.  Eight lanes add
+// the eight wave values.
+static_assert(kVerWaves == 8, "eight lanes hold the wave values");
 __device__ __forceinline__ void block_max2(StatShared& sh, int& par, float& a, float& b) {
   a = wave_fmax(a);
   b = wave_fmax(b);
@@ -229,15 +232,15 @@ __device__ __forceinline__ void block_max2(StatShared& sh, int& par, float& a, f
     sh.redg[par][threadIdx.x >> 6] = b;
   }
   __syncthreads();
-  a = row_fmax(sh.redf[par][threadIdx.x & 15]);
-  b = row_fmax(sh.redg[par][threadIdx.x & 15]);
+  a = oct_fmax(sh.redf[par][threadIdx.x & 7]);
+  b = oct_fmax(sh.redg[par][threadIdx.x & 7]);
   par ^= 1;
 }
 __device__ __forceinline__ float block_max(StatShared& sh, int& par, float a) {
   a = wave_fmax(a);
   if ((threadIdx.x & 63) == 0) sh.redf[par][threadIdx.x >> 6] = a;
   __syncthreads();
-  a = row_fmax(sh.redf[par][threadIdx.x & 15]);
+  a = oct_fmax(sh.redf[par][threadIdx.x & 7]);
   par ^= 1;
   return a;
 }
@@ -245,7 +248,7 @@ __device__ __forceinline__ double block_sum(StatShared& sh, int& par, double a) 
   a = wave_add(a);
   if ((threadIdx.x & 63) == 0) sh.redd[par][threadIdx.x >> 6] = a;
   __syncthreads();
-  a = row_add(sh.redd[par][threadIdx.x & 15]);
+  a = oct_add(sh.redd[par][threadIdx.x & 7]);
   par ^= 1;
   return a;
 }
@@ -260,10 +263,10 @@ __device__ __forceinline__ void block_add(StatShared& sh, int& par, uint32_t& a,
     sh.redm[par][w] = m;
   }
   __syncthreads();
-  const int w = threadIdx.x & 15;
-  a = row_add(sh.redc[par][w]);
-  b = row_add(sh.rede[par][w]);
-  m = row_add(sh.redm[par][w]);
+  const int w = threadIdx.x & 7;
+  a = oct_add(sh.redc[par][w]);
+  b = oct_add(sh.rede[par][w]);
+  m = oct_add(sh.redm[par][w]);
   par ^= 1;
 }
 
@@ -459,13 +462,13 @@ __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id,
   return r;
 }
 
-// kTiles > 0: a row (V <= kTiles * kVerTile) that is searched as a whole stays in LDS; 0: it is re-read.
-// kLists: the groups' lists are searched first.
-template <bool kHalf, int kTiles, bool kLists>
-__global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) {
+// kLists: the groups' lists are searched first.  A row that is searched as a whole is read twice more:
+// for the histogram and for the entries of one bin.  (Kept in LDS, 128 KiB left one workgroup per CU, whose
+// loads and arithmetic then took turns.)
+template <bool kHalf, bool kLists>
+__global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kernel(VerifyArgs p) {
   typedef typename Raw<kHalf>::type R;
   __shared__ StatShared sh;
-  __shared__ R lrow[kTiles > 0 ? kTiles * kVerThreads : 1];
   const int T = p.K + 1;
   const int b = blockIdx.x / T, i = blockIdx.x - b * T;
   const int n = p.n_draft ? p.n_draft[b] : p.K;
@@ -517,40 +520,38 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
     if ((j + 1) * kVerTile > V && j * kVerTile + 4 * t >= V) l = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     return l;
   };
-  // f(four entries) over this lane's part of the row, four tiles' loads at a time; padding is -inf.
-  // first: from memory, into LDS if the row fits there; then from where it is.
-  auto each_row = [&](bool first, auto&& f) __attribute__((always_inline)) {
+  // f(four entries) over this lane's part of the row, four tiles' loads at a time; padding is -inf
+  auto each_row = [&](auto&& f) __attribute__((always_inline)) {
     for (int j = 0; j < tiles; j += 4) {
       R x[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (kTiles == 0 || first) x[u] = load_raw<kHalf>(row, min((j + u) * kVerTile + 4 * t, V - 4));
-        else x[u] = lrow[min(j + u, tiles - 1) * kVerThreads + t];
-      }
+      for (int u = 0; u < 4; ++u) x[u] = load_raw<kHalf>(row, min((j + u) * kVerTile + 4 * t, V - 4));
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (j + u >= tiles) break;
-        if (kTiles > 0 && first) lrow[(j + u) * kVerThreads + t] = x[u];
         f(entries(j + u, x[u]));
       }
     }
   };
 
-  // The lists: one entry per lane.
-  bool listed = kLists && sum.reach < INFINITY, loaded = false;
-  float mine = -INFINITY;
-  int mine_at = -1;
+  // The lists: two entries per lane.
+  bool listed = kLists && sum.reach < INFINITY;
+  float mine[2] = {-INFINITY, -INFINITY};
+  int mine_at[2] = {-1, -1};
   if (listed) {
-    const int g = t / p.cap, k = t - g * p.cap;
-    if (g < p.groups && k < p.group_count[id * p.groups + g]) {
-      const float2 e = p.list[(id * p.groups + g) * p.cap + k];
-      mine = e.x;
-      mine_at = __builtin_bit_cast(int, e.y);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = t + u * kVerThreads, g = at / p.cap, k = at - g * p.cap;
+      if (g < p.groups && k < p.group_count[id * p.groups + g]) {
+        const float2 e = p.list[(id * p.groups + g) * p.cap + k];
+        mine[u] = e.x;
+        mine_at[u] = __builtin_bit_cast(int, e.y);
+      }
     }
   }
   auto each4 = [&](auto&& f) __attribute__((always_inline)) {
-    if (kLists && listed) f(f4{mine, -INFINITY, -INFINITY, -INFINITY});
-    else each_row(!loaded, f);
+    if (kLists && listed) f(f4{mine[0], mine[1], -INFINITY, -INFINITY});
+    else each_row(f);
   };
   auto each = [&](auto&& f) __attribute__((always_inline)) {
     each4([&](f4 x) __attribute__((always_inline)) {
@@ -598,31 +599,42 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
         }
       }
     });
-    loaded = loaded || !listed;
     __syncthreads();
-    // inclusive prefix over the bins (two per lane) and the first bin that reaches the budget
-    const uint32_t c0 = sh.cnt[2 * t], c1 = sh.cnt[2 * t + 1];
-    const uint64_t m0 = sh.mass[2 * t], m1 = sh.mass[2 * t + 1];
-    uint32_t ci = wave_scan(c0 + c1, lane);
-    uint64_t mi = wave_scan(m0 + m1, lane);
+    // inclusive prefix over the bins (four per lane) and the first bin that reaches the budget
+    constexpr int kPer = kVerBins / kVerThreads;
+    uint32_t c[kPer], ci = 0;
+    uint64_t m[kPer], mi = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      ci += c[k] = sh.cnt[kPer * t + k];
+      mi += m[k] = sh.mass[kPer * t + k];
+    }
+    const uint32_t c_own = ci;
+    const uint64_t m_own = mi;
+    ci = wave_scan(ci, lane);
+    mi = wave_scan(mi, lane);
     if (lane == 63) {
       sh.redc[par][wv] = ci;
       sh.redm[par][wv] = mi;
     }
     __syncthreads();
-    ci += row_add((lane & 15) < wv ? sh.redc[par][lane & 15] : 0u);
-    mi += row_add((lane & 15) < wv ? sh.redm[par][lane & 15] : (uint64_t)0);
+    ci += oct_add((lane & 7) < wv ? sh.redc[par][lane & 7] : 0u);
+    mi += oct_add((lane & 7) < wv ? sh.redm[par][lane & 7] : (uint64_t)0);
     par ^= 1;
-    if (enough(ci - c1, mi - m1)) {
-      if (!enough(ci - c1 - c0, mi - m1 - m0)) {
-        sh.bin = 2 * t;
-        sh.before_c = ci - c1 - c0;
-        sh.before_m = mi - m1 - m0;
+    if (enough(ci, mi) && !enough(ci - c_own, mi - m_own)) {
+      uint32_t cb = ci - c_own;
+      uint64_t mb = mi - m_own;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        if (enough(cb + c[k], mb + m[k])) {
+          sh.bin = kPer * t + k;
+          sh.before_c = cb;
+          sh.before_m = mb;
+          break;
+        }
+        cb += c[k];
+        mb += m[k];
       }
-    } else if (enough(ci, mi)) {
-      sh.bin = 2 * t + 1;
-      sh.before_c = ci - c1;
-      sh.before_m = mi - m1;
     }
     __syncthreads();
     const bool found = sh.bin < kVerBins;
@@ -750,21 +762,25 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
   // The token if the sequence stops here: all kept entries are listed.  Sorted by index (places counted,
   // so that the sums' order does not hang on the order of the atomics), then the prefix sums in one wave.
   if (kLists && listed) {
-    double w = 0.0;
-    if (mine >= st.tau) {
-      w = kept_of(p, st, mine) / st.z;
-      if (i < n) {
-        if (p.q) w = fmax(w - (double)p.q[((int64_t)b * p.K + i) * V + mine_at], 0.0);
-        else if (mine_at == p.drafts[(int64_t)b * p.K + i]) w = 0.0;
-      }
+    double w[2] = {0.0, 0.0};
+    const int d = i < n && !p.q ? p.drafts[(int64_t)b * p.K + i] : -1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!(mine[u] >= st.tau && mine[u] > -INFINITY)) continue;
+      w[u] = kept_of(p, st, mine[u]) / st.z;
+      if (i < n && p.q) w[u] = fmax(w[u] - (double)p.q[((int64_t)b * p.K + i) * V + mine_at[u]], 0.0);
+      if (mine_at[u] == d) w[u] = 0.0;
     }
     if (t == 0) sh.n_cand = 0;
     __syncthreads();
-    if (mine >= st.tau && mine > -INFINITY) {
-      const int at = atomicAdd(&sh.n_cand, 1);
-      if (at < kVerDraw) {
-        sh.draw.w[at] = w;
-        sh.draw.at[at] = mine_at;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (mine[u] >= st.tau && mine[u] > -INFINITY) {
+        const int at = atomicAdd(&sh.n_cand, 1);
+        if (at < kVerDraw) {
+          sh.draw.w[at] = w[u];
+          sh.draw.at[at] = mine_at[u];
+        }
       }
     }
     __syncthreads();
@@ -773,7 +789,10 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(VerifyArgs p) 
       if (t < kept) {
         const int my = sh.draw.at[t];
         int place = 0;
-        for (int k = 0; k < kept; ++k) place += sh.draw.at[k] < my ? 1 : 0;
+        for (int k = 0; k < kept; k += 4) {
+          const int4 o = *reinterpret_cast<const int4*>(&sh.draw.at[k]);
+          place += (o.x < my) + (o.y < my && k + 1 < kept) + (o.z < my && k + 2 < kept) + (o.w < my && k + 3 < kept);
+        }
         sh.draw.sorted_w[place] = sh.draw.w[t];
         sh.draw.sorted_at[place] = my;
       }
@@ -1059,21 +1078,13 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
   }
 }
 
-// Rows of up to 128 KiB stay in LDS while they are searched, longer ones are re-read from memory; with
-// lists the row is read only where they do not reach down to tau.
 template <bool kHalf>
 void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
-  constexpr int kTileBytes = kVerTile * (kHalf ? 2 : 4);
-  constexpr int kSmall = (32 << 10) / kTileBytes, kLarge = (128 << 10) / kTileBytes;
   const unsigned rows = (unsigned)B * (a.K + 1);
-  const int tiles = (a.V + kVerTile - 1) / kVerTile;
   hipLaunchKernelGGL(verify_sums_kernel<kHalf>, dim3(rows * ((a.groups + 3) / 4)), dim3(256), 0, s, a);
   if (a.truncate) {
-    const dim3 grid(rows), block(kVerThreads);
-    if (a.cap > 0) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0, true>), grid, block, 0, s, a);
-    else if (tiles > kLarge) hipLaunchKernelGGL((verify_rows_kernel<kHalf, 0, false>), grid, block, 0, s, a);
-    else if (tiles <= kSmall) hipLaunchKernelGGL((verify_rows_kernel<kHalf, kSmall, false>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((verify_rows_kernel<kHalf, kLarge, false>), grid, block, 0, s, a);
+    if (a.cap > 0) hipLaunchKernelGGL((verify_rows_kernel<kHalf, true>), dim3(rows), dim3(kVerThreads), 0, s, a);
+    else hipLaunchKernelGGL((verify_rows_kernel<kHalf, false>), dim3(rows), dim3(kVerThreads), 0, s, a);
   }
   if (a.truncate ? a.cap == 0 : a.q != nullptr)
     hipLaunchKernelGGL(verify_parts_kernel<kHalf>, dim3(B * ((a.segs + 4 * kPartSegs - 1) / (4 * kPartSegs))), dim3(256), 0,
@@ -1134,7 +1145,7 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
              "%s: vocabulary size must be a multiple of 4 and at most 1048576, got %d", fn, V);
   VK_REQUIRE(temperature >= 0.001 && temperature <= 1000, "%s: temperature %g outside [0.001, 1000]", fn,
              temperature);
-  // (256 threads per 8192 entries of a row, 1024 per row: fewer than 2^32 in a launch)
+  // (256 threads per 8192 entries of a row, 512 per row: fewer than 2^32 in a launch)
   VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= (1 << 21) / ((V + 131071) / 131072), "%s: B*(K+1) too large", fn);
   if (B == 0) return VKWR_OK;
   VK_REQUIRE(logits && uniforms && tokens && accepted && (K == 0 || drafts), "%s: null pointer", fn);
