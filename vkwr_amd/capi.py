@@ -459,15 +459,31 @@ def sample(logits, states, out, temperature=1.0, top_k=-1, top_p=1.0, penalties=
         _check(st, "vkwr_sampling_repetition_topk_topp")
 
 
-def _dev(t, dtype, n, what):
-    """Pointer of a tensor that a kernel reads or writes as n values of dtype: contiguous, on the
-    current device, with exactly n entries."""
-    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.numel() != n:
+class _Tensors:
+    """Addresses of the tensors of one call: contiguous, of the given type and size, on the current device
+    (whose current stream the call goes to)."""
+
+    __slots__ = ("dev",)
+
+    def __init__(self):
+        self.dev = torch.cuda.current_device() if torch.cuda.is_initialized() else 0
+
+    def __call__(self, t, dtype, n, what):
+        if t.dtype != dtype or t.get_device() != self.dev or t.numel() != n or not t.is_contiguous():
+            self._refuse(t, dtype, n, what)
+        return t.data_ptr()
+
+    def optional(self, t, dtype, n, what):
+        return None if t is None else self(t, dtype, n, what)
+
+    def stream(self):
+        return torch._C._cuda_getCurrentRawStream(self.dev)
+
+    def _refuse(self, t, dtype, n, what):
+        if t.is_cuda and t.get_device() != self.dev:
+            raise ValueError(f"{what}: on {t.device}, but the current device is cuda:{self.dev}")
         raise TypeError(f"{what}: expected a contiguous {dtype} CUDA tensor of {n} entries, got "
                         f"{t.dtype} {t.device} shape {tuple(t.shape)} contiguous={t.is_contiguous()}")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
-    return ctypes.c_void_p(t.data_ptr())
 
 
 def wkv_drafts_slots(B, T, C, H, pool, slots, r, w, k, v, a, b, y, kept=None, pending=None, pending_rows=None):
@@ -475,7 +491,7 @@ def wkv_drafts_slots(B, T, C, H, pool, slots, r, w, k, v, a, b, y, kept=None, pe
     sequence i takes kept[i] tokens of the pending vectors (w, k, v, a, b), each [n, P, C] -- row
     pending_rows[i], or i -- its state is written, and r..b [B, T, C] run on from it into y [B, T, C]
     without being written.  T = 0 (r..y may be None): only the kept tokens; no pending: only drafts."""
-    h = torch.float16
+    at, h, i32 = _Tensors(), torch.float16, torch.int32
     n_slots = pool.shape[0]
     P = n_pending = 0
     pv = [None] * 5
@@ -483,13 +499,13 @@ def wkv_drafts_slots(B, T, C, H, pool, slots, r, w, k, v, a, b, y, kept=None, pe
         raise ValueError("wkv_drafts_slots: kept and pending go together")
     if pending is not None:
         n_pending, P = pending[0].shape[:2]
-        pv = [_dev(t, h, n_pending * P * C, "pending") for t in pending]
+        pv = [at(t, h, n_pending * P * C, "pending") for t in pending]
     n = B * T * C
-    ins = [_dev(t, h, n, "r, w, k, v, a, b, y") for t in (r, w, k, v, a, b, y)] if T else [None] * 7
-    _check(_wkv_drafts(B, P, T, C, H, _dev(pool, torch.float32, n_slots * H * 4096, "pool"), n_slots,
-                       _dev(slots, torch.int32, B, "slots"), _dev(kept, torch.int32, B, "kept") if P else None,
-                       n_pending, None if pending_rows is None else _dev(pending_rows, torch.int32, B, "pending_rows"),
-                       *pv, *ins, _stream()), "vkwr_wkv7_fp32_drafts_slots")
+    ins = [at(t, h, n, "r, w, k, v, a, b, y") for t in (r, w, k, v, a, b, y)] if T else [None] * 7
+    _check(_wkv_drafts(B, P, T, C, H, at(pool, torch.float32, n_slots * H * 4096, "pool"), n_slots,
+                       at(slots, i32, B, "slots"), at(kept, i32, B, "kept") if P else None, n_pending,
+                       at.optional(pending_rows, i32, B, "pending_rows"), *pv, *ins, at.stream()),
+           "vkwr_wkv7_fp32_drafts_slots")
 
 
 def verify_workspace_bytes(B, K, V):
@@ -507,15 +523,14 @@ def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_draft=None, draf
     K = T - 1
     if logits.dtype not in (torch.float16, torch.float32):
         raise TypeError(f"logits: fp16 or fp32, got {logits.dtype}")
-    i32, f32 = torch.int32, torch.float32
+    at, i32, f32 = _Tensors(), torch.int32, torch.float32
     if workspace is None:
         workspace = torch.empty(_verify_ws(B, K, V), dtype=torch.uint8, device=logits.device)
-    _check(_verify(B, K, V, _dev(logits, logits.dtype, B * T * V, "logits"), int(logits.dtype == torch.float16),
-                   _dev(drafts, i32, B * K, "drafts"), None if n_draft is None else _dev(n_draft, i32, B, "n_draft"),
-                   None if draft_probs is None else _dev(draft_probs, f32, B * K * V, "draft_probs"),
-                   _dev(uniforms, f32, B * T, "uniforms"), _dev(tokens, i32, B * T, "tokens"),
-                   _dev(accepted, i32, B, "accepted"), temperature, top_k, top_p,
-                   _dev(workspace, torch.uint8, workspace.numel(), "workspace"), workspace.numel(), _stream()),
+    _check(_verify(B, K, V, at(logits, logits.dtype, B * T * V, "logits"), int(logits.dtype == torch.float16),
+                   at(drafts, i32, B * K, "drafts"), at.optional(n_draft, i32, B, "n_draft"),
+                   at.optional(draft_probs, f32, B * K * V, "draft_probs"), at(uniforms, f32, B * T, "uniforms"),
+                   at(tokens, i32, B * T, "tokens"), at(accepted, i32, B, "accepted"), temperature, top_k, top_p,
+                   at(workspace, torch.uint8, workspace.numel(), "workspace"), workspace.numel(), at.stream()),
            "vkwr_sampling_verify_drafts")
 
 
@@ -544,9 +559,9 @@ def lora_plan(adapters, plan):
     m = adapters.numel()
     if m > plan.max_rows:
         raise ValueError(f"lora plan of {plan.max_rows} rows, got {m}")
-    _check(_lora_plan(m, plan.n_adapters, _dev(adapters, torch.int32, m, "adapters"),
-                      _dev(plan.buf, torch.uint8, plan.buf.numel(), "plan"), plan.buf.numel(), _stream()),
-           "vkwr_lora_plan")
+    at, nbytes = _Tensors(), plan.buf.numel()
+    _check(_lora_plan(m, plan.n_adapters, at(adapters, torch.int32, m, "adapters"),
+                      at(plan.buf, torch.uint8, nbytes, "plan"), nbytes, at.stream()), "vkwr_lora_plan")
     plan.m = m
 
 
@@ -559,15 +574,16 @@ def lora_target(x, a, b, y, base=None, epilogue=EPI_NONE):
     h = torch.float16
     if tuple(b.shape) != (G, n, rank):
         raise ValueError(f"lora_target: a {tuple(a.shape)} and b {tuple(b.shape)} do not match")
-    t = LoraTarget(_dev(x, h, m * k, "x"), _dev(a, h, G * rank * k, "a"), _dev(b, h, G * n * rank, "b"),
-                   None if base is None else _dev(base, h, m * n, "base"), _dev(y, h, m * n, "y"), n, k, epilogue)
+    at = _Tensors()
+    t = LoraTarget(at(x, h, m * k, "x"), at(a, h, G * rank * k, "a"), at(b, h, G * n * rank, "b"),
+                   at.optional(base, h, m * n, "base"), at(y, h, m * n, "y"), n, k, epilogue)
     t.sizes = (m, G, rank)
     t.tensors = (x, a, b, y, base)  # what the pointers point to
     return t
 
 
 def _lora_targets(targets):
-    if not 1 <= len(targets) <= LORA_MAX_TARGETS or len({t.sizes for t in targets}) != 1:
+    if not 1 <= len(targets) <= LORA_MAX_TARGETS or any(t.sizes != targets[0].sizes for t in targets):
         raise ValueError("lora: 1 to 8 targets with the same rows, adapters and rank")
     return targets[0].sizes, (LoraTarget * len(targets))(*targets)
 
@@ -589,6 +605,6 @@ def lora(plan, targets, scale=None, workspace=None):
         raise ValueError(f"lora: plan of {plan.m} rows and {plan.n_adapters} adapters, targets of {m} and {G}")
     if workspace is None:
         workspace = torch.empty(lora_workspace_bytes(m, G, targets), dtype=torch.uint8, device=plan.buf.device)
-    _check(_lora(m, G, rank, None if scale is None else _dev(scale, torch.float32, G, "scale"), _ptr(plan.buf),
-                 len(targets), arr, _dev(workspace, torch.uint8, workspace.numel(), "workspace"), workspace.numel(),
-                 _stream()), "vkwr_lora_f16")
+    at, nbytes = _Tensors(), workspace.numel()
+    _check(_lora(m, G, rank, at.optional(scale, torch.float32, G, "scale"), plan.buf.data_ptr(), len(targets), arr,
+                 at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()), "vkwr_lora_f16")

@@ -827,12 +827,12 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
   }
 }
 
-// What the last two kernels share: the row a sequence stops at and the weights it draws from.  Four
-// waves; without a filter they make the rows' statistics from the groups' sums, a row each at a time.
+// What the last two kernels share: the row a sequence stops at and the weights it draws from.  Without a
+// filter the workgroup's kWaves waves make the rows' statistics from the groups' sums, a row each.
 struct StopShared {
   RowStat stat[64];
 };
-template <bool kHalf>
+template <bool kHalf, int kWaves>
 struct Stop {
   const VerifyArgs& p;
   int64_t id;      // row b (K + 1) + j
@@ -852,7 +852,7 @@ struct Stop {
         last = last || !p.stat[(int64_t)b * T + k0 + lane].ok;
       } else {
         if (k0 > 0) __syncthreads();
-        for (int k = wv; k < 64 && k0 + k <= n; k += 4) {
+        for (int k = wv; k < 64 && k0 + k <= n; k += kWaves) {
           const int64_t r = (int64_t)b * T + k0 + k;
           const int d = k0 + k < n ? p.drafts[(int64_t)b * p.K + k0 + k] : -1;
           const bool in = d >= 0 && d < p.V;
@@ -918,7 +918,7 @@ __global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
   const int b = blockIdx.x / parts, part = blockIdx.x - b * parts, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int n = p.n_draft ? p.n_draft[b] : p.K;
   if (n < 0 || n > p.K) return;
-  const Stop<kHalf> stop(p, shared, b, n, lane, wv);
+  const Stop<kHalf, 4> stop(p, shared, b, n, lane, wv);
   if (!p.truncate && !stop.beyond) return;
   const int seg0 = (part * 4 + wv) * kPartSegs;
   f4 l[kPartSegs], qv[kPartSegs];
@@ -943,11 +943,11 @@ __global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
   }
 }
 
-constexpr int kDrawThreads = 256;
+constexpr int kDrawThreads = 512;
 struct DrawShared {
   StopShared stop;
   double sum[kMaxSegs];
-  double red[4];
+  double red[kDrawThreads / 64];
   int first, last;
 };
 
@@ -964,7 +964,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
     if (t == 0) p.accepted[b] = -1;
     return;
   }
-  Stop<kHalf> stop(p, sh.stop, b, n, lane, wv);
+  Stop<kHalf, kDrawThreads / 64> stop(p, sh.stop, b, n, lane, wv);
   const int j = stop.j;
   for (int k = t; k < T; k += kDrawThreads)
     if (k != j) out[k] = k < j ? p.drafts[(int64_t)b * p.K + k] : -1;
@@ -981,13 +981,13 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
     stop.weights(stop.load_l(at), stop.load_q(at), at, w);
     return wave_add((w[0] + w[1]) + (w[2] + w[3]));
   };
-  const int per = (segs + kDrawThreads - 1) / kDrawThreads;  // segments per lane of the scan: at most 16
+  const int per = (segs + kDrawThreads - 1) / kDrawThreads;  // segments per lane of the scan: at most 8
   const int k0 = min(t * per, segs), k1 = min(k0 + per, segs);
   double total, run0;
   for (bool again = false;; again = true) {
     if (again || (p.truncate && !parts)) {
       // nothing beyond the drafter's probabilities (then p itself), or lists that did not reach down to tau
-      for (int k = wv; k < segs; k += 4) {
+      for (int k = wv; k < segs; k += kDrawThreads / 64) {
         const double s = segment(k);
         if (lane == 0) sh.sum[k] = s;
       }
@@ -1022,9 +1022,9 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
     const double incl = wave_scan(s, lane);
     if (lane == 63) sh.red[wv] = incl;
     __syncthreads();
-    const double r0 = sh.red[0], r1 = sh.red[1], r2 = sh.red[2], r3 = sh.red[3];
-    total = (r0 + r1) + (r2 + r3);
-    run0 = (wv == 0 ? 0.0 : wv == 1 ? r0 : wv == 2 ? r0 + r1 : r0 + r1 + r2) + incl - s;
+    const double of_wave = sh.red[lane & 7];
+    total = oct_add(of_wave);
+    run0 = oct_add((lane & 7) < wv ? of_wave : 0.0) + incl - s;
     if (total > 0.0 || !stop.beyond) break;
     stop.beyond = false;
     __syncthreads();
@@ -1113,14 +1113,18 @@ VerifySpace verify_space(int64_t B, int64_t K, int64_t V) {
   return w;
 }
 
-// Lists pay where they nearly always reach down to the top_k-th entry: a group's share of the top_k,
-// m = top_k / groups on average and m + 5 sqrt(m) + 3 hardly ever exceeded if they are spread at random,
-// within the 4 rank entries that a list holds at least.
+// Lists pay where they nearly always reach down to the top_k-th entry.  The r-th largest of 16 lane maxima
+// of 32 entries each has about 64 (-ln(1 - r / 16)) of a group's 2048 entries above it; the largest r
+// that leaves the list a third of room is taken.  That has to hold a group's share of the top_k: m = top_k
+// / groups on average, hardly ever more than m + 5 sqrt(m) + 3 where they are spread at random.  24
+// sequences of 5 drafts, 65536 entries, top_k 40: 41 us without lists, 28 with.
 void use_lists(VerifyArgs& a) {
   a.cap = a.truncate && a.top_k < a.V ? list_cap(a.groups) : 0;
-  a.rank = a.cap / 8;
+  a.rank = 0;
+  const auto above = [](int r) { return -64.0 * std::log1p(-r / 16.0); };
+  while (a.rank < 14 && above(a.rank + 1) * 1.33 <= a.cap) ++a.rank;
   const double m = (double)a.top_k / a.groups;
-  if (4.0 * a.rank < (a.groups > 1 ? m + 5.0 * std::sqrt(m) + 3.0 : m)) a.cap = a.rank = 0;
+  if (above(a.rank) < (a.groups > 1 ? m + 5.0 * std::sqrt(m) + 3.0 : m)) a.cap = a.rank = 0;
 }
 
 }  // namespace
