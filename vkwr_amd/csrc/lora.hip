@@ -33,7 +33,7 @@ constexpr int kMaxTargets = 8;
 constexpr int kMaxRank = 128;
 constexpr int kMaxAdapters = 8192;
 constexpr int kRankBlock = 64;     // ranks per shrink workgroup
-constexpr int kColBlock = 256;     // output columns per expand workgroup (64 per wave)
+constexpr int kColBlock = 256;     // fewest output columns per expand workgroup
 constexpr int kNone = -1, kBad = -2;
 
 struct Tile {
@@ -79,9 +79,17 @@ __global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const
     }
     return live ? atomicAdd(&cnt[bin], 1) : 0;
   };
+  // the first 4096 rows' bins stay in registers between the two passes
+  constexpr int kHeld = 4;
+  int held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) held[u] = u * 1024 + t < m ? bin_of(u * 1024 + t) : -1;
   for (int k = t; k < nb; k += 1024) cnt[k] = 0;
   __syncthreads();
-  for (int64_t i0 = 0; i0 < m; i0 += 1024) {
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (u * 1024 < m) place(held[u] >= 0, held[u] >= 0 ? held[u] : 0);
+  for (int64_t i0 = kHeld * 1024; i0 < m; i0 += 1024) {
     const bool live = i0 + t < m;
     place(live, live ? bin_of(i0 + t) : 0);
   }
@@ -126,7 +134,13 @@ __global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const
     row += c;
   }
   __syncthreads();
-  for (int64_t i0 = 0; i0 < m; i0 += 1024) {
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    if (u * 1024 >= m) break;
+    const int at = place(held[u] >= 0, held[u] >= 0 ? held[u] : 0);
+    if (held[u] >= 0) order[at] = u * 1024 + t;
+  }
+  for (int64_t i0 = kHeld * 1024; i0 < m; i0 += 1024) {
     const bool live = i0 + t < m;
     const int at = place(live, live ? bin_of(i0 + t) : 0);
     if (live) order[at] = (int32_t)(i0 + t);
@@ -146,7 +160,7 @@ struct LoraArgs {
   int G;
   const float* scale;
   float* h;        // [parts][target][m][rank_pad]
-  int rank, rank_pad, n_targets, parts, rank_blocks;
+  int rank, rank_pad, n_targets, parts, rank_blocks, cols;
   Target t[kMaxTargets];
 };
 
@@ -154,225 +168,274 @@ __device__ __forceinline__ fv4 mfma(hv8 a, hv8 b, fv4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Grid: x = part, y = tile, z = target * rank_blocks + rank block.  Four waves cut the part's K
-// between them; their sums are added in wave order through LDS.
+// x A^T of NS blocks of 16 rows over the 32-deep steps s0 .. s1 - 1, two steps' loads together.
+template <int NS, int RT>
+__device__ __forceinline__ void shrink_steps(const _Float16* const* xr, const _Float16* const* ar, int kg, int K, int s0,
+                                             int s1, fv4 (&acc)[NS][RT]) {
+  const hv8 zero = {};
+  for (int st = s0; st < s1; st += 2) {
+    hv8 fa[2][RT], fb[2][NS];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k = 32 * (st + u) + kg;
+      const bool in = st + u < s1 && k < K;
+#pragma unroll
+      for (int j = 0; j < RT; ++j) fa[u][j] = in ? *reinterpret_cast<const hv8*>(ar[j] + k) : zero;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) fb[u][s] = in ? *reinterpret_cast<const hv8*>(xr[s] + k) : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[s][j] = mfma(fa[u][j], fb[u][s], acc[s][j]);
+  }
+}
+
+// Grid: x = part, y = tile, z = target * rank_blocks + rank block.  Up to 16 rows: the eight waves cut the
+// part's K between them; more: four of them, each for half of the row blocks.  The waves' sums are added
+// in K order through LDS.
+constexpr int kShrinkWaves = 8;
 template <int RT>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
-  __shared__ fv4 lds[4][kSub][RT][64];
-  const PlanHead* head = reinterpret_cast<const PlanHead*>(p.plan);
-  if ((int)blockIdx.y >= head->n_adapter || head->m != p.m || head->G != p.G) return;
-  const Tile tile = plan_tiles(p.plan)[blockIdx.y];
+__global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs p) {
+  __shared__ fv4 lds[3 * kSub][RT][64];
+  const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
+  const Tile tile = plan_tiles(p.plan)[blockIdx.y];  // blockIdx.y < tiles_cap: in the buffer, if stale
+  if ((int)blockIdx.y >= head.n_adapter || head.m != p.m || head.G != p.G) return;
   const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
-  const int ti = blockIdx.z / p.rank_blocks, rb = blockIdx.z - ti * p.rank_blocks;
+  const int ti = blockIdx.z / p.rank_blocks, r0 = (blockIdx.z - ti * p.rank_blocks) * kRankBlock;
   const Target& tg = p.t[ti];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int K = tg.k, ns = (tile.rows + 15) >> 4;
   const int li = lane & 15, kg = 8 * (lane >> 4);
-  const _Float16* xr[kSub];
+  // waves along the rows and along K; row blocks per wave
+  const int rw = ns > 1 ? 2 : 1, kw = kShrinkWaves / rw, per = (ns + rw - 1) / rw;
+  const int ri = wv % rw, ki = wv / rw;
+  const _Float16* xr[2];
 #pragma unroll
-  for (int s = 0; s < kSub; ++s)
-    xr[s] = tg.x + (int64_t)order[min(16 * s + li, tile.rows - 1)] * K;
-  const int r0 = rb * kRankBlock;
+  for (int s = 0; s < 2; ++s)
+    xr[s] = tg.x + (int64_t)order[min(16 * min(ri * per + s, ns - 1) + li, tile.rows - 1)] * K;
   const _Float16* ar[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j)
     ar[j] = tg.a + ((int64_t)tile.adapter * p.rank + min(r0 + 16 * j + li, p.rank - 1)) * K;
   // this wave's 32-deep steps of the part
-  const int steps = (K + 31) >> 5, chunks = 4 * p.parts, c = 4 * blockIdx.x + wv;
+  const int steps = (K + 31) >> 5, chunks = kw * p.parts, c = kw * blockIdx.x + ki;
   const int s0 = (int)((int64_t)steps * c / chunks), s1 = (int)((int64_t)steps * (c + 1) / chunks);
-  fv4 acc[kSub][RT];
+  fv4 acc[2][RT];
 #pragma unroll
-  for (int s = 0; s < kSub; ++s)
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int j = 0; j < RT; ++j) acc[s][j] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
-  const hv8 zero = {};
-  for (int st = s0; st < s1; ++st) {
-    const int k = 32 * st + kg;
-    const bool in = k < K;
-    hv8 fa[RT];
+  if (per == 1) shrink_steps<1, RT>(xr, ar, kg, K, s0, s1, *reinterpret_cast<fv4(*)[1][RT]>(&acc));
+  else shrink_steps<2, RT>(xr, ar, kg, K, s0, s1, acc);
+  // waves behind the first along K hand their sums over: 7 of one block, or 3 for each of up to 4 blocks
+  if (ki > 0) {
 #pragma unroll
-    for (int j = 0; j < RT; ++j) fa[j] = in ? *reinterpret_cast<const hv8*>(ar[j] + k) : zero;
+    for (int s = 0; s < 2; ++s) {
+      if (s >= per) break;
 #pragma unroll
-    for (int s = 0; s < kSub; ++s) {
-      if (s >= ns) break;
-      const hv8 fb = in ? *reinterpret_cast<const hv8*>(xr[s] + k) : zero;
-#pragma unroll
-      for (int j = 0; j < RT; ++j) acc[s][j] = mfma(fa[j], fb, acc[s][j]);
+      for (int j = 0; j < RT; ++j) lds[rw == 1 ? ki - 1 : (ki - 1) * kSub + ri * per + s][j][lane] = acc[s][j];
     }
   }
-#pragma unroll
-  for (int s = 0; s < kSub; ++s) {
-    if (s >= ns) break;
-#pragma unroll
-    for (int j = 0; j < RT; ++j) lds[wv][s][j][lane] = acc[s][j];
-  }
   __syncthreads();
+  if (ki > 0) return;
   // lane (row li, ranks 16 j + 4 (lane / 16) ..): four consecutive ranks
   float* h = p.h + ((int64_t)(blockIdx.x * p.n_targets + ti) * p.m + tile.row0) * p.rank_pad + r0;
-  for (int i = tid; i < ns * RT * 64; i += 256) {
-    const int l = i & 63, j = (i >> 6) % RT, s = (i >> 6) / RT;
-    const int r = 16 * s + (l & 15);
-    if (r >= tile.rows || r0 + 16 * j >= p.rank_pad) continue;
-    const fv4 v = ((lds[0][s][j][l] + lds[1][s][j][l]) + lds[2][s][j][l]) + lds[3][s][j][l];
-    *reinterpret_cast<fv4*>(h + (int64_t)r * p.rank_pad + 16 * j + 4 * (l >> 4)) = v;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int blk = ri * per + s, r = 16 * blk + li;
+    if (s >= per || blk >= ns) break;
+    if (r >= tile.rows) continue;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      if (r0 + 16 * j >= p.rank_pad) break;
+      fv4 v = acc[s][j];
+      if (rw == 1) {
+#pragma unroll
+        for (int k = 0; k < kShrinkWaves - 1; ++k) v += lds[k][j][lane];
+      } else {
+#pragma unroll
+        for (int k = 0; k < kShrinkWaves / 2 - 1; ++k) v += lds[k * kSub + blk][j][lane];
+      }
+      *reinterpret_cast<fv4*>(h + (int64_t)r * p.rank_pad + 16 * j + 4 * (lane >> 4)) = v;
+    }
   }
 }
 
-// Grid: x = column block over all targets, y = tile.
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
+__device__ __forceinline__ float relu2(float f) {
+  f = f > 0.0f ? f : (f != f ? f : 0.0f);
+  return f * f;
+}
+
+// Grid: x = block of p.cols columns over all targets, y = tile.  Up to 16 rows: the kW waves take 64 columns
+// each at a time; more: half of the waves for each half of the row blocks.
+template <int kW>
+__global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
   extern __shared__ char dyn[];
-  const PlanHead* head = reinterpret_cast<const PlanHead*>(p.plan);
-  if ((int)blockIdx.y >= head->n_tiles || head->m != p.m || head->G != p.G) return;
+  const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
   const Tile tile = plan_tiles(p.plan)[blockIdx.y];
+  if ((int)blockIdx.y >= head.n_tiles || head.m != p.m || head.G != p.G) return;
   const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
   int ti = 0;
   while (ti + 1 < p.n_targets && (int)blockIdx.x >= p.t[ti + 1].col_block0) ++ti;
   const Target& tg = p.t[ti];
-  const int N = tg.n, c0 = ((int)blockIdx.x - tg.col_block0) * kColBlock;
+  const int N = tg.n, c0 = ((int)blockIdx.x - tg.col_block0) * p.cols, c1 = min(c0 + p.cols, N);
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   if (tile.adapter < 0) {
     // no adapter: the epilogue alone; an index out of range: NaN
     if (tile.adapter == kNone && !tg.relu2 && tg.base == tg.y) return;
-    for (int i = tid; i < tile.rows * (kColBlock / 8); i += 256) {
-      const int c = c0 + 8 * (i % (kColBlock / 8));
-      if (c >= N) continue;
-      const int64_t at = (int64_t)order[i / (kColBlock / 8)] * N + c;
+    const int per_row = (c1 - c0) >> 3;
+    for (int i = tid; i < tile.rows * per_row; i += 64 * kW) {
+      const int r = i / per_row;
+      const int64_t at = (int64_t)order[r] * N + c0 + 8 * (i - r * per_row);
       h8 v = ld8(tg.base + at);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (tile.adapter == kBad) v.v[e] = (_Float16)__builtin_nanf("");
-        else if (tg.relu2) {
-          const float f = (float)v.v[e], z = f > 0.0f ? f : (f != f ? f : 0.0f);
-          v.v[e] = f16_of(z * z);
-        }
+        else if (tg.relu2) v.v[e] = f16_of(relu2((float)v.v[e]));
       }
       st8(tg.y + at, v);
     }
     return;
   }
-  const int ns = (tile.rows + 15) >> 4, chunks = p.rank_pad >> 4;
-  hv8* const hf = reinterpret_cast<hv8*>(dyn);                                   // [chunk][sub][lane]
-  uint32_t* const rmax = reinterpret_cast<uint32_t*>(hf + chunks * kSub * 64);   // [kTileM] largest |h| of a row
-  if (tid < kTileM) rmax[tid] = 0;
-  __syncthreads();
-  // h = scale * (sum of the parts, in order), 8 ranks of a row per item; at most 4 items a lane
+  const int ns = (tile.rows + 15) >> 4, chunks = (p.rank + 15) >> 4;
+  const int li = lane & 15, grp = lane >> 4;
+  const _Float16* const bw = tg.b + (int64_t)tile.adapter * N * p.rank;
+  const hv8 zero = {};
+  // Product row li of column tile t is output column cw + 16 (li / 4) + 4 t + li % 4, so that a lane of
+  // group grp ends up with the 16 consecutive columns cw + 16 grp ..
+  auto weights = [&](int cw, int ch, hv8 (&fa)[4]) __attribute__((always_inline)) {
+    const int rk = 16 * ch + 8 * (grp & 1);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int col = cw + 16 * (li >> 2) + 4 * t + (li & 3);
+      fa[t] = rk < p.rank && col < c1 ? *reinterpret_cast<const hv8*>(bw + (int64_t)col * p.rank + rk) : zero;
+    }
+  };
+  const int rw = ns > 1 ? 2 : 1, per = (ns + rw - 1) / rw;  // waves along the rows; row blocks per wave
+  const int ri = wv % rw, ci = wv / rw, pass = 64 * (kW / rw);
+  int64_t rows[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) rows[s] = (int64_t)order[min(16 * (ri * per + s) + li, tile.rows - 1)] * N;
+  hv8 fa[4];  // requested before h is waited for
+  weights(c0 + 64 * ci, 0, fa);
+
+  hv8* const hf = reinterpret_cast<hv8*>(dyn);                          // [chunk][sub][lane]
+  int* const back = reinterpret_cast<int*>(hf + chunks * kSub * 64);    // [kTileM] powers of two taken out of the rows
+  // h = scale * (sum of the parts, in order), 8 ranks of a row per item, at most 4 items a lane; a row's
+  // items lie in neighbouring lanes (rank_pad / 8, a power of two)
   const float sc = p.scale ? p.scale[tile.adapter] : 1.0f;
-  const int groups = p.rank_pad >> 3, items = tile.rows * groups;
-  constexpr int kItems = kTileM * (kMaxRank / 8) / 256;
-  float hv[kItems][8];
+  const int groups = p.rank_pad >> 3, gbits = 31 - __builtin_clz(groups);
   const float* h0 = p.h + ((int64_t)ti * p.m + tile.row0) * p.rank_pad;
   const int64_t plane = (int64_t)p.n_targets * p.m * p.rank_pad;
-#pragma unroll
-  for (int u = 0; u < kItems; ++u) {
-    const int i = tid + 256 * u;
-    if (i >= items) break;
-    const int r = i / groups, gr = i - r * groups;
-    const float* src = h0 + (int64_t)r * p.rank_pad + 8 * gr;
-    fv4 lo = *reinterpret_cast<const fv4*>(src), hi = *reinterpret_cast<const fv4*>(src + 4);
-    for (int q = 1; q < p.parts; ++q) {
-      lo += *reinterpret_cast<const fv4*>(src + q * plane);
-      hi += *reinterpret_cast<const fv4*>(src + q * plane + 4);
-    }
+  for (int i = tid; i - tid < 16 * ns * groups; i += 64 * kW) {
+    const int r = i >> gbits, gr = i & (groups - 1);
+    float hv[8];
     uint32_t mx = 0;
+    const bool live = r < tile.rows && 8 * gr < p.rank;  // rows behind the tile's and ranks of the padding: 0
+    {
+      const float* src = h0 + (int64_t)min(r, tile.rows - 1) * p.rank_pad + 8 * gr;
+      fv4 lo = *reinterpret_cast<const fv4*>(src), hi = *reinterpret_cast<const fv4*>(src + 4);
+      for (int q = 1; q < p.parts; ++q) {
+        lo += *reinterpret_cast<const fv4*>(src + q * plane);
+        hi += *reinterpret_cast<const fv4*>(src + q * plane + 4);
+      }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      hv[u][e] = 8 * gr < p.rank ? (e < 4 ? lo[e & 3] : hi[e & 3]) * sc : 0.0f;  // ranks of the padding: 0
-      mx = max(mx, __builtin_bit_cast(uint32_t, hv[u][e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; ++e) {
+        hv[e] = live ? (e < 4 ? lo[e & 3] : hi[e & 3]) * sc : 0.0f;
+        mx = max(mx, __builtin_bit_cast(uint32_t, hv[e]) & 0x7fffffffu);
+      }
     }
-    atomicMax(&rmax[r], mx);  // a maximum does not depend on the order
-  }
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kItems; ++u) {
-    const int i = tid + 256 * u;
-    if (i >= items) break;
-    const int r = i / groups, gr = i - r * groups;
-    const int ex = (int)(rmax[r] >> 23);                  // biased exponent of the row's largest value
-    const int sh = ex == 0 || ex == 255 ? 0 : 127 - ex;   // zeros (and denormals), infinities, NaN: as they are
+    for (int d = 1; d < groups; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d, 64));
+    const int ex = (int)(mx >> 23);                      // biased exponent of the row's largest value
+    const int sh = ex == 0 || ex == 255 ? 0 : 127 - ex;  // zeros (and denormals), infinities, NaN: as they are
+    if (r < kTileM && gr == 0) back[r] = -sh;
     hv8 vh, vl;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float f = __builtin_ldexpf(hv[u][e], sh);
+      const float f = __builtin_ldexpf(hv[e], sh);
       vh[e] = (_Float16)f;
       // an infinity has no second half
       vl[e] = __builtin_isinf((float)vh[e]) ? (_Float16)0.0f : (_Float16)(f - (float)vh[e]);
     }
     // k groups 0, 1 of the product: ranks 0-7, 8-15 of the chunk's first half; 2, 3: second half
-    hv8* d = hf + ((gr >> 1) * kSub + (r >> 4)) * 64 + (r & 15);
-    d[16 * (gr & 1)] = vh;
-    d[16 * (2 + (gr & 1))] = vl;
+    if (r < kTileM && (gr >> 1) < chunks) {
+      hv8* d = hf + ((gr >> 1) * kSub + (r >> 4)) * 64 + (r & 15);
+      d[16 * (gr & 1)] = vh;
+      d[16 * (2 + (gr & 1))] = vl;
+    }
   }
   __syncthreads();
-  const int cw = c0 + 64 * wv;
-  if (cw >= N) return;
-  const int li = lane & 15, grp = lane >> 4;
-  // product row li of column tile t is output column cw + 16 (li / 4) + 4 t + li % 4, so that a lane
-  // of group grp ends up with the 16 consecutive columns cw + 16 grp ..
-  fv4 acc[kSub][4];
+  for (int cw = c0 + 64 * ci; cw < c1; cw += pass) {
+    const bool in0 = cw + 16 * grp < c1, in1 = cw + 16 * grp + 8 < c1;
+    fv4 acc[2][4];
+    h8 base[2][2];
 #pragma unroll
-  for (int s = 0; s < kSub; ++s)
+    for (int s = 0; s < 2; ++s) {
+      if (s >= per) break;
+      const int64_t at = rows[s] + cw + 16 * grp;
+      if (in0) base[s][0] = ld8(tg.base + at);
+      if (in1) base[s][1] = ld8(tg.base + at + 8);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[s][t] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
-  const hv8 zero = {};
-  for (int ch = 0; ch < chunks; ++ch) {
-    const int rk = 16 * ch + 8 * (grp & 1);
-    hv8 fa[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int col = cw + 16 * (li >> 2) + 4 * t + (li & 3);
-      fa[t] = rk < p.rank && col < N
-                  ? *reinterpret_cast<const hv8*>(tg.b + ((int64_t)tile.adapter * N + col) * p.rank + rk)
-                  : zero;
+      for (int t = 0; t < 4; ++t) acc[s][t] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    for (int ch = 0; ch < chunks; ++ch) {
+      hv8 next[4];
+      const bool last = ch + 1 == chunks;
+      if (!last || cw + pass < c1) weights(last ? cw + pass : cw, last ? 0 : ch + 1, next);
 #pragma unroll
-    for (int s = 0; s < kSub; ++s) {
-      if (s >= ns) break;
-      const hv8 fb = hf[(ch * kSub + s) * 64 + lane];
+      for (int s = 0; s < 2; ++s) {
+        if (s >= per) break;
+        const hv8 fb = hf[(ch * kSub + min(ri * per + s, kSub - 1)) * 64 + lane];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], fb, acc[s][t]);
-    }
-  }
-#pragma unroll
-  for (int s = 0; s < kSub; ++s) {
-    if (s >= ns) break;
-    const int r = 16 * s + li;
-    if (r >= tile.rows) continue;
-    const int ex = (int)(rmax[r] >> 23);
-    const int back = ex == 0 || ex == 255 ? 0 : ex - 127;
-    const int64_t at = (int64_t)order[r] * N + cw + 16 * grp;
-#pragma unroll
-    for (int hf2 = 0; hf2 < 2; ++hf2) {
-      if (cw + 16 * grp + 8 * hf2 >= N) continue;
-      h8 v = ld8(tg.base + at + 8 * hf2);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float f = (float)v.v[e] + __builtin_ldexpf(acc[s][2 * hf2 + (e >> 2)][e & 3], back);
-        if (tg.relu2) {
-          f = f > 0.0f ? f : (f != f ? f : 0.0f);
-          f = f * f;
-        }
-        v.v[e] = f16_of(f);
+        for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], fb, acc[s][t]);
       }
-      st8(tg.y + at + 8 * hf2, v);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) fa[t] = next[t];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s >= per) break;
+      const int r = 16 * (ri * per + s) + li;
+      if (r >= tile.rows) continue;
+      const int bk = back[r];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (!(q ? in1 : in0)) continue;
+        h8 v = base[s][q];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = (float)v.v[e] + __builtin_ldexpf(acc[s][2 * q + (e >> 2)][e & 3], bk);
+          v.v[e] = f16_of(tg.relu2 ? relu2(f) : f);
+        }
+        st8(tg.y + rows[s] + cw + 16 * grp + 8 * q, v);
+      }
     }
   }
 }
 
 struct LoraPlan {
-  int parts, rank_pad, rank_blocks;
+  int parts, rank_pad, rank_blocks, cols;
   int64_t bytes;
 };
 
-// K parts: enough workgroups for the chip where the rows make few tiles, each wave's share of a part
-// at least 64 deep.
-LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min) {
+// K parts of the first product: enough workgroups for the chip, at least 256 deep each.  Columns of the
+// second product per workgroup: 256 (four waves), or where that leaves enough workgroups 512 and 1024
+// (eight waves; each workgroup adds h's parts up anew).  The number of tiles is known on the device only;
+// the rows of a step that has them scattered make one per adapter.
+LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min, int64_t n_max) {
   LoraPlan s{};
-  s.rank_pad = (rank + 15) / 16 * 16;
+  s.rank_pad = 16;
+  while (s.rank_pad < rank) s.rank_pad *= 2;
   s.rank_blocks = (rank + kRankBlock - 1) / kRankBlock;
-  const int64_t tiles = (m < G ? m : G) + m / kTileM;
+  const int64_t tiles = std::min<int64_t>(m, G) + m / kTileM;
   int64_t parts = 1;
-  while (parts < 8 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 256) parts *= 2;
+  while (parts < 4 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 256) parts *= 2;
   s.parts = (int)parts;
+  s.cols = kColBlock;
+  while (s.cols < 4 * kColBlock && tiles * n_targets * (n_max / (2 * s.cols)) >= 1024) s.cols *= 2;
   s.bytes = parts * n_targets * m * s.rank_pad * 4;
   return s;
 }
@@ -399,6 +462,12 @@ int64_t least_k(int n_targets, const vkwr_lora_target* t) {
   int64_t k = t[0].k;
   for (int i = 1; i < n_targets; ++i) k = t[i].k < k ? t[i].k : k;
   return k;
+}
+
+int64_t most_n(int n_targets, const vkwr_lora_target* t) {
+  int64_t n = t[0].n;
+  for (int i = 1; i < n_targets; ++i) n = std::max(n, t[i].n);
+  return n;
 }
 
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -434,11 +503,11 @@ extern "C" int64_t vkwr_lora_workspace_bytes(int64_t m, int n_adapters, int rank
                                              const vkwr_lora_target* targets) {
   clear_error();
   if (check_lora("vkwr_lora_workspace_bytes", m, n_adapters, rank, n_targets, targets)) return -1;
-  const int64_t k = least_k(n_targets, targets);
-  int64_t most = lora_split(m, n_adapters, rank, n_targets, k).bytes;
+  const int64_t k = least_k(n_targets, targets), n = most_n(n_targets, targets);
+  int64_t most = lora_split(m, n_adapters, rank, n_targets, k, n).bytes;
   // fewer rows can be cut into more parts; from 512 row tiles on there is one part
   for (int64_t r = 1; r < m && r < 512 * kTileM; ++r)
-    most = std::max(most, lora_split(r, n_adapters, rank, n_targets, k).bytes);
+    most = std::max(most, lora_split(r, n_adapters, rank, n_targets, k, n).bytes);
   return most;
 }
 
@@ -449,7 +518,8 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
   const char* fn = "vkwr_lora_f16";
   if (int e = check_lora(fn, m, n_adapters, rank, n_targets, targets)) return e;
   if (m == 0) return VKWR_OK;
-  const LoraPlan sp = lora_split(m, n_adapters, rank, n_targets, least_k(n_targets, targets));
+  const LoraPlan sp =
+      lora_split(m, n_adapters, rank, n_targets, least_k(n_targets, targets), most_n(n_targets, targets));
   VK_REQUIRE(plan && (uintptr_t)plan % 16 == 0, "%s: null or misaligned plan", fn);
   VK_REQUIRE(workspace && workspace_bytes >= sp.bytes && (uintptr_t)workspace % 16 == 0,
              "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn, (long long)sp.bytes,
@@ -466,6 +536,7 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
   a.n_targets = n_targets;
   a.parts = sp.parts;
   a.rank_blocks = sp.rank_blocks;
+  a.cols = sp.cols;
   int cols = 0;
   for (int i = 0; i < n_targets; ++i) {
     const vkwr_lora_target& t = targets[i];
@@ -485,16 +556,18 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
                     reinterpret_cast<const _Float16*>(t.b), reinterpret_cast<const _Float16*>(base),
                     reinterpret_cast<_Float16*>(t.y), (int)t.n, (int)t.k,
                     t.epilogue == VKWR_GEMM_EPI_RELU_SQUARE, cols};
-    cols += (int)((t.n + kColBlock - 1) / kColBlock);
+    cols += (int)((t.n + sp.cols - 1) / sp.cols);
   }
   VK_REQUIRE(a.tiles_cap <= 65535, "%s: %lld row tiles, at most 65535", fn, (long long)a.tiles_cap);
   const hipStream_t s = (hipStream_t)stream;
   const dim3 grid(sp.parts, (unsigned)a.tiles_cap, n_targets * sp.rank_blocks);
-  const int rt = (rank < kRankBlock ? sp.rank_pad : kRankBlock) / 16;
-  if (rt == 1) hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(256), 0, s, a);
-  else if (rt == 2) hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(256), 0, s, a);
-  hipLaunchKernelGGL(lora_expand_kernel, dim3(cols, (unsigned)a.tiles_cap), dim3(256),
-                     sp.rank_pad / 16 * kSub * 1024 + kTileM * 4, s, a);
+  const int rt = std::min(sp.rank_pad, kRankBlock) / 16;
+  if (rt == 1) hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(64 * kShrinkWaves), 0, s, a);
+  else if (rt == 2) hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(64 * kShrinkWaves), 0, s, a);
+  else hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(64 * kShrinkWaves), 0, s, a);
+  const dim3 egrid(cols, (unsigned)a.tiles_cap);
+  const int lds = (rank + 15) / 16 * kSub * 1024 + kTileM * 4;
+  if (sp.cols == kColBlock) hipLaunchKernelGGL(lora_expand_kernel<4>, egrid, dim3(256), lds, s, a);
+  else hipLaunchKernelGGL(lora_expand_kernel<8>, egrid, dim3(512), lds, s, a);
   return check_launch(fn);
 }
