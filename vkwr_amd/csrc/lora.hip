@@ -12,9 +12,8 @@
 //   expand  the parts added in order, y = epi(base + scale h B^T)
 // Both run on the matrix cores with 16 rows of x (or h) as the columns of v_mfma_f32_16x16x32_f16,
 // the adapter's rows as its rows.  h is not rounded to fp16: it enters the second product as a sum
-// of two halves (fp16(h) and fp16(h - fp16(h)), 22 bits), 16 ranks filling the 32-deep product, after
-// a power of two per row has brought its largest value to [1, 2) so that neither half leaves
-// fp16's range.
+// of two halves (fp16(h) and fp16(h - fp16(h)), 22 bits), a product each, after a power of two per row
+// has brought its largest value to [1, 2) so that neither half leaves fp16's range.
 
 #include <algorithm>
 
@@ -168,38 +167,67 @@ __device__ __forceinline__ fv4 mfma(hv8 a, hv8 b, fv4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// x A^T of NS blocks of 16 rows over the 32-deep steps s0 .. s1 - 1, two steps' loads together.
-template <int NS, int RT>
-__device__ __forceinline__ void shrink_steps(const _Float16* const* xr, const _Float16* const* ar, int kg, int K, int s0,
-                                             int s1, fv4 (&acc)[NS][RT]) {
+// x A^T of 16 rows over the 32-deep steps s0 .. s1 - 1: two steps' loads together, up to 32 ranks
+// requested while the two before are multiplied.
+template <int RT>
+__device__ __forceinline__ void shrink_steps(const _Float16* xr, const _Float16* const* ar, int kg, int K, int s0, int s1,
+                                             fv4 (&acc)[RT]) {
   const hv8 zero = {};
-  for (int st = s0; st < s1; st += 2) {
-    hv8 fa[2][RT], fb[2][NS];
+  struct Pair {
+    hv8 a[2][RT], b[2];
+  };
+  auto load = [&](Pair& f, int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int k = 32 * (st + u) + kg;
       const bool in = st + u < s1 && k < K;
+      f.b[u] = in ? *reinterpret_cast<const hv8*>(xr + k) : zero;
 #pragma unroll
-      for (int j = 0; j < RT; ++j) fa[u][j] = in ? *reinterpret_cast<const hv8*>(ar[j] + k) : zero;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) fb[u][s] = in ? *reinterpret_cast<const hv8*>(xr[s] + k) : zero;
+      for (int j = 0; j < RT; ++j) f.a[u][j] = in ? *reinterpret_cast<const hv8*>(ar[j] + k) : zero;
     }
+  };
+  auto multiply = [&](const Pair& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int j = 0; j < RT; ++j) acc[s][j] = mfma(fa[u][j], fb[u][s], acc[s][j]);
+      for (int j = 0; j < RT; ++j) acc[j] = mfma(f.a[u][j], f.b[u], acc[j]);
+  };
+  Pair p;
+  if constexpr (RT > 2) {  // no registers for two pairs
+    for (int st = s0; st < s1; st += 2) {
+      load(p, st);
+      multiply(p);
+    }
+    return;
+  }
+  Pair q;
+  load(p, s0);
+  for (int st = s0; st < s1; st += 4) {
+    if (st + 2 < s1) load(q, st + 2);
+    multiply(p);
+    if (st + 2 >= s1) break;
+    if (st + 4 < s1) load(p, st + 4);
+    multiply(q);
   }
 }
 
-// Grid: x = part, y = tile, z = target * rank_blocks + rank block.  Up to 16 rows: the eight waves cut the
-// part's K between them; more: four of them, each for half of the row blocks.  The waves' sums are added
-// in K order through LDS.
+// Grid: x = part, y = tile, z = target * rank_blocks + rank block.  A wave takes one block of 16 rows; the
+// eight waves cut the part's K in 8 for one block, in 4 for two, in 2 for three or four.  The waves' sums
+// are added in K order through LDS.
+//
+// Tiles of three or four blocks (prompt chunks) go through LDS: the 16 rows of an operand, 2 K bytes apart,
+// fall on the same sets of the vector cache, so that operands loaded straight into registers, 64 bytes of
+// a row at a time, came in twice (four projections of 2304 rows, K = 4096, rank 64: 107 us; through LDS
+// {STAGED_US}).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
+// chunk c at place c ^ (r & 7) -- in a ring of four, three of them in flight.
 constexpr int kShrinkWaves = 8;
+constexpr int kStageK = 64, kStages = 4;
+constexpr int kStageHalfs = 2 * kTileM * kStageK;
 template <int RT>
-__global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs p) {
-  __shared__ fv4 lds[3 * kSub][RT][64];
+__global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[kStages * kStageHalfs * 2];  // the ring, then the waves' sums
+  fv4(*const lds)[RT][64] = reinterpret_cast<fv4(*)[RT][64]>(smem);
+  static_assert((kShrinkWaves - 1) * kRankBlock / 16 * 1024 <= kStages * kStageHalfs * 2, "the sums fit");
   const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
   const Tile tile = plan_tiles(p.plan)[blockIdx.y];  // blockIdx.y < tiles_cap: in the buffer, if stale
   if ((int)blockIdx.y >= head.n_adapter || head.m != p.m || head.G != p.G) return;
@@ -209,58 +237,75 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int K = tg.k, ns = (tile.rows + 15) >> 4;
   const int li = lane & 15, kg = 8 * (lane >> 4);
-  // waves along the rows and along K; row blocks per wave
-  const int rw = ns > 1 ? 2 : 1, kw = kShrinkWaves / rw, per = (ns + rw - 1) / rw;
-  const int ri = wv % rw, ki = wv / rw;
-  const _Float16* xr[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-    xr[s] = tg.x + (int64_t)order[min(16 * min(ri * per + s, ns - 1) + li, tile.rows - 1)] * K;
+  const int rbits = ns == 1 ? 0 : ns == 2 ? 1 : 2;  // 2^rbits waves along the rows
+  const int ri = wv & ((1 << rbits) - 1), ki = wv >> rbits;
+  const int r = 16 * ri + li;
+  const _Float16* xr = tg.x + (int64_t)order[min(r, tile.rows - 1)] * K;
   const _Float16* ar[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j)
     ar[j] = tg.a + ((int64_t)tile.adapter * p.rank + min(r0 + 16 * j + li, p.rank - 1)) * K;
   // this wave's 32-deep steps of the part
-  const int steps = (K + 31) >> 5, chunks = kw * p.parts, c = kw * blockIdx.x + ki;
+  const int steps = (K + 31) >> 5, chunks = (kShrinkWaves >> rbits) * p.parts;
+  const int c = (kShrinkWaves >> rbits) * blockIdx.x + ki;
   const int s0 = (int)((int64_t)steps * c / chunks), s1 = (int)((int64_t)steps * (c + 1) / chunks);
-  fv4 acc[2][RT];
+  fv4 acc[RT];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int j = 0; j < RT; ++j) acc[j] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (rbits < 2) {
+    if (ri < ns) shrink_steps<RT>(xr, ar, kg, K, s0, s1, acc);
+  } else {
+    const int blocks = (K + kStageK - 1) / kStageK;
+    const int b0 = (int)((int64_t)blocks * blockIdx.x / p.parts), b1 = (int)((int64_t)blocks * (blockIdx.x + 1) / p.parts);
+    // DMA instruction: 8 rows; wave w fills rows 8 w .. of x and rows 8 (w mod 2 RT) .. of A
+    _Float16* const ring = reinterpret_cast<_Float16*>(smem);
+    const int w = __builtin_amdgcn_readfirstlane(wv), aw = w % (2 * RT);
+    const int xrow = 8 * w + (lane >> 3), arow = 8 * aw + (lane >> 3);
+    const _Float16* const xs = tg.x + (int64_t)order[min(xrow, tile.rows - 1)] * K;
+    const _Float16* const as = tg.a + ((int64_t)tile.adapter * p.rank + min(r0 + arow, p.rank - 1)) * K;
+    const int xc = 8 * ((lane & 7) ^ (xrow & 7)), ac = 8 * ((lane & 7) ^ (arow & 7));
+    auto issue = [&](int blk) __attribute__((always_inline)) {
+      _Float16* const to = ring + ((blk - b0) % kStages) * kStageHalfs;
+      // chunks past the end of K: the row's last one, made zero when they are read
+      dma16(xs + min(blk * kStageK + xc, K - 8), to + w * 512);
+      dma16(as + min(blk * kStageK + ac, K - 8), to + kTileM * kStageK + aw * 512);
+    };
+    for (int b = b0; b < min(b0 + kStages - 1, b1); ++b) issue(b);
+    const int cc = 4 * ki + (lane >> 4);  // this lane's chunk: wave half ki multiplies 32 of the 64 k
+    for (int b = b0; b < b1; ++b) {
+      // stage b has landed once at most the two stages behind it are outstanding (two DMA each); the
+      // barrier also ends the reads of the buffer that is filled next
+      if (b + 2 < b1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else if (b + 1 < b1) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (b + kStages - 1 < b1) issue(b + kStages - 1);
+      const _Float16* const st = ring + ((b - b0) % kStages) * kStageHalfs;
+      const hv8 zero = {};
+      const bool in = b * kStageK + 8 * cc < K;
+      hv8 fb = *reinterpret_cast<const hv8*>(st + r * kStageK + 8 * (cc ^ (r & 7)));
+      fb = in ? fb : zero;
 #pragma unroll
-    for (int j = 0; j < RT; ++j) acc[s][j] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (per == 1) shrink_steps<1, RT>(xr, ar, kg, K, s0, s1, *reinterpret_cast<fv4(*)[1][RT]>(&acc));
-  else shrink_steps<2, RT>(xr, ar, kg, K, s0, s1, acc);
-  // waves behind the first along K hand their sums over: 7 of one block, or 3 for each of up to 4 blocks
+      for (int j = 0; j < RT; ++j) {
+        const int row = 16 * j + li;
+        const hv8 fa = *reinterpret_cast<const hv8*>(st + (kTileM + row) * kStageK + 8 * (cc ^ (row & 7)));
+        acc[j] = mfma(in ? fa : zero, fb, acc[j]);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the ring is read
+  }
   if (ki > 0) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s >= per) break;
-#pragma unroll
-      for (int j = 0; j < RT; ++j) lds[rw == 1 ? ki - 1 : (ki - 1) * kSub + ri * per + s][j][lane] = acc[s][j];
-    }
+    for (int j = 0; j < RT; ++j) lds[((ki - 1) << rbits) + ri][j][lane] = acc[j];
   }
   __syncthreads();
-  if (ki > 0) return;
+  if (ki > 0 || r >= tile.rows) return;
   // lane (row li, ranks 16 j + 4 (lane / 16) ..): four consecutive ranks
   float* h = p.h + ((int64_t)(blockIdx.x * p.n_targets + ti) * p.m + tile.row0) * p.rank_pad + r0;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int blk = ri * per + s, r = 16 * blk + li;
-    if (s >= per || blk >= ns) break;
-    if (r >= tile.rows) continue;
-#pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      if (r0 + 16 * j >= p.rank_pad) break;
-      fv4 v = acc[s][j];
-      if (rw == 1) {
-#pragma unroll
-        for (int k = 0; k < kShrinkWaves - 1; ++k) v += lds[k][j][lane];
-      } else {
-#pragma unroll
-        for (int k = 0; k < kShrinkWaves / 2 - 1; ++k) v += lds[k * kSub + blk][j][lane];
-      }
-      *reinterpret_cast<fv4*>(h + (int64_t)r * p.rank_pad + 16 * j + 4 * (lane >> 4)) = v;
-    }
+  for (int j = 0; j < RT; ++j) {
+    if (r0 + 16 * j >= p.rank_pad) break;
+    for (int k = 0; k < (kShrinkWaves >> rbits) - 1; ++k) acc[j] += lds[(k << rbits) + ri][j][lane];
+    *reinterpret_cast<fv4*>(h + (int64_t)r * p.rank_pad + 16 * j + 4 * (lane >> 4)) = acc[j];
   }
 }
 
@@ -300,17 +345,18 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
     }
     return;
   }
-  const int ns = (tile.rows + 15) >> 4, chunks = (p.rank + 15) >> 4;
+  const int ns = (tile.rows + 15) >> 4, chunks = (p.rank + 31) >> 5;
   const int li = lane & 15, grp = lane >> 4;
   const _Float16* const bw = tg.b + (int64_t)tile.adapter * N * p.rank;
   const hv8 zero = {};
-  // Product row li of column tile t is output column cw + 16 (li / 4) + 4 t + li % 4, so that a lane of
-  // group grp ends up with the 16 consecutive columns cw + 16 grp ..
+  // Product row li of column tile t is output column cw + 32 (t / 2) + 8 (li / 4) + 4 (t % 2) + li % 4, so that
+  // a lane of group grp ends up with the columns cw + 32 q + 8 grp .. + 7 (q = 0, 1): four lanes cover 64
+  // consecutive bytes of a row.
   auto weights = [&](int cw, int ch, hv8 (&fa)[4]) __attribute__((always_inline)) {
-    const int rk = 16 * ch + 8 * (grp & 1);
+    const int rk = 32 * ch + 8 * grp;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int col = cw + 16 * (li >> 2) + 4 * t + (li & 3);
+      const int col = cw + 32 * (t >> 1) + 8 * (li >> 2) + 4 * (t & 1) + (li & 3);
       fa[t] = rk < p.rank && col < c1 ? *reinterpret_cast<const hv8*>(bw + (int64_t)col * p.rank + rk) : zero;
     }
   };
@@ -322,8 +368,8 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
   hv8 fa[4];  // requested before h is waited for
   weights(c0 + 64 * ci, 0, fa);
 
-  hv8* const hf = reinterpret_cast<hv8*>(dyn);                          // [chunk][sub][lane]
-  int* const back = reinterpret_cast<int*>(hf + chunks * kSub * 64);    // [kTileM] powers of two taken out of the rows
+  hv8* const hf = reinterpret_cast<hv8*>(dyn);                          // [chunk][sub][half][lane]
+  int* const back = reinterpret_cast<int*>(hf + chunks * kSub * 128);    // [kTileM] powers of two taken out of the rows
   // h = scale * (sum of the parts, in order), 8 ranks of a row per item, at most 4 items a lane; a row's
   // items lie in neighbouring lanes (rank_pad / 8, a power of two)
   const float sc = p.scale ? p.scale[tile.adapter] : 1.0f;
@@ -360,24 +406,23 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
       // an infinity has no second half
       vl[e] = __builtin_isinf((float)vh[e]) ? (_Float16)0.0f : (_Float16)(f - (float)vh[e]);
     }
-    // k groups 0, 1 of the product: ranks 0-7, 8-15 of the chunk's first half; 2, 3: second half
-    if (r < kTileM && (gr >> 1) < chunks) {
-      hv8* d = hf + ((gr >> 1) * kSub + (r >> 4)) * 64 + (r & 15);
-      d[16 * (gr & 1)] = vh;
-      d[16 * (2 + (gr & 1))] = vl;
+    if (r < kTileM && (gr >> 2) < chunks) {
+      hv8* d = hf + ((gr >> 2) * kSub + (r >> 4)) * 128 + 16 * (gr & 3) + (r & 15);
+      d[0] = vh;
+      d[64] = vl;
     }
   }
   __syncthreads();
   for (int cw = c0 + 64 * ci; cw < c1; cw += pass) {
-    const bool in0 = cw + 16 * grp < c1, in1 = cw + 16 * grp + 8 < c1;
+    const bool in0 = cw + 8 * grp < c1, in1 = cw + 8 * grp + 32 < c1;
     fv4 acc[2][4];
     h8 base[2][2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (s >= per) break;
-      const int64_t at = rows[s] + cw + 16 * grp;
+      const int64_t at = rows[s] + cw + 8 * grp;
       if (in0) base[s][0] = ld8(tg.base + at);
-      if (in1) base[s][1] = ld8(tg.base + at + 8);
+      if (in1) base[s][1] = ld8(tg.base + at + 32);
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[s][t] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -388,9 +433,12 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s >= per) break;
-        const hv8 fb = hf[(ch * kSub + min(ri * per + s, kSub - 1)) * 64 + lane];
+        const hv8* fb = hf + (ch * kSub + min(ri * per + s, kSub - 1)) * 128 + lane;
+        const hv8 hi = fb[0], lo = fb[64];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], fb, acc[s][t]);
+        for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], hi, acc[s][t]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], lo, acc[s][t]);
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) fa[t] = next[t];
@@ -410,7 +458,7 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
           const float f = (float)v.v[e] + __builtin_ldexpf(acc[s][2 * q + (e >> 2)][e & 3], bk);
           v.v[e] = f16_of(tg.relu2 ? relu2(f) : f);
         }
-        st8(tg.y + rows[s] + cw + 16 * grp + 8 * q, v);
+        st8(tg.y + rows[s] + cw + 8 * grp + 32 * q, v);
       }
     }
   }
@@ -427,7 +475,7 @@ struct LoraPlan {
 // the rows of a step that has them scattered make one per adapter.
 LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min, int64_t n_max) {
   LoraPlan s{};
-  s.rank_pad = 16;
+  s.rank_pad = 32;  // a power of two, so that a row's groups of 8 lie in neighbouring lanes
   while (s.rank_pad < rank) s.rank_pad *= 2;
   s.rank_blocks = (rank + kRankBlock - 1) / kRankBlock;
   const int64_t tiles = std::min<int64_t>(m, G) + m / kTileM;
@@ -561,12 +609,12 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
   VK_REQUIRE(a.tiles_cap <= 65535, "%s: %lld row tiles, at most 65535", fn, (long long)a.tiles_cap);
   const hipStream_t s = (hipStream_t)stream;
   const dim3 grid(sp.parts, (unsigned)a.tiles_cap, n_targets * sp.rank_blocks);
-  const int rt = std::min(sp.rank_pad, kRankBlock) / 16;
+  const int rt = (std::min(rank, kRankBlock) + 15) / 16;
   if (rt == 1) hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(64 * kShrinkWaves), 0, s, a);
   else if (rt == 2) hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(64 * kShrinkWaves), 0, s, a);
   else hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(64 * kShrinkWaves), 0, s, a);
   const dim3 egrid(cols, (unsigned)a.tiles_cap);
-  const int lds = (rank + 15) / 16 * kSub * 1024 + kTileM * 4;
+  const int lds = (rank + 31) / 32 * kSub * 2048 + kTileM * 4;
   if (sp.cols == kColBlock) hipLaunchKernelGGL(lora_expand_kernel<4>, egrid, dim3(256), lds, s, a);
   else hipLaunchKernelGGL(lora_expand_kernel<8>, egrid, dim3(512), lds, s, a);
   return check_launch(fn);
