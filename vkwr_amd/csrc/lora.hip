@@ -365,8 +365,20 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
   int64_t rows[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) rows[s] = (int64_t)order[min(16 * (ri * per + s) + li, tile.rows - 1)] * N;
-  hv8 fa[4];  // requested before h is waited for
+  // requested before h is waited for: the first pass's weights and base
+  hv8 fa[4];
+  h8 base[2][2];
+  auto load_base = [&](int cw) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s >= per) break;
+      const int64_t at = rows[s] + cw + 8 * grp;
+      if (cw + 8 * grp < c1) base[s][0] = ld8(tg.base + at);
+      if (cw + 8 * grp + 32 < c1) base[s][1] = ld8(tg.base + at + 32);
+    }
+  };
   weights(c0 + 64 * ci, 0, fa);
+  load_base(c0 + 64 * ci);
 
   hv8* const hf = reinterpret_cast<hv8*>(dyn);                          // [chunk][sub][half][lane]
   int* const back = reinterpret_cast<int*>(hf + chunks * kSub * 128);    // [kTileM] powers of two taken out of the rows
@@ -383,10 +395,23 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
     const bool live = r < tile.rows && 8 * gr < p.rank;  // rows behind the tile's and ranks of the padding: 0
     {
       const float* src = h0 + (int64_t)min(r, tile.rows - 1) * p.rank_pad + 8 * gr;
-      fv4 lo = *reinterpret_cast<const fv4*>(src), hi = *reinterpret_cast<const fv4*>(src + 4);
-      for (int q = 1; q < p.parts; ++q) {
-        lo += *reinterpret_cast<const fv4*>(src + q * plane);
-        hi += *reinterpret_cast<const fv4*>(src + q * plane + 4);
+      fv4 lo = fv4{0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+      if (live) {
+        for (int q0 = 0; q0 < p.parts; q0 += 4) {  // four parts' loads together
+          fv4 x[4], y[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float* at = src + min(q0 + q, p.parts - 1) * plane;
+            x[q] = *reinterpret_cast<const fv4*>(at);
+            y[q] = *reinterpret_cast<const fv4*>(at + 4);
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (q0 + q >= p.parts) break;
+            lo += x[q];
+            hi += y[q];
+          }
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -416,16 +441,11 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
   for (int cw = c0 + 64 * ci; cw < c1; cw += pass) {
     const bool in0 = cw + 8 * grp < c1, in1 = cw + 8 * grp + 32 < c1;
     fv4 acc[2][4];
-    h8 base[2][2];
+    if (cw != c0 + 64 * ci) load_base(cw);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s >= per) break;
-      const int64_t at = rows[s] + cw + 8 * grp;
-      if (in0) base[s][0] = ld8(tg.base + at);
-      if (in1) base[s][1] = ld8(tg.base + at + 32);
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[s][t] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
     for (int ch = 0; ch < chunks; ++ch) {
       hv8 next[4];
       const bool last = ch + 1 == chunks;
@@ -469,7 +489,9 @@ struct LoraPlan {
   int64_t bytes;
 };
 
-// K parts of the first product: enough workgroups for the chip, at least 256 deep each.  Columns of the
+// K parts of the first product: enough workgroups for the chip, at least 512 deep each (128 rows, 40
+// adapters, rank 32, K = 2048, N = 8192: 18.4 us with 4 parts, 20.5 with 8, which the second product has to
+// add; 434 rows of K = 8192: 23.2 with 4, 21.2 with 8).  Columns of the
 // second product per workgroup: 256 (four waves), or where that leaves enough workgroups 512 and 1024
 // (eight waves; each workgroup adds h's parts up anew).  The number of tiles is known on the device only;
 // the rows of a step that has them scattered make one per adapter.
@@ -480,7 +502,7 @@ LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min, in
   s.rank_blocks = (rank + kRankBlock - 1) / kRankBlock;
   const int64_t tiles = std::min<int64_t>(m, G) + m / kTileM;
   int64_t parts = 1;
-  while (parts < 4 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 256) parts *= 2;
+  while (parts < 8 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 512) parts *= 2;
   s.parts = (int)parts;
   s.cols = kColBlock;
   while (s.cols < 4 * kColBlock && tiles * n_targets * (n_max / (2 * s.cols)) >= 1024) s.cols *= 2;
