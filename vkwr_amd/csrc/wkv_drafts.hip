@@ -18,8 +18,9 @@
 // FMA chains and a butterfly over the eight lanes of the row -- the order of the row-split prefill
 // and decode kernels, so a draft's y and state are their bits whatever the split.
 //
-// Token vectors are staged in LDS as fp32 (the decay computed once per token and channel) in chunks
-// of kDraftTC tokens, the kept and the new tokens as one sequence.
+// Token vectors are staged in LDS as fp32 in chunks of kDraftTC tokens, the kept and the new tokens as one
+// sequence; the decay is computed once per token and channel, with a channel on every lane (as one of six
+// vectors in 16-byte pieces, a sixth of each wave's lanes computed eight of them while the others waited).
 
 #include "vk_capi.h"
 #include "vk_common.cuh"
@@ -49,7 +50,10 @@ __device__ __forceinline__ float row_sum8(float x) {
   return x;
 }
 
-// kRPL state rows per lane: 8 / kRPL waves per (sequence, head).
+// kRPL state rows per lane: 8 / kRPL waves per (sequence, head).  Few chains (up to two per CU) are bound by
+// the latency of one and take kRPL = 1 (one sequence of 32 heads, 5 + 5 tokens: 6.3 us against 9.0 with 2),
+// the others 2 (128 sequences of 64 heads: 72 us; 84 with 1, 80 with 4, 114 with 8, whose single wave has
+// nothing beside it to cover its loads).
 template <int kRPL>
 __global__ __launch_bounds__(64 * (8 / kRPL)) void wkv7_fp32_drafts_kernel(DraftArgs p) {
   constexpr int kThreads = 64 * (8 / kRPL);
@@ -96,26 +100,38 @@ __global__ __launch_bounds__(64 * (8 / kRPL)) void wkv7_fp32_drafts_kernel(Draft
   for (int c0 = 0; c0 < total; c0 += kDraftTC) {
     const int n = min(kDraftTC, total - c0);
     if (c0 > 0) __syncthreads();  // the chunk before is read
-    for (int piece = tid; piece < n * kDraftVecs * 8; piece += kThreads) {
-      const int part = piece & 7, tv = piece >> 3;
-      const int tt = tv / kDraftVecs, vec = tv - tt * kDraftVecs;
-      const int t = c0 + tt;
-      const _Float16* src;
-      if (t < nk) {
-        if (vec == 0) continue;  // kept tokens need no r
-        src = (vec == 1 ? p.pend[0] : vec == 2 ? p.pend[1] : vec == 3 ? p.pend[2] : vec == 4 ? p.pend[3] : p.pend[4]) +
-              pend0 + (size_t)t * p.C;
-      } else {
-        src = (vec == 0 ? p.r : vec == 1 ? p.w : vec == 2 ? p.k : vec == 3 ? p.v : vec == 4 ? p.a : p.b) + ytok +
-              (size_t)(t - nk) * p.C;
-      }
-      const hv8 x = *reinterpret_cast<const hv8*>(src + part * 8);
-      float f[8];
+    // r, k, v, a, b in pieces of 8 channels, w channel by channel: all loads, then all stores
+    constexpr int kPieces = (kDraftTC * 40 + kThreads - 1) / kThreads, kChannels = kDraftTC * kHead / kThreads;
+    hv8 x[kPieces];
+    _Float16 xw[kChannels];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = vec == 1 ? decay((float)x[e]) : (float)x[e];
-      f4* d = &vl[(tt * kDraftVecs + vec) * 16 + part * 2];
-      d[0] = f4{f[0], f[1], f[2], f[3]};
-      d[1] = f4{f[4], f[5], f[6], f[7]};
+    for (int u = 0; u < kPieces; ++u) {
+      const int piece = tid + u * kThreads, tv = piece >> 3, tt = tv / 5, vec = tv - tt * 5, t = c0 + tt;
+      if (tt >= n || (t < nk && vec == 0)) continue;  // kept tokens need no r
+      const _Float16* src = t < nk ? (vec == 1 ? p.pend[1] : vec == 2 ? p.pend[2] : vec == 3 ? p.pend[3] : p.pend[4]) +
+                                         pend0 + (size_t)t * p.C
+                                   : (vec == 0 ? p.r : vec == 1 ? p.k : vec == 2 ? p.v : vec == 3 ? p.a : p.b) + ytok +
+                                         (size_t)(t - nk) * p.C;
+      x[u] = *reinterpret_cast<const hv8*>(src + (piece & 7) * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < kChannels; ++u) {
+      const int e = tid + u * kThreads, tt = e >> 6, t = c0 + tt;
+      if (tt >= n) continue;
+      xw[u] = t < nk ? p.pend[0][pend0 + (size_t)t * p.C + (e & 63)] : p.w[ytok + (size_t)(t - nk) * p.C + (e & 63)];
+    }
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u) {
+      const int piece = tid + u * kThreads, tv = piece >> 3, tt = tv / 5, vec = tv - tt * 5;
+      if (tt >= n || (c0 + tt < nk && vec == 0)) continue;
+      f4* d = &vl[(tt * kDraftVecs + vec + (vec > 0 ? 1 : 0)) * 16 + (piece & 7) * 2];
+      d[0] = f4{(float)x[u][0], (float)x[u][1], (float)x[u][2], (float)x[u][3]};
+      d[1] = f4{(float)x[u][4], (float)x[u][5], (float)x[u][6], (float)x[u][7]};
+    }
+#pragma unroll
+    for (int u = 0; u < kChannels; ++u) {
+      const int e = tid + u * kThreads, tt = e >> 6;
+      if (tt < n) reinterpret_cast<float*>(&vl[(tt * kDraftVecs + 1) * 16])[e & 63] = decay((float)xw[u]);
     }
     __syncthreads();
     for (int tt = 0; tt < n; ++tt) {
@@ -189,6 +205,9 @@ extern "C" int vkwr_wkv7_fp32_drafts_slots(int B, int P, int T, int C, int H, fl
   DraftArgs p{P, T, C, H, n_slots, n_pending, pool, slots, kept, pending_rows,
               {h16(pw), h16(pk), h16(pv), h16(pa), h16(pb)}, h16(r), h16(w), h16(k), h16(v), h16(a), h16(b),
               reinterpret_cast<_Float16*>(y)};
-  hipLaunchKernelGGL(wkv7_fp32_drafts_kernel<2>, dim3(B * H), dim3(256), 0, (hipStream_t)stream, p);
+  if ((int64_t)B * H <= 2 * (int64_t)device_cus())
+    hipLaunchKernelGGL(wkv7_fp32_drafts_kernel<1>, dim3(B * H), dim3(512), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL(wkv7_fp32_drafts_kernel<2>, dim3(B * H), dim3(256), 0, (hipStream_t)stream, p);
   return check_launch(fn);
 }
