@@ -30,11 +30,17 @@ of T tokens gives the same recurrent state and last-token logits as T decode
 steps (same arithmetic per token, GEMM rows independent); tests/test_serving_gpu.py
 checks that, and the decode rows against DecodeEngine.
 
-Every buffer is preallocated for `max_rows` rows, so a step allocates nothing.
+With `adapters` (adapters.py) each sequence of a step may have a low-rank adapter of its own beside the
+shared projections: x A^T B^T is added to r, k, v before the low-rank outputs, to o, to the FFN key before
+the squared ReLU (which the adapters' launch then applies) and to the FFN value.
+
+Every buffer is preallocated for `max_rows` rows, so a step allocates nothing (the adapters' scratch
+grows to its size in the first steps).
 """
 import torch
 
 from vkwr_amd import capi
+from vkwr.model_executor.adapters import AdapterStep
 from vkwr.model_executor.rwkv7 import HEAD
 
 TMIX_MIX = ("x_r", "x_w", "x_k", "x_v", "x_a", "x_g")
@@ -58,7 +64,7 @@ def _pad_rank(w1, w2, r):
 class MixedEngine:
     """Forward step over up to `max_rows` rows in decode and prefill groups."""
 
-    def __init__(self, model, max_rows, max_seqs=None):
+    def __init__(self, model, max_rows, max_seqs=None, adapters=None):
         cfg = model.cfg
         self.model, self.cfg, self.max_rows = model, cfg, max_rows
         self.max_seqs = max_seqs or max_rows
@@ -105,6 +111,7 @@ class MixedEngine:
         self.side = torch.cuda.Stream(device=dev) if dev.type == "cuda" else None
         self.fork = torch.cuda.Event() if dev.type == "cuda" else None
         self.join = torch.cuda.Event() if dev.type == "cuda" else None
+        self.adapters = None if adapters is None else AdapterStep(adapters, max_rows, dev)
 
     # -- GEMM batches (shared by planning and execution)
     def _proj(self, L, W, R, first):
@@ -176,16 +183,38 @@ class MixedEngine:
             s.join.record(s.side)
             main.wait_event(s.join)
 
+    def _begin_adapters(self, groups, adapter_ids):
+        """The step's adapters, or None.  groups: (B, T, first row, slots, first sequence)."""
+        if adapter_ids is None:
+            return None
+        if self.adapters is None:
+            raise ValueError("adapter_ids given to an engine without adapters")
+        self.adapters.begin([(B, T, r0, q0) for B, T, r0, _, q0 in groups], adapter_ids)
+        return self.adapters
+
+    def _ffn(self, l, L, R, adapters):
+        """relu(xk K^T)^2 V^T of the rows, into ffn."""
+        s, gp = self, capi.gemm_problem
+        square = capi.EPI_RELU_SQUARE
+        late = adapters is not None and "key" in adapters.pool.names  # the square follows the adapters
+        capi.gemm([gp(s.xk[:R], L["key"], s.act[:R], epilogue=capi.EPI_NONE if late else square)], s.ws)
+        if late:
+            adapters.add(l, [("key", s.xk, s.act)], square)
+        capi.gemm([gp(s.act[:R], L["value"], s.ffn[:R])], s.ws)
+        if adapters is not None:
+            adapters.add(l, [("value", s.act, s.ffn)])
+
     def _head_problem(self, S):
         return [capi.gemm_problem(self.h[:S], self.model.head, self.logits[:S])]
 
     # -- the step
-    def step(self, state, decode=None, prefill=()):
+    def step(self, state, decode=None, prefill=(), adapter_ids=None):
         """decode: (tokens [Bd] int32, slots [Bd] int32) or None; prefill: sequence of
         (tokens [Bg, Tg] int32, slots [Bg] int32).  All on the device, slots distinct over the
         whole step and < state.n_slots.  Updates `state` in place and returns logits
         [Bd + sum Bg, V]: the decode rows, then each prefill sequence's last chunk token
-        (a view valid until the next step)."""
+        (a view valid until the next step).  adapter_ids (engines with adapters): int32 [sequences] on
+        the device in the order of the logits, negative for none; not given: no adapters."""
         cfg, m, s = self.cfg, self.model, self
         assert state.layout == capi.WKV_STATE_STD, "the mixed step uses the row-major WKV pool"
         C, H = cfg.n_embd, cfg.n_head
@@ -207,6 +236,7 @@ class MixedEngine:
         ws = self.ws
         torch.index_select(m.emb, 0, s.tok[:R], out=s.x0[:R])
         shift_groups = [(r0, B, T, slots) for B, T, r0, slots, _ in groups]
+        adapters = self._begin_adapters(groups, adapter_ids)
         x, res_in = s.x0[:R], None
         for l, L in enumerate(m.layers):
             first = l == 0
@@ -217,18 +247,22 @@ class MixedEngine:
             capi.layer_norm_shift_rows(x, L["ln1_w"], L["ln1_b"], res, [L[k] for k in TMIX_MIX],
                                        [t[:R] for t in s.mix], state.att_shift[l], shift_groups, residual=res_in)
             capi.gemm(self._proj(L, s.lw[l], R, first), ws)
+            if adapters is not None:
+                adapters.add(l, [("Wr", s.mix[0], s.r), ("Wk", s.mix[2], s.k),
+                                 ("Wv", s.mix[3], s.v_first if first else s.v)])
             capi.gemm(self._rank_out(L, s.lw[l], R, first), ws)
             v = (s.v_first if first else s.v_new)[:R]
             capi.kk_a_gate(R, 1, C, H, s.k[:R], L["k_k"], L["a0"], s.a12[:R], L["k_a"], s.new_k[:R],
                            s.neg_kk[:R], s.kka[:R])
             self._wkv_gn(groups, state.wkv[l], v, L)
             capi.gemm([capi.gemm_problem(s.o_in[:R], L["Wo"], s.o[:R])], ws)
+            if adapters is not None:
+                adapters.add(l, [("Wo", s.o_in, s.o)])
             # ---- channel mix
             res2 = s.res[0][:R]
             capi.layer_norm_shift_rows(s.o[:R], L["ln2_w"], L["ln2_b"], res2, [L["x_k_ffn"]], [s.xk[:R]],
                                        state.ffn_shift[l], shift_groups, residual=res)
-            capi.gemm([capi.gemm_problem(s.xk[:R], L["key"], s.act[:R], epilogue=capi.EPI_RELU_SQUARE)], ws)
-            capi.gemm([capi.gemm_problem(s.act[:R], L["value"], s.ffn[:R])], ws)
+            self._ffn(l, L, R, adapters)
             x, res_in = s.ffn[:R], res2
         for B, T, r0, _, q0 in groups:
             n = B * T

@@ -16,12 +16,18 @@ Finished sequences release their slot immediately, so waiting requests are
 admitted the next step (256 decode rows + 4 x 512 prefill
 rows per step, 2048-slot pool).  The default sampler is greedy (argmax); pass
 `sample` to use another, e.g. a ``GpuSampler`` (temperature / top-k / top-p on
-the vkwr_sampling kernels).
+the vkwr_sampling kernels).  A request may name an adapter of the engine's pool.
+
+`SpeculativeBatcher` does the same on a `DraftEngine`: generating sequences run
+their last token and up to `max_draft` drafts in one draft step, `verify_drafts`
+accepts or rejects them, and a sequence advances by one token or more.
 """
 from collections import deque
 from dataclasses import dataclass, field
 
 import torch
+
+from vkwr_amd import capi
 
 
 @dataclass
@@ -30,6 +36,7 @@ class Request:
     max_new_tokens: int
     rid: int = -1
     slot: int = -1
+    adapter: int = -1                  # of the engine's AdapterPool; -1: none
     pos: int = 0                       # prompt tokens consumed
     output: list = field(default_factory=list)
 
@@ -89,9 +96,12 @@ class ContinuousBatcher:
         self.steps = 0
         self.tokens_processed = 0
 
-    def submit(self, prompt, max_new_tokens):
+    def submit(self, prompt, max_new_tokens, adapter=-1):
         assert len(prompt) >= 1 and max_new_tokens >= 1
-        req = Request(list(prompt), max_new_tokens, rid=self._next_id)
+        n = self.engine.adapters.pool.n_adapters if self.engine.adapters is not None else 0
+        if not -1 <= adapter < n:
+            raise ValueError(f"adapter {adapter} of {n}")
+        req = Request(list(prompt), max_new_tokens, rid=self._next_id, adapter=adapter)
         self._next_id += 1
         self.waiting.append(req)
         return req
@@ -112,23 +122,31 @@ class ContinuousBatcher:
         if len(set(slots)) != len(slots) or any(s not in self.slots._used for s in slots):
             raise RuntimeError(f"invalid slot table for this step: {slots}")
 
-    def step(self):
-        """Runs one forward step; returns the requests that finished in it."""
+    def _adapter_ids(self, reqs):
+        """Adapter indices of these requests, or None where no request has one."""
+        ids = [r.adapter for r in reqs]
+        return self._i32(ids) if any(i >= 0 for i in ids) else None
+
+    def _admit(self):
         while self.waiting and self.slots.available:
             req = self.waiting.popleft()
             req.slot = self.slots.alloc()
             self._reset_slot(req.slot)
             self.running.append(req)
+
+    def _decoding(self):
+        """The generating sequences of this step."""
         decoding = [r for r in self.running if not r.prefilling]
         if len(decoding) > self.max_decode:
             # more generating sequences than decode rows: rotate, so none starves
             start = self._rr % len(decoding)
-            dec = (decoding[start:] + decoding[:start])[: self.max_decode]
             self._rr = start + self.max_decode
-        else:
-            dec = decoding
-        rows = len(dec)
-        groups = {}  # chunk length -> requests
+            return (decoding[start:] + decoding[:start])[: self.max_decode]
+        return decoding
+
+    def _chunks(self, rows):
+        """Prompt chunks of this step beside `rows` decode rows: chunk length -> requests."""
+        groups = {}
         n_chunks = 0
         for r in self.running:
             if not r.prefilling or n_chunks == self.max_prefill_chunks:
@@ -139,6 +157,14 @@ class ContinuousBatcher:
             groups.setdefault(t, []).append(r)
             rows += t
             n_chunks += 1
+        return groups
+
+    def step(self):
+        """Runs one forward step; returns the requests that finished in it."""
+        self._admit()
+        dec = self._decoding()
+        groups = self._chunks(len(dec))
+        rows = len(dec) + sum(t * len(reqs) for t, reqs in groups.items())
         if rows == 0:
             return []
         self._check_slots(dec + [r for reqs in groups.values() for r in reqs])
@@ -150,7 +176,8 @@ class ContinuousBatcher:
             toks = self._i32([r.prompt[r.pos:r.pos + t] for r in reqs])
             prefill.append((toks, self._i32([r.slot for r in reqs])))
             order.append((t, reqs))
-        logits = self.engine.step(self.state, decode=decode, prefill=prefill)
+        ids = self._adapter_ids(dec + [r for _, reqs in order for r in reqs])
+        logits = self.engine.step(self.state, decode=decode, prefill=prefill, adapter_ids=ids)
         nxt = self.sample(logits).tolist()
         for i, r in enumerate(dec):
             r.output.append(nxt[i])
@@ -177,4 +204,91 @@ class ContinuousBatcher:
         return done
 
 
-__all__ = ["Request", "SlotAllocator", "ContinuousBatcher"]
+def prompt_lookup(tokens, n, match=2):
+    """Up to n drafts: what followed the latest earlier occurrence of the last `match` tokens."""
+    if len(tokens) <= match:
+        return []
+    tail = tokens[-match:]
+    for i in range(len(tokens) - match - 1, -1, -1):
+        if tokens[i:i + match] == tail:
+            return tokens[i + match:i + match + n]
+    return []
+
+
+class SpeculativeBatcher(ContinuousBatcher):
+    """Continuous batching with drafted tokens on a DraftEngine.  `draft(tokens, n)` proposes up to n
+    tokens behind a sequence's tokens (default: looked up in them); top_k = 1 generates greedily.
+    Prompt chunks run as in ContinuousBatcher, in a step of their own before the drafts'."""
+
+    def __init__(self, engine, state, draft=prompt_lookup, temperature=1.0, top_k=1, top_p=1.0, seed=0, **kw):
+        kw.setdefault("max_decode", engine.draft_seqs)
+        if kw["max_decode"] > engine.draft_seqs:
+            raise ValueError(f"{kw['max_decode']} generating sequences, the engine drafts {engine.draft_seqs}")
+        super().__init__(engine, state, **kw)
+        B, T = engine.draft_seqs, engine.max_draft + 1
+        self.draft, self.filter = draft, dict(temperature=temperature, top_k=top_k, top_p=top_p)
+        self.gen = torch.Generator(device=self.device).manual_seed(seed)
+        self.ws = torch.empty(capi.verify_workspace_bytes(B, T - 1, engine.cfg.vocab), dtype=torch.uint8,
+                              device=self.device)
+        self.drafted = self.accepted = 0
+
+    def _verify(self, logits, drafts, n_draft):
+        """logits [B, T, V]: (tokens, accepted) on the device."""
+        B, T, _ = logits.shape
+        tokens = torch.empty(B, T, dtype=torch.int32, device=self.device)
+        accepted = torch.empty(B, dtype=torch.int32, device=self.device)
+        u = torch.rand(B, T, generator=self.gen, device=self.device)
+        capi.verify_drafts(logits, drafts, u, tokens, accepted, n_draft=n_draft, workspace=self.ws, **self.filter)
+        return tokens, accepted
+
+    def _finish(self):
+        finished = [r for r in self.running if r.done]
+        for r in finished:
+            self.engine.drop([r.slot])
+            self.slots.free(r.slot)
+        self.running = [r for r in self.running if not r.done]
+        return finished
+
+    def step(self):
+        """Prompt chunks, then one draft step of the generating sequences; returns the requests that
+        finished."""
+        self._admit()
+        groups = self._chunks(0)
+        if groups:
+            order = [(t, reqs) for t, reqs in groups.items()]
+            flat = [r for _, reqs in order for r in reqs]
+            self._check_slots(flat)
+            prefill = [(self._i32([r.prompt[r.pos:r.pos + t] for r in reqs]), self._i32([r.slot for r in reqs]))
+                       for t, reqs in order]
+            logits = self.engine.step(self.state, prefill=prefill, adapter_ids=self._adapter_ids(flat))
+            none = torch.empty(len(flat), 0, dtype=torch.int32, device=self.device)
+            nxt = self._verify(logits[:, None, :], none, None)[0][:, 0].tolist()
+            for (t, r), token in zip([(t, r) for t, reqs in order for r in reqs], nxt):
+                r.pos += t
+                self.tokens_processed += t
+                if not r.prefilling:
+                    r.output.append(token)
+            done = self._finish()
+        else:
+            done = []
+        dec = self._decoding()
+        if dec:
+            self._check_slots(dec)
+            K = self.engine.max_draft
+            drafts = [list(self.draft(r.prompt + r.output, min(K, r.max_new_tokens - len(r.output) - 1)))[:K] for r in dec]
+            T = 1 + max(len(d) for d in drafts)
+            rows = self._i32([[r.output[-1]] + d + [0] * (T - 1 - len(d)) for r, d in zip(dec, drafts)])
+            logits = self.engine.draft_step(self.state, rows, [r.slot for r in dec], adapter_ids=self._adapter_ids(dec))
+            tokens, accepted = self._verify(logits, rows[:, 1:].contiguous(), self._i32([len(d) for d in drafts]))
+            self.engine.accept(accepted)
+            for r, d, new, n in zip(dec, drafts, tokens.tolist(), accepted.tolist()):
+                r.output += new[:min(n + 1, r.max_new_tokens - len(r.output))]
+                self.drafted += len(d)
+                self.accepted += n
+            self.tokens_processed += rows.numel()
+        if groups or dec:
+            self.steps += 1
+        return done + self._finish()
+
+
+__all__ = ["Request", "SlotAllocator", "ContinuousBatcher", "SpeculativeBatcher", "prompt_lookup"]

@@ -598,11 +598,13 @@ def lora_workspace_bytes(max_rows, n_adapters, targets):
 
 
 def lora(plan, targets, scale=None, workspace=None):
-    """Adds each row's adapter to 1..8 projections that the rows of `plan` go through (vkwr_lora_f16).
-    scale: fp32 [G] (None: 1).  workspace: uint8, lora_workspace_bytes (None: allocated)."""
-    (m, G, rank), arr = _lora_targets(targets)
-    if plan.m != m or plan.n_adapters != G:
-        raise ValueError(f"lora: plan of {plan.m} rows and {plan.n_adapters} adapters, targets of {m} and {G}")
+    """Adds each row's adapter to 1..8 projections that the rows of `plan` go through (vkwr_lora_f16): the
+    first plan.m rows of the targets, the others are left as they were.  scale: fp32 [G] (None: 1).
+    workspace: uint8, lora_workspace_bytes (None: allocated)."""
+    (rows, G, rank), arr = _lora_targets(targets)
+    m = plan.m
+    if m is None or m > rows or plan.n_adapters != G:
+        raise ValueError(f"lora: plan of {m} rows and {plan.n_adapters} adapters, targets of {rows} and {G}")
     if workspace is None:
         workspace = torch.empty(lora_workspace_bytes(m, G, targets), dtype=torch.uint8, device=plan.buf.device)
     at, nbytes = _Tensors(), workspace.numel()
