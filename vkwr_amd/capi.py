@@ -466,12 +466,20 @@ class _Tensors:
     __slots__ = ("dev",)
 
     def __init__(self):
-        self.dev = torch.cuda.current_device() if torch.cuda.is_initialized() else 0
+        self.dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else 0
 
     def __call__(self, t, dtype, n, what):
-        if t.dtype != dtype or t.get_device() != self.dev or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not dtype or t.get_device() != self.dev or t.numel() != n or not t.is_contiguous():
             self._refuse(t, dtype, n, what)
         return t.data_ptr()
+
+    def all(self, ts, dtype, n, what):
+        dev, out = self.dev, []
+        for t in ts:
+            if t.dtype is not dtype or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+                self._refuse(t, dtype, n, what)
+            out.append(t.data_ptr())
+        return out
 
     def optional(self, t, dtype, n, what):
         return None if t is None else self(t, dtype, n, what)
@@ -499,9 +507,9 @@ def wkv_drafts_slots(B, T, C, H, pool, slots, r, w, k, v, a, b, y, kept=None, pe
         raise ValueError("wkv_drafts_slots: kept and pending go together")
     if pending is not None:
         n_pending, P = pending[0].shape[:2]
-        pv = [at(t, h, n_pending * P * C, "pending") for t in pending]
+        pv = at.all(pending, h, n_pending * P * C, "pending")
     n = B * T * C
-    ins = [at(t, h, n, "r, w, k, v, a, b, y") for t in (r, w, k, v, a, b, y)] if T else [None] * 7
+    ins = at.all((r, w, k, v, a, b, y), h, n, "r, w, k, v, a, b, y") if T else [None] * 7
     _check(_wkv_drafts(B, P, T, C, H, at(pool, torch.float32, n_slots * H * 4096, "pool"), n_slots,
                        at(slots, i32, B, "slots"), at(kept, i32, B, "kept") if P else None, n_pending,
                        at.optional(pending_rows, i32, B, "pending_rows"), *pv, *ins, at.stream()),

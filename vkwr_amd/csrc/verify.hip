@@ -432,10 +432,14 @@ struct RowSummary {
 };
 __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id, int lane) {
   RowSummary r;
-  float mx = -INFINITY, below = -INFINITY, reach = -INFINITY;
+  const bool sums = !p.truncate || p.use_mass;
+  float mx = -INFINITY, below = -INFINITY, reach = -INFINITY, gm = -INFINITY;
+  double gs = 0.0;
   int count = 0;
-  for (int g = lane; g < p.groups; g += 64) {
-    mx = fmaxf(mx, p.group_max[id * p.groups + g]);
+  for (int g = lane; g < p.groups; g += 64) {  // one round up to 131072 entries
+    gm = p.group_max[id * p.groups + g];
+    if (sums) gs = p.group_sum[id * p.groups + g];
+    mx = fmaxf(mx, gm);
     if (p.cap > 0) {
       const float f = p.group_floor[id * p.groups + g];
       below = fmaxf(below, -f);
@@ -445,9 +449,13 @@ __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id,
   }
   mx = wave_fmax(mx);
   double m = 0.0;
-  if (!p.truncate || p.use_mass) {
-    for (int g = lane; g < p.groups; g += 64)
-      m += p.group_sum[id * p.groups + g] * group_factor(p, p.group_max[id * p.groups + g], mx);
+  if (sums) {
+    if (p.groups <= 64) {
+      m = gs * group_factor(p, gm, mx);
+    } else {
+      for (int g = lane; g < p.groups; g += 64)
+        m += p.group_sum[id * p.groups + g] * group_factor(p, p.group_max[id * p.groups + g], mx);
+    }
     m = wave_add(m);
   }
   r.mode = mx == INFINITY ? kInfOnly : mx == -INFINITY ? kAllLow : kNanZero;
@@ -460,6 +468,40 @@ __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id,
     r.reach = wave_fmax(reach);
   }
   return r;
+}
+
+// Draft k of sequence b: its logit as stored, the drafter's probability and the uniform.
+struct Draft {
+  bool in;  // in the vocabulary
+  float l, q, u;
+};
+template <bool kHalf>
+__device__ __forceinline__ Draft load_draft(const VerifyArgs& p, int b, int k) {
+  const int64_t id = (int64_t)b * (p.K + 1) + k, at = (int64_t)b * p.K + k;
+  const int d = p.drafts[at];
+  Draft r{d >= 0 && d < p.V, 0.0f, 1.0f, p.u[id]};
+  if (r.in) {
+    const void* row = row_at<kHalf>(p, id);
+    r.l = kHalf ? (float)reinterpret_cast<const _Float16*>(row)[d] : reinterpret_cast<const float*>(row)[d];
+    if (p.q) r.q = p.q[at * p.V + d];
+  }
+  return r;
+}
+
+// With top_p alone the kept mass is top_p S exactly, so p(d) <= x_d / (top_p S), which rejects many a draft
+// without tau; and if tau <= l_d, p(d) >= (x_d - (1 - top_p) S) / (top_p S) (the entries above d hold at most
+// S - n x_d if n are tied with it, so d keeps (top_p S - (S - n x_d)) / n or all of x_d), which also says that
+// tau <= l_d where it is positive.  Margins of 1e-9 for the rounding of either side.
+enum { kUnsure, kAccept, kReject };
+template <bool kHalf>
+__device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int lane) {
+  const Draft d = load_draft<kHalf>(p, b, k);
+  const RowSummary s = summarize(p, (int64_t)b * (p.K + 1) + k, lane);
+  if (!d.in) return kReject;
+  const double x = exp2_neg((double)read_as(d.l, s.mode) - (double)s.max, p.scale, p.d_min);
+  const double goal = p.top_p * s.mass, uq = (double)d.u * (double)d.q;
+  if (!(uq * goal < x * (1.0 + 1.0e-9))) return kReject;
+  return uq * goal < (x - (1.0 - p.top_p) * s.mass) - 1.0e-9 * s.mass ? kAccept : kUnsure;
 }
 
 // kLists: the groups' lists are searched first.  A row that is searched as a whole is read twice more:
@@ -478,18 +520,28 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
   const void* row = row_at<kHalf>(p, id);
   const int tiles = (V + kVerTile - 1) / kVerTile;
   int par = 0;
-  // what the draft's test needs, requested early
-  int draft = -1;
-  float draft_l = -INFINITY, draft_q = 1.0f, draft_u = 0.0f;
-  const float last_u = p.u[(int64_t)b * T + p.K];
-  if (t == 0 && i < n) {
-    draft = p.drafts[(int64_t)b * p.K + i];
-    draft_u = p.u[id];
-    if (draft >= 0 && draft < V) {
-      draft_l = kHalf ? (float)reinterpret_cast<const _Float16*>(row)[draft] : reinterpret_cast<const float*>(row)[draft];
-      if (p.q) draft_q = p.q[((int64_t)b * p.K + i) * V + draft];
+  if (!kLists && p.use_mass && p.top_k == V) {
+    // Rows that a quick test can do without: those behind a rejection, and accepted ones (no statistics
+    // but the verdict are read of them).  128 sequences of 4 drafts, fp32 logits: 82 -> {QUICK_US} us.
+    if (t == 0) sh.bin = sh.n_cand = 0;
+    __syncthreads();
+    for (int k = wv; k <= i && k < n; k += kVerWaves) {
+      const int v = quick_test<kHalf>(p, b, k, lane);
+      if (lane == 0 && k < i && v == kReject) sh.bin = 1;
+      if (lane == 0 && k == i && v == kAccept) sh.n_cand = 1;
     }
+    __syncthreads();
+    if (sh.bin != 0) return;
+    if (sh.n_cand != 0) {
+      if (t == 0) p.stat[id].ok = 1;
+      return;
+    }
+    __syncthreads();
   }
+  // what the draft's test needs, requested early
+  Draft draft{false, 0.0f, 1.0f, 0.0f};
+  const float last_u = p.u[(int64_t)b * T + p.K];
+  if (t == 0 && i < n) draft = load_draft<kHalf>(p, b, i);
   const RowSummary sum = summarize(p, id, lane);
   const float mx = sum.max;
   const int mode = sum.mode;
@@ -821,8 +873,8 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
     }
   }
   if (t == 0) {
-    if (draft >= 0 && draft < V)
-      st.ok = (double)draft_u * (double)draft_q < kept_of(p, st, read_as(draft_l, mode)) / st.z ? 1 : 0;
+    if (draft.in)
+      st.ok = (double)draft.u * (double)draft.q < kept_of(p, st, read_as(draft.l, mode)) / st.z ? 1 : 0;
     p.stat[id] = st;
   }
 }
@@ -854,15 +906,11 @@ struct Stop {
         if (k0 > 0) __syncthreads();
         for (int k = wv; k < 64 && k0 + k <= n; k += kWaves) {
           const int64_t r = (int64_t)b * T + k0 + k;
-          const int d = k0 + k < n ? p.drafts[(int64_t)b * p.K + k0 + k] : -1;
-          const bool in = d >= 0 && d < p.V;
-          const float l = !in ? 0.0f : kHalf ? (float)reinterpret_cast<const _Float16*>(row_at<kHalf>(p, r))[d]
-                                             : reinterpret_cast<const float*>(row_at<kHalf>(p, r))[d];
-          const double qd = in && p.q ? (double)p.q[((int64_t)b * p.K + k0 + k) * p.V + d] : 1.0;
-          const double u = (double)p.u[r];
+          Draft d{false, 0.0f, 1.0f, 0.0f};
+          if (k0 + k < n) d = load_draft<kHalf>(p, b, k0 + k);
           const RowSummary sum = summarize(p, r, lane);
           RowStat s{sum.mass, 1.0, sum.max, -INFINITY, 0, sum.mode, -1, 0};
-          s.ok = in && u * qd < kept_of(p, s, read_as(l, sum.mode)) / s.z ? 1 : 0;
+          s.ok = d.in && (double)d.u * (double)d.q < kept_of(p, s, read_as(d.l, sum.mode)) / s.z ? 1 : 0;
           if (lane == 0) sh.stat[k] = s;
         }
         __syncthreads();
@@ -1007,7 +1055,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
         }
         sh.sum[k] = s;
       }
-      if (own >= 0 && wv == 0) {
+      if (own >= 0 && wv == kDrawThreads / 64 - 1) {  // the wave with the fewest sums to load
         const double s = segment(own);
         if (lane == 0) sh.sum[own] = s;
       }
