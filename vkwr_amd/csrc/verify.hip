@@ -40,13 +40,12 @@
 namespace vk {
 namespace {
 
-constexpr int kVerThreads = 512;   // per row: three workgroups fit on a CU, and one's loads cover another's work
-constexpr int kVerWaves = kVerThreads / 64;
+constexpr int kListThreads = 512;  // rows' kernel: rows searched in lists
+constexpr int kMaxWaves = 1024 / 64;
 constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
 constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
-constexpr int kVerList = 2 * kVerThreads;  // listed entries of a row: two per lane
+constexpr int kVerList = 2 * kListThreads;  // listed entries of a row: two per lane
 constexpr int kVerDraw = 256;    // kept entries that the rows' kernel draws from directly
-constexpr int kVerTile = 4 * kVerThreads;  // consecutive entries a row's workgroup reads at once
 constexpr int kVerMaxV = 1 << 20;
 constexpr int kSeg = 256;        // consecutive entries whose weights are added up for the draw (one wave's 64 x 4)
 constexpr int kMaxSegs = kVerMaxV / kSeg;
@@ -192,10 +191,10 @@ struct StatShared {
     } draw;
   };
   uint32_t cnt[kVerBins];
-  uint64_t redm[2][kVerWaves];
-  double redd[2][kVerWaves];
-  uint32_t redc[2][kVerWaves], rede[2][kVerWaves];
-  float redf[2][kVerWaves], redg[2][kVerWaves];
+  uint64_t redm[2][kMaxWaves];
+  double redd[2][kMaxWaves];
+  uint32_t redc[2][kMaxWaves], rede[2][kMaxWaves];
+  float redf[2][kMaxWaves], redg[2][kMaxWaves];
   alignas(16) float cand[kVerCand];
   uint64_t candm[kVerCand];
   int n_cand, bin;
@@ -219,11 +218,23 @@ __device__ __forceinline__ float row_fmax(float x) {
   x = oct_fmax(x);
   return fmaxf(x, dpp<0x140>(x));
 }
+// ... that W consecutive lanes hold, W = 8 or 16.
+template <int W, class X>
+__device__ __forceinline__ X lanes_add(X x) {
+  static_assert(W == 8 || W == 16, "half a row of lanes or a row");
+  x = oct_add(x);
+  if constexpr (W == 16) x += dpp<0x140>(x);
+  return x;
+}
+template <int W>
+__device__ __forceinline__ float lanes_fmax(float x) {
+  return W == 16 ? row_fmax(x) : oct_fmax(x);
+}
 
 // Block reductions with one barrier: consecutive ones alternate between two buffers (par), so a wave
-// overwrites a buffer only behind the barrier that every wave reaches after reading it.  Eight lanes add
-// the eight wave values.
-static_assert(kVerWaves == 8, "eight lanes hold the wave values");
+// overwrites a buffer only behind the barrier that every wave reaches after reading it.  W lanes add the W
+// waves' values.
+template <int W>
 __device__ __forceinline__ void block_max2(StatShared& sh, int& par, float& a, float& b) {
   a = wave_fmax(a);
   b = wave_fmax(b);
@@ -232,26 +243,29 @@ __device__ __forceinline__ void block_max2(StatShared& sh, int& par, float& a, f
     sh.redg[par][threadIdx.x >> 6] = b;
   }
   __syncthreads();
-  a = oct_fmax(sh.redf[par][threadIdx.x & 7]);
-  b = oct_fmax(sh.redg[par][threadIdx.x & 7]);
+  a = lanes_fmax<W>(sh.redf[par][threadIdx.x & (W - 1)]);
+  b = lanes_fmax<W>(sh.redg[par][threadIdx.x & (W - 1)]);
   par ^= 1;
 }
+template <int W>
 __device__ __forceinline__ float block_max(StatShared& sh, int& par, float a) {
   a = wave_fmax(a);
   if ((threadIdx.x & 63) == 0) sh.redf[par][threadIdx.x >> 6] = a;
   __syncthreads();
-  a = oct_fmax(sh.redf[par][threadIdx.x & 7]);
+  a = lanes_fmax<W>(sh.redf[par][threadIdx.x & (W - 1)]);
   par ^= 1;
   return a;
 }
+template <int W>
 __device__ __forceinline__ double block_sum(StatShared& sh, int& par, double a) {
   a = wave_add(a);
   if ((threadIdx.x & 63) == 0) sh.redd[par][threadIdx.x >> 6] = a;
   __syncthreads();
-  a = oct_add(sh.redd[par][threadIdx.x & 7]);
+  a = lanes_add<W>(sh.redd[par][threadIdx.x & (W - 1)]);
   par ^= 1;
   return a;
 }
+template <int W>
 __device__ __forceinline__ void block_add(StatShared& sh, int& par, uint32_t& a, uint32_t& b, uint64_t& m) {
   a = wave_add(a);
   b = wave_add(b);
@@ -263,10 +277,10 @@ __device__ __forceinline__ void block_add(StatShared& sh, int& par, uint32_t& a,
     sh.redm[par][w] = m;
   }
   __syncthreads();
-  const int w = threadIdx.x & 7;
-  a = oct_add(sh.redc[par][w]);
-  b = oct_add(sh.rede[par][w]);
-  m = oct_add(sh.redm[par][w]);
+  const int w = threadIdx.x & (W - 1);
+  a = lanes_add<W>(sh.redc[par][w]);
+  b = lanes_add<W>(sh.rede[par][w]);
+  m = lanes_add<W>(sh.redm[par][w]);
   par ^= 1;
 }
 
@@ -507,8 +521,11 @@ __device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int
 // kLists: the groups' lists are searched first.  A row that is searched as a whole is read twice more:
 // for the histogram and for the entries of one bin.  (Kept in LDS, 128 KiB left one workgroup per CU, whose
 // loads and arithmetic then took turns.)
-template <bool kHalf, bool kLists>
-__global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kernel(VerifyArgs p) {
+template <bool kHalf, bool kLists, int kThreads>
+__global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(VerifyArgs p) {
+  static_assert(!kLists || kThreads == kListThreads, "two listed entries per lane");
+  constexpr int W = kThreads / 64;
+  constexpr int kTile = 4 * kThreads;  // consecutive entries read at once
   typedef typename Raw<kHalf>::type R;
   __shared__ StatShared sh;
   const int T = p.K + 1;
@@ -518,14 +535,15 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = p.V;
   const int64_t id = (int64_t)b * T + i;
   const void* row = row_at<kHalf>(p, id);
-  const int tiles = (V + kVerTile - 1) / kVerTile;
+  const int tiles = (V + kTile - 1) / kTile;
   int par = 0;
   if (!kLists && p.use_mass && p.top_k == V) {
     // Rows that a quick test can do without: those behind a rejection, and accepted ones (no statistics
-    // but the verdict are read of them).  128 sequences of 4 drafts, fp32 logits: 82 -> {QUICK_US} us.
+    // but the verdict are read of them).  Of 128 sequences' 566 rows (4 drafts,
+    // nucleus 0.95) 271 are left.
     if (t == 0) sh.bin = sh.n_cand = 0;
     __syncthreads();
-    for (int k = wv; k <= i && k < n; k += kVerWaves) {
+    for (int k = wv; k <= i && k < n; k += W) {
       const int v = quick_test<kHalf>(p, b, k, lane);
       if (lane == 0 && k < i && v == kReject) sh.bin = 1;
       if (lane == 0 && k == i && v == kAccept) sh.n_cand = 1;
@@ -569,17 +587,18 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
     for (int e = 0; e < 4; ++e) l[e] = __builtin_isnan(l[e]) ? 0.0f : l[e];
     if (mode != kNanZero)
       for (int e = 0; e < 4; ++e) l[e] = read_as(l[e], mode);
-    if ((j + 1) * kVerTile > V && j * kVerTile + 4 * t >= V) l = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if ((j + 1) * kTile > V && j * kTile + 4 * t >= V) l = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     return l;
   };
-  // f(four entries) over this lane's part of the row, four tiles' loads at a time; padding is -inf
+  // f(four entries) over this lane's part of the row, eight tiles' loads at a time; padding is -inf
   auto each_row = [&](auto&& f) __attribute__((always_inline)) {
-    for (int j = 0; j < tiles; j += 4) {
-      R x[4];
+    constexpr int kB = 8;
+    for (int j = 0; j < tiles; j += kB) {
+      R x[kB];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = load_raw<kHalf>(row, min((j + u) * kVerTile + 4 * t, V - 4));
+      for (int u = 0; u < kB; ++u) x[u] = load_raw<kHalf>(row, min((j + u) * kTile + 4 * t, V - 4));
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kB; ++u) {
         if (j + u >= tiles) break;
         f(entries(j + u, x[u]));
       }
@@ -593,7 +612,7 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
   if (listed) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int at = t + u * kVerThreads, g = at / p.cap, k = at - g * p.cap;
+      const int at = t + u * kThreads, g = at / p.cap, k = at - g * p.cap;
       if (g < p.groups && k < p.group_count[id * p.groups + g]) {
         const float2 e = p.list[(id * p.groups + g) * p.cap + k];
         mine[u] = e.x;
@@ -626,7 +645,7 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
     const float far = mx - floor;
     const float s = far > 0.0f ? fminf(fmaxf(p.bin_scale, (float)(kVerBins - 1) / far), FLT_MAX) : p.bin_scale;
     auto bin_at = [&](float l) __attribute__((always_inline)) { return fminf((mx - l) * s, (float)(kVerBins - 1)); };
-    for (int k = t; k < kVerBins; k += kVerThreads) {
+    for (int k = t; k < kVerBins; k += kThreads) {
       sh.cnt[k] = 0;
       sh.mass[k] = 0;
     }
@@ -652,8 +671,8 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
       }
     });
     __syncthreads();
-    // inclusive prefix over the bins (four per lane) and the first bin that reaches the budget
-    constexpr int kPer = kVerBins / kVerThreads;
+    // inclusive prefix over the bins (kPer per lane) and the first bin that reaches the budget
+    constexpr int kPer = kVerBins / kThreads;
     uint32_t c[kPer], ci = 0;
     uint64_t m[kPer], mi = 0;
 #pragma unroll
@@ -670,8 +689,8 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
       sh.redm[par][wv] = mi;
     }
     __syncthreads();
-    ci += oct_add((lane & 7) < wv ? sh.redc[par][lane & 7] : 0u);
-    mi += oct_add((lane & 7) < wv ? sh.redm[par][lane & 7] : (uint64_t)0);
+    ci += lanes_add<W>((lane & (W - 1)) < wv ? sh.redc[par][lane & (W - 1)] : 0u);
+    mi += lanes_add<W>((lane & (W - 1)) < wv ? sh.redm[par][lane & (W - 1)] : (uint64_t)0);
     par ^= 1;
     if (enough(ci, mi) && !enough(ci - c_own, mi - m_own)) {
       uint32_t cb = ci - c_own;
@@ -754,11 +773,11 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
           }
         }
       }
-      st.tau = block_max(sh, par, t < in_bin && enough(c, m) ? v : -INFINITY);
+      st.tau = block_max<W>(sh, par, t < in_bin && enough(c, m) ? v : -INFINITY);
       ngt = t < in_bin && v > st.tau ? 1 : 0;
       neq = t < in_bin && v == st.tau ? 1 : 0;
       mgt = ngt ? sh.candm[t] : 0;
-      block_add(sh, par, ngt, neq, mgt);
+      block_add<W>(sh, par, ngt, neq, mgt);
       ngt += before_c;
       mgt += before_m;
     } else {
@@ -776,7 +795,7 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
             m += p.use_mass ? mass_of(weight(l)) : 0;
           }
         });
-        block_add(sh, par, c, none, m);
+        block_add<W>(sh, par, c, none, m);
         if (enough(c, m)) lo = mid;
         else hi = mid - 1u;
       }
@@ -784,13 +803,13 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
       float least = -INFINITY;
       const float lov = of_key(lo);
       each([&](float l) { least = l >= lov ? fmaxf(least, -l) : least; });
-      st.tau = -block_max(sh, par, least);
+      st.tau = -block_max<W>(sh, par, least);
       each([&](float l) {
         ngt += l > st.tau ? 1 : 0;
         neq += l == st.tau ? 1 : 0;
         mgt += l > st.tau && p.use_mass ? mass_of(weight(l)) : 0;
       });
-      block_add(sh, par, ngt, neq, mgt);
+      block_add<W>(sh, par, ngt, neq, mgt);
     }
     if (!p.use_mass) {  // the mass above tau was not needed so far
       mgt = 0;
@@ -799,7 +818,7 @@ __global__ __launch_bounds__(kVerThreads, kLists ? 4 : 6) void verify_rows_kerne
 #pragma unroll
         for (int e = 0; e < 4; ++e) mgt += x[e] > st.tau ? mass_of(weight(x[e])) : 0;
       });
-      block_add(sh, par, none, none2, mgt);
+      block_add<W>(sh, par, none, none2, mgt);
     }
     const double x = weight(st.tau);
     double comp = by_count ? (double)((int64_t)p.top_k - (int64_t)ngt) / (double)neq : 1.0;
@@ -1131,8 +1150,14 @@ void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
   const unsigned rows = (unsigned)B * (a.K + 1);
   hipLaunchKernelGGL(verify_sums_kernel<kHalf>, dim3(rows * ((a.groups + 3) / 4)), dim3(256), 0, s, a);
   if (a.truncate) {
-    if (a.cap > 0) hipLaunchKernelGGL((verify_rows_kernel<kHalf, true>), dim3(rows), dim3(kVerThreads), 0, s, a);
-    else hipLaunchKernelGGL((verify_rows_kernel<kHalf, false>), dim3(rows), dim3(kVerThreads), 0, s, a);
+    // As a whole: up to a row per CU 16 waves each, more rows 8, two workgroups to a CU (nucleus of 65536
+    // entries, 4 drafts: 16 sequences 67 us with 16 waves, 77 with 8; 128 sequences 140 and 128).
+    if (a.cap > 0)
+      hipLaunchKernelGGL((verify_rows_kernel<kHalf, true, kListThreads>), dim3(rows), dim3(kListThreads), 0, s, a);
+    else if (rows <= (unsigned)device_cus())
+      hipLaunchKernelGGL((verify_rows_kernel<kHalf, false, 1024>), dim3(rows), dim3(1024), 0, s, a);
+    else
+      hipLaunchKernelGGL((verify_rows_kernel<kHalf, false, 512>), dim3(rows), dim3(512), 0, s, a);
   }
   if (a.truncate ? a.cap == 0 : a.q != nullptr)
     hipLaunchKernelGGL(verify_parts_kernel<kHalf>, dim3(B * ((a.segs + 4 * kPartSegs - 1) / (4 * kPartSegs))), dim3(256), 0,
@@ -1197,7 +1222,7 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
              "%s: vocabulary size must be a multiple of 4 and at most 1048576, got %d", fn, V);
   VK_REQUIRE(temperature >= 0.001 && temperature <= 1000, "%s: temperature %g outside [0.001, 1000]", fn,
              temperature);
-  // (256 threads per 8192 entries of a row, 512 per row: fewer than 2^32 in a launch)
+  // (256 threads per 8192 entries of a row, 1024 per row: fewer than 2^32 in a launch)
   VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= (1 << 21) / ((V + 131071) / 131072), "%s: B*(K+1) too large", fn);
   if (B == 0) return VKWR_OK;
   VK_REQUIRE(logits && uniforms && tokens && accepted && (K == 0 || drafts), "%s: null pointer", fn);
