@@ -1,5 +1,7 @@
 """Verification of drafted tokens (capi.verify_drafts) against the 64-bit oracle: whole numbers, so
 every one has to be equal."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -211,3 +213,23 @@ def test_batch_independence_graph_and_stream(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(tokens, want_t) and torch.equal(accepted, want_a)
+
+
+@pytest.mark.gpu
+def test_masses_that_all_round_down(gpu):
+    """2^20 - 2 equal weights, each rounded down by a third of 2^-43: the kept mass is 4e-8 short, and the
+    first draft's acceptance, whose border lies in between, may fall either way, but what follows it has to
+    fit: the second draft's row is then judged, or not looked at.  (The weights are exp(l / temperature); N
+    x = 1 + 4e-8 puts 1/2 between 1 / (mass as rounded) and 1 / mass.)"""
+    V = 1 << 20
+    x = (1.0 + 4e-8) / (V - 2)
+    assert 0.2 < x * 2.0 ** 43 % 1.0 < 0.45
+    l = torch.full((1, 3, V), -13.875)
+    l[..., 0], l[..., V - 1] = 0.0, -30.0
+    drafts = torch.zeros(1, 2, dtype=torch.int32)
+    u = torch.tensor([[0.5, 0.9, 0.0]])
+    tokens, accepted = torch.empty(1, 3, dtype=torch.int32, device=gpu), torch.empty(1, dtype=torch.int32, device=gpu)
+    ws = torch.full((capi.verify_workspace_bytes(1, 2, V),), 255, dtype=torch.uint8, device=gpu)
+    capi.verify_drafts(l.to(gpu), drafts.to(gpu), u.to(gpu), tokens, accepted, temperature=-13.875 / math.log(x),
+                       top_p=1.0 - 1e-9, workspace=ws)
+    assert (accepted.item(), tokens[0].tolist()) in ((1, [0, 1, -1]), (0, [1, -1, -1]))

@@ -17,7 +17,7 @@
 // 64 bits: weights by a polynomial of relative error 1.1e-12, masses as integers in units of 2^-43
 // (sums of up to 2^20 weights <= 1 do not overflow, and integer sums do not depend on their order),
 // the draw's prefix sums in fp64.  A token differs from that of exact arithmetic only where a
-// uniform lies within ~1e-11 of a border.
+// uniform lies within ~1e-11 of a border (6e-8 where 2^20 equal weights round the same way).
 //
 // Launches:
 //   sums   every row in groups of 2048 entries, a wave each: the group's largest logit, its mass relative
@@ -192,9 +192,8 @@ struct StatShared {
   };
   uint32_t cnt[kVerBins];
   uint64_t redm[2][kMaxWaves];
-  double redd[2][kMaxWaves];
   uint32_t redc[2][kMaxWaves], rede[2][kMaxWaves];
-  float redf[2][kMaxWaves], redg[2][kMaxWaves];
+  float redf[2][kMaxWaves];
   alignas(16) float cand[kVerCand];
   uint64_t candm[kVerCand];
   int n_cand, bin;
@@ -235,33 +234,11 @@ __device__ __forceinline__ float lanes_fmax(float x) {
 // overwrites a buffer only behind the barrier that every wave reaches after reading it.  W lanes add the W
 // waves' values.
 template <int W>
-__device__ __forceinline__ void block_max2(StatShared& sh, int& par, float& a, float& b) {
-  a = wave_fmax(a);
-  b = wave_fmax(b);
-  if ((threadIdx.x & 63) == 0) {
-    sh.redf[par][threadIdx.x >> 6] = a;
-    sh.redg[par][threadIdx.x >> 6] = b;
-  }
-  __syncthreads();
-  a = lanes_fmax<W>(sh.redf[par][threadIdx.x & (W - 1)]);
-  b = lanes_fmax<W>(sh.redg[par][threadIdx.x & (W - 1)]);
-  par ^= 1;
-}
-template <int W>
 __device__ __forceinline__ float block_max(StatShared& sh, int& par, float a) {
   a = wave_fmax(a);
   if ((threadIdx.x & 63) == 0) sh.redf[par][threadIdx.x >> 6] = a;
   __syncthreads();
   a = lanes_fmax<W>(sh.redf[par][threadIdx.x & (W - 1)]);
-  par ^= 1;
-  return a;
-}
-template <int W>
-__device__ __forceinline__ double block_sum(StatShared& sh, int& par, double a) {
-  a = wave_add(a);
-  if ((threadIdx.x & 63) == 0) sh.redd[par][threadIdx.x >> 6] = a;
-  __syncthreads();
-  a = lanes_add<W>(sh.redd[par][threadIdx.x & (W - 1)]);
   par ^= 1;
   return a;
 }
@@ -505,7 +482,8 @@ __device__ __forceinline__ Draft load_draft(const VerifyArgs& p, int b, int k) {
 // With top_p alone the kept mass is top_p S exactly, so p(d) <= x_d / (top_p S), which rejects many a draft
 // without tau; and if tau <= l_d, p(d) >= (x_d - (1 - top_p) S) / (top_p S) (the entries above d hold at most
 // S - n x_d if n are tied with it, so d keeps (top_p S - (S - n x_d)) / n or all of x_d), which also says that
-// tau <= l_d where it is positive.  Margins of 1e-9 for the rounding of either side.
+// tau <= l_d where it is positive.  Margins of 1e-7 for the rounding of either side: 2^19 units of 2^-43 at most
+// (6e-8) where all of a row's masses round the same way; a rejection here and the full test never disagree.
 enum { kUnsure, kAccept, kReject };
 template <bool kHalf>
 __device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int lane) {
@@ -514,8 +492,8 @@ __device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int
   if (!d.in) return kReject;
   const double x = exp2_neg((double)read_as(d.l, s.mode) - (double)s.max, p.scale, p.d_min);
   const double goal = p.top_p * s.mass, uq = (double)d.u * (double)d.q;
-  if (!(uq * goal < x * (1.0 + 1.0e-9))) return kReject;
-  return uq * goal < (x - (1.0 - p.top_p) * s.mass) - 1.0e-9 * s.mass ? kAccept : kUnsure;
+  if (!(uq * goal < x * (1.0 + 1.0e-7))) return kReject;
+  return uq * goal < (x - (1.0 - p.top_p) * s.mass) - 1.0e-7 * s.mass ? kAccept : kUnsure;
 }
 
 // kLists: the groups' lists are searched first.  A row that is searched as a whole is read twice more:
@@ -1186,6 +1164,11 @@ VerifySpace verify_space(int64_t B, int64_t K, int64_t V) {
   return w;
 }
 
+// A launch has fewer than 2^32 threads: 256 per 8192 entries of a row, 1024 per row.
+bool verify_rows_fit(int64_t B, int64_t K, int64_t V) {
+  return B * (K + 1) <= (1 << 22) / std::max<int64_t>(4, (V + 8191) / 8192);
+}
+
 // Lists pay where they nearly always reach down to the top_k-th entry.  The r-th largest of 16 lane maxima
 // of 32 entries each has about 64 (-ln(1 - r / 16)) of a group's 2048 entries above it; the largest r
 // that leaves the list a third of room is taken.  That has to hold a group's share of the top_k: m = top_k
@@ -1206,7 +1189,7 @@ void use_lists(VerifyArgs& a) {
 using namespace vk;
 
 extern "C" int64_t vkwr_sampling_verify_workspace_bytes(int B, int K, int V) {
-  if (B <= 0 || K < 0 || V <= 0) return 0;
+  if (B <= 0 || K < 0 || V <= 0 || V > kVerMaxV || !verify_rows_fit(B, K, V)) return 0;  // refused
   return verify_space(B, K, V).bytes;
 }
 
@@ -1222,8 +1205,7 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
              "%s: vocabulary size must be a multiple of 4 and at most 1048576, got %d", fn, V);
   VK_REQUIRE(temperature >= 0.001 && temperature <= 1000, "%s: temperature %g outside [0.001, 1000]", fn,
              temperature);
-  // (256 threads per 8192 entries of a row, 1024 per row: fewer than 2^32 in a launch)
-  VK_REQUIRE((int64_t)B * ((int64_t)K + 1) <= (1 << 21) / ((V + 131071) / 131072), "%s: B*(K+1) too large", fn);
+  VK_REQUIRE(verify_rows_fit(B, K, V), "%s: B*(K+1) too large", fn);
   if (B == 0) return VKWR_OK;
   VK_REQUIRE(logits && uniforms && tokens && accepted && (K == 0 || drafts), "%s: null pointer", fn);
   VK_REQUIRE((uintptr_t)logits % (logits_f16 ? 8 : 16) == 0 && (uintptr_t)draft_probs % 16 == 0,
