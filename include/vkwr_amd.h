@@ -112,7 +112,8 @@ VKWR_EXPORT int vkwr_wkv7_fp32_step_rows_slots(int B, int C, int H, float* pool,
  * products are in the order of vkwr_wkv7_fp32_step_rows_slots: P + T tokens give the bits of that
  * many of its steps.  slots distinct; a slot outside [0, n_slots), a kept count outside [0, P] or,
  * where kept[i] > 0, a pending row outside [0, n_pending) makes the sequence's y rows NaN and leaves
- * its pool entry untouched.  pool and token vectors 16-byte aligned.  No counterpart in the reference. */
+ * its pool entry untouched.  pool and token vectors 16-byte aligned, P + T <= 2^24.  No counterpart in
+ * the reference. */
 VKWR_EXPORT int vkwr_wkv7_fp32_drafts_slots(int B, int P, int T, int C, int H, float* pool, int n_slots,
                                             const int32_t* slots, const int32_t* kept, int n_pending,
                                             const int32_t* pending_rows, const uint16_t* pw,
@@ -537,10 +538,13 @@ typedef struct vkwr_lora_target {
 VKWR_EXPORT int64_t vkwr_lora_workspace_bytes(int64_t m, int n_adapters, int rank, int n_targets,
                                               const vkwr_lora_target* targets);
 
-/* 1..8 projections in two launches, on a plan made for the same m and n_adapters (with another one
- * nothing is written).  scale [n_adapters] fp32 (device) or NULL (1).  rank a multiple of 8 up to 128
- * (zero rows and columns pad an adapter of lower rank exactly), n and k multiples of 8; all pointers 16-byte aligned.  y must not
- * overlap any x, another y or base, nor its own base unless they are equal (rejected). */
+/* 1..8 projections in two launches, on a plan that vkwr_lora_plan has filled, in a buffer of
+ * vkwr_lora_plan_bytes(m, n_adapters) bytes or more (one made for another m or n_adapters: nothing is
+ * written).  scale [n_adapters] fp32 (device) or NULL (1).  rank a multiple of 8 up to 128 (zero rows and
+ * columns pad an adapter of lower rank exactly), n and k multiples of 8; all pointers 16-byte aligned.
+ * y must not overlap any x, another y or base, nor its own base unless they are equal (rejected).  Calls
+ * that may run at the same time (two streams, two replayed graphs) need workspaces of their own, and
+ * vkwr_lora_plan must not run beside calls that read the plan it fills. */
 VKWR_EXPORT int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* scale, const void* plan,
                               int n_targets, const vkwr_lora_target* targets, void* workspace,
                               int64_t workspace_bytes, void* stream);
@@ -691,8 +695,9 @@ VKWR_EXPORT int vkwr_sampling_repetition_topk_topp(int B, int T, int V, const fl
  * accepted [B] int32: the number of accepted drafts.  n_draft outside [0, K]: accepted -1 and every
  * token -1.  A draft outside [0, V) has p = 0.  Deterministic, and independent of the batch.
  * V, temperature, top_k, top_p as above; logits 16-byte (fp16: 8-byte) and draft_probs 16-byte
- * aligned; workspace: vkwr_sampling_verify_workspace_bytes(B, K, V) bytes, 16-byte aligned.
- * No counterpart in the reference. */
+ * aligned; workspace: vkwr_sampling_verify_workspace_bytes(B, K, V) bytes (0 for sizes that are refused;
+ * it grows with B and K), 16-byte aligned, one for each of the calls that may run at the same time.
+ * tokens and accepted must not overlap the inputs.  No counterpart in the reference. */
 VKWR_EXPORT int64_t vkwr_sampling_verify_workspace_bytes(int B, int K, int V);
 VKWR_EXPORT int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logits, int logits_f16,
                                             const int32_t* drafts, const int32_t* n_draft,

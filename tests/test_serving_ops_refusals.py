@@ -28,6 +28,10 @@ def test_wkv_drafts_refuses(change, text):
     assert drafts(**change) == 1 and text in err()
 
 
+def test_wkv_drafts_refuses_too_many_tokens():
+    assert drafts(B=1, H=1, C=64, T=2 ** 24) == 1 and "too large" in err()
+
+
 def test_wkv_drafts_empty_work():
     assert drafts(B=0) == 0
     assert drafts(Pn=0, T=0, kept=None) == 0
@@ -56,6 +60,14 @@ def test_verify_sizes():
     assert verify(B=0) == 0
     assert capi.verify_workspace_bytes(2, 2, 8) >= 192
     assert capi.verify_workspace_bytes(0, 2, 8) == 0
+
+
+@pytest.mark.parametrize("V,rows", [(8, 1 << 20), (32768, 1 << 20), (65536, 1 << 19), (1 << 20, 1 << 15)])
+def test_verify_launch_limits(V, rows):
+    assert verify(B=rows, K=0, V=V) == 1 and "workspace" in err()  # the size itself is taken
+    assert verify(B=rows + 1, K=0, V=V) == 1 and "too large" in err()
+    assert capi.verify_workspace_bytes(rows, 0, V) > 0 and capi.verify_workspace_bytes(rows + 1, 0, V) == 0
+    assert capi.verify_workspace_bytes(2 ** 30, 2 ** 30, V) == 0 and capi.verify_workspace_bytes(1, 1, 1 << 21) == 0
 
 
 def target(n=64, k=64, x=0x10000, a=0x20000, b=0x30000, base=None, y=0x40000, epilogue=0):

@@ -585,20 +585,20 @@ def lora_target(x, a, b, y, base=None, epilogue=EPI_NONE):
     at = _Tensors()
     t = LoraTarget(at(x, h, m * k, "x"), at(a, h, G * rank * k, "a"), at(b, h, G * n * rank, "b"),
                    at.optional(base, h, m * n, "base"), at(y, h, m * n, "y"), n, k, epilogue)
-    t.sizes = (m, G, rank)
+    t.sizes = (m, G, rank, at.dev)
     t.tensors = (x, a, b, y, base)  # what the pointers point to
     return t
 
 
 def _lora_targets(targets):
     if not 1 <= len(targets) <= LORA_MAX_TARGETS or any(t.sizes != targets[0].sizes for t in targets):
-        raise ValueError("lora: 1 to 8 targets with the same rows, adapters and rank")
+        raise ValueError("lora: 1 to 8 targets with the same rows, adapters, rank and device")
     return targets[0].sizes, (LoraTarget * len(targets))(*targets)
 
 
 def lora_workspace_bytes(max_rows, n_adapters, targets):
     """Workspace of `lora` for these targets at any row count up to max_rows."""
-    (_, G, rank), arr = _lora_targets(targets)
+    (_, G, rank, _), arr = _lora_targets(targets)
     n = _lora_ws(max_rows, n_adapters, rank, len(targets), arr)
     if n < 0:
         raise RuntimeError(f"vkwr_lora_workspace_bytes: {_LIB.vkwr_last_error().decode()}")
@@ -609,12 +609,15 @@ def lora(plan, targets, scale=None, workspace=None):
     """Adds each row's adapter to 1..8 projections that the rows of `plan` go through (vkwr_lora_f16): the
     first plan.m rows of the targets, the others are left as they were.  scale: fp32 [G] (None: 1).
     workspace: uint8, lora_workspace_bytes (None: allocated)."""
-    (rows, G, rank), arr = _lora_targets(targets)
+    (rows, G, rank, _), arr = _lora_targets(targets)
     m = plan.m
     if m is None or m > rows or plan.n_adapters != G:
         raise ValueError(f"lora: plan of {m} rows and {plan.n_adapters} adapters, targets of {rows} and {G}")
     if workspace is None:
         workspace = torch.empty(lora_workspace_bytes(m, G, targets), dtype=torch.uint8, device=plan.buf.device)
     at, nbytes = _Tensors(), workspace.numel()
-    _check(_lora(m, G, rank, at.optional(scale, torch.float32, G, "scale"), plan.buf.data_ptr(), len(targets), arr,
+    if targets[0].sizes[3] != at.dev:
+        raise ValueError(f"lora: targets on cuda:{targets[0].sizes[3]}, but the current device is cuda:{at.dev}")
+    _check(_lora(m, G, rank, at.optional(scale, torch.float32, G, "scale"),
+                 at(plan.buf, torch.uint8, plan.buf.numel(), "plan"), len(targets), arr,
                  at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()), "vkwr_lora_f16")

@@ -218,7 +218,7 @@ __device__ __forceinline__ void shrink_steps(const _Float16* xr, const _Float16*
 // Tiles of three or four blocks (prompt chunks) go through LDS: the 16 rows of an operand, 2 K bytes apart,
 // fall on the same sets of the vector cache, so that operands loaded straight into registers, 64 bytes of
 // a row at a time, came in twice (four projections of 2304 rows, K = 4096, rank 64: 107 us; through LDS
-// {STAGED_US}).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
+// 35.5).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
 // chunk c at place c ^ (r & 7) -- in a ring of four, three of them in flight.
 constexpr int kShrinkWaves = 8;
 constexpr int kStageK = 64, kStages = 4;
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraA
   fv4(*const lds)[RT][64] = reinterpret_cast<fv4(*)[RT][64]>(smem);
   static_assert((kShrinkWaves - 1) * kRankBlock / 16 * 1024 <= kStages * kStageHalfs * 2, "the sums fit");
   const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
-  const Tile tile = plan_tiles(p.plan)[blockIdx.y];  // blockIdx.y < tiles_cap: in the buffer, if stale
+  const Tile tile = plan_tiles(p.plan)[blockIdx.y];  // blockIdx.y < tiles_cap: inside the plan, stale or not
   if ((int)blockIdx.y >= head.n_adapter || head.m != p.m || head.G != p.G) return;
   const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
   const int ti = blockIdx.z / p.rank_blocks, r0 = (blockIdx.z - ti * p.rank_blocks) * kRankBlock;

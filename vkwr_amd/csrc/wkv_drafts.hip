@@ -191,7 +191,7 @@ extern "C" int vkwr_wkv7_fp32_drafts_slots(int B, int P, int T, int C, int H, fl
   VK_REQUIRE(B >= 0 && P >= 0 && T >= 0 && H >= 0 && n_slots >= 0 && n_pending >= 0,
              "%s: negative size (B=%d P=%d T=%d H=%d n_slots=%d n_pending=%d)", fn, B, P, T, H, n_slots, n_pending);
   VK_REQUIRE(C == (int64_t)H * kHead, "%s: only head size 64 is supported (C=%d H=%d)", fn, C, H);
-  VK_REQUIRE((int64_t)B * H < (1 << 23) && (int64_t)P + T <= 0x7fffffff, "%s: B*H or P+T too large", fn);
+  VK_REQUIRE((int64_t)B * H < (1 << 23) && (int64_t)P + T <= (1 << 24), "%s: B*H or P+T too large", fn);
   VK_REQUIRE((kept != nullptr) == (P > 0), "%s: kept must be given exactly when P > 0", fn);
   if (B == 0 || H == 0 || P + T == 0) return VKWR_OK;
   VK_REQUIRE(pool && slots, "%s: null pointer", fn);
