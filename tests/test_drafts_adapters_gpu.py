@@ -249,3 +249,87 @@ def test_sampled_speculation_with_filter(gpu):
         runs.append([r.output for r in reqs])
         assert all(len(o) == 12 and all(0 <= t < cfg.vocab for t in o) for o in runs[-1])
     assert runs[0] == runs[1]
+
+
+def test_step_writes_the_kept_tokens_first(gpu):
+    """A plain step after a draft step equals one after an explicit flush; another state's step leaves the
+    kept tokens for theirs."""
+    from vkwr.model_executor import DraftEngine
+    cfg, model, state = _tiny(gpu, 6)
+    g = torch.Generator().manual_seed(31)
+    tok = torch.randint(0, cfg.vocab, (2, 3), generator=g).to(torch.int32).to(gpu)
+    pre = torch.randint(0, cfg.vocab, (1, 4), generator=g).to(torch.int32).to(gpu)
+    runs = []
+    for explicit in (True, False):
+        eng, s, other = DraftEngine(model, 2, 2, max_rows=16), _clone(state), _clone(state)
+        eng.draft_step(s, tok, [3, 5])
+        with pytest.raises(RuntimeError):
+            eng.step(s, decode=(_i32([1], gpu), _i32([3], gpu)))
+        eng.accept(_i32([2, 0], gpu))
+        eng.step(other, decode=(_i32([1], gpu), _i32([3], gpu)))
+        assert set(eng.rows_of) == {3, 5}
+        if explicit:
+            eng.flush(s, [5, 3, 5])
+        out = eng.step(s, decode=(_i32([7], gpu), _i32([3], gpu)), prefill=[(pre, _i32([5], gpu))]).clone()
+        assert not eng.rows_of
+        runs.append((out, s.wkv, s.att_shift))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_padding_behind_short_drafts_is_free(gpu):
+    from vkwr.model_executor import DraftEngine
+    cfg, model, state = _tiny(gpu, 4)
+    outs = []
+    for pad in (0, -1, 2 ** 31 - 1):
+        eng, s = DraftEngine(model, 2, 3), _clone(state)
+        tok = _i32([[5, 6, pad, pad], [9, 10, 11, 12]], gpu)
+        lg = eng.draft_step(s, tok, [2, 0]).clone()
+        eng.accept(_i32([1, 2], gpu))
+        eng.flush(s)
+        outs.append((lg[0, :2], lg[1], s.wkv, s.att_shift))
+    for o in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(o, outs[0]))
+
+
+def test_engines_refuse_wrong_counts(gpu):
+    from vkwr.model_executor import DraftEngine
+    cfg, model, state = _tiny(gpu, 4)
+    eng = DraftEngine(model, 2, 2, adapters=_pool(model, gpu)[0])
+    dec = (_i32([3, 9], gpu), _i32([0, 2], gpu))
+    tok = _i32([[1, 2], [3, 4]], gpu)
+    before = state.wkv.clone()
+    for ids in (_i32([1], gpu), _i32([1, 0, 2], gpu), torch.tensor([1, 0], device=gpu)):
+        with pytest.raises(ValueError):
+            eng.step(state, decode=dec, adapter_ids=ids)
+        with pytest.raises(ValueError):
+            eng.draft_step(state, tok, [0, 2], adapter_ids=ids)
+    assert torch.equal(state.wkv, before)
+    eng.draft_step(state, tok, [0, 2], adapter_ids=_i32([1, -1], gpu))
+    for acc in (_i32([1], gpu), torch.tensor([1, 1], device=gpu), torch.tensor([1, 1], dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            eng.accept(acc)
+    eng.accept(_i32([1, 1], gpu))  # still open
+    eng.flush(state)
+
+
+def test_more_prompt_chunks_than_draft_rows(gpu):
+    from vkwr.model_executor import DraftEngine, SpeculativeBatcher
+    cfg, model, state = _tiny(gpu, 6)
+    eng = DraftEngine(model, 1, 7, max_rows=64)
+    sched = SpeculativeBatcher(eng, state, max_prefill_chunks=6, chunk=8)
+    reqs = [sched.submit([3 + i, 4, 5, 3 + i, 4], 4) for i in range(6)]
+    assert len(sched.run()) == 6
+    for r in reqs:
+        _replay(model, r, gpu)
+
+
+def test_adapters_scratch_is_whole_from_the_start(gpu):
+    """Steps of every size, in any order, run in the scratch that the engine was built with."""
+    from vkwr.model_executor import MixedEngine
+    cfg, model, state = _tiny(gpu, 8)
+    eng = MixedEngine(model, 64, adapters=_pool(model, gpu)[0])
+    at = eng.adapters.ws.data_ptr()
+    for T in (1, 9, 2, 60):
+        tok = torch.ones(1, T, dtype=torch.int32, device=gpu)
+        eng.step(state, prefill=[(tok, _i32([1], gpu))], adapter_ids=_i32([2], gpu))
+    assert eng.adapters.ws.data_ptr() == at

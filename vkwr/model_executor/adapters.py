@@ -60,38 +60,44 @@ class AdapterPool:
 
 
 class AdapterStep:
-    """What an engine keeps to run a pool's adapters: the rows' indices and their plan, the projections'
-    descriptions and the scratch."""
+    """What an engine keeps to run a pool's adapters: the rows' indices and their plan, and scratch for all
+    the sets of projections that `targets` has described."""
 
     def __init__(self, pool, max_rows, device):
         self.pool, self.max_rows = pool, max_rows
         self.ids = torch.empty(max_rows, dtype=torch.int32, device=device)
         self.plan = capi.lora_plan_empty(max_rows, pool.n_adapters, device)
-        self.targets, self.ws = {}, torch.empty(0, dtype=torch.uint8, device=device)
+        self.ws = torch.empty(0, dtype=torch.uint8, device=device)
+
+    def targets(self, layer, items, epilogue=capi.EPI_NONE):
+        """The pool's projections among items (name, x, y): y, of the engine's full-size buffers, gets the
+        adapters added in place.  Called while the engine is built, so that the scratch is never replaced
+        under a captured step."""
+        items = [it for it in items if it[0] in self.pool.names]
+        if not items:
+            return None
+        L = self.pool.layers[layer]
+        rows = min(t.shape[0] for _, x, y in items for t in (x, y))
+        ts = [capi.lora_target(x[:rows], *L[n], y[:rows], epilogue=epilogue) for n, x, y in items]
+        need = capi.lora_workspace_bytes(self.max_rows, self.pool.n_adapters, ts)
+        if need > self.ws.numel():
+            self.ws = torch.empty(need, dtype=torch.uint8, device=self.ids.device)
+        return ts
 
     def begin(self, groups, adapter_ids):
         """groups: (B, T, first row, first sequence); adapter_ids int32 [sequences] on the device."""
+        n = sum(B for B, _, _, _ in groups)
+        if adapter_ids.dtype != torch.int32 or tuple(adapter_ids.shape) != (n,):
+            raise ValueError(f"adapter_ids: expected int32 [{n}], got {adapter_ids.dtype} {tuple(adapter_ids.shape)}")
         rows = 0
         for B, T, r0, q0 in groups:
             self.ids[r0:r0 + B * T].view(B, T).copy_(adapter_ids[q0:q0 + B, None])
             rows = max(rows, r0 + B * T)
         capi.lora_plan(self.ids[:rows], self.plan)
 
-    def add(self, layer, items, epilogue=capi.EPI_NONE):
-        """Adds the adapters of `layer` to the projections (name, x, y) of full-size buffers, in place."""
-        items = [it for it in items if it[0] in self.pool.names]
-        if not items:
-            return
-        key = (layer, epilogue) + tuple((n, x.data_ptr(), y.data_ptr()) for n, x, y in items)
-        ts = self.targets.get(key)
-        if ts is None:
-            L = self.pool.layers[layer]
-            rows = min(t.shape[0] for _, x, y in items for t in (x, y))
-            ts = self.targets[key] = [capi.lora_target(x[:rows], *L[n], y[:rows], epilogue=epilogue) for n, x, y in items]
-            need = capi.lora_workspace_bytes(self.max_rows, self.pool.n_adapters, ts)
-            if need > self.ws.numel():
-                self.ws = torch.empty(need, dtype=torch.uint8, device=self.ids.device)
-        capi.lora(self.plan, ts, scale=self.pool.scale, workspace=self.ws)
+    def add(self, targets):
+        if targets is not None:
+            capi.lora(self.plan, targets, scale=self.pool.scale, workspace=self.ws)
 
 
 __all__ = ["AdapterPool", "AdapterStep", "ADAPTED"]

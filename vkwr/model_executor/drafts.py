@@ -13,8 +13,8 @@ rejected tokens again, so the step leaves the states alone:
           shift pools.
 
 Between steps the WKV pool is behind by the kept tokens of the sequences of the last draft step: `flush`
-writes them (before the pool is read by anything else), `drop` forgets them (finished sequences).
-Sequences that a draft step leaves out are flushed by it.
+writes them (before the pool is read by anything else), `drop` forgets them (finished sequences, slots that
+are reset).  Sequences that a draft step leaves out are flushed by it, all of them by `step`.
 
 Per layer as MixedEngine's step, with the fused LayerNorm + shift launches replaced by LayerNorm (its rows
 kept) and a token shift on gathered shift rows.
@@ -48,11 +48,22 @@ class DraftEngine(MixedEngine):
         self.rows_of = {}        # slot -> its sequence in the last draft step, where tokens are to be written
         self.T, self.kept = 0, None
         self.pool_of = None
+        if adapters is not None:  # layer 0's values go to the kept vectors
+            self.adapted_first = [self._adapted_rkv(0, self.pend[i][0]["v"]) for i in range(2)]
+
+    def step(self, state, decode=None, prefill=(), adapter_ids=None, flush=True):
+        """MixedEngine's step, the kept tokens written first.  flush=False: not (for the caller whose
+        slots here have none)."""
+        if self.open is not None:
+            raise RuntimeError("step: the last step's drafts are not accepted yet")
+        if flush and self.pool_of is state.wkv:
+            self.flush(state)
+        return super().step(state, decode, prefill, adapter_ids)
 
     def draft_step(self, state, tokens, slots, adapter_ids=None):
         """tokens [B, T] int32 on the device (the last generated token, then the drafts; anything behind a
-        short draft), slots: B distinct slot numbers (host).  Returns logits [B, T, V] (a view valid until
-        the next step); `accept` has to follow."""
+        short draft: a number outside the vocabulary runs as the nearest inside), slots: B distinct slot
+        numbers (host).  Returns logits [B, T, V] (a view valid until the next step); `accept` has to follow."""
         B, T = tokens.shape
         slots = [int(i) for i in slots]
         if self.open is not None:
@@ -66,6 +77,7 @@ class DraftEngine(MixedEngine):
             raise ValueError("draft_step: the row-major WKV pool is needed")
         if self.rows_of and self.pool_of is not state.wkv:
             raise RuntimeError("draft_step: kept tokens of another state are not written yet (flush)")
+        adapters = self._begin_adapters([(B, T, 0, None, 0)], adapter_ids)
         self.flush(state, [i for i in self.rows_of if i not in set(slots)])
         cfg, m, s = self.cfg, self.model, self
         C, H, R, ws = cfg.n_embd, cfg.n_head, B * T, self.ws
@@ -82,9 +94,8 @@ class DraftEngine(MixedEngine):
         att = state.att_shift.index_select(1, sl64)  # [L, B, C]
         ffn = state.ffn_shift.index_select(1, sl64)
         att0, ffn0 = att.clone(), ffn.clone()
-        s.tok[:R].copy_(tokens.reshape(-1))
+        s.tok[:R].copy_(tokens.reshape(-1).clamp(0, cfg.vocab - 1))
         torch.index_select(m.emb, 0, s.tok[:R], out=s.x0[:R])
-        adapters = self._begin_adapters([(B, T, 0, None, 0)], adapter_ids)
         own = s.w, s.v_first, s.v_new
         x, res_in = s.x0[:R], None
         try:
@@ -102,8 +113,7 @@ class DraftEngine(MixedEngine):
                 capi.token_shift(B, T, C, y, att[l], [L[k] for k in TMIX_MIX], [t[:R] for t in s.mix])
                 capi.gemm(self._proj(L, s.lw[l], R, first), ws)
                 if adapters is not None:
-                    adapters.add(l, [("Wr", s.mix[0], s.r), ("Wk", s.mix[2], s.k),
-                                     ("Wv", s.mix[3], s.v_first if first else s.v)])
+                    adapters.add(self.adapted_first[self.which ^ 1] if first else self.adapted[l]["rkv"])
                 capi.gemm(self._rank_out(L, s.lw[l], R, first), ws)
                 v = N["v"][:R]
                 capi.kk_a_gate(R, 1, C, H, s.k[:R], L["k_k"], L["a0"], s.a12[:R], L["k_a"], N["new_k"][:R],
@@ -117,7 +127,7 @@ class DraftEngine(MixedEngine):
                                           L["lnx_b"], s.g[:R], s.o_in[:R])
                 capi.gemm([capi.gemm_problem(s.o_in[:R], L["Wo"], s.o[:R])], ws)
                 if adapters is not None:
-                    adapters.add(l, [("Wo", s.o_in, s.o)])
+                    adapters.add(self.adapted[l]["o"])
                 res2 = s.res[0][:R]
                 y = self.ys[1][l, :R]
                 capi.layer_norm(s.o[:R], L["ln2_w"], L["ln2_b"], y, residual=res, x_out=res2)
@@ -140,8 +150,9 @@ class DraftEngine(MixedEngine):
             raise RuntimeError("accept: no draft step is open")
         state, slots, sl, att0, ffn0 = self.open
         B, T = self.B, self.T
-        if accepted.numel() != B:
-            raise ValueError(f"accept: {accepted.numel()} counts for {B} sequences")
+        if tuple(accepted.shape) != (B,) or accepted.dtype != torch.int32 or accepted.device != sl.device:
+            raise ValueError(f"accept: expected int32 [{B}] on {sl.device}, got {accepted.dtype} "
+                             f"{tuple(accepted.shape)} on {accepted.device}")
         self.open = None
         self.kept = (accepted + 1).clamp(min=0, max=T).to(torch.int32)
         last = (self.kept - 1).clamp(min=0).long()
@@ -156,7 +167,7 @@ class DraftEngine(MixedEngine):
         """Writes the kept tokens of these slots (None: all) to the WKV pool."""
         if self.open is not None:
             raise RuntimeError("flush: the last step's drafts are not accepted yet")
-        todo = [i for i in (self.rows_of if slots is None else slots) if i in self.rows_of]
+        todo = [i for i in dict.fromkeys(self.rows_of if slots is None else slots) if i in self.rows_of]
         if not todo:
             return
         if self.pool_of is not state.wkv:

@@ -34,8 +34,7 @@ With `adapters` (adapters.py) each sequence of a step may have a low-rank adapte
 shared projections: x A^T B^T is added to r, k, v before the low-rank outputs, to o, to the FFN key before
 the squared ReLU (which the adapters' launch then applies) and to the FFN value.
 
-Every buffer is preallocated for `max_rows` rows, so a step allocates nothing (the adapters' scratch
-grows to its size in the first steps).
+Every buffer is preallocated for `max_rows` rows, so a step allocates nothing.
 """
 import torch
 
@@ -111,7 +110,10 @@ class MixedEngine:
         self.side = torch.cuda.Stream(device=dev) if dev.type == "cuda" else None
         self.fork = torch.cuda.Event() if dev.type == "cuda" else None
         self.join = torch.cuda.Event() if dev.type == "cuda" else None
-        self.adapters = None if adapters is None else AdapterStep(adapters, max_rows, dev)
+        self.adapters, self.adapted = None, []
+        if adapters is not None:
+            self.adapters = AdapterStep(adapters, max_rows, dev)
+            self.adapted = [self._adapted(l) for l in range(cfg.n_layer)]
 
     # -- GEMM batches (shared by planning and execution)
     def _proj(self, L, W, R, first):
@@ -183,6 +185,17 @@ class MixedEngine:
             s.join.record(s.side)
             main.wait_event(s.join)
 
+    def _adapted_rkv(self, l, v):
+        s = self
+        return s.adapters.targets(l, [("Wr", s.mix[0], s.r), ("Wk", s.mix[2], s.k), ("Wv", s.mix[3], v)])
+
+    def _adapted(self, l):
+        """Layer l's adapters: the sets of projections that one pair of launches each takes."""
+        s, t = self, self.adapters.targets
+        return {"rkv": s._adapted_rkv(l, s.v if l else s.v_first),
+                "o": t(l, [("Wo", s.o_in, s.o)]), "key": t(l, [("key", s.xk, s.act)], capi.EPI_RELU_SQUARE),
+                "value": t(l, [("value", s.act, s.ffn)])}
+
     def _begin_adapters(self, groups, adapter_ids):
         """The step's adapters, or None.  groups: (B, T, first row, slots, first sequence)."""
         if adapter_ids is None:
@@ -196,13 +209,13 @@ class MixedEngine:
         """relu(xk K^T)^2 V^T of the rows, into ffn."""
         s, gp = self, capi.gemm_problem
         square = capi.EPI_RELU_SQUARE
-        late = adapters is not None and "key" in adapters.pool.names  # the square follows the adapters
+        late = adapters is not None and self.adapted[l]["key"] is not None  # the square follows the adapters
         capi.gemm([gp(s.xk[:R], L["key"], s.act[:R], epilogue=capi.EPI_NONE if late else square)], s.ws)
         if late:
-            adapters.add(l, [("key", s.xk, s.act)], square)
+            adapters.add(self.adapted[l]["key"])
         capi.gemm([gp(s.act[:R], L["value"], s.ffn[:R])], s.ws)
         if adapters is not None:
-            adapters.add(l, [("value", s.act, s.ffn)])
+            adapters.add(self.adapted[l]["value"])
 
     def _head_problem(self, S):
         return [capi.gemm_problem(self.h[:S], self.model.head, self.logits[:S])]
@@ -248,8 +261,7 @@ class MixedEngine:
                                        [t[:R] for t in s.mix], state.att_shift[l], shift_groups, residual=res_in)
             capi.gemm(self._proj(L, s.lw[l], R, first), ws)
             if adapters is not None:
-                adapters.add(l, [("Wr", s.mix[0], s.r), ("Wk", s.mix[2], s.k),
-                                 ("Wv", s.mix[3], s.v_first if first else s.v)])
+                adapters.add(self.adapted[l]["rkv"])
             capi.gemm(self._rank_out(L, s.lw[l], R, first), ws)
             v = (s.v_first if first else s.v_new)[:R]
             capi.kk_a_gate(R, 1, C, H, s.k[:R], L["k_k"], L["a0"], s.a12[:R], L["k_a"], s.new_k[:R],
@@ -257,7 +269,7 @@ class MixedEngine:
             self._wkv_gn(groups, state.wkv[l], v, L)
             capi.gemm([capi.gemm_problem(s.o_in[:R], L["Wo"], s.o[:R])], ws)
             if adapters is not None:
-                adapters.add(l, [("Wo", s.o_in, s.o)])
+                adapters.add(self.adapted[l]["o"])
             # ---- channel mix
             res2 = s.res[0][:R]
             capi.layer_norm_shift_rows(s.o[:R], L["ln2_w"], L["ln2_b"], res2, [L["x_k_ffn"]], [s.xk[:R]],

@@ -98,7 +98,8 @@ class ContinuousBatcher:
 
     def submit(self, prompt, max_new_tokens, adapter=-1):
         assert len(prompt) >= 1 and max_new_tokens >= 1
-        n = self.engine.adapters.pool.n_adapters if self.engine.adapters is not None else 0
+        adapters = getattr(self.engine, "adapters", None)
+        n = 0 if adapters is None else adapters.pool.n_adapters
         if not -1 <= adapter < n:
             raise ValueError(f"adapter {adapter} of {n}")
         req = Request(list(prompt), max_new_tokens, rid=self._next_id, adapter=adapter)
@@ -123,9 +124,9 @@ class ContinuousBatcher:
             raise RuntimeError(f"invalid slot table for this step: {slots}")
 
     def _adapter_ids(self, reqs):
-        """Adapter indices of these requests, or None where no request has one."""
+        """The step's argument for these requests' adapters, where one of them has any."""
         ids = [r.adapter for r in reqs]
-        return self._i32(ids) if any(i >= 0 for i in ids) else None
+        return {"adapter_ids": self._i32(ids)} if any(i >= 0 for i in ids) else {}
 
     def _admit(self):
         while self.waiting and self.slots.available:
@@ -176,8 +177,8 @@ class ContinuousBatcher:
             toks = self._i32([r.prompt[r.pos:r.pos + t] for r in reqs])
             prefill.append((toks, self._i32([r.slot for r in reqs])))
             order.append((t, reqs))
-        ids = self._adapter_ids(dec + [r for _, reqs in order for r in reqs])
-        logits = self.engine.step(self.state, decode=decode, prefill=prefill, adapter_ids=ids)
+        logits = self.engine.step(self.state, decode=decode, prefill=prefill,
+                                  **self._adapter_ids(dec + [r for _, reqs in order for r in reqs]))
         nxt = self.sample(logits).tolist()
         for i, r in enumerate(dec):
             r.output.append(nxt[i])
@@ -228,8 +229,9 @@ class SpeculativeBatcher(ContinuousBatcher):
         B, T = engine.draft_seqs, engine.max_draft + 1
         self.draft, self.filter = draft, dict(temperature=temperature, top_k=top_k, top_p=top_p)
         self.gen = torch.Generator(device=self.device).manual_seed(seed)
-        self.ws = torch.empty(capi.verify_workspace_bytes(B, T - 1, engine.cfg.vocab), dtype=torch.uint8,
-                              device=self.device)
+        V = engine.cfg.vocab
+        need = max(capi.verify_workspace_bytes(B, T - 1, V), capi.verify_workspace_bytes(self.max_prefill_chunks, 0, V))
+        self.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self.drafted = self.accepted = 0
 
     def _verify(self, logits, drafts, n_draft):
@@ -260,7 +262,8 @@ class SpeculativeBatcher(ContinuousBatcher):
             self._check_slots(flat)
             prefill = [(self._i32([r.prompt[r.pos:r.pos + t] for r in reqs]), self._i32([r.slot for r in reqs]))
                        for t, reqs in order]
-            logits = self.engine.step(self.state, prefill=prefill, adapter_ids=self._adapter_ids(flat))
+            # (a prompt's slot is fresh: no kept tokens)
+            logits = self.engine.step(self.state, prefill=prefill, flush=False, **self._adapter_ids(flat))
             none = torch.empty(len(flat), 0, dtype=torch.int32, device=self.device)
             nxt = self._verify(logits[:, None, :], none, None)[0][:, 0].tolist()
             for (t, r), token in zip([(t, r) for t, reqs in order for r in reqs], nxt):
@@ -278,7 +281,7 @@ class SpeculativeBatcher(ContinuousBatcher):
             drafts = [list(self.draft(r.prompt + r.output, min(K, r.max_new_tokens - len(r.output) - 1)))[:K] for r in dec]
             T = 1 + max(len(d) for d in drafts)
             rows = self._i32([[r.output[-1]] + d + [0] * (T - 1 - len(d)) for r, d in zip(dec, drafts)])
-            logits = self.engine.draft_step(self.state, rows, [r.slot for r in dec], adapter_ids=self._adapter_ids(dec))
+            logits = self.engine.draft_step(self.state, rows, [r.slot for r in dec], **self._adapter_ids(dec))
             tokens, accepted = self._verify(logits, rows[:, 1:].contiguous(), self._i32([len(d) for d in drafts]))
             self.engine.accept(accepted)
             for r, d, new, n in zip(dec, drafts, tokens.tolist(), accepted.tolist()):
