@@ -326,13 +326,17 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
 #pragma unroll
   for (int k = 0; k < kGroupSegs; ++k) {
     l[k] = to_f4(raw[k]);
-    const bool in = at0 + k * kSeg < p.V;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      l[k][e] = !in ? -INFINITY : __builtin_isnan(l[k][e]) ? 0.0f : l[k][e];
-      lane_max = fmaxf(lane_max, l[k][e]);
-    }
+    for (int e = 0; e < 4; ++e) l[k][e] = __builtin_isnan(l[k][e]) ? 0.0f : l[k][e];
   }
+  if ((group + 1) * (kGroupSegs * kSeg) > p.V) {  // padding of the last group
+#pragma unroll
+    for (int k = 0; k < kGroupSegs; ++k)
+      if (at0 + k * kSeg >= p.V) l[k] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  }
+#pragma unroll
+  for (int k = 0; k < kGroupSegs; ++k)
+    lane_max = fmaxf(lane_max, fmaxf(fmaxf(l[k][0], l[k][1]), fmaxf(l[k][2], l[k][3])));
   const float mx = wave_fmax(lane_max);
   if (p.cap > 0) {
     // The rank-th largest lane maximum of each row of 16 lanes, the smallest of the four: 4 rank entries
@@ -358,21 +362,22 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
       at = INFINITY;
       count = 0;
     }
-    float2* out = p.list + (id * p.groups + group) * p.cap;
-    int base = 0;
     if (count > 0) {
+      // Lane by lane: a bit per entry, the lanes' places by a scan, then each lane's listed entries (one or
+      // two) read again.
+      uint32_t in = 0;
 #pragma unroll
       for (int k = 0; k < kGroupSegs; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = l[k][e] >= at;
-          const uint64_t m = __ballot(in);
-          if (m == 0) continue;
-          if (in)
-            out[base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] =
-                make_float2(l[k][e], __builtin_bit_cast(float, at0 + k * kSeg + e));
-          base += __builtin_popcountll(m);
-        }
+        for (int e = 0; e < 4; ++e) in |= l[k][e] >= at ? 1u << (4 * k + e) : 0u;
+      const int own = __builtin_popcount(in);
+      float2* out = p.list + (id * p.groups + group) * p.cap + (wave_scan(own, lane) - own);
+      while (in != 0) {
+        const int bit = __builtin_ctz(in), i = at0 + (bit >> 2) * kSeg + (bit & 3);
+        in &= in - 1;
+        const float x = kHalf ? (float)reinterpret_cast<const _Float16*>(row)[i] : reinterpret_cast<const float*>(row)[i];
+        *out++ = make_float2(__builtin_isnan(x) ? 0.0f : x, __builtin_bit_cast(float, i));
+      }
     }
     if (lane == 0) {
       p.group_floor[id * p.groups + group] = at;
@@ -383,8 +388,13 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
   if (p.truncate && !p.use_mass) return;
   double total = 0.0;
   if (mx > -INFINITY) {
-    const bool inf = mx == INFINITY;
-    const double mxd = inf ? 0.0 : (double)mx;
+    if (mx == INFINITY) {
+#pragma unroll
+      for (int k = 0; k < kGroupSegs; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l[k][e] = read_as(l[k][e], kInfOnly);
+    }
+    const double mxd = mx == INFINITY ? 0.0 : (double)mx;
 #pragma unroll
     for (int k0 = 0; k0 < kGroupSegs; k0 += 4) {
       double s[4];
@@ -393,7 +403,7 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
         double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          w[e] = exp2_neg((double)(inf ? read_as(l[k0 + u][e], kInfOnly) : l[k0 + u][e]) - mxd, p.scale, p.d_min);
+          w[e] = exp2_neg((double)l[k0 + u][e] - mxd, p.scale, p.d_min);
         s[u] = (w[0] + w[1]) + (w[2] + w[3]);
       }
       total += (s[0] + s[1]) + (s[2] + s[3]);
@@ -421,32 +431,40 @@ struct RowSummary {
   float floor;  // top_k entries or more lie at or above it (-inf: not known)
   float reach;  // all entries from it up are listed
 };
-__device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id, int lane) {
-  RowSummary r;
-  const bool sums = !p.truncate || p.use_mass;
-  float mx = -INFINITY, below = -INFINITY, reach = -INFINITY, gm = -INFINITY;
-  double gs = 0.0;
-  int count = 0;
-  for (int g = lane; g < p.groups; g += 64) {  // one round up to 131072 entries
-    gm = p.group_max[id * p.groups + g];
-    if (sums) gs = p.group_sum[id * p.groups + g];
-    mx = fmaxf(mx, gm);
+// The lane's first group (up to 131072 entries: its only one), to be requested early.
+struct GroupLoads {
+  float max, floor;
+  double sum;
+  int count;
+};
+__device__ __forceinline__ GroupLoads load_group(const VerifyArgs& p, int64_t id, int g) {
+  GroupLoads x{-INFINITY, -INFINITY, 0.0, 0};
+  if (g < p.groups) {
+    x.max = p.group_max[id * p.groups + g];
+    if (!p.truncate || p.use_mass) x.sum = p.group_sum[id * p.groups + g];
     if (p.cap > 0) {
-      const float f = p.group_floor[id * p.groups + g];
-      below = fmaxf(below, -f);
-      reach = fmaxf(reach, f);
-      count += p.group_count[id * p.groups + g];
+      x.floor = p.group_floor[id * p.groups + g];
+      x.count = p.group_count[id * p.groups + g];
     }
   }
+  return x;
+}
+__device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id, int lane, const GroupLoads& first) {
+  RowSummary r;
+  const bool sums = !p.truncate || p.use_mass;
+  float mx = first.max, below = -INFINITY, reach = -INFINITY;
+  const int count = first.count;  // lists: at most 64 groups
+  if (p.cap > 0 && lane < p.groups) {
+    below = -first.floor;
+    reach = first.floor;
+  }
+  for (int g = lane + 64; g < p.groups; g += 64) mx = fmaxf(mx, p.group_max[id * p.groups + g]);
   mx = wave_fmax(mx);
   double m = 0.0;
   if (sums) {
-    if (p.groups <= 64) {
-      m = gs * group_factor(p, gm, mx);
-    } else {
-      for (int g = lane; g < p.groups; g += 64)
-        m += p.group_sum[id * p.groups + g] * group_factor(p, p.group_max[id * p.groups + g], mx);
-    }
+    m = first.sum * group_factor(p, first.max, mx);
+    for (int g = lane + 64; g < p.groups; g += 64)
+      m += p.group_sum[id * p.groups + g] * group_factor(p, p.group_max[id * p.groups + g], mx);
     m = wave_add(m);
   }
   r.mode = mx == INFINITY ? kInfOnly : mx == -INFINITY ? kAllLow : kNanZero;
@@ -459,6 +477,10 @@ __device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id,
     r.reach = wave_fmax(reach);
   }
   return r;
+}
+
+__device__ __forceinline__ RowSummary summarize(const VerifyArgs& p, int64_t id, int lane) {
+  return summarize(p, id, lane, load_group(p, id, lane));
 }
 
 // Draft k of sequence b: its logit as stored, the drafter's probability and the uniform.
@@ -508,10 +530,32 @@ __global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(VerifyArgs p) 
   __shared__ StatShared sh;
   const int T = p.K + 1;
   const int b = blockIdx.x / T, i = blockIdx.x - b * T;
-  const int n = p.n_draft ? p.n_draft[b] : p.K;
-  if (n < 0 || n > p.K || i > n) return;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = p.V;
   const int64_t id = (int64_t)b * T + i;
+  // What does not depend on another load is requested first, needed or not: the chain of loads is a third
+  // of the kernel's time where the lists decide.  Two listed entries per lane (in the lists' room if not
+  // written).
+  const GroupLoads own_group = load_group(p, id, lane);
+  float2 listed_at[2] = {};
+  int list_group[2] = {}, list_place[2] = {}, list_count[2] = {};
+  if (kLists) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = t + u * kThreads;
+      list_group[u] = at / p.cap;
+      list_place[u] = at - list_group[u] * p.cap;
+      if (list_group[u] < p.groups) {
+        listed_at[u] = p.list[(id * p.groups + list_group[u]) * p.cap + list_place[u]];
+        list_count[u] = p.group_count[id * p.groups + list_group[u]];
+      }
+    }
+  }
+  const int n = p.n_draft ? p.n_draft[b] : p.K;
+  const float last_u = p.u[(int64_t)b * T + p.K];
+  Draft draft{false, 0.0f, 1.0f, 0.0f};
+  if (t == 0 && i < p.K) draft = load_draft<kHalf>(p, b, i);
+  if (n < 0 || n > p.K || i > n) return;
+  if (i == n) draft.in = false;
   const void* row = row_at<kHalf>(p, id);
   const int tiles = (V + kTile - 1) / kTile;
   int par = 0;
@@ -534,11 +578,7 @@ __global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(VerifyArgs p) 
     }
     __syncthreads();
   }
-  // what the draft's test needs, requested early
-  Draft draft{false, 0.0f, 1.0f, 0.0f};
-  const float last_u = p.u[(int64_t)b * T + p.K];
-  if (t == 0 && i < n) draft = load_draft<kHalf>(p, b, i);
-  const RowSummary sum = summarize(p, id, lane);
+  const RowSummary sum = summarize(p, id, lane, own_group);
   const float mx = sum.max;
   const int mode = sum.mode;
   const double mxd = (double)mx, all = sum.mass;
@@ -570,7 +610,7 @@ __global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(VerifyArgs p) 
   };
   // f(four entries) over this lane's part of the row, eight tiles' loads at a time; padding is -inf
   auto each_row = [&](auto&& f) __attribute__((always_inline)) {
-    constexpr int kB = 8;
+    constexpr int kB = kLists ? 2 : 8;  // (searched in lists: seldom here, and no registers for more)
     for (int j = 0; j < tiles; j += kB) {
       R x[kB];
 #pragma unroll
@@ -590,11 +630,9 @@ __global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(VerifyArgs p) 
   if (listed) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int at = t + u * kThreads, g = at / p.cap, k = at - g * p.cap;
-      if (g < p.groups && k < p.group_count[id * p.groups + g]) {
-        const float2 e = p.list[(id * p.groups + g) * p.cap + k];
-        mine[u] = e.x;
-        mine_at[u] = __builtin_bit_cast(int, e.y);
+      if (list_place[u] < list_count[u]) {
+        mine[u] = listed_at[u].x;
+        mine_at[u] = __builtin_bit_cast(int, listed_at[u].y);
       }
     }
   }
