@@ -32,7 +32,7 @@ constexpr int kMaxTargets = 8;
 constexpr int kMaxRank = 128;
 constexpr int kMaxAdapters = 8192;
 constexpr int kRankBlock = 64;     // ranks per shrink workgroup
-constexpr int kColBlock = 256;     // fewest output columns per expand workgroup
+constexpr int kExpandWaves = 4;
 constexpr int kNone = -1, kBad = -2;
 
 struct Tile {
@@ -314,10 +314,9 @@ __device__ __forceinline__ float relu2(float f) {
   return f * f;
 }
 
-// Grid: x = block of p.cols columns over all targets, y = tile.  Up to 16 rows: the kW waves take 64 columns
+// Grid: x = block of p.cols columns over all targets, y = tile.  Up to 16 rows: the waves take 64 columns
 // each at a time; more: half of the waves for each half of the row blocks.
-template <int kW>
-__global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
+__global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraArgs p) {
   extern __shared__ char dyn[];
   const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
   const Tile tile = plan_tiles(p.plan)[blockIdx.y];
@@ -332,7 +331,7 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
     // no adapter: the epilogue alone; an index out of range: NaN
     if (tile.adapter == kNone && !tg.relu2 && tg.base == tg.y) return;
     const int per_row = (c1 - c0) >> 3;
-    for (int i = tid; i < tile.rows * per_row; i += 64 * kW) {
+    for (int i = tid; i < tile.rows * per_row; i += 64 * kExpandWaves) {
       const int r = i / per_row;
       const int64_t at = (int64_t)order[r] * N + c0 + 8 * (i - r * per_row);
       h8 v = ld8(tg.base + at);
@@ -361,7 +360,7 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
     }
   };
   const int rw = ns > 1 ? 2 : 1, per = (ns + rw - 1) / rw;  // waves along the rows; row blocks per wave
-  const int ri = wv % rw, ci = wv / rw, pass = 64 * (kW / rw);
+  const int ri = wv % rw, ci = wv / rw, pass = 64 * (kExpandWaves / rw);
   int64_t rows[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) rows[s] = (int64_t)order[min(16 * (ri * per + s) + li, tile.rows - 1)] * N;
@@ -388,7 +387,7 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
   const int groups = p.rank_pad >> 3, gbits = 31 - __builtin_clz(groups);
   const float* h0 = p.h + ((int64_t)ti * p.m + tile.row0) * p.rank_pad;
   const int64_t plane = (int64_t)p.n_targets * p.m * p.rank_pad;
-  for (int i = tid; i - tid < 16 * ns * groups; i += 64 * kW) {
+  for (int i = tid; i - tid < 16 * ns * groups; i += 64 * kExpandWaves) {
     const int r = i >> gbits, gr = i & (groups - 1);
     float hv[8];
     uint32_t mx = 0;
@@ -447,9 +446,7 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[s][t] = fv4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int ch = 0; ch < chunks; ++ch) {
-      hv8 next[4];
-      const bool last = ch + 1 == chunks;
-      if (!last || cw + pass < c1) weights(last ? cw + pass : cw, last ? 0 : ch + 1, next);
+      if (ch > 0 || cw != c0 + 64 * ci) weights(cw, ch, fa);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s >= per) break;
@@ -460,8 +457,6 @@ __global__ __launch_bounds__(64 * kW, 4) void lora_expand_kernel(LoraArgs p) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[s][t] = mfma(fa[t], lo, acc[s][t]);
       }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) fa[t] = next[t];
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -492,9 +487,11 @@ struct LoraPlan {
 // K parts of the first product: enough workgroups for the chip, at least 512 deep each (128 rows, 40
 // adapters, rank 32, K = 2048, N = 8192: 18.4 us with 4 parts, 20.5 with 8, which the second product has to
 // add; 434 rows of K = 8192: 23.2 with 4, 21.2 with 8).  Columns of the
-// second product per workgroup: 256 (four waves), or where that leaves enough workgroups 512 and 1024
-// (eight waves; each workgroup adds h's parts up anew).  The number of tiles is known on the device only;
-// the rows of a step that has them scattered make one per adapter.
+// second product per workgroup: 256, or 128 where that leaves few workgroups (423 rows, 2 adapters of 16, N =
+// 2048: 18.6 us, 21.0 with 256; 128 rows, 40 adapters, N = 8192: 21.1 and 18.4, as each adds h's parts up
+// anew; wider ones expose their later columns' loads: 2304 rows, 4 of 4096, 67 us, 72 with 1024 columns and
+// eight waves).  The number of tiles is known on the device only; the rows of a step that has them scattered
+// make one per adapter.
 LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min, int64_t n_max) {
   LoraPlan s{};
   s.rank_pad = 32;  // a power of two, so that a row's groups of 8 lie in neighbouring lanes
@@ -504,8 +501,8 @@ LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min, in
   int64_t parts = 1;
   while (parts < 8 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 512) parts *= 2;
   s.parts = (int)parts;
-  s.cols = kColBlock;
-  while (s.cols < 4 * kColBlock && tiles * n_targets * (n_max / (2 * s.cols)) >= 1024) s.cols *= 2;
+  s.cols = 256;
+  while (s.cols > 128 && tiles * n_targets * (n_max / s.cols) < 512) s.cols /= 2;
   s.bytes = parts * n_targets * m * s.rank_pad * 4;
   return s;
 }
@@ -637,7 +634,6 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
   else hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(64 * kShrinkWaves), 0, s, a);
   const dim3 egrid(cols, (unsigned)a.tiles_cap);
   const int lds = (rank + 31) / 32 * kSub * 2048 + kTileM * 4;
-  if (sp.cols == kColBlock) hipLaunchKernelGGL(lora_expand_kernel<4>, egrid, dim3(256), lds, s, a);
-  else hipLaunchKernelGGL(lora_expand_kernel<8>, egrid, dim3(512), lds, s, a);
+  hipLaunchKernelGGL(lora_expand_kernel, egrid, dim3(64 * kExpandWaves), lds, s, a);
   return check_launch(fn);
 }
