@@ -168,3 +168,22 @@ def test_plan_of_many_rows(gpu):
                                            "b": (0.2 * torch.randn(G, N, R, generator=g)).half(),
                                            "base": torch.randn(m, N, generator=g).half()}]}
     check(gpu, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [17, 65, 70, 97, 150])
+def test_equal_rows_of_an_adapter_are_equal(gpu, n):
+    """The plan puts an adapter's rows into its tiles, the last of which is shorter, in any order: equal rows
+    have to get equal bits wherever they are."""
+    d = make(n + 40, 3, 16, [(256, 4096), (72, 200)], seed=n)
+    d["ids"][:] = 1
+    d["ids"][n:] = torch.arange(40, dtype=torch.int32) % 2 * 2
+    for t in d["t"]:
+        t["x"][:n], t["base"][:n] = t["x"][0].clone(), t["base"][0].clone()
+    first = None
+    for _ in range(3):
+        ys = [y.cpu() for y in run_lora(gpu, d)]
+        for y in ys:
+            assert torch.equal(y[:n], y[:1].expand(n, -1))
+        assert first is None or all(torch.equal(a, b) for a, b in zip(first, ys))
+        first = ys

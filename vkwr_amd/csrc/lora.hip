@@ -36,7 +36,8 @@ constexpr int kExpandWaves = 4;
 constexpr int kNone = -1, kBad = -2;
 
 struct Tile {
-  int adapter, row0, rows, pad;
+  int adapter, row0, rows;
+  int blocks;  // blocks of 16 rows that the adapter has, 4 of more: how the first product cuts K
 };
 struct PlanHead {
   int n_tiles;     // all tiles
@@ -55,7 +56,9 @@ __device__ __forceinline__ const int32_t* plan_order(const void* plan, int64_t t
 
 // One workgroup: counts per bin (adapters, then rows without one, then indices out of range), prefix
 // sums of counts and tiles, tiles, and the rows' places.  Rows of one bin are placed in the order
-// in which their waves get there; what is computed for a row does not depend on its place.
+// in which their waves get there, in any of the adapter's tiles; what is computed for a row does not depend
+// on its place, as all tiles of an adapter cut K alike.  Bound by the
+// latency of its dozen dependent steps: 4 us up to 4096 rows.
 __global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const int32_t* adapters, void* plan,
                                                          int64_t tiles_cap) {
   extern __shared__ int lds[];
@@ -127,7 +130,7 @@ __global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const
     const int c = cnt[k];
     if (k == G) head->n_adapter = tile;
     for (int r = 0; r < c; r += kTileM)
-      tiles[tile++] = Tile{k < G ? k : k == G ? kNone : kBad, row + r, min(kTileM, c - r), 0};
+      tiles[tile++] = Tile{k < G ? k : k == G ? kNone : kBad, row + r, min(kTileM, c - r), min((c + 15) / 16, kSub)};
     if (k == nb - 1) head->n_tiles = tile;
     cnt[k] = row;
     row += c;
@@ -218,7 +221,7 @@ __device__ __forceinline__ void shrink_steps(const _Float16* xr, const _Float16*
 // Tiles of three or four blocks (prompt chunks) go through LDS: the 16 rows of an operand, 2 K bytes apart,
 // fall on the same sets of the vector cache, so that operands loaded straight into registers, 64 bytes of
 // a row at a time, came in twice (four projections of 2304 rows, K = 4096, rank 64: 107 us; through LDS
-// 35.5).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
+// 36, 3.9 TB/s of the 142 MB that x and A are).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
 // chunk c at place c ^ (r & 7) -- in a ring of four, three of them in flight.
 constexpr int kShrinkWaves = 8;
 constexpr int kStageK = 64, kStages = 4;
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraA
   const int ti = blockIdx.z / p.rank_blocks, r0 = (blockIdx.z - ti * p.rank_blocks) * kRankBlock;
   const Target& tg = p.t[ti];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int K = tg.k, ns = (tile.rows + 15) >> 4;
+  const int K = tg.k, ns = tile.blocks;
   const int li = lane & 15, kg = 8 * (lane >> 4);
   const int rbits = ns == 1 ? 0 : ns == 2 ? 1 : 2;  // 2^rbits waves along the rows
   const int ri = wv & ((1 << rbits) - 1), ki = wv >> rbits;
@@ -315,7 +318,10 @@ __device__ __forceinline__ float relu2(float f) {
 }
 
 // Grid: x = block of p.cols columns over all targets, y = tile.  Up to 16 rows: the waves take 64 columns
-// each at a time; more: half of the waves for each half of the row blocks.
+// each at a time; more: half of the waves for each half of the row blocks.  Bound by memory where there are
+// many rows (2304 rows, four projections of N = 4096, rank 64, 32 adapters: 67 us for 218 MB of base, y and
+// B), else by its chain of loads: tile, row numbers, h's parts, B and base.  A fragment of B for each of four
+// waves along the rows instead of two (6 waves per SIMD) took 103 us, base and y past the caches 81.
 __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraArgs p) {
   extern __shared__ char dyn[];
   const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
