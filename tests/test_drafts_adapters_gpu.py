@@ -333,3 +333,51 @@ def test_adapters_scratch_is_whole_from_the_start(gpu):
         tok = torch.ones(1, T, dtype=torch.int32, device=gpu)
         eng.step(state, prefill=[(tok, _i32([1], gpu))], adapter_ids=_i32([2], gpu))
     assert eng.adapters.ws.data_ptr() == at
+
+
+def test_captured_steps_follow_the_adapter_indices(gpu):
+    """A captured mixed step with adapters, replayed with other indices, tokens and slots: the eager step's
+    logits and states."""
+    from vkwr.model_executor import MixedEngine
+    cfg, model, state = _tiny(gpu, 8)
+    pool, _ = _pool(model, gpu)
+    eng, eager = MixedEngine(model, 32, adapters=pool), MixedEngine(model, 32, adapters=pool)
+    tok, slots, ids = _i32([1, 2, 3], gpu), _i32([0, 1, 2], gpu), _i32([0, 1, -1, 2], gpu)
+    pre, pslot = torch.ones(1, 5, dtype=torch.int32, device=gpu), _i32([3], gpu)
+    s1 = _clone(state)
+
+    def step(e, s):
+        return e.step(s, decode=(tok, slots), prefill=[(pre, pslot)], adapter_ids=ids)
+
+    step(eng, _clone(state))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(eng, s1)
+    s2 = _clone(s1)
+    for seed in (1, 2, 3):
+        g = torch.Generator().manual_seed(seed)
+        tok.copy_(torch.randint(0, cfg.vocab, (3,), generator=g))
+        pre.copy_(torch.randint(0, cfg.vocab, (1, 5), generator=g))
+        ids.copy_(torch.randint(-1, 3, (4,), generator=g))
+        perm = torch.randperm(8, generator=g)
+        slots.copy_(perm[:3])
+        pslot.copy_(perm[3:4])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step(eager, s2))
+        assert torch.equal(s1.wkv, s2.wkv) and torch.equal(s1.att_shift, s2.att_shift)
+
+
+def test_no_drafts_at_all(gpu):
+    """max_draft = 0: plain decoding through the draft step."""
+    from vkwr.model_executor import DraftEngine, SpeculativeBatcher
+    cfg, model, state = _tiny(gpu, 4)
+    eng = DraftEngine(model, 2, 0, max_rows=24)
+    sched = SpeculativeBatcher(eng, state, max_decode=1, max_prefill_chunks=1, chunk=8)
+    reqs = [sched.submit([5, 6, 7, 5, 6], n) for n in (1, 2, 5)]
+    assert len(sched.run()) == 3 and sched.drafted == 0
+    for r in reqs:
+        assert len(r.output) == r.max_new_tokens
+        _replay(model, r, gpu)

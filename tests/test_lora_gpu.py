@@ -191,3 +191,35 @@ def test_equal_rows_of_an_adapter_are_equal(gpu, n):
             assert torch.equal(y[:n], y[:1].expand(n, -1))
         assert first is None or all(torch.equal(a, b) for a, b in zip(first, ys))
         first = ys
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(gpu):
+    """The last adapter of pools of more than 2^31 entries."""
+    G, R, N, K, m = 300, 128, 65536, 65536, 3
+    d = make(m, 1, R, [(N, K)], seed=8, none=0.0)
+    t = d["t"][0]
+    a = torch.zeros(G, R, K, dtype=torch.float16, device=gpu)
+    b = torch.zeros(G, N, R, dtype=torch.float16, device=gpu)
+    a[-1], b[-1] = t["a"][0].to(gpu), t["b"][0].to(gpu)
+    y = t["base"].to(gpu)
+    plan = capi.lora_plan_empty(m, G, gpu)
+    capi.lora_plan(torch.full((m,), G - 1, dtype=torch.int32, device=gpu), plan)
+    capi.lora(plan, [capi.lora_target(t["x"].to(gpu), a, b, y)])
+    want, err = ref.lora(t["x"], t["a"], t["b"], t["base"], torch.zeros(m, dtype=torch.int32), None, False)
+    assert ((y.cpu().double() - want).abs() <= err + HALF16 * (want.abs() + err) + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_plan_are_left(gpu):
+    d = make(70, 3, 16, [(264, 72)], seed=9, none=0.3)
+    t = d["t"][0]
+    x, a, b = t["x"].to(gpu), t["a"].to(gpu), t["b"].to(gpu)
+    plan = capi.lora_plan_empty(70, 3, gpu)
+    for m in (41, 0, 1):
+        y = t["base"].to(gpu)
+        capi.lora_plan(d["ids"][:m].to(gpu), plan)
+        capi.lora(plan, [capi.lora_target(x, a, b, y)], scale=d["scale"].to(gpu))
+        assert torch.equal(y[m:].cpu(), t["base"][m:])
+        want, err = ref.lora(t["x"][:m], t["a"], t["b"], t["base"][:m], d["ids"][:m], d["scale"], False)
+        assert ((y[:m].cpu().double() - want).abs() <= err + HALF16 * (want.abs() + err) + 2.0 ** -25).all()

@@ -233,3 +233,47 @@ def test_masses_that_all_round_down(gpu):
     capi.verify_drafts(l.to(gpu), drafts.to(gpu), u.to(gpu), tokens, accepted, temperature=-13.875 / math.log(x),
                        top_p=1.0 - 1e-9, workspace=ws)
     assert (accepted.item(), tokens[0].tolist()) in ((1, [0, 1, -1]), (0, [1, -1, -1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [63, 64, 130])
+@pytest.mark.parametrize("filt", [{}, {"top_k": 40, "top_p": 0.9}, {"top_p": 0.95}, {"top_k": 300}],
+                         ids=["all", "k40p90", "p95", "k300"])
+def test_many_drafts(gpu, K, filt):
+    """More rows per sequence than a wave has lanes; the first rejection anywhere among them."""
+    d = make(6, K, 1000, seed=K, probs=False)
+    d["drafts"] = d["logits"][:, :K].float().argmax(-1).to(torch.int32)
+    d["u"][:, :K] *= 1e-9
+    for b, at in enumerate((0, 62, 63, 64, K - 1)):
+        if at < K:
+            d["u"][b, at] = 1.0 - 2.0 ** -24
+    d["n_draft"] = torch.tensor([K, K, K, K, K, min(K, 64)], dtype=torch.int32)
+    wt, wa = check(gpu, d, **filt)
+    assert wa[5] == min(K, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("filt", [{}, {"top_k": 40, "top_p": 0.9}, {"top_p": 0.95}], ids=["all", "k40p90", "p95"])
+def test_offsets_past_32_bits(gpu, filt, probs):
+    """The last sequences of more than 2^31 logits, as in a call of their own."""
+    B, K, V, last = 8400, 3, 65536, 3
+    d = make(last, K, V, seed=71)
+    logits = torch.zeros(B, K + 1, V, dtype=torch.float16, device=gpu)
+    logits[-last:] = d["logits"].to(gpu)
+    drafts, u = torch.zeros(B, K, dtype=torch.int32, device=gpu), torch.zeros(B, K + 1, device=gpu)
+    drafts[-last:], u[-last:] = d["drafts"].to(gpu), d["u"].to(gpu)
+    n = torch.zeros(B, dtype=torch.int32, device=gpu)
+    n[-last:] = d["n_draft"].to(gpu)
+    q = None
+    if probs:
+        q = torch.zeros(B, K, V, device=gpu)
+        q[-last:] = d["q"].to(gpu)
+    outs = []
+    for s in (slice(0, B), slice(B - last, B)):
+        tokens = torch.empty(s.stop - s.start, K + 1, dtype=torch.int32, device=gpu)
+        accepted = torch.empty(s.stop - s.start, dtype=torch.int32, device=gpu)
+        capi.verify_drafts(logits[s], drafts[s], u[s], tokens, accepted, n_draft=n[s], draft_probs=None if q is None else q[s],
+                           **filt)
+        outs.append((tokens[-last:], accepted[-last:]))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])

@@ -149,3 +149,17 @@ def test_graph_replays_and_another_stream(gpu):
         y2, p2 = run(gpu, B, P, T, H, d, pool=p2)
     side.synchronize()
     assert torch.equal(y2, want_y) and torch.equal(p2, want_pool)
+
+
+@pytest.mark.gpu
+def test_pool_past_32_bits(gpu):
+    """Slots on either side of the pool's 2^31st entry."""
+    B, P, T, H = 2, 2, 2, 64
+    d = make(B, P, T, H, seed=5, n_slots=2)
+    y, pool = run(gpu, B, P, T, H, d)
+    big = torch.zeros(8400, H, 64, 64, device=gpu)
+    at = [8191, 8399]
+    big[at] = d["pool"].to(gpu)
+    e = {**d, "slots": torch.tensor([at[i] for i in d["slots"].tolist()], dtype=torch.int32)}
+    y2, _ = run(gpu, B, P, T, H, e, pool=big)
+    assert torch.equal(y, y2) and torch.equal(big[at], pool) and not big[:8191].any() and not big[8192:8399].any()
