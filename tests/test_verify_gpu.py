@@ -277,3 +277,39 @@ def test_offsets_past_32_bits(gpu, filt, probs):
                            **filt)
         outs.append((tokens[-last:], accepted[-last:]))
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("V", [65536, 20004, 1220, 131076])
+@pytest.mark.parametrize("filt", [{"top_p": 0.95}, {"top_p": 0.6, "temperature": 0.7}, {"top_k": 5000, "top_p": 0.9}],
+                         ids=["p95", "p60", "k5000p90"])
+def test_nucleus_of_peaked_and_flat_rows(gpu, V, half, probs, filt):
+    """Rows whose kept entries are a few, hundreds, and most of the row, next to each other in a sequence;
+    replayed over scratch that holds anything."""
+    d = make(9, 4, V, seed=V + 1, half=False, probs=probs)
+    f = torch.tensor([0.3, 1.0, 3.0, 8.0, 20.0])
+    l = d["logits"] * f[torch.randint(0, 5, (9, 5, 1), generator=torch.Generator().manual_seed(V))]
+    d["logits"] = l.half() if half else l
+    d["n_draft"][:] = 4
+    if not probs:
+        d["drafts"] = l[:, :4].argmax(-1).to(torch.int32)
+    wt, wa = check(gpu, d, **filt)
+    c = lambda t: None if t is None else t.to(gpu)  # noqa: E731
+    ins, q = [c(d[k]) for k in ("logits", "drafts", "u")], c(d["q"])
+    tokens = torch.empty(9, 5, dtype=torch.int32, device=gpu)
+    accepted = torch.empty(9, dtype=torch.int32, device=gpu)
+    ws = torch.zeros(capi.verify_workspace_bytes(9, 4, V), dtype=torch.uint8, device=gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        capi.verify_drafts(*ins, tokens, accepted, draft_probs=q, workspace=ws, **filt)
+    for fill in (255, 1, 0):
+        ws.fill_(fill)
+        tokens.fill_(5)
+        g.replay()
+        torch.cuda.synchronize()
+        np.testing.assert_array_equal(tokens.cpu().numpy(), wt)
+        np.testing.assert_array_equal(accepted.cpu().numpy(), wa)

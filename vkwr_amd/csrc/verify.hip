@@ -21,13 +21,13 @@
 //
 // Launches:
 //   sums   every row in groups of 2048 entries, a wave each: the group's largest logit, its mass relative
-//          to that (without a filter also that of its 8 segments of 256), and for a small top_k a list of
-//          its largest entries
+//          to that (without a filter also that of its 8 segments of 256), and for a small top_k or a
+//          nucleus a list of its largest entries
 //   rows   (with a filter) one workgroup per row: tau, comp, Z and the test of the row's draft; from the
 //          lists, where they reach down to tau, also the token if the sequence stops at this row;
-//          otherwise from the whole row
-//   parts  (with a larger top_k or a drafter's distribution) the segments' sums of w for the row that
-//          each sequence stops at, by several workgroups
+//          otherwise from the whole row (of a nucleus, in a launch of its own)
+//   parts  (with a drafter's distribution, and where lists may not do) the segments' sums of w for the row
+//          that each sequence stops at, by several workgroups
 //   draw   one workgroup per sequence: the segment that the uniform falls on, and the entry
 
 #include <algorithm>
@@ -56,7 +56,8 @@ struct RowStat {
   double z, comp;
   float max, tau;
   int ok, mode;
-  int token, pad;  // the new token if the sequence stops here; -1: not known yet
+  int token;    // the new token if the sequence stops here; -1: not known yet
+  int verdict;  // where a second launch searches what the lists leave open
 };
 static_assert(sizeof(RowStat) == 40, "row stat size");
 // How a row's logits are read so that only finite values and -inf (weight 0) remain:
@@ -66,6 +67,8 @@ enum {
                 // weighs nothing): +inf -> 0, anything else -> -inf
   kAllLow = 2   // -inf everywhere: all entries tied
 };
+
+enum { kOpen = 0, kAccepted = 1, kRejected = 2 };  // kRejected: rows behind a rejection too
 
 struct VerifyArgs {
   int K, V;
@@ -82,6 +85,7 @@ struct VerifyArgs {
   double* part_sum;    // [B, segs]
   int segs, groups;
   int cap, rank;       // entries listed per group (0: no lists); maxima that a row of lanes gives
+  int again;           // rows that the lists leave open are searched by a launch of their own
   double scale, d_min;  // log2(e) / temperature; -1023 / scale (weight 0)
   float bin_scale;
   int top_k;
@@ -311,7 +315,8 @@ __device__ __forceinline__ double kept_of(const VerifyArgs& p, const RowStat& st
 }
 
 // One wave per group of kGroupSegs segments, four groups per workgroup.  fp32: bound by memory (566 rows of
-// 65536: 32 us, 4.7 TB/s); fp16: by its 20 instructions an entry for the mass (144 rows with lists: 15 us).
+// 65536: 32 us, 4.7 TB/s, or 38 where it looks for nuclei's lists); fp16: by its 20 instructions an entry for
+// the mass (144 rows with lists: 15 us).
 template <bool kHalf>
 __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
   const int T = p.K + 1, wgs = (p.groups + 3) / 4;
@@ -347,7 +352,50 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
   for (int k = 0; k < kGroupSegs; ++k)
     lane_max = fmaxf(lane_max, fmaxf(fmaxf(l[k][0], l[k][1]), fmaxf(l[k][2], l[k][3])));
   const float mx = wave_fmax(lane_max);
-  if (p.cap > 0) {
+  if (lane == 0) p.group_max[id * p.groups + group] = mx;
+  bool flat = false;
+  if (!p.truncate || p.use_mass) {
+    double total = 0.0;
+    if (mx > -INFINITY) {
+      if (mx == INFINITY) {
+        lane_max = read_as(lane_max, kInfOnly);
+#pragma unroll
+        for (int k = 0; k < kGroupSegs; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l[k][e] = read_as(l[k][e], kInfOnly);
+      }
+      const double mxd = mx == INFINITY ? 0.0 : (double)mx;
+#pragma unroll
+      for (int k0 = 0; k0 < kGroupSegs; k0 += 4) {
+        double s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          double w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = exp2_neg((double)l[k0 + u][e] - mxd, p.scale, p.d_min);
+          s[u] = (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        total += (s[0] + s[1]) + (s[2] + s[3]);
+        if (!p.truncate) {
+          const double w = wave_add4(s, lane);
+          const int seg = group * kGroupSegs + k0 + lane;
+          if (lane < 4 && seg < p.segs) p.seg_sum[id * p.segs + seg] = w;
+        }
+      }
+      total = wave_add(total);
+      // A list holds about what the lanes' maxima are.  Where those are less than half of top_p of the mass,
+      // either no entry of the group is kept (its list is empty, from just above its largest up), or more
+      // are than lists hold.
+      if (p.again) flat = !(wave_add(exp2_neg((double)lane_max - mxd, p.scale, p.d_min)) >= 0.5 * p.top_p * total);
+    }
+    if (lane == 0) p.group_sum[id * p.groups + group] = total;
+  }
+  if (flat) {
+    if (lane == 0) {
+      p.group_floor[id * p.groups + group] = mx == INFINITY ? mx : of_key(key_of(mx) + 1u);
+      p.group_count[id * p.groups + group] = 0;
+    }
+  } else if (p.cap > 0) {
     // The rank-th largest lane maximum of each row of 16 lanes, the smallest of the four: 4 rank entries
     // or more lie at or above it.  More than cap (likely entries side by side): halved from there to the
     // largest, until cap / 2 to cap do.
@@ -357,84 +405,50 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
       lm = lm == at ? -INFINITY : lm;
     }
     at = fmaxf(fminf(fminf(lane_read(at, 0), lane_read(at, 16)), fminf(lane_read(at, 32), lane_read(at, 48))), -FLT_MAX);
-    auto count_from = [&](float x) __attribute__((always_inline)) {
-      int c = 0;
+    // A bit per entry of the lane from x up, the first one highest: a compare and m = 2 m + carry each.
+    auto from = [&](float x) __attribute__((always_inline)) {
+      uint32_t m = 0;
 #pragma unroll
       for (int k = 0; k < kGroupSegs; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c += __builtin_popcountll(__ballot(l[k][e] >= x));
-      return c;
+        for (int e = 0; e < 4; ++e)
+          asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(m) : "v"(l[k][e]), "v"(x) : "vcc");
+      return m;
     };
-    int count = count_from(at);
+    uint32_t in = from(at);
+    int place = wave_scan(__builtin_popcount(in), lane), count = lane_read(place, 63);
     if (count > p.cap) {
       float lo = at, hi = mx;
       at = INFINITY;
-      count = 0;
+      in = 0;
+      count = place = 0;
       for (int k = 0; k < 12 && 2 * count < p.cap; ++k) {
         const float mid = 0.5f * lo + 0.5f * hi;
-        const int c = count_from(mid);
+        const uint32_t some = from(mid);
+        const int to = wave_scan(__builtin_popcount(some), lane), c = lane_read(to, 63);
         if (c > p.cap) {
           lo = mid;
         } else {
           hi = at = mid;
+          in = some;
+          place = to;
           count = c;
         }
       }
     }
-    if (count > 0) {
-      // Lane by lane: a bit per entry, the lanes' places by a scan, then each lane's listed entries (one or
-      // two) read again.
-      uint32_t in = 0;
-#pragma unroll
-      for (int k = 0; k < kGroupSegs; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) in |= l[k][e] >= at ? 1u << (4 * k + e) : 0u;
-      const int own = __builtin_popcount(in);
-      float2* out = p.list + (id * p.groups + group) * p.cap + (wave_scan(own, lane) - own);
-      while (in != 0) {
-        const int bit = __builtin_ctz(in), i = at0 + (bit >> 2) * step + (bit & 3);
-        in &= in - 1;
-        const float x = kHalf ? (float)reinterpret_cast<const _Float16*>(row)[i] : reinterpret_cast<const float*>(row)[i];
-        *out++ = make_float2(__builtin_isnan(x) ? 0.0f : x, __builtin_bit_cast(float, i));
-      }
+    // lane by lane, each lane's listed entries (one or two) read again
+    float2* out = p.list + (id * p.groups + group) * p.cap + (place - __builtin_popcount(in));
+    while (in != 0) {
+      const int e = __builtin_clz(in), i = at0 + (e >> 2) * step + (e & 3);
+      in &= ~(0x80000000u >> e);
+      const float x = kHalf ? (float)reinterpret_cast<const _Float16*>(row)[i] : reinterpret_cast<const float*>(row)[i];
+      *out++ = make_float2(__builtin_isnan(x) ? 0.0f : x, __builtin_bit_cast(float, i));
     }
     if (lane == 0) {
       p.group_floor[id * p.groups + group] = at;
       p.group_count[id * p.groups + group] = count;
     }
   }
-  if (lane == 0) p.group_max[id * p.groups + group] = mx;
-  if (p.truncate && !p.use_mass) return;
-  double total = 0.0;
-  if (mx > -INFINITY) {
-    if (mx == INFINITY) {
-#pragma unroll
-      for (int k = 0; k < kGroupSegs; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) l[k][e] = read_as(l[k][e], kInfOnly);
-    }
-    const double mxd = mx == INFINITY ? 0.0 : (double)mx;
-#pragma unroll
-    for (int k0 = 0; k0 < kGroupSegs; k0 += 4) {
-      double s[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        double w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = exp2_neg((double)l[k0 + u][e] - mxd, p.scale, p.d_min);
-        s[u] = (w[0] + w[1]) + (w[2] + w[3]);
-      }
-      total += (s[0] + s[1]) + (s[2] + s[3]);
-      if (!p.truncate) {
-        const double w = wave_add4(s, lane);
-        const int seg = group * kGroupSegs + k0 + lane;
-        if (lane < 4 && seg < p.segs) p.seg_sum[id * p.segs + seg] = w;
-      }
-    }
-    total = wave_add(total);
-  }
-  if (lane == 0) p.group_sum[id * p.groups + group] = total;
 }
 
 // What a group's sums, relative to its own largest logit, are in units of the row's largest weight.
@@ -540,7 +554,7 @@ __device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int
 // kLists: the groups' lists are searched first.  A row that is searched as a whole is read twice more:
 // for the histogram and for the entries of one bin.  (Kept in LDS, 128 KiB left one workgroup per CU, whose
 // loads and arithmetic then took turns.)  Bound by one workgroup's chain: lists, 144 rows 9 us; whole rows,
-// 640 of which 271 are searched, 65536 fp32 entries, 66 us, of which 23 vector instructions.
+// 640 of which 271 are searched, 65536 fp32 entries, 63 us, of which 23 vector instructions.
 template <bool kHalf, bool kLists, int kThreads>
 __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(VerifyArgs p) {
   static_assert(!kLists || kThreads == kListThreads, "four listed entries per lane");
@@ -581,10 +595,9 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
   const void* row = row_at<kHalf>(p, id);
   const int tiles = (V + kTile - 1) / kTile;
   int par = 0;
-  if (!kLists && p.use_mass && p.top_k == V) {
+  if (kLists == (p.cap > 0) && p.use_mass && p.top_k == V) {
     // Rows that a quick test can do without: those behind a rejection, and accepted ones (no statistics
-    // but the verdict are read of them).  Of 128 sequences' 566 rows (4 drafts,
-    // nucleus 0.95) 271 are left.
+    // but the verdict are read of them).  Of 128 sequences' 566 rows (4 drafts, nucleus 0.95) 271 are left.
     if (t == 0) sh.bin = sh.n_cand = 0;
     __syncthreads();
     for (int k = wv; k <= i && k < n; k += W) {
@@ -593,12 +606,22 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
       if (lane == 0 && k == i && v == kAccept) sh.n_cand = 1;
     }
     __syncthreads();
-    if (sh.bin != 0) return;
-    if (sh.n_cand != 0) {
-      if (t == 0) p.stat[id].ok = 1;
+    if (sh.bin != 0 || sh.n_cand != 0) {
+      if (t == 0) {
+        p.stat[id].ok = sh.bin != 0 ? 0 : 1;
+        p.stat[id].verdict = sh.bin != 0 ? kRejected : kAccepted;
+      }
       return;
     }
     __syncthreads();
+  }
+  if (!kLists && p.cap > 0) {  // the launch behind the lists': open rows that no known rejection is before
+    bool out = false;
+    for (int k = lane; k <= i; k += 64) {
+      const int v = p.stat[(int64_t)b * T + k].verdict;  // (not written by this launch's others)
+      out = out || v == kRejected || (k == i && v != kOpen);
+    }
+    if (__ballot(out) != 0) return;
   }
   const RowSummary sum = summarize(p, id, lane, own_group);
   const float mx = sum.max;
@@ -658,6 +681,11 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
       }
     }
   }
+  uint32_t none = 0, none2 = 0;
+  if (kLists && !listed && p.again) {
+    if (t == 0) p.stat[id].verdict = kOpen;
+    return;
+  }
   auto each4 = [&](auto&& f) __attribute__((always_inline)) {
     if (kLists && listed) f(f4{mine[0], mine[1], mine[2], mine[3]});
     else each_row(f);
@@ -674,8 +702,7 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
   st.mode = mode;
   st.ok = 0;
   st.token = -1;
-  st.pad = 0;
-  uint32_t none = 0, none2 = 0;
+  st.verdict = kOpen;
   for (;;) {
     const float floor = listed ? fmaxf(floor0, sum.reach) : floor0;
     // Histogram of (mx - l) in kBins equal steps: 32 per octave of the weight, or finer where the
@@ -748,6 +775,10 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
     __syncthreads();
     const bool found = sh.bin < kBins;
     if (kLists && !found && listed && sum.reach > -FLT_MAX) {  // tau lies below the lists' reach: the whole row
+      if (p.again) {
+        if (t == 0) p.stat[id].verdict = kOpen;
+        return;
+      }
       __syncthreads();
       listed = false;
       continue;
@@ -932,6 +963,7 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
   if (t == 0) {
     if (draft.in)
       st.ok = (double)draft.u * (double)draft.q < kept_of(p, st, read_as(draft.l, mode)) / st.z ? 1 : 0;
+    if (kLists && p.again) st.verdict = st.ok ? kAccepted : kRejected;
     p.stat[id] = st;
   }
 }
@@ -1025,7 +1057,7 @@ __global__ __launch_bounds__(256) void verify_parts_kernel(VerifyArgs p) {
   const int n = p.n_draft ? p.n_draft[b] : p.K;
   if (n < 0 || n > p.K) return;
   const Stop<kHalf, 4> stop(p, shared, b, n, lane, wv);
-  if (!p.truncate && !stop.beyond) return;
+  if (p.truncate ? stop.st.token >= 0 : !stop.beyond) return;
   const int seg0 = (part * 4 + wv) * kPartSegs;
   f4 l[kPartSegs], qv[kPartSegs];
 #pragma unroll
@@ -1080,7 +1112,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
     if (t == 0) out[j] = stop.st.token;
     return;
   }
-  const bool parts = p.truncate ? p.cap == 0 : stop.q != nullptr;  // the parts' kernel has run
+  const bool parts = p.truncate ? p.cap == 0 || p.again : stop.q != nullptr;  // the parts' kernel has run
   // the sum of segment k by one wave (the rows' and parts' kernels' order of additions aside)
   auto segment = [&](int k) {
     double w[4];
@@ -1194,12 +1226,12 @@ void launch_verify(const VerifyArgs& a, int B, hipStream_t s) {
     // entries, 4 drafts: 16 sequences 67 us with 16 waves, 77 with 8; 128 sequences 140 and 128).
     if (a.cap > 0)
       hipLaunchKernelGGL((verify_rows_kernel<kHalf, true, kListThreads>), dim3(rows), dim3(kListThreads), 0, s, a);
-    else if (rows <= (unsigned)device_cus())
+    if ((a.cap == 0 || a.again) && rows <= (unsigned)device_cus())
       hipLaunchKernelGGL((verify_rows_kernel<kHalf, false, 1024>), dim3(rows), dim3(1024), 0, s, a);
-    else
+    else if (a.cap == 0 || a.again)
       hipLaunchKernelGGL((verify_rows_kernel<kHalf, false, 512>), dim3(rows), dim3(512), 0, s, a);
   }
-  if (a.truncate ? a.cap == 0 : a.q != nullptr)
+  if (a.truncate ? a.cap == 0 || a.again : a.q != nullptr)
     hipLaunchKernelGGL(verify_parts_kernel<kHalf>, dim3(B * ((a.segs + 4 * kPartSegs - 1) / (4 * kPartSegs))), dim3(256), 0,
                        s, a);
   hipLaunchKernelGGL(verify_draw_kernel<kHalf>, dim3(B), dim3(kDrawThreads), 0, s, a);
@@ -1237,13 +1269,19 @@ bool verify_rows_fit(int64_t B, int64_t K, int64_t V) {
 // / groups on average, hardly ever more than m + 5 sqrt(m) + 3 where they are spread at random.  24
 // sequences of 5 drafts, 65536 entries, top_k 40: 41 us without lists, 26.5 with, 87 where all 40 are side by
 // side in one group, whose list ends above the last of them.
+// A nucleus (top_p without a top_k that lists hold) is a few entries or most of the row; rows that the lists
+// leave open are searched as a whole by a launch of their own.  128 sequences of 4 drafts, 65536 fp32
+// entries: nuclei of 4 entries 70 us (96 without lists), of 85 72 (109), of 32000 149 (130); 4 sequences: 21 (42),
+// 23 (49), 69 (63).
 void use_lists(VerifyArgs& a) {
-  a.cap = a.truncate && a.top_k < a.V ? list_cap(a.groups) : 0;
+  a.cap = a.truncate ? list_cap(a.groups) : 0;
   a.rank = 0;
   const auto above = [](int r) { return -64.0 * std::log1p(-r / 16.0); };
   while (a.rank < 14 && above(a.rank + 1) * 1.33 <= a.cap) ++a.rank;
   const double m = (double)a.top_k / a.groups;
-  if (above(a.rank) < (a.groups > 1 ? m + 5.0 * std::sqrt(m) + 3.0 : m)) a.cap = a.rank = 0;
+  const bool hold = a.top_k < a.V && above(a.rank) >= (a.groups > 1 ? m + 5.0 * std::sqrt(m) + 3.0 : m);
+  a.again = a.cap > 0 && !hold && a.use_mass;
+  if (!hold && !a.again) a.cap = a.rank = 0;
 }
 
 }  // namespace
