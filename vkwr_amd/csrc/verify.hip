@@ -32,6 +32,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 
 #include "vk_capi.h"
@@ -87,6 +88,7 @@ struct VerifyArgs {
   int cap, rank;       // entries listed per group (0: no lists); maxima that a row of lanes gives
   int again;           // rows that the lists leave open are searched by a launch of their own
   double scale, d_min;  // log2(e) / temperature; -1023 / scale (weight 0)
+  double unscale, light;  // 1 / scale; (1 - top_p) / V
   float bin_scale;
   int top_k;
   double top_p;
@@ -586,6 +588,9 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
       }
     }
   }
+  int lookup = -1;  // the draft that a drafter without a distribution gave
+  if (kLists && !p.q && i < p.K)  // (an ordinary scalar load is moved to its use, far behind)
+    lookup = __hip_atomic_load(p.drafts + (int64_t)b * p.K + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
   const int n = p.n_draft ? p.n_draft[b] : p.K;
   const float last_u = p.u[(int64_t)b * T + p.K];
   Draft draft{false, 0.0f, 1.0f, 0.0f};
@@ -639,8 +644,8 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
   // the roundings of the logarithm and of the sum).  Masked entries have no weight.
   float floor0 = sum.floor;
   if (p.use_mass) {
-    const float least = (float)((1.0 - p.top_p) * all / (double)V);
-    if (least > 1.0e-30f) floor0 = fmaxf(floor0, (float)(mxd + ((double)__log2f(least) - 0.01) / p.scale));
+    const float least = (float)(p.light * all);
+    if (least > 1.0e-30f) floor0 = fmaxf(floor0, (float)(mxd + ((double)__log2f(least) - 0.01) * p.unscale));
   }
   floor0 = fmaxf(floor0, -FLT_MAX);
 
@@ -899,39 +904,51 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
     break;
   }
 
+  const double unit = 1.0 / st.z;
+  if (t == 0 && draft.in)
+    st.ok = (double)draft.u * (double)draft.q < kept_of(p, st, read_as(draft.l, mode)) * unit ? 1 : 0;
   // The token if the sequence stops here: all kept entries are listed.  Sorted by index (places counted,
   // so that the sums' order does not hang on the order of the atomics), then the prefix sums in one wave.
   if (kLists && listed) {
+    if (t == 0) {
+      sh.n_cand = 0;
+      sh.bin = st.ok;
+    }
+    if (t < kVerDraw) sh.draw.at[t] = INT_MAX;
+    const int d = i < n ? lookup : -1;
     double w[4] = {0.0, 0.0, 0.0, 0.0};
-    const int d = i < n && !p.q ? p.drafts[(int64_t)b * p.K + i] : -1;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (!(mine[u] >= st.tau && mine[u] > -INFINITY)) continue;
-      w[u] = kept_of(p, st, mine[u]) / st.z;
+      w[u] = kept_of(p, st, mine[u]) * unit;
       if (i < n && p.q) w[u] = fmax(w[u] - (double)p.q[((int64_t)b * p.K + i) * V + mine_at[u]], 0.0);
       if (mine_at[u] == d) w[u] = 0.0;
     }
-    if (t == 0) sh.n_cand = 0;
     __syncthreads();
+    if (sh.bin == 0) {  // not where the draft is accepted
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (mine[u] >= st.tau && mine[u] > -INFINITY) {
-        const int at = atomicAdd(&sh.n_cand, 1);
-        if (at < kVerDraw) {
-          sh.draw.w[at] = w[u];
-          sh.draw.at[at] = mine_at[u];
+      for (int u = 0; u < 4; ++u) {
+        if (mine[u] >= st.tau && mine[u] > -INFINITY) {
+          const int at = atomicAdd(&sh.n_cand, 1);
+          if (at < kVerDraw) {
+            sh.draw.w[at] = w[u];
+            sh.draw.at[at] = mine_at[u];
+          }
         }
       }
     }
     __syncthreads();
     const int kept = sh.n_cand;
-    if (kept <= kVerDraw) {
+    if (kept > 0 && kept <= kVerDraw) {
       if (t < kept) {
         const int my = sh.draw.at[t];
         int place = 0;
-        for (int k = 0; k < kept; k += 4) {
-          const int4 o = *reinterpret_cast<const int4*>(&sh.draw.at[k]);
-          place += (o.x < my) + (o.y < my && k + 1 < kept) + (o.z < my && k + 2 < kept) + (o.w < my && k + 3 < kept);
+        for (int k = 0; k < kept; k += 16) {
+          int4 o[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) o[u] = *reinterpret_cast<const int4*>(&sh.draw.at[k + 4 * u]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) place += (o[u].x < my) + (o[u].y < my) + (o[u].z < my) + (o[u].w < my);
         }
         sh.draw.sorted_w[place] = sh.draw.w[t];
         sh.draw.sorted_at[place] = my;
@@ -961,8 +978,6 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
     }
   }
   if (t == 0) {
-    if (draft.in)
-      st.ok = (double)draft.u * (double)draft.q < kept_of(p, st, read_as(draft.l, mode)) / st.z ? 1 : 0;
     if (kLists && p.again) st.verdict = st.ok ? kAccepted : kRejected;
     p.stat[id] = st;
   }
@@ -1344,6 +1359,8 @@ extern "C" int vkwr_sampling_verify_drafts(int B, int K, int V, const void* logi
   a.groups = (a.segs + kGroupSegs - 1) / kGroupSegs;
   a.scale = 1.4426950408889634 / temperature;
   a.d_min = -1023.0 / a.scale;
+  a.unscale = 1.0 / a.scale;
+  a.light = (1.0 - top_p) / V;
   a.bin_scale = (float)(32.0 * a.scale);
   a.top_k = top_k;
   a.top_p = top_p;
