@@ -41,7 +41,8 @@
 namespace vk {
 namespace {
 
-constexpr int kListThreads = 256;  // rows' kernel: rows searched in lists (37 of 7 drafts: 13.2 us, 14.6 with 512)
+constexpr int kListThreads = 256;  // rows' kernel: rows searched in lists (320 rows of 1220:
+                                    // a call of 19.2 us, 21.0 with 512)
 constexpr int kMaxWaves = 1024 / 64;
 constexpr int kVerBins = 2048;   // histogram of (max - l) for the threshold
 constexpr int kVerCand = 512;    // entries of one bin that are ranked directly
@@ -555,7 +556,7 @@ __device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int
 
 // kLists: the groups' lists are searched first.  A row that is searched as a whole is read twice more:
 // for the histogram and for the entries of one bin.  (Kept in LDS, 128 KiB left one workgroup per CU, whose
-// loads and arithmetic then took turns.)  Bound by one workgroup's chain: lists, 144 rows 9 us; whole rows,
+// loads and arithmetic then took turns.)  Bound by one workgroup's chain: lists, 144 rows 8 us; whole rows,
 // 640 of which 271 are searched, 65536 fp32 entries, 63 us, of which 23 vector instructions.
 template <bool kHalf, bool kLists, int kThreads>
 __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(VerifyArgs p) {
