@@ -516,7 +516,8 @@ VKWR_EXPORT int vkwr_tmix_groupnorm_bonus_gate_frag_f16(int B, int T, int C, int
 
 /* The plan of a step: its rows ordered by adapter, made on the device from adapters [m] int32 (device)
  * once for all projections of the step.  plan: device memory of vkwr_lora_plan_bytes(m, n_adapters)
- * bytes (-1 on invalid arguments; it grows with m), 16-byte aligned.  1 <= n_adapters <= 8192. */
+ * bytes (-1 on invalid arguments; it grows with m), 16-byte aligned.  1 <= n_adapters <= 8192,
+ * min(m, n_adapters + 2) + m / 64 <= 65535. */
 VKWR_EXPORT int64_t vkwr_lora_plan_bytes(int64_t m, int n_adapters);
 VKWR_EXPORT int vkwr_lora_plan(int64_t m, int n_adapters, const int32_t* adapters, void* plan,
                                int64_t plan_bytes, void* stream);

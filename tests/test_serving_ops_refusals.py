@@ -98,6 +98,8 @@ def test_lora_plan_and_workspace_sizes():
     assert capi._lora_plan_bytes(-1, 2) == -1 and capi._lora_plan_bytes(4, 0) == -1
     assert capi._lora_plan(4, 2, P, P, 8, None) == 1 and "plan of" in err()
     assert capi._lora_plan(4, 2, None, P, 1 << 20, None) == 1 and "null" in err()
+    assert capi._lora_plan_bytes(65535 * 64, 2) == -1 and capi._lora_plan_bytes(65531 * 64, 2) > 0
+    assert capi._lora_plan(2 ** 31 - 100, 2, P, P, 2 ** 62, None) == 1 and "tiles" in err()
     sizes = [capi._lora_plan_bytes(m, 100) for m in range(0, 3000, 7)]
     assert sizes == sorted(sizes)
     arr = (capi.LoraTarget * 1)(target(n=2048, k=2048))

@@ -31,6 +31,7 @@ constexpr int kSub = kTileM / 16;
 constexpr int kMaxTargets = 8;
 constexpr int kMaxRank = 128;
 constexpr int kMaxAdapters = 8192;
+constexpr int kMaxTiles = 65535;   // rows of the grid
 constexpr int kRankBlock = 64;     // ranks per shrink workgroup
 constexpr int kExpandWaves = 4;
 constexpr int kNone = -1, kBad = -2;
@@ -50,6 +51,8 @@ __host__ __device__ inline int64_t max_tiles(int64_t m, int64_t G) { return (m <
 __device__ __forceinline__ const Tile* plan_tiles(const void* plan) {
   return reinterpret_cast<const Tile*>(reinterpret_cast<const char*>(plan) + sizeof(PlanHead));
 }
+// The rows' numbers, kTileM places per tile (those behind its rows hold anything): where a workgroup's rows
+// are hangs on no other load.
 __device__ __forceinline__ const int32_t* plan_order(const void* plan, int64_t tiles) {
   return reinterpret_cast<const int32_t*>(plan_tiles(plan) + tiles);
 }
@@ -62,7 +65,7 @@ __device__ __forceinline__ const int32_t* plan_order(const void* plan, int64_t t
 __global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const int32_t* adapters, void* plan,
                                                          int64_t tiles_cap) {
   extern __shared__ int lds[];
-  int* const cnt = lds;          // [G + 2] counts, then next free place
+  int* const cnt = lds;          // [G + 2] counts, then next free place (of the tiles' kTileM each)
   int* const red = lds + G + 2;  // [32]
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, nb = G + 2;
   Tile* const tiles = const_cast<Tile*>(plan_tiles(plan));
@@ -132,7 +135,7 @@ __global__ __launch_bounds__(1024) void lora_plan_kernel(int64_t m, int G, const
     for (int r = 0; r < c; r += kTileM)
       tiles[tile++] = Tile{k < G ? k : k == G ? kNone : kBad, row + r, min(kTileM, c - r), min((c + 15) / 16, kSub)};
     if (k == nb - 1) head->n_tiles = tile;
-    cnt[k] = row;
+    cnt[k] = (tile - (c + kTileM - 1) / kTileM) * kTileM;  // its first tile's first place
     row += c;
   }
   __syncthreads();
@@ -154,7 +157,6 @@ struct Target {
   _Float16* y;
   int n, k;
   int relu2;
-  int col_block0;  // expand: this target's first column block
 };
 struct LoraArgs {
   const void* plan;
@@ -162,9 +164,45 @@ struct LoraArgs {
   int G;
   const float* scale;
   float* h;        // [parts][target][m][rank_pad]
-  int rank, rank_pad, n_targets, parts, rank_blocks, cols;
+  int rank, rank_pad, n_targets, parts, cols;
   Target t[kMaxTargets];
 };
+
+// What a workgroup is to do: the arguments in one round of scalar loads, the plan's in a second.  (Left to
+// the compiler they came one by one where they are used, a dozen round trips one after the other.)
+struct Work {
+  const _Float16 *x, *a, *b, *base;
+  _Float16* y;
+  int n, k, relu2;
+  const float* scale;
+  float* h;
+  int64_t m;
+  int rank, rank_pad, n_targets, parts, cols;
+  int tiles, adapter_tiles;  // 0: a plan for something else
+  Tile tile;
+  const int32_t* order;
+  int mine;  // lane l: row number l of the tile
+};
+__device__ __forceinline__ Work work_of(const LoraArgs& p) {
+  const Target& t = p.t[blockIdx.z];
+  Work w{t.x, t.a, t.b, t.base, t.y, t.n, t.k, t.relu2, p.scale, p.h, p.m, p.rank, p.rank_pad, p.n_targets, p.parts, p.cols};
+  const void* plan = p.plan;
+  const int64_t cap = p.tiles_cap;
+  const int G = p.G;
+  asm volatile("" ::"s"(w.x), "s"(w.a), "s"(w.b), "s"(w.base), "s"(w.y), "s"(w.n), "s"(w.k), "s"(w.relu2), "s"(w.scale),
+               "s"(w.h), "s"(w.m), "s"(w.rank), "s"(w.rank_pad), "s"(w.n_targets), "s"(w.parts), "s"(w.cols), "s"(plan),
+               "s"(cap), "s"(G));
+  w.order = plan_order(plan, cap) + (int64_t)blockIdx.y * kTileM;
+  w.mine = __hip_atomic_load(w.order + (threadIdx.x & 63), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+  const PlanHead head = *reinterpret_cast<const PlanHead*>(plan);
+  w.tile = plan_tiles(plan)[blockIdx.y];  // blockIdx.y < tiles_cap: inside the plan, stale or not
+  asm volatile("" ::"s"(head.n_tiles), "s"(head.n_adapter), "s"(head.m), "s"(head.G), "s"(w.tile.adapter), "s"(w.tile.row0),
+               "s"(w.tile.rows), "s"(w.tile.blocks));
+  const bool ours = head.m == w.m && head.G == G;
+  w.tiles = ours ? head.n_tiles : 0;
+  w.adapter_tiles = ours ? head.n_adapter : 0;
+  return w;
+}
 
 __device__ __forceinline__ fv4 mfma(hv8 a, hv8 b, fv4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -214,7 +252,7 @@ __device__ __forceinline__ void shrink_steps(const _Float16* xr, const _Float16*
   }
 }
 
-// Grid: x = part, y = tile, z = target * rank_blocks + rank block.  A wave takes one block of 16 rows; the
+// Grid: x = rank block * parts + part, y = tile, z = target.  A wave takes one block of 16 rows; the
 // eight waves cut the part's K in 8 for one block, in 4 for two, in 2 for three or four.  The waves' sums
 // are added in K order through LDS.
 //
@@ -231,26 +269,25 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraA
   __shared__ __attribute__((aligned(1024))) char smem[kStages * kStageHalfs * 2];  // the ring, then the waves' sums
   fv4(*const lds)[RT][64] = reinterpret_cast<fv4(*)[RT][64]>(smem);
   static_assert((kShrinkWaves - 1) * kRankBlock / 16 * 1024 <= kStages * kStageHalfs * 2, "the sums fit");
-  const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
-  const Tile tile = plan_tiles(p.plan)[blockIdx.y];  // blockIdx.y < tiles_cap: inside the plan, stale or not
-  if ((int)blockIdx.y >= head.n_adapter || head.m != p.m || head.G != p.G) return;
-  const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
-  const int ti = blockIdx.z / p.rank_blocks, r0 = (blockIdx.z - ti * p.rank_blocks) * kRankBlock;
-  const Target& tg = p.t[ti];
+  const Work tg = work_of(p);
+  const Tile tile = tg.tile;
+  if ((int)blockIdx.y >= tg.adapter_tiles) return;
+  auto row_of = [&](int r) { return (int64_t)__shfl(tg.mine, min(r, tile.rows - 1), 64); };
+  const int rb = (int)blockIdx.x >= tg.parts ? 1 : 0, part = (int)blockIdx.x - rb * tg.parts, r0 = rb * kRankBlock;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int K = tg.k, ns = tile.blocks;
   const int li = lane & 15, kg = 8 * (lane >> 4);
   const int rbits = ns == 1 ? 0 : ns == 2 ? 1 : 2;  // 2^rbits waves along the rows
   const int ri = wv & ((1 << rbits) - 1), ki = wv >> rbits;
   const int r = 16 * ri + li;
-  const _Float16* xr = tg.x + (int64_t)order[min(r, tile.rows - 1)] * K;
+  const _Float16* xr = tg.x + row_of(r) * K;
   const _Float16* ar[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j)
-    ar[j] = tg.a + ((int64_t)tile.adapter * p.rank + min(r0 + 16 * j + li, p.rank - 1)) * K;
+    ar[j] = tg.a + ((int64_t)tile.adapter * tg.rank + min(r0 + 16 * j + li, tg.rank - 1)) * K;
   // this wave's 32-deep steps of the part
-  const int steps = (K + 31) >> 5, chunks = (kShrinkWaves >> rbits) * p.parts;
-  const int c = (kShrinkWaves >> rbits) * blockIdx.x + ki;
+  const int steps = (K + 31) >> 5, chunks = (kShrinkWaves >> rbits) * tg.parts;
+  const int c = (kShrinkWaves >> rbits) * part + ki;
   const int s0 = (int)((int64_t)steps * c / chunks), s1 = (int)((int64_t)steps * (c + 1) / chunks);
   fv4 acc[RT];
 #pragma unroll
@@ -259,13 +296,13 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraA
     if (ri < ns) shrink_steps<RT>(xr, ar, kg, K, s0, s1, acc);
   } else {
     const int blocks = (K + kStageK - 1) / kStageK;
-    const int b0 = (int)((int64_t)blocks * blockIdx.x / p.parts), b1 = (int)((int64_t)blocks * (blockIdx.x + 1) / p.parts);
+    const int b0 = (int)((int64_t)blocks * part / tg.parts), b1 = (int)((int64_t)blocks * (part + 1) / tg.parts);
     // DMA instruction: 8 rows; wave w fills rows 8 w .. of x and rows 8 (w mod 2 RT) .. of A
     _Float16* const ring = reinterpret_cast<_Float16*>(smem);
     const int w = __builtin_amdgcn_readfirstlane(wv), aw = w % (2 * RT);
     const int xrow = 8 * w + (lane >> 3), arow = 8 * aw + (lane >> 3);
-    const _Float16* const xs = tg.x + (int64_t)order[min(xrow, tile.rows - 1)] * K;
-    const _Float16* const as = tg.a + ((int64_t)tile.adapter * p.rank + min(r0 + arow, p.rank - 1)) * K;
+    const _Float16* const xs = tg.x + row_of(xrow) * K;
+    const _Float16* const as = tg.a + ((int64_t)tile.adapter * tg.rank + min(r0 + arow, tg.rank - 1)) * K;
     const int xc = 8 * ((lane & 7) ^ (xrow & 7)), ac = 8 * ((lane & 7) ^ (arow & 7));
     auto issue = [&](int blk) __attribute__((always_inline)) {
       _Float16* const to = ring + ((blk - b0) % kStages) * kStageHalfs;
@@ -303,12 +340,12 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraA
   __syncthreads();
   if (ki > 0 || r >= tile.rows) return;
   // lane (row li, ranks 16 j + 4 (lane / 16) ..): four consecutive ranks
-  float* h = p.h + ((int64_t)(blockIdx.x * p.n_targets + ti) * p.m + tile.row0) * p.rank_pad + r0;
+  float* h = tg.h + ((int64_t)(part * tg.n_targets + (int)blockIdx.z) * tg.m + tile.row0) * tg.rank_pad + r0;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
-    if (r0 + 16 * j >= p.rank_pad) break;
+    if (r0 + 16 * j >= tg.rank_pad) break;
     for (int k = 0; k < (kShrinkWaves >> rbits) - 1; ++k) acc[j] += lds[(k << rbits) + ri][j][lane];
-    *reinterpret_cast<fv4*>(h + (int64_t)r * p.rank_pad + 16 * j + 4 * (lane >> 4)) = acc[j];
+    *reinterpret_cast<fv4*>(h + (int64_t)r * tg.rank_pad + 16 * j + 4 * (lane >> 4)) = acc[j];
   }
 }
 
@@ -317,21 +354,18 @@ __device__ __forceinline__ float relu2(float f) {
   return f * f;
 }
 
-// Grid: x = block of p.cols columns over all targets, y = tile.  Up to 16 rows: the waves take 64 columns
+// Grid: x = block of cols columns, y = tile, z = target.  Up to 16 rows: the waves take 64 columns
 // each at a time; more: half of the waves for each half of the row blocks.  Bound by memory where there are
-// many rows (2304 rows, four projections of N = 4096, rank 64, 32 adapters: 67 us for 218 MB of base, y and
+// many rows (2304 rows, four projections of N = 4096, rank 64, 32 adapters: 66 us for 218 MB of base, y and
 // B), else by its chain of loads: tile, row numbers, h's parts, B and base.  A fragment of B for each of four
 // waves along the rows instead of two (6 waves per SIMD) took 103 us, base and y past the caches 81.
 __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraArgs p) {
   extern __shared__ char dyn[];
-  const PlanHead head = *reinterpret_cast<const PlanHead*>(p.plan);
-  const Tile tile = plan_tiles(p.plan)[blockIdx.y];
-  if ((int)blockIdx.y >= head.n_tiles || head.m != p.m || head.G != p.G) return;
-  const int32_t* order = plan_order(p.plan, p.tiles_cap) + tile.row0;
-  int ti = 0;
-  while (ti + 1 < p.n_targets && (int)blockIdx.x >= p.t[ti + 1].col_block0) ++ti;
-  const Target& tg = p.t[ti];
-  const int N = tg.n, c0 = ((int)blockIdx.x - tg.col_block0) * p.cols, c1 = min(c0 + p.cols, N);
+  const Work tg = work_of(p);
+  const Tile tile = tg.tile;
+  const int N = tg.n, c0 = (int)blockIdx.x * tg.cols, c1 = min(c0 + tg.cols, N);
+  if ((int)blockIdx.y >= tg.tiles || c0 >= N) return;
+  const int32_t* const order = tg.order;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   if (tile.adapter < 0) {
     // no adapter: the epilogue alone; an index out of range: NaN
@@ -350,9 +384,9 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
     }
     return;
   }
-  const int ns = (tile.rows + 15) >> 4, chunks = (p.rank + 31) >> 5;
+  const int ns = (tile.rows + 15) >> 4, chunks = (tg.rank + 31) >> 5;
   const int li = lane & 15, grp = lane >> 4;
-  const _Float16* const bw = tg.b + (int64_t)tile.adapter * N * p.rank;
+  const _Float16* const bw = tg.b + (int64_t)tile.adapter * N * tg.rank;
   const hv8 zero = {};
   // Product row li of column tile t is output column cw + 32 (t / 2) + 8 (li / 4) + 4 (t % 2) + li % 4, so that
   // a lane of group grp ends up with the columns cw + 32 q + 8 grp .. + 7 (q = 0, 1): four lanes cover 64
@@ -362,14 +396,14 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int col = cw + 32 * (t >> 1) + 8 * (li >> 2) + 4 * (t & 1) + (li & 3);
-      fa[t] = rk < p.rank && col < c1 ? *reinterpret_cast<const hv8*>(bw + (int64_t)col * p.rank + rk) : zero;
+      fa[t] = rk < tg.rank && col < c1 ? *reinterpret_cast<const hv8*>(bw + (int64_t)col * tg.rank + rk) : zero;
     }
   };
   const int rw = ns > 1 ? 2 : 1, per = (ns + rw - 1) / rw;  // waves along the rows; row blocks per wave
   const int ri = wv % rw, ci = wv / rw, pass = 64 * (kExpandWaves / rw);
   int64_t rows[2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) rows[s] = (int64_t)order[min(16 * (ri * per + s) + li, tile.rows - 1)] * N;
+  for (int s = 0; s < 2; ++s) rows[s] = (int64_t)__shfl(tg.mine, min(16 * (ri * per + s) + li, tile.rows - 1), 64) * N;
   // requested before h is waited for: the first pass's weights and base
   hv8 fa[4];
   h8 base[2][2];
@@ -389,30 +423,30 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
   int* const back = reinterpret_cast<int*>(hf + chunks * kSub * 128);    // [kTileM] powers of two taken out of the rows
   // h = scale * (sum of the parts, in order), 8 ranks of a row per item, at most 4 items a lane; a row's
   // items lie in neighbouring lanes (rank_pad / 8, a power of two)
-  const float sc = p.scale ? p.scale[tile.adapter] : 1.0f;
-  const int groups = p.rank_pad >> 3, gbits = 31 - __builtin_clz(groups);
-  const float* h0 = p.h + ((int64_t)ti * p.m + tile.row0) * p.rank_pad;
-  const int64_t plane = (int64_t)p.n_targets * p.m * p.rank_pad;
+  const float sc = tg.scale ? tg.scale[tile.adapter] : 1.0f;
+  const int groups = tg.rank_pad >> 3, gbits = 31 - __builtin_clz(groups);
+  const float* h0 = tg.h + ((int64_t)blockIdx.z * tg.m + tile.row0) * tg.rank_pad;
+  const int64_t plane = (int64_t)tg.n_targets * tg.m * tg.rank_pad;
   for (int i = tid; i - tid < 16 * ns * groups; i += 64 * kExpandWaves) {
     const int r = i >> gbits, gr = i & (groups - 1);
     float hv[8];
     uint32_t mx = 0;
-    const bool live = r < tile.rows && 8 * gr < p.rank;  // rows behind the tile's and ranks of the padding: 0
+    const bool live = r < tile.rows && 8 * gr < tg.rank;  // rows behind the tile's and ranks of the padding: 0
     {
-      const float* src = h0 + (int64_t)min(r, tile.rows - 1) * p.rank_pad + 8 * gr;
+      const float* src = h0 + (int64_t)min(r, tile.rows - 1) * tg.rank_pad + 8 * gr;
       fv4 lo = fv4{0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
       if (live) {
-        for (int q0 = 0; q0 < p.parts; q0 += 4) {  // four parts' loads together
+        for (int q0 = 0; q0 < tg.parts; q0 += 4) {  // four parts' loads together
           fv4 x[4], y[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float* at = src + min(q0 + q, p.parts - 1) * plane;
+            const float* at = src + min(q0 + q, tg.parts - 1) * plane;
             x[q] = *reinterpret_cast<const fv4*>(at);
             y[q] = *reinterpret_cast<const fv4*>(at + 4);
           }
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            if (q0 + q >= p.parts) break;
+            if (q0 + q >= tg.parts) break;
             lo += x[q];
             hi += y[q];
           }
@@ -553,8 +587,8 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 using namespace vk;
 
 extern "C" int64_t vkwr_lora_plan_bytes(int64_t m, int n_adapters) {
-  if (m < 0 || m > 0x7fffffff - 64 || n_adapters < 1 || n_adapters > kMaxAdapters) return -1;
-  return (int64_t)sizeof(PlanHead) + max_tiles(m, n_adapters) * (int64_t)sizeof(Tile) + 4 * m;
+  if (m < 0 || n_adapters < 1 || n_adapters > kMaxAdapters || max_tiles(m, n_adapters) > kMaxTiles) return -1;
+  return (int64_t)sizeof(PlanHead) + max_tiles(m, n_adapters) * (int64_t)(sizeof(Tile) + 4 * kTileM);
 }
 
 extern "C" int vkwr_lora_plan(int64_t m, int n_adapters, const int32_t* adapters, void* plan, int64_t plan_bytes,
@@ -562,8 +596,8 @@ extern "C" int vkwr_lora_plan(int64_t m, int n_adapters, const int32_t* adapters
   clear_error();
   const char* fn = "vkwr_lora_plan";
   const int64_t need = vkwr_lora_plan_bytes(m, n_adapters);
-  VK_REQUIRE(need >= 0, "%s: bad size (m=%lld, %d adapters; at most %d adapters)", fn, (long long)m, n_adapters,
-             kMaxAdapters);
+  VK_REQUIRE(need >= 0, "%s: bad size (m=%lld, %d adapters; at most %d adapters and %d row tiles)", fn, (long long)m,
+             n_adapters, kMaxAdapters, kMaxTiles);
   VK_REQUIRE(m == 0 || adapters, "%s: null pointer", fn);
   VK_REQUIRE(plan && plan_bytes >= need && (uintptr_t)plan % 16 == 0,
              "%s: needs a 16-byte aligned plan of %lld bytes, got %lld", fn, (long long)need, (long long)plan_bytes);
@@ -608,9 +642,8 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
   a.rank_pad = sp.rank_pad;
   a.n_targets = n_targets;
   a.parts = sp.parts;
-  a.rank_blocks = sp.rank_blocks;
   a.cols = sp.cols;
-  int cols = 0;
+  int64_t widest = 0;
   for (int i = 0; i < n_targets; ++i) {
     const vkwr_lora_target& t = targets[i];
     const uint16_t* base = t.base ? t.base : t.y;
@@ -628,17 +661,17 @@ extern "C" int vkwr_lora_f16(int64_t m, int n_adapters, int rank, const float* s
     a.t[i] = Target{reinterpret_cast<const _Float16*>(t.x), reinterpret_cast<const _Float16*>(t.a),
                     reinterpret_cast<const _Float16*>(t.b), reinterpret_cast<const _Float16*>(base),
                     reinterpret_cast<_Float16*>(t.y), (int)t.n, (int)t.k,
-                    t.epilogue == VKWR_GEMM_EPI_RELU_SQUARE, cols};
-    cols += (int)((t.n + sp.cols - 1) / sp.cols);
+                    t.epilogue == VKWR_GEMM_EPI_RELU_SQUARE};
+    widest = std::max(widest, t.n);
   }
-  VK_REQUIRE(a.tiles_cap <= 65535, "%s: %lld row tiles, at most 65535", fn, (long long)a.tiles_cap);
+  VK_REQUIRE(a.tiles_cap <= kMaxTiles, "%s: %lld row tiles, at most %d", fn, (long long)a.tiles_cap, kMaxTiles);
   const hipStream_t s = (hipStream_t)stream;
-  const dim3 grid(sp.parts, (unsigned)a.tiles_cap, n_targets * sp.rank_blocks);
+  const dim3 grid(sp.parts * sp.rank_blocks, (unsigned)a.tiles_cap, n_targets);
   const int rt = (std::min(rank, kRankBlock) + 15) / 16;
   if (rt == 1) hipLaunchKernelGGL(lora_shrink_kernel<1>, grid, dim3(64 * kShrinkWaves), 0, s, a);
   else if (rt == 2) hipLaunchKernelGGL(lora_shrink_kernel<2>, grid, dim3(64 * kShrinkWaves), 0, s, a);
   else hipLaunchKernelGGL(lora_shrink_kernel<4>, grid, dim3(64 * kShrinkWaves), 0, s, a);
-  const dim3 egrid(cols, (unsigned)a.tiles_cap);
+  const dim3 egrid((unsigned)((widest + sp.cols - 1) / sp.cols), (unsigned)a.tiles_cap, n_targets);
   const int lds = (rank + 31) / 32 * kSub * 2048 + kTileM * 4;
   hipLaunchKernelGGL(lora_expand_kernel, egrid, dim3(64 * kExpandWaves), lds, s, a);
   return check_launch(fn);
