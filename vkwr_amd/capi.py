@@ -543,6 +543,7 @@ def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_draft=None, draf
 
 
 LORA_MAX_TARGETS = 8
+_LORA_ARRAYS = [LoraTarget * n for n in range(LORA_MAX_TARGETS + 1)]
 
 
 class LoraPlan:
@@ -591,9 +592,14 @@ def lora_target(x, a, b, y, base=None, epilogue=EPI_NONE):
 
 
 def _lora_targets(targets):
-    if not 1 <= len(targets) <= LORA_MAX_TARGETS or any(t.sizes != targets[0].sizes for t in targets):
+    n = len(targets)
+    sizes = targets[0].sizes if n else None
+    for t in targets:
+        if t.sizes != sizes:
+            n = 0
+    if not 1 <= n <= LORA_MAX_TARGETS:
         raise ValueError("lora: 1 to 8 targets with the same rows, adapters, rank and device")
-    return targets[0].sizes, (LoraTarget * len(targets))(*targets)
+    return sizes, _LORA_ARRAYS[n](*targets)
 
 
 def lora_workspace_bytes(max_rows, n_adapters, targets):

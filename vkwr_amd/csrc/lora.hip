@@ -416,8 +416,6 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
       if (cw + 8 * grp + 32 < c1) base[s][1] = ld8(tg.base + at + 32);
     }
   };
-  weights(c0 + 64 * ci, 0, fa);
-  load_base(c0 + 64 * ci);
 
   hv8* const hf = reinterpret_cast<hv8*>(dyn);                          // [chunk][sub][half][lane]
   int* const back = reinterpret_cast<int*>(hf + chunks * kSub * 128);    // [kTileM] powers of two taken out of the rows
@@ -427,28 +425,39 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
   const int groups = tg.rank_pad >> 3, gbits = 31 - __builtin_clz(groups);
   const float* h0 = tg.h + ((int64_t)blockIdx.z * tg.m + tile.row0) * tg.rank_pad;
   const int64_t plane = (int64_t)tg.n_targets * tg.m * tg.rank_pad;
+  struct Parts {
+    fv4 x[4], y[4];
+  };
+  auto load_parts = [&](Parts& f, int i, int q0) __attribute__((always_inline)) {  // four parts together
+    const float* src = h0 + (int64_t)min(i >> gbits, tile.rows - 1) * tg.rank_pad + 8 * (i & (groups - 1));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float* at = src + min(q0 + q, tg.parts - 1) * plane;
+      f.x[q] = *reinterpret_cast<const fv4*>(at);
+      f.y[q] = *reinterpret_cast<const fv4*>(at + 4);
+    }
+  };
+  auto live_at = [&](int i) { return (i >> gbits) < tile.rows && 8 * (i & (groups - 1)) < tg.rank; };
+  // requested first, as the others wait for it
+  Parts ph;
+  if (live_at(tid)) load_parts(ph, tid, 0);
+  weights(c0 + 64 * ci, 0, fa);
+  load_base(c0 + 64 * ci);
   for (int i = tid; i - tid < 16 * ns * groups; i += 64 * kExpandWaves) {
     const int r = i >> gbits, gr = i & (groups - 1);
     float hv[8];
     uint32_t mx = 0;
     const bool live = r < tile.rows && 8 * gr < tg.rank;  // rows behind the tile's and ranks of the padding: 0
     {
-      const float* src = h0 + (int64_t)min(r, tile.rows - 1) * tg.rank_pad + 8 * gr;
       fv4 lo = fv4{0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
       if (live) {
-        for (int q0 = 0; q0 < tg.parts; q0 += 4) {  // four parts' loads together
-          fv4 x[4], y[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float* at = src + min(q0 + q, tg.parts - 1) * plane;
-            x[q] = *reinterpret_cast<const fv4*>(at);
-            y[q] = *reinterpret_cast<const fv4*>(at + 4);
-          }
+        for (int q0 = 0; q0 < tg.parts; q0 += 4) {
+          if (i != tid || q0 > 0) load_parts(ph, i, q0);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             if (q0 + q >= tg.parts) break;
-            lo += x[q];
-            hi += y[q];
+            lo += ph.x[q];
+            hi += ph.y[q];
           }
         }
       }
@@ -524,9 +533,10 @@ struct LoraPlan {
   int64_t bytes;
 };
 
-// K parts of the first product: enough workgroups for the chip, at least 512 deep each (128 rows, 40
-// adapters, rank 32, K = 2048, N = 8192: 18.4 us with 4 parts, 20.5 with 8, which the second product has to
-// add; 434 rows of K = 8192: 23.2 with 4, 21.2 with 8).  Columns of the
+// K parts of the first product: enough workgroups for the chip, at least 512 deep each, or 256 where that
+// leaves fewer than 128 (128 rows, 40 adapters, rank 32, K = 2048, N = 8192: 16.0 us with 4 parts, 16.5 with 8,
+// which the second product has to add; 434 rows of K = 8192: 16.7 with 8, 15.8 with 16; 27 rows of 7 adapters, K =
+// 2560: 15.2 with 4, 14.3 with 8).  Columns of the
 // second product per workgroup: 256, or 128 where that leaves few workgroups (423 rows, 2 adapters of 16, N =
 // 2048: 18.6 us, 21.0 with 256; 128 rows, 40 adapters, N = 8192: 21.1 and 18.4, as each adds h's parts up
 // anew; wider ones expose their later columns' loads: 2304 rows, 4 of 4096, 67 us, 72 with 1024 columns and
@@ -538,8 +548,9 @@ LoraPlan lora_split(int64_t m, int G, int rank, int n_targets, int64_t k_min, in
   while (s.rank_pad < rank) s.rank_pad *= 2;
   s.rank_blocks = (rank + kRankBlock - 1) / kRankBlock;
   const int64_t tiles = std::min<int64_t>(m, G) + m / kTileM;
+  const int64_t each = tiles * n_targets * s.rank_blocks;
   int64_t parts = 1;
-  while (parts < 8 && parts * tiles * n_targets * s.rank_blocks < 512 && k_min / (2 * parts) >= 512) parts *= 2;
+  while (parts < 16 && parts * each < 512 && k_min / (2 * parts) >= (parts * each < 128 ? 256 : 512)) parts *= 2;
   s.parts = (int)parts;
   s.cols = 256;
   while (s.cols > 128 && tiles * n_targets * (n_max / s.cols) < 512) s.cols /= 2;
