@@ -1196,8 +1196,11 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
       }
       run += s;
     }
-    if (first < segs) atomicMin(&sh.first, first);
-    if (last >= 0) atomicMax(&sh.last, last);
+    // lanes hold segments in order; an atomic per wave (per lane the compiler puts a loop over the lanes around
+    // it, 4 us)
+    const uint64_t hit = __ballot(first < segs), any = __ballot(last >= 0);
+    if (hit && lane == __builtin_ctzll(hit)) atomicMin(&sh.first, first);
+    if (any && lane == 63 - __builtin_clzll(any)) atomicMax(&sh.last, last);
   }
   __syncthreads();
   // the segment that holds the target (rounding short of the end: the last with weight), by one wave
