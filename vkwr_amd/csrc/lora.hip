@@ -259,7 +259,7 @@ __device__ __forceinline__ void shrink_steps(const _Float16* xr, const _Float16*
 // Tiles of three or four blocks (prompt chunks) go through LDS: the 16 rows of an operand, 2 K bytes apart,
 // fall on the same sets of the vector cache, so that operands loaded straight into registers, 64 bytes of
 // a row at a time, came in twice (four projections of 2304 rows, K = 4096, rank 64: 107 us; through LDS
-// 36, 3.9 TB/s of the 142 MB that x and A are).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
+// 34, 4.2 TB/s of the 142 MB that x and A are).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
 // chunk c at place c ^ (r & 7) -- in a ring of four, three of them in flight.
 constexpr int kShrinkWaves = 8;
 constexpr int kStageK = 64, kStages = 4;

@@ -1105,7 +1105,7 @@ struct DrawShared {
   int first, last;
 };
 
-// One workgroup per sequence: the segment that holds the target, then the entry.  Seven dependent loads: 10 us,
+// One workgroup per sequence: the segment that holds the target, then the entry.  Dependent loads: 6 us,
 // or 4 where the rows' kernel left the token.
 template <bool kHalf>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p) {
