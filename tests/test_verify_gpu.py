@@ -273,8 +273,8 @@ def test_offsets_past_32_bits(gpu, filt, probs):
     for s in (slice(0, B), slice(B - last, B)):
         tokens = torch.empty(s.stop - s.start, K + 1, dtype=torch.int32, device=gpu)
         accepted = torch.empty(s.stop - s.start, dtype=torch.int32, device=gpu)
-        capi.verify_drafts(logits[s], drafts[s], u[s], tokens, accepted, n_draft=n[s], draft_probs=None if q is None else q[s],
-                           **filt)
+        capi.verify_drafts(logits[s], drafts[s], u[s], tokens, accepted, n_draft=n[s],
+                           draft_probs=None if q is None else q[s], **filt)
         outs.append((tokens[-last:], accepted[-last:]))
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
 

@@ -185,7 +185,8 @@ struct Work {
 };
 __device__ __forceinline__ Work work_of(const LoraArgs& p) {
   const Target& t = p.t[blockIdx.z];
-  Work w{t.x, t.a, t.b, t.base, t.y, t.n, t.k, t.relu2, p.scale, p.h, p.m, p.rank, p.rank_pad, p.n_targets, p.parts, p.cols};
+  Work w{t.x,    t.a,        t.b,         t.base,  t.y,    t.n, t.k, t.relu2, p.scale, p.h, p.m,
+         p.rank, p.rank_pad, p.n_targets, p.parts, p.cols, 0,   0,   {},      nullptr, 0};
   const void* plan = p.plan;
   const int64_t cap = p.tiles_cap;
   const int G = p.G;
@@ -259,8 +260,8 @@ __device__ __forceinline__ void shrink_steps(const _Float16* xr, const _Float16*
 // Tiles of three or four blocks (prompt chunks) go through LDS: the 16 rows of an operand, 2 K bytes apart,
 // fall on the same sets of the vector cache, so that operands loaded straight into registers, 64 bytes of
 // a row at a time, came in twice (four projections of 2304 rows, K = 4096, rank 64: 107 us; through LDS
-// 34, 4.2 TB/s of the 142 MB that x and A are).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each, written by DMA, row r's 16-byte
-// chunk c at place c ^ (r & 7) -- in a ring of four, three of them in flight.
+// 34, 4.2 TB/s of the 142 MB that x and A are).  Stages of 64 k -- 64 rows of x and 64 of A, 128 bytes each,
+// written by DMA, row r's 16-byte chunk c at place c ^ (r & 7) -- in a ring of four, three of them in flight.
 constexpr int kShrinkWaves = 8;
 constexpr int kStageK = 64, kStages = 4;
 constexpr int kStageHalfs = 2 * kTileM * kStageK;
@@ -296,7 +297,8 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 4) void lora_shrink_kernel(LoraA
     if (ri < ns) shrink_steps<RT>(xr, ar, kg, K, s0, s1, acc);
   } else {
     const int blocks = (K + kStageK - 1) / kStageK;
-    const int b0 = (int)((int64_t)blocks * part / tg.parts), b1 = (int)((int64_t)blocks * (part + 1) / tg.parts);
+    const int b0 = (int)((int64_t)blocks * part / tg.parts);
+    const int b1 = (int)((int64_t)blocks * (part + 1) / tg.parts);
     // DMA instruction: 8 rows; wave w fills rows 8 w .. of x and rows 8 (w mod 2 RT) .. of A
     _Float16* const ring = reinterpret_cast<_Float16*>(smem);
     const int w = __builtin_amdgcn_readfirstlane(wv), aw = w % (2 * RT);
