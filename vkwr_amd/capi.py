@@ -555,6 +555,12 @@ class LoraPlan:
             raise ValueError(f"lora plan: bad size ({max_rows} rows, {n_adapters} adapters)")
         self.max_rows, self.n_adapters, self.m = max_rows, n_adapters, None
         self.buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.nbytes, self.ptr, self.dev = nbytes, self.buf.data_ptr(), self.buf.get_device()
+
+    def on(self, dev):
+        if dev != self.dev:
+            raise ValueError(f"lora plan on {self.buf.device}, but the current device is cuda:{dev}")
+        return self.ptr
 
 
 def lora_plan_empty(max_rows, n_adapters, device):
@@ -568,9 +574,9 @@ def lora_plan(adapters, plan):
     m = adapters.numel()
     if m > plan.max_rows:
         raise ValueError(f"lora plan of {plan.max_rows} rows, got {m}")
-    at, nbytes = _Tensors(), plan.buf.numel()
-    _check(_lora_plan(m, plan.n_adapters, at(adapters, torch.int32, m, "adapters"),
-                      at(plan.buf, torch.uint8, nbytes, "plan"), nbytes, at.stream()), "vkwr_lora_plan")
+    at = _Tensors()
+    _check(_lora_plan(m, plan.n_adapters, at(adapters, torch.int32, m, "adapters"), plan.on(at.dev), plan.nbytes,
+                      at.stream()), "vkwr_lora_plan")
     plan.m = m
 
 
@@ -625,5 +631,5 @@ def lora(plan, targets, scale=None, workspace=None):
     if targets[0].sizes[3] != at.dev:
         raise ValueError(f"lora: targets on cuda:{targets[0].sizes[3]}, but the current device is cuda:{at.dev}")
     _check(_lora(m, G, rank, at.optional(scale, torch.float32, G, "scale"),
-                 at(plan.buf, torch.uint8, plan.buf.numel(), "plan"), len(targets), arr,
+                 plan.on(at.dev), len(targets), arr,
                  at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()), "vkwr_lora_f16")
