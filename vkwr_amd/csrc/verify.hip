@@ -675,7 +675,7 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
   };
 
   // The lists: four entries per lane.
-  bool listed = kLists && sum.reach < INFINITY;
+  bool listed = kLists && sum.reach <= mx;  // (else none is listed)
   float mine[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   int mine_at[4] = {-1, -1, -1, -1};
   if (listed) {
