@@ -65,9 +65,9 @@ static_assert(sizeof(RowStat) == 40, "row stat size");
 // How a row's logits are read so that only finite values and -inf (weight 0) remain:
 enum {
   kNanZero = 0, // NaN -> 0
-  kInfOnly = 1, // +inf present (it stands for the largest float, beside which every finite value
-                // weighs nothing): +inf -> 0, anything else -> -inf
-  kAllLow = 2   // -inf everywhere: all entries tied
+  kInfOnly = 1, // the largest is FLT_MAX, which +inf stands for and beside which every other value weighs
+                // nothing (its neighbours are 2e31 apart): FLT_MAX and +inf -> 0, anything else -> -inf
+  kAllLow = 2   // nothing above -FLT_MAX, which -inf stands for: all entries tied
 };
 
 enum { kOpen = 0, kAccepted = 1, kRejected = 2 };  // kRejected: rows behind a rejection too
@@ -273,9 +273,15 @@ __device__ __forceinline__ void block_add(StatShared& sh, int& par, uint32_t& a,
 }
 
 __device__ __forceinline__ float read_as(float l, int mode) {
-  if (mode == kInfOnly) return l == INFINITY ? 0.0f : -INFINITY;
+  if (mode == kInfOnly) return l >= FLT_MAX ? 0.0f : -INFINITY;
   if (mode == kAllLow) return 0.0f;
   return __builtin_isnan(l) ? 0.0f : l;
+}
+
+// The largest logit of a group, with those at the ends of the range as the infinities that they are tied with:
+// what tells how a row is read.
+__device__ __forceinline__ float saturated(float x) {
+  return x >= FLT_MAX ? INFINITY : x <= -FLT_MAX ? -INFINITY : x;
 }
 
 // Order-preserving key of a finite float.
@@ -354,7 +360,7 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
 #pragma unroll
   for (int k = 0; k < kGroupSegs; ++k)
     lane_max = fmaxf(lane_max, fmaxf(fmaxf(l[k][0], l[k][1]), fmaxf(l[k][2], l[k][3])));
-  const float mx = wave_fmax(lane_max);
+  const float mx = saturated(wave_fmax(lane_max));
   if (lane == 0) p.group_max[id * p.groups + group] = mx;
   bool flat = false;
   if (!p.truncate || p.use_mass) {
