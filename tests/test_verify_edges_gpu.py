@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests.test_verify_gpu import check, make
+from vkwr_amd import capi
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,22 @@ def test_infinities_beside_the_ends_of_the_range(gpu, V, probs, filt):
     l[7, :, 1], l[7, :, 2:] = F, -INF
     d["n_draft"][:] = 3
     check(gpu, d, **filt)
+
+
+def test_uniform_of_zero_on_weights_that_underflow(gpu):
+    """Without a filter a segment's sum is kept relative to its group's largest logit: in units of the row's it
+    may be a denormal where every single weight is 0 (here 2^-1039 beside 2^-1010 in its group, 1 in the next).
+    A uniform of 0 has to fall on an entry that has a weight, in vocabulary order."""
+    V = 4096
+    for drafted in (0, 1):
+        l = torch.full((2, drafted + 1, V), -INF)
+        l[:, :, 3:200] = -720.0
+        l[:, :, 256:260] = -700.0
+        l[:, :, 2048:2050] = 0.0
+        tokens = torch.full((2, drafted + 1), -5, dtype=torch.int32, device=gpu)
+        accepted = torch.empty(2, dtype=torch.int32, device=gpu)
+        u = torch.zeros(2, drafted + 1)
+        u[:, 0] = 0.0 if drafted == 0 else 0.9  # the draft, half of the row's mass, is rejected
+        capi.verify_drafts(l.to(gpu), torch.full((2, drafted), 2048, dtype=torch.int32, device=gpu), u.to(gpu), tokens,
+                           accepted)
+        assert tokens[:, 0].tolist() == [256, 256] and accepted.tolist() == [0, 0]

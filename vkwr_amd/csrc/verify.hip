@@ -1164,7 +1164,10 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs p)
         else if (stop.st.mode == kAllLow) s = (double)(min(p.V, (k + 1) * kSeg) - k * kSeg) * stop.unit;
         else {
           const float gm = p.group_max[stop.id * p.groups + k / kGroupSegs];
-          s = gm > -INFINITY ? src[k] * group_factor(p, gm, top) * stop.unit : 0.0;
+          s = gm > -INFINITY ? src[k] * group_factor(p, gm, top) : 0.0;
+          // (weights end at 2^-1022: a sum of 256 down to 2^-1013 has one that is more than 0, a smaller one
+          // may have none, and a uniform of 0 would fall on it)
+          s = s >= 0x1p-1013 ? s * stop.unit : 0.0;
         }
         sh.sum[k] = s;
       }
