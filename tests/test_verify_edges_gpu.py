@@ -51,3 +51,29 @@ def test_uniform_of_zero_on_weights_that_underflow(gpu):
         capi.verify_drafts(l.to(gpu), torch.full((2, drafted), 2048, dtype=torch.int32, device=gpu), u.to(gpu), tokens,
                            accepted)
         assert tokens[:, 0].tolist() == [256, 256] and accepted.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("filt", [{}, {"top_p": 0.95}, {"top_k": 2, "top_p": 0.95}], ids=["all", "p95", "k2p95"])
+@pytest.mark.parametrize("reject", [3, 63, 64, 65, 100000, 262143])
+def test_hundreds_of_thousands_of_drafts(gpu, filt, reject):
+    """The work has to grow with the drafts, not with their square: what each row tests of those before it is
+    bounded.  (One sequence; entry 1 of 8 holds all but e^-20 of each row, and is drafted up to `reject`.)"""
+    K, V = 262143, 8
+    l = torch.full((1, K + 1, V), -20.0)
+    l[:, :, 1] = 0.0
+    drafts = torch.ones(1, K, dtype=torch.int32)
+    if reject < K:
+        drafts[0, reject] = 2
+    u = torch.full((1, K + 1), 0.5)
+    args = [t.to(gpu) for t in (l.half(), drafts, u)]
+    tokens = torch.full((1, K + 1), -5, dtype=torch.int32, device=gpu)
+    accepted = torch.empty(1, dtype=torch.int32, device=gpu)
+    ws = torch.empty(capi.verify_workspace_bytes(1, K, V), dtype=torch.uint8, device=gpu)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    capi.verify_drafts(*args, tokens, accepted, workspace=ws, **filt)
+    end.record()
+    torch.cuda.synchronize()
+    assert accepted.item() == reject
+    assert (tokens[0, :reject + 1] == 1).all() and (tokens[0, reject + 1:] == -1).all()
+    assert start.elapsed_time(end) < 2000.0  # milliseconds

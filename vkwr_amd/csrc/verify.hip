@@ -549,6 +549,9 @@ __device__ __forceinline__ Draft load_draft(const VerifyArgs& p, int b, int k) {
 // tau <= l_d where it is positive.  Margins of 1e-7 for the rounding of either side: 2^19 units of 2^-43 at most
 // (6e-8) where all of a row's masses round the same way; a rejection here and the full test never disagree.
 enum { kUnsure, kAccept, kReject };
+// A row looks at this many drafts before its own: without an end K drafts were K^2 / 2 tests (262143 drafts of
+// one sequence: 34 thousand million).  Rows behind a later rejection are searched for nothing.
+constexpr int kQuickRows = 64;
 template <bool kHalf>
 __device__ __forceinline__ int quick_test(const VerifyArgs& p, int b, int k, int lane) {
   const Draft d = load_draft<kHalf>(p, b, k);
@@ -612,10 +615,13 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
     // but the verdict are read of them).  Of 128 sequences' 566 rows (4 drafts, nucleus 0.95) 271 are left.
     if (t == 0) sh.bin = sh.n_cand = 0;
     __syncthreads();
-    for (int k = wv; k <= i && k < n; k += W) {
-      const int v = quick_test<kHalf>(p, b, k, lane);
-      if (lane == 0 && k < i && v == kReject) sh.bin = 1;
-      if (lane == 0 && k == i && v == kAccept) sh.n_cand = 1;
+    const int before = min(i, kQuickRows);  // of the drafts before row i the first ones; then its own
+    for (int k = wv; k <= before; k += W) {
+      const int at = k < before ? k : i;
+      if (at >= n) continue;
+      const int v = quick_test<kHalf>(p, b, at, lane);
+      if (lane == 0 && at < i && v == kReject) sh.bin = 1;
+      if (lane == 0 && at == i && v == kAccept) sh.n_cand = 1;
     }
     __syncthreads();
     if (sh.bin != 0 || sh.n_cand != 0) {
@@ -628,12 +634,10 @@ __global__ __launch_bounds__(kThreads, kLists ? 3 : 4) void verify_rows_kernel(V
     __syncthreads();
   }
   if (!kLists && p.cap > 0) {  // the launch behind the lists': open rows that no known rejection is before
-    bool out = false;
-    for (int k = lane; k <= i; k += 64) {
-      const int v = p.stat[(int64_t)b * T + k].verdict;  // (not written by this launch's others)
-      out = out || v == kRejected || (k == i && v != kOpen);
-    }
-    if (__ballot(out) != 0) return;
+    static_assert(kQuickRows <= 64, "a lane each");
+    const int own = p.stat[id].verdict;  // (neither these are written by this launch's others)
+    const int v = lane < min(i, kQuickRows) ? p.stat[(int64_t)b * T + lane].verdict : kOpen;
+    if (own != kOpen || __ballot(v == kRejected) != 0) return;
   }
   const RowSummary sum = summarize(p, id, lane, own_group);
   const float mx = sum.max;
