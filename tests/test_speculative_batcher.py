@@ -1,0 +1,130 @@
+"""The batchers' own logic on the CPU: an engine whose logits are a fixed function of a sequence's last tokens,
+and the 64-bit oracle in place of the verification kernel."""
+import types
+
+import pytest
+import torch
+
+from oracle import serving_ref
+from vkwr.model_executor import ContinuousBatcher, SpeculativeBatcher
+from vkwr_amd import capi
+
+V = 16
+
+
+def logits_of(tokens):
+    """Small whole numbers, so that the largest are tied more often than not."""
+    g = torch.Generator().manual_seed(hash(tuple(tokens[-2:])) % 2 ** 31)
+    return torch.randint(0, 4, (V,), generator=g).float()
+
+
+class Engine:
+    """A sequence's tokens are its state: their number, then the tokens."""
+
+    def __init__(self, draft_seqs=4, max_draft=3, max_rows=64):
+        self.draft_seqs, self.max_draft, self.max_rows, self.max_seqs = draft_seqs, max_draft, max_rows, max_rows
+        self.cfg = types.SimpleNamespace(vocab=V)
+        self.model = types.SimpleNamespace(head=torch.empty(0))
+        self.kept = None
+
+    def _tokens(self, state, slot):
+        s = state.wkv[0, slot]
+        return s[1:1 + int(s[0])].int().tolist()
+
+    def _append(self, state, slot, tokens):
+        s = state.wkv[0, slot]
+        n = int(s[0])
+        s[1 + n:1 + n + len(tokens)] = torch.tensor(tokens).float()
+        s[0] = n + len(tokens)
+
+    def step(self, state, decode=None, prefill=(), adapter_ids=None, flush=True):
+        out = []
+        groups = ([(decode[0][:, None], decode[1])] if decode else []) + list(prefill)
+        for tokens, slots in groups:
+            for t, slot in zip(tokens.tolist(), slots.tolist()):
+                self._append(state, slot, t)
+                out.append(logits_of(self._tokens(state, slot)))
+        return torch.stack(out)
+
+    def draft_step(self, state, tokens, slots, adapter_ids=None):
+        assert self.kept is None
+        self.kept = (state, tokens.tolist(), slots)
+        return torch.stack([torch.stack([logits_of(self._tokens(state, slot) + t[:i + 1]) for i in range(len(t))])
+                            for t, slot in zip(tokens.tolist(), slots)])
+
+    def accept(self, accepted):
+        (state, tokens, slots), self.kept = self.kept, None
+        for t, slot, n in zip(tokens, slots, accepted.tolist()):
+            self._append(state, slot, t[:n + 1])
+
+    def drop(self, slots, state=None):
+        pass
+
+
+def make_state(n_slots=4):
+    return types.SimpleNamespace(n_slots=n_slots, wkv=torch.zeros(1, n_slots, 200), att_shift=torch.zeros(1, n_slots, 1),
+                                 ffn_shift=torch.zeros(1, n_slots, 1))
+
+
+@pytest.fixture
+def oracle(monkeypatch):
+    def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_draft=None, draft_probs=None, workspace=None, **filt):
+        wt, wa = serving_ref.verify(logits.numpy(), drafts.numpy(), uniforms.numpy(),
+                                    None if n_draft is None else n_draft.numpy(), draft_probs, **filt)
+        tokens.copy_(torch.from_numpy(wt))
+        accepted.copy_(torch.from_numpy(wa))
+
+    monkeypatch.setattr(capi, "verify_drafts", verify_drafts)
+
+
+def run(batcher, prompts):
+    reqs = [batcher.submit(p, 5 + 4 * i) for i, p in enumerate(prompts)]
+    batcher.run()
+    return [r.output for r in reqs]
+
+
+PROMPTS = [[1, 2, 3, 1, 2], [7], [4, 4, 4, 4], [9, 8, 9, 8, 9], [0, 0], [15, 3, 2]]
+
+
+@pytest.mark.parametrize("filt", [{}, {"top_k": 1, "top_p": 0.5}, {"top_k": 7, "top_p": 0.0}])
+def test_greedy_tokens_are_the_first_of_the_largest(oracle, filt):
+    """Whatever the seed, the drafts and the other sequences of a step, and the tokens of plain decoding; the
+    drafts here are often right, tied with the right one, or behind a short draft."""
+    want = run(ContinuousBatcher(Engine(), make_state(), max_decode=4, chunk=3), PROMPTS)
+    tied = 0
+    for p, o in zip(PROMPTS, want):
+        for i, t in enumerate(o):
+            l = logits_of((p + o[:i]))
+            assert t == int((l == l.max()).nonzero()[0])
+            tied += int((l == l.max()).sum()) > 1
+    assert tied > 10
+
+    def largest(tokens, n):  # the last of the largest
+        out = []
+        for _ in range(n if len(tokens) % 3 else 1):
+            l = logits_of(tokens + out)
+            out.append(int((l == l.max()).nonzero()[-1 if len(out) else 0]))
+        return out[:n]
+
+    def zeros(tokens, n):
+        return [0] * (n - len(tokens) % 2)
+
+    for seed in (0, 1):
+        for draft in ({}, {"draft": largest}, {"draft": zeros}):
+            b = SpeculativeBatcher(Engine(), make_state(), max_decode=4, chunk=3, seed=seed, **draft, **filt)
+            assert run(b, PROMPTS) == want
+    for n in (1, 3):
+        assert run(SpeculativeBatcher(Engine(n), make_state(2), chunk=3, draft=largest, **filt), PROMPTS) == want
+
+
+def test_accepted_drafts_save_steps(oracle):
+    def exact(tokens, n):
+        out = []
+        for _ in range(n):
+            l = logits_of(tokens + out)
+            out.append(int(l.argmax()))
+        return out
+
+    b = SpeculativeBatcher(Engine(), make_state(), draft=exact, chunk=8)
+    run(b, PROMPTS[:1] * 4)
+    assert b.accepted == b.drafted > 0

@@ -1,0 +1,30 @@
+"""Speculative decoding on the tiny RWKV-7 shape: tied logits, and kept tokens of sequences that are gone."""
+import pytest
+import torch
+
+from tests.test_drafts_adapters_gpu import _i32, _tiny
+
+pytestmark = pytest.mark.gpu
+
+
+def test_greedy_takes_the_lowest_of_tied_logits(gpu):
+    """Vocabulary entries 2 i and 2 i + 1 share their head's row, so every logit is tied with its neighbour's:
+    even tokens only, whatever the seed, and though the drafts are odd ones too."""
+    from vkwr.model_executor import DraftEngine, SpeculativeBatcher
+    cfg, model, state = _tiny(gpu, 4)
+    model.head[1::2] = model.head[::2]
+    outs = []
+
+    def either(tokens, n):
+        return [(known[len(tokens) + i] + i % 2) if len(tokens) + i < len(known) else 0 for i in range(n)]
+
+    known = []
+    for seed, kw in ((0, {}), (1, {}), (2, {"draft": either}), (3, {"draft": either, "top_p": 0.0, "top_k": 5})):
+        sched = SpeculativeBatcher(DraftEngine(model, 3, 3, max_rows=32), state, max_prefill_chunks=2, chunk=8, seed=seed, **kw)
+        reqs = [sched.submit([6, 8, 6, 8, 6], 16) for _ in range(3)]
+        sched.run()
+        outs.append([r.output for r in reqs])
+        known = reqs[0].prompt + reqs[0].output
+        assert all(t % 2 == 0 for r in reqs for t in r.output)
+    assert outs[0] == outs[1]
+    assert sched.drafted > sched.accepted > 0

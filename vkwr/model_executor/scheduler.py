@@ -218,7 +218,8 @@ def prompt_lookup(tokens, n, match=2):
 
 class SpeculativeBatcher(ContinuousBatcher):
     """Continuous batching with drafted tokens on a DraftEngine.  `draft(tokens, n)` proposes up to n
-    tokens behind a sequence's tokens (default: looked up in them); top_k = 1 generates greedily.
+    tokens behind a sequence's tokens (default: looked up in them); top_k = 1 generates greedily, the lowest
+    index among equal logits, whatever the drafts and the seed.
     Prompt chunks run as in ContinuousBatcher, in a step of their own before the drafts'."""
 
     def __init__(self, engine, state, draft=prompt_lookup, temperature=1.0, top_k=1, top_p=1.0, seed=0, **kw):
@@ -230,18 +231,42 @@ class SpeculativeBatcher(ContinuousBatcher):
         self.draft, self.filter = draft, dict(temperature=temperature, top_k=top_k, top_p=top_p)
         self.gen = torch.Generator(device=self.device).manual_seed(seed)
         V = engine.cfg.vocab
-        need = max(capi.verify_workspace_bytes(B, T - 1, V), capi.verify_workspace_bytes(self.max_prefill_chunks, 0, V))
+        # top_k = 1 (top_p = 0 stands for it): a row of its own per token
+        self.greedy = top_k == 1 or top_p == 0
+        P = self.max_prefill_chunks
+        sizes = ((B * T, 0), (P, 0)) if self.greedy else ((B, T - 1), (P, 0))
+        need = max(capi.verify_workspace_bytes(b, k, V) for b, k in sizes)
         self.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self.zeros = torch.zeros(max(B * T, P), 1, device=self.device)
         self.drafted = self.accepted = 0
 
     def _verify(self, logits, drafts, n_draft):
-        """logits [B, T, V]: (tokens, accepted) on the device."""
+        """logits [B, T, V], n_draft: the drafts' lengths (host); (tokens, accepted) on the device."""
         B, T, _ = logits.shape
+        if self.greedy:
+            return self._verify_greedy(logits, drafts, n_draft)
         tokens = torch.empty(B, T, dtype=torch.int32, device=self.device)
         accepted = torch.empty(B, dtype=torch.int32, device=self.device)
         u = torch.rand(B, T, generator=self.gen, device=self.device)
-        capi.verify_drafts(logits, drafts, u, tokens, accepted, n_draft=n_draft, workspace=self.ws, **self.filter)
+        capi.verify_drafts(logits, drafts, u, tokens, accepted, n_draft=self._i32(n_draft), workspace=self.ws,
+                           **self.filter)
         return tokens, accepted
+
+    def _verify_greedy(self, logits, drafts, n_draft):
+        """As _verify, where only a row's first largest logit will do (fp16 logits are often tied, and the filter
+        keeps all entries that are): every row's token is drawn with the uniform 0, which falls on the first kept
+        entry, and compared with the draft.  Rows behind a short draft (a length of -1) are not looked at."""
+        B, T, V = logits.shape
+        best = torch.empty(B * T, 1, dtype=torch.int32, device=self.device)
+        count = torch.empty(B * T, dtype=torch.int32, device=self.device)
+        capi.verify_drafts(logits.view(B * T, 1, V), drafts.new_empty(B * T, 0), self.zeros[:B * T], best, count,
+                           n_draft=self._i32([0 if t <= n else -1 for n in n_draft for t in range(T)]),
+                           workspace=self.ws, **self.filter)
+        best = best.view(B, T)
+        # (behind a short draft: drafts of -1, which no row's token is)
+        accepted = (best[:, :T - 1] == drafts).to(torch.int32).cumprod(1).sum(1, dtype=torch.int32)
+        kept = torch.arange(T, device=self.device) <= accepted[:, None]
+        return torch.where(kept, best, -1), accepted
 
     def _finish(self):
         finished = [r for r in self.running if r.done]
@@ -265,7 +290,7 @@ class SpeculativeBatcher(ContinuousBatcher):
             # (a prompt's slot is fresh: no kept tokens)
             logits = self.engine.step(self.state, prefill=prefill, flush=False, **self._adapter_ids(flat))
             none = torch.empty(len(flat), 0, dtype=torch.int32, device=self.device)
-            nxt = self._verify(logits[:, None, :], none, None)[0][:, 0].tolist()
+            nxt = self._verify(logits[:, None, :], none, [0] * len(flat))[0][:, 0].tolist()
             for (t, r), token in zip([(t, r) for t, reqs in order for r in reqs], nxt):
                 r.pos += t
                 self.tokens_processed += t
@@ -280,9 +305,9 @@ class SpeculativeBatcher(ContinuousBatcher):
             K = self.engine.max_draft
             drafts = [list(self.draft(r.prompt + r.output, min(K, r.max_new_tokens - len(r.output) - 1)))[:K] for r in dec]
             T = 1 + max(len(d) for d in drafts)
-            rows = self._i32([[r.output[-1]] + d + [0] * (T - 1 - len(d)) for r, d in zip(dec, drafts)])
+            rows = self._i32([[r.output[-1]] + d + [-1] * (T - 1 - len(d)) for r, d in zip(dec, drafts)])
             logits = self.engine.draft_step(self.state, rows, [r.slot for r in dec], **self._adapter_ids(dec))
-            tokens, accepted = self._verify(logits, rows[:, 1:].contiguous(), self._i32([len(d) for d in drafts]))
+            tokens, accepted = self._verify(logits, rows[:, 1:].contiguous(), [len(d) for d in drafts])
             self.engine.accept(accepted)
             for r, d, new, n in zip(dec, drafts, tokens.tolist(), accepted.tolist()):
                 r.output += new[:min(n + 1, r.max_new_tokens - len(r.output))]
