@@ -28,3 +28,22 @@ def test_greedy_takes_the_lowest_of_tied_logits(gpu):
         assert all(t % 2 == 0 for r in reqs for t in r.output)
     assert outs[0] == outs[1]
     assert sched.drafted > sched.accepted > 0
+
+
+def test_sequences_that_end_leave_another_states_kept_tokens(gpu):
+    """One engine for two states: a request that ends on the one in slot 2 has nothing to do with the tokens kept
+    of slot 2 of the other."""
+    from vkwr.model_executor import DraftEngine, RWKV7State, SpeculativeBatcher
+    from vkwr_amd import capi
+    cfg, model, state = _tiny(gpu, 4)
+    eng = DraftEngine(model, 2, 2, max_rows=24)
+    eng.draft_step(state, _i32([[5, 6, 7], [8, 9, 10]], gpu), [2, 0])
+    eng.accept(_i32([2, 1], gpu))
+    before = state.wkv.clone()
+    other = SpeculativeBatcher(eng, RWKV7State(cfg, 4, gpu, std=0.0, layout=capi.WKV_STATE_STD), max_prefill_chunks=4, chunk=4)
+    reqs = [other.submit([1 + i, 2, 3], 1) for i in range(4)]
+    assert len(other.run()) == 4 and all(len(r.output) == 1 for r in reqs)
+    assert set(eng.rows_of) == {0, 2}
+    eng.flush(state)
+    changed = (state.wkv != before).flatten(2).any(-1).any(0)
+    assert changed.tolist() == [True, False, True, False]

@@ -184,8 +184,10 @@ class DraftEngine(MixedEngine):
                                   pending_rows=rows)
         self.drop(todo)
 
-    def drop(self, slots):
-        """Forgets the kept tokens of these slots (sequences that end)."""
+    def drop(self, slots, state=None):
+        """Forgets the kept tokens of these slots (sequences that end); given a state, only if they are its."""
+        if state is not None and self.pool_of is not state.wkv:
+            return
         for i in slots:
             self.rows_of.pop(i, None)
 

@@ -271,7 +271,7 @@ class SpeculativeBatcher(ContinuousBatcher):
     def _finish(self):
         finished = [r for r in self.running if r.done]
         for r in finished:
-            self.engine.drop([r.slot])
+            self.engine.drop([r.slot], self.state)
             self.slots.free(r.slot)
         self.running = [r for r in self.running if not r.done]
         return finished
