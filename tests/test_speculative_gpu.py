@@ -47,3 +47,30 @@ def test_sequences_that_end_leave_another_states_kept_tokens(gpu):
     eng.flush(state)
     changed = (state.wkv != before).flatten(2).any(-1).any(0)
     assert changed.tolist() == [True, False, True, False]
+
+
+@pytest.mark.parametrize("plain", [False, True])
+def test_a_new_sequence_takes_no_kept_tokens_of_the_slots_last_user(gpu, plain):
+    """A batcher that is left in the middle of its requests, then another one on the same engine and state."""
+    from vkwr.model_executor import ContinuousBatcher, DraftEngine, SpeculativeBatcher
+    cfg, model, state = _tiny(gpu, 3)
+
+    def serve(eng):
+        if plain:
+            sched = ContinuousBatcher(eng, state, max_decode=3, max_prefill_chunks=3, chunk=8)
+        else:
+            sched = SpeculativeBatcher(eng, state, max_prefill_chunks=3, chunk=8)
+        reqs = [sched.submit([2 + i, 4, 2 + i, 4], 8) for i in range(3)]
+        sched.run()
+        return [r.output for r in reqs], state.wkv.clone()
+
+    want = serve(DraftEngine(model, 3, 2, max_rows=32))
+    eng = DraftEngine(model, 3, 2, max_rows=32)
+    left = SpeculativeBatcher(eng, state, max_prefill_chunks=3, chunk=8)
+    for _ in range(3):
+        left.submit([9, 7, 5, 9, 7], 40)
+    for _ in range(3):
+        left.step()
+    assert set(eng.rows_of) == {0, 1, 2}
+    got = serve(eng)
+    assert got[0] == want[0] and torch.equal(got[1], want[1])

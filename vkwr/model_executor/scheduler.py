@@ -112,6 +112,9 @@ class ContinuousBatcher:
         st.wkv[:, slot].zero_()
         st.att_shift[:, slot].zero_()
         st.ffn_shift[:, slot].zero_()
+        drop = getattr(self.engine, "drop", None)  # a DraftEngine: what it keeps of the slot's last user
+        if drop is not None:
+            drop([slot], st)
 
     def _i32(self, values):
         return torch.tensor(values, dtype=torch.int32).to(self.device, non_blocking=True)
