@@ -74,3 +74,22 @@ def test_a_new_sequence_takes_no_kept_tokens_of_the_slots_last_user(gpu, plain):
     assert set(eng.rows_of) == {0, 1, 2}
     got = serve(eng)
     assert got[0] == want[0] and torch.equal(got[1], want[1])
+
+
+def test_drop_waits_for_accept(gpu):
+    """Between a draft step and its accept nothing is kept yet: a drop there would be undone by the accept."""
+    from vkwr.model_executor import DraftEngine, RWKV7State
+    from vkwr_amd import capi
+    cfg, model, state = _tiny(gpu, 4)
+    other = RWKV7State(cfg, 4, gpu, layout=capi.WKV_STATE_STD)
+    eng = DraftEngine(model, 2, 2)
+    eng.draft_step(state, _i32([[5, 6], [8, 9]], gpu), [2, 0])
+    for args in (([2],), ([2], state)):
+        with pytest.raises(RuntimeError):
+            eng.drop(*args)
+    eng.drop([2], other)
+    eng.accept(_i32([1, 1], gpu))
+    eng.drop([2], other)
+    assert set(eng.rows_of) == {0, 2}
+    eng.drop([2], state)
+    assert set(eng.rows_of) == {0}

@@ -185,7 +185,10 @@ class DraftEngine(MixedEngine):
         self.drop(todo)
 
     def drop(self, slots, state=None):
-        """Forgets the kept tokens of these slots (sequences that end); given a state, only if they are its."""
+        """Forgets the kept tokens of these slots (sequences that end); given a state, only if they are its.
+        Not between a draft step and its accept, which is what says that tokens are kept."""
+        if self.open is not None and (state is None or self.open[0].wkv is state.wkv):
+            raise RuntimeError("drop: the last step's drafts are not accepted yet")
         if state is not None and self.pool_of is not state.wkv:
             return
         for i in slots:
