@@ -16,8 +16,10 @@ def lora(x, a, b, base, adapters, scale=None, relu2=False):
     """y [m, n] float64 and a bound of the error of the fp32 computation before the rounding to
     fp16.  The sum over k: every addition rounds its partial sum, whose size is about
     s = sqrt(sum (x a)^2) for terms of random sign, so the errors walk to u s sqrt(k) at most in
-    the rms; 8 of those are allowed.  h enters the second product within 2^-22 of itself and of
-    its row's largest value 2^-25; that product's r + 2 roundings count u each."""
+    the rms; 8 of those are allowed.  h enters the second product as two fp16 halves of a value
+    whose row's largest is at least 2^14: within 2^-22 of itself, and where the second half is a
+    denormal, half of 2^-24, which is 2^-39 of that largest; that product's r + 2 roundings count
+    u each."""
     x, a, b, y = x.double(), a.double(), b.double(), base.double().clone()
     G, R, K = a.shape
     err = torch.zeros_like(y)
@@ -30,7 +32,7 @@ def lora(x, a, b, base, adapters, scale=None, relu2=False):
         s = 1.0 if scale is None else float(scale[g])
         h = s * (a[g] @ x[i])
         eh = 8 * U32 * math.sqrt(K) * abs(s) * torch.sqrt((a[g] ** 2) @ (x[i] ** 2)) + 2.0 ** -22 * h.abs()
-        eh = eh + 2.0 ** -25 * (h.abs().max() if R else 0.0) + 2 * U32 * h.abs()
+        eh = eh + 2.0 ** -39 * (h.abs().max() if R else 0.0) + 2 * U32 * h.abs()
         y[i] += b[g] @ h
         err[i] = b[g].abs() @ eh + (R + 2) * U32 * (b[g].abs() @ h.abs())
     err = err + U32 * y.abs()

@@ -12,8 +12,10 @@
 //   expand  the parts added in order, y = epi(base + scale h B^T)
 // Both run on the matrix cores with 16 rows of x (or h) as the columns of v_mfma_f32_16x16x32_f16,
 // the adapter's rows as its rows.  h is not rounded to fp16: it enters the second product as a sum
-// of two halves (fp16(h) and fp16(h - fp16(h)), 22 bits), a product each, after a power of two per row
-// has brought its largest value to [1, 2) so that neither half leaves fp16's range.
+// of two halves (fp16(h) and fp16(h - fp16(h)), a product each), after a power of two per row has brought its
+// largest value to [2^14, 2^15), the top of fp16's range, as what is far below the largest leaves it at the
+// lower end: 22 bits of each value, and never more than 2^-39 of the row's largest off.  (128 products with
+// fp16 entries of B stay below 2^38 in the fp32 sums.)
 
 #include <algorithm>
 
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
     }
     for (int d = 1; d < groups; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d, 64));
     const int ex = (int)(mx >> 23);                      // biased exponent of the row's largest value
-    const int sh = ex == 0 || ex == 255 ? 0 : 127 - ex;  // zeros (and denormals), infinities, NaN: as they are
+    const int sh = ex == 255 ? 0 : 141 - max(ex, 1);     // to [2^14, 2^15); infinities, NaN: as they are
     if (r < kTileM && gr == 0) back[r] = -sh;
     hv8 vh, vl;
 #pragma unroll
