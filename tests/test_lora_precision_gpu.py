@@ -34,3 +34,19 @@ def test_ranks_of_different_sizes(gpu, m, R, K, last):
     t["a"], t["b"] = (t["a"].float() * f[:, None]).half(), (t["b"].float() / f).half()
     assert t["b"].abs().max() < 60000
     cancelled(gpu, d)
+
+
+def test_an_infinite_rank_leaves_the_others_finite(gpu):
+    """One rank of an adapter overflows (an infinity in A) beside inner values beyond fp16's range: the result is
+    that infinity, not the NaN of two."""
+    m, R, K, N = 5, 8, 64, 16
+    a = torch.ones(1, R, K).half()
+    a[0, 0, 0] = float("inf")
+    x = torch.full((m, K), 8192.0).half()    # inner values of 2^19 where finite
+    x[3] = 2.0
+    b = torch.full((1, N, R), -2.0 ** -10).half()
+    b[0, ::2, 0] = 2.0 ** -10                # (odd columns: of the same sign as the others)
+    d = {"ids": torch.zeros(m, dtype=torch.int32), "scale": None,
+         "t": [{"x": x, "a": a, "b": b, "base": torch.zeros(m, N).half()}]}
+    y = run_lora(gpu, d)[0].float().cpu()
+    assert (y[:, ::2] == float("inf")).all() and (y[:, 1::2] == -float("inf")).all()

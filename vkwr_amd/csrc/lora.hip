@@ -468,12 +468,12 @@ __global__ __launch_bounds__(64 * kExpandWaves, 4) void lora_expand_kernel(LoraA
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         hv[e] = live ? (e < 4 ? lo[e & 3] : hi[e & 3]) * sc : 0.0f;
-        mx = max(mx, __builtin_bit_cast(uint32_t, hv[e]) & 0x7fffffffu);
+        const uint32_t size = __builtin_bit_cast(uint32_t, hv[e]) & 0x7fffffffu;
+        mx = max(mx, size < 0x7f800000u ? size : 0);  // the largest finite one: infinities, NaN pass as they are
       }
     }
     for (int d = 1; d < groups; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d, 64));
-    const int ex = (int)(mx >> 23);                      // biased exponent of the row's largest value
-    const int sh = ex == 255 ? 0 : 141 - max(ex, 1);     // to [2^14, 2^15); infinities, NaN: as they are
+    const int sh = 141 - max((int)(mx >> 23), 1);  // its biased exponent becomes that of [2^14, 2^15)
     if (r < kTileM && gr == 0) back[r] = -sh;
     hv8 vh, vl;
 #pragma unroll
