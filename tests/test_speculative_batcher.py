@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import serving_ref
-from vkwr.model_executor import ContinuousBatcher, SpeculativeBatcher
+from vkwr.model_executor import ContinuousBatcher, Request, SpeculativeBatcher
 from vkwr_amd import capi
 
 V = 16
@@ -128,3 +128,9 @@ def test_accepted_drafts_save_steps(oracle):
     b = SpeculativeBatcher(Engine(), make_state(), draft=exact, chunk=8)
     run(b, PROMPTS[:1] * 4)
     assert b.accepted == b.drafted > 0
+
+
+def test_request_fields_keep_their_places():
+    """Fields that came later stand behind those that callers may give by position."""
+    r = Request([1, 2, 3], 4, 5, 6, 2, [9])
+    assert (r.rid, r.slot, r.pos, r.output, r.adapter) == (5, 6, 2, [9], -1) and r.prefilling

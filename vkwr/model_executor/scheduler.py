@@ -36,9 +36,9 @@ class Request:
     max_new_tokens: int
     rid: int = -1
     slot: int = -1
-    adapter: int = -1                  # of the engine's AdapterPool; -1: none
     pos: int = 0                       # prompt tokens consumed
     output: list = field(default_factory=list)
+    adapter: int = -1                  # of the engine's AdapterPool; -1: none
 
     @property
     def prefilling(self):
