@@ -134,3 +134,10 @@ def test_request_fields_keep_their_places():
     """Fields that came later stand behind those that callers may give by position."""
     r = Request([1, 2, 3], 4, 5, 6, 2, [9])
     assert (r.rid, r.slot, r.pos, r.output, r.adapter) == (5, 6, 2, [9], -1) and r.prefilling
+
+
+def test_a_sample_function_is_refused():
+    """(It would not be called: the verification draws the tokens.)"""
+    with pytest.raises(TypeError):
+        SpeculativeBatcher(Engine(), make_state(), chunk=8, sample=lambda logits: logits.argmax(-1))
+    SpeculativeBatcher(Engine(), make_state(), chunk=8, sample=None)

@@ -226,6 +226,8 @@ class SpeculativeBatcher(ContinuousBatcher):
     Prompt chunks run as in ContinuousBatcher, in a step of their own before the drafts'."""
 
     def __init__(self, engine, state, draft=prompt_lookup, temperature=1.0, top_k=1, top_p=1.0, seed=0, **kw):
+        if kw.get("sample") is not None:
+            raise TypeError("tokens are drawn by verify_drafts (temperature, top_k, top_p): no sample function")
         kw.setdefault("max_decode", engine.draft_seqs)
         if kw["max_decode"] > engine.draft_seqs:
             raise ValueError(f"{kw['max_decode']} generating sequences, the engine drafts {engine.draft_seqs}")
