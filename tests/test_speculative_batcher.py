@@ -141,3 +141,69 @@ def test_a_sample_function_is_refused():
     with pytest.raises(TypeError):
         SpeculativeBatcher(Engine(), make_state(), chunk=8, sample=lambda logits: logits.argmax(-1))
     SpeculativeBatcher(Engine(), make_state(), chunk=8, sample=None)
+
+
+class Counted(int):
+    """A token that counts its comparisons."""
+    count = 0
+
+    def __eq__(self, other):
+        Counted.count += 1
+        return int(self) == int(other)
+
+    __hash__ = int.__hash__
+
+
+def test_looked_up_drafts_are_prompt_lookups(oracle):
+    """What the batcher looks up is what prompt_lookup finds in the whole sequence, at every step."""
+    from vkwr.model_executor.scheduler import prompt_lookup
+    seen = []
+
+    def spy(tokens, n):
+        seen.append((tuple(tokens), n))
+        return prompt_lookup(tokens, n)
+
+    outs = [run(SpeculativeBatcher(Engine(), make_state(), chunk=3, **kw), PROMPTS) for kw in ({}, {"draft": spy})]
+    assert outs[0] == outs[1]
+    calls = []
+    b = SpeculativeBatcher(Engine(), make_state(), chunk=3)
+    draft = b._draft
+    b._draft = lambda r, n: calls.append((tuple(r.prompt + r.output), n, draft(r, n))) or calls[-1][2]
+    assert run(b, PROMPTS) == outs[0] and not b.lookups
+    assert [c[:2] for c in calls] == seen
+    assert all(d == prompt_lookup(list(t), n) for t, n, d in calls) and any(d for _, _, d in calls)
+
+
+def test_lookups_of_growing_sequences():
+    from vkwr.model_executor.scheduler import _Lookup, prompt_lookup
+    g = torch.Generator().manual_seed(3)
+    for trial in range(40):
+        r = Request(torch.randint(0, 4, (1 + trial % 5,), generator=g).tolist(), 100)
+        look = _Lookup(r.prompt)
+        for _ in range(30):
+            n = int(torch.randint(0, 5, (1,), generator=g))
+            assert look(r, n) == prompt_lookup(r.prompt + r.output, n)
+            r.output += torch.randint(0, 4, (1 + n,), generator=g).tolist()
+
+
+def test_looking_up_drafts_does_not_walk_the_sequence(oracle):
+    """A prompt of different tokens: a step compares no more than a few of them."""
+    import vkwr.model_executor.scheduler as scheduler
+
+    class Long(Engine):
+        def step(self, state, decode=None, prefill=(), adapter_ids=None, flush=True):
+            return torch.stack([logits_of(t) for tokens, _ in prefill for t in tokens.tolist()])
+
+        def draft_step(self, state, tokens, slots, adapter_ids=None):
+            return torch.stack([torch.stack([logits_of(t[:i + 1]) for i in range(len(t))]) for t in tokens.tolist()])
+
+        def accept(self, accepted):
+            pass
+
+    b = scheduler.SpeculativeBatcher(Long(max_rows=4000), make_state(), chunk=3000)
+    b.submit([Counted(i) for i in range(3000)], 12)
+    b.step()
+    Counted.count = 0
+    for _ in range(5):
+        b.step()
+    assert Counted.count < 1000

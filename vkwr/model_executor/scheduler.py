@@ -219,6 +219,24 @@ def prompt_lookup(tokens, n, match=2):
     return []
 
 
+class _Lookup:
+    """prompt_lookup of one growing sequence by an index of its pairs of tokens: the steps of a call are the
+    tokens that came since the last, not the sequence's (a list scanned anew took 0.66 ms of 8192 tokens, once a
+    sequence and step)."""
+
+    def __init__(self, prompt):
+        self.tokens, self.places, self.seen = list(prompt), {}, 0
+
+    def __call__(self, request, n):
+        t = self.tokens
+        t += request.output[len(t) - len(request.prompt):]
+        for i in range(self.seen, len(t) - 2):  # all pairs but the last
+            self.places[t[i], t[i + 1]] = i
+        self.seen = max(len(t) - 2, 0)
+        at = self.places.get(tuple(t[-2:]))
+        return [] if at is None else t[at + 2:at + 2 + n]
+
+
 class SpeculativeBatcher(ContinuousBatcher):
     """Continuous batching with drafted tokens on a DraftEngine.  `draft(tokens, n)` proposes up to n
     tokens behind a sequence's tokens (default: looked up in them); top_k = 1 generates greedily, the lowest
@@ -244,6 +262,14 @@ class SpeculativeBatcher(ContinuousBatcher):
         self.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self.zeros = torch.zeros(max(B * T, P), 1, device=self.device)
         self.drafted = self.accepted = 0
+        self.lookups = {}  # request id -> _Lookup
+
+    def _draft(self, r, n):
+        if self.draft is prompt_lookup:
+            if r.rid not in self.lookups:
+                self.lookups[r.rid] = _Lookup(r.prompt)
+            return self.lookups[r.rid](r, n)
+        return list(self.draft(r.prompt + r.output, n))[:self.engine.max_draft]
 
     def _verify(self, logits, drafts, n_draft):
         """logits [B, T, V], n_draft: the drafts' lengths (host); (tokens, accepted) on the device."""
@@ -277,6 +303,7 @@ class SpeculativeBatcher(ContinuousBatcher):
         finished = [r for r in self.running if r.done]
         for r in finished:
             self.engine.drop([r.slot], self.state)
+            self.lookups.pop(r.rid, None)
             self.slots.free(r.slot)
         self.running = [r for r in self.running if not r.done]
         return finished
@@ -308,7 +335,7 @@ class SpeculativeBatcher(ContinuousBatcher):
         if dec:
             self._check_slots(dec)
             K = self.engine.max_draft
-            drafts = [list(self.draft(r.prompt + r.output, min(K, r.max_new_tokens - len(r.output) - 1)))[:K] for r in dec]
+            drafts = [self._draft(r, min(K, r.max_new_tokens - len(r.output) - 1)) for r in dec]
             T = 1 + max(len(d) for d in drafts)
             rows = self._i32([[r.output[-1]] + d + [-1] * (T - 1 - len(d)) for r, d in zip(dec, drafts)])
             logits = self.engine.draft_step(self.state, rows, [r.slot for r in dec], **self._adapter_ids(dec))
