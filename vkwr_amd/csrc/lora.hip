@@ -626,10 +626,19 @@ extern "C" int64_t vkwr_lora_workspace_bytes(int64_t m, int n_adapters, int rank
   clear_error();
   if (check_lora("vkwr_lora_workspace_bytes", m, n_adapters, rank, n_targets, targets)) return -1;
   const int64_t k = least_k(n_targets, targets), n = most_n(n_targets, targets);
-  int64_t most = lora_split(m, n_adapters, rank, n_targets, k, n).bytes;
-  // fewer rows can be cut into more parts; from 512 row tiles on there is one part
-  for (int64_t r = 1; r < m && r < 512 * kTileM; ++r)
-    most = std::max(most, lora_split(r, n_adapters, rank, n_targets, k, n).bytes);
+  // Fewer rows can be cut into more parts (a power of two up to 16, which never grows with the rows), so for each
+  // number of parts the most rows that have it.
+  int64_t most = 0;
+  for (int64_t rows = m; rows > 0;) {
+    const LoraPlan s = lora_split(rows, n_adapters, rank, n_targets, k, n);
+    most = std::max(most, s.bytes);
+    int64_t lo = 0, hi = rows;  // the most rows with more parts: [lo, hi)
+    while (hi - lo > 1) {
+      const int64_t mid = lo + (hi - lo) / 2;
+      (lora_split(mid, n_adapters, rank, n_targets, k, n).parts > s.parts ? lo : hi) = mid;
+    }
+    rows = lo;
+  }
   return most;
 }
 
