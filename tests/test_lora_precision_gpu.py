@@ -50,3 +50,24 @@ def test_an_infinite_rank_leaves_the_others_finite(gpu):
          "t": [{"x": x, "a": a, "b": b, "base": torch.zeros(m, N).half()}]}
     y = run_lora(gpu, d)[0].float().cpu()
     assert (y[:, ::2] == float("inf")).all() and (y[:, 1::2] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("K", [200, 2048, 8192])
+def test_a_row_in_different_company(gpu, K):
+    """A row alone, among other adapters' rows, and among 20, 40 and 200 of its own adapter's: operands straight
+    into registers or through LDS, K in few and many parts.  Each is within the sums' bound of the exact value and
+    rounded once, so any two are within twice the bound and a whole step of fp16 of each other."""
+    N, R, G = 264, 24, 4
+    d = make(240, G, R, [(N, K)], seed=K, none=0.0)
+    t = d["t"][0]
+    d["ids"][:] = 1
+    want, err = ref.lora(t["x"][:1], t["a"], t["b"], t["base"][:1], d["ids"][:1], d["scale"])
+    got = []
+    for own, others in ((1, 0), (1, 39), (20, 0), (40, 0), (40, 200), (200, 0), (200, 40)):
+        ids = torch.ones(own + others, dtype=torch.int32)
+        ids[own:] = torch.tensor([-1, 0, 2, 3], dtype=torch.int32).repeat(others // 4 + 1)[:others]
+        e = {"ids": ids, "scale": d["scale"], "t": [{**t, "x": t["x"][:own + others], "base": t["base"][:own + others]}]}
+        got.append(run_lora(gpu, e)[0][:1].cpu().double())
+        assert ((got[-1] - want).abs() <= err + HALF16 * (want.abs() + err) + 2.0 ** -25).all()
+    for y in got[1:]:
+        assert ((y - got[0]).abs() <= 2 * err + 2 * HALF16 * (want.abs() + err) + 2.0 ** -24).all()
