@@ -511,8 +511,11 @@ VKWR_EXPORT int vkwr_tmix_groupnorm_bonus_gate_frag_f16(int B, int T, int C, int
  *
  * y[i] = epilogue(base[i] + scale[g] * (x[i] A_g^T) B_g^T), g = adapters[i], for the rows i of a step
  * whose requests use different low-rank adapters beside one shared projection (base = its output).
- * g < 0: no adapter, y[i] = epilogue(base[i]); g >= n_adapters: y[i] = NaN.  fp32 sums; x A^T enters
- * the second product with 22 bits; one rounding to fp16.  No counterpart in the reference. */
+ * g < 0: no adapter, y[i] = epilogue(base[i]); g >= n_adapters: y[i] = NaN.  fp32 sums; each value of
+ * x A^T enters the second product with 22 bits (or within 2^-39 of its row's largest); one rounding to fp16.
+ * The order of the sums over k, and with it a row's last bits, depends on m and on how many rows share the
+ * adapter, not on the order of the rows.  a and b finite: an infinity or NaN in them makes the results it
+ * goes into infinities or NaN.  No counterpart in the reference. */
 
 /* The plan of a step: its rows ordered by adapter, made on the device from adapters [m] int32 (device)
  * once for all projections of the step.  plan: device memory of vkwr_lora_plan_bytes(m, n_adapters)
@@ -686,7 +689,9 @@ VKWR_EXPORT int vkwr_sampling_repetition_topk_topp(int B, int T, int V, const fl
 /* Verification of drafted tokens.  Sequence b has K + 1 rows of logits [B, K+1, V] (fp16 where
  * logits_f16, else fp32; row i: after i drafts) and n_draft[b] <= K (NULL: K) drafts [B, K] int32.
  * Per row p is the distribution that the ops above draw from (same filter; probabilities, masses and
- * sums in 64 bits, ties by logit).  Draft i, in order, is accepted while
+ * sums in 64 bits, ties by logit: top_k = 1 keeps every entry that is tied at the largest, of which
+ * uniforms[b, K] = 0 draws the lowest index; weights below 2^-1022 of the row's largest are 0).  Draft i, in
+ * order, is accepted while
  *   uniforms[b, i] * q(d_i) < p_i(d_i),
  * q = draft_probs [B, K, V] fp32 (finite, >= 0), or 1 where draft_probs is NULL (a drafter that
  * proposes single tokens).  At the first rejected draft the new token is drawn from max(p_i - q_i, 0)

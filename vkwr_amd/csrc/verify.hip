@@ -324,8 +324,9 @@ __device__ __forceinline__ double kept_of(const VerifyArgs& p, const RowStat& st
 }
 
 // One wave per group of kGroupSegs segments, four groups per workgroup.  fp32: bound by memory (566 rows of
-// 65536: 32 us, 4.7 TB/s, or 38 where it looks for nuclei's lists); fp16: by its 20 instructions an entry for
-// the mass (144 rows with lists: 15 us).
+// 65536: 32 us, 4.7 TB/s), or where it looks for nuclei's lists by its vector instructions (38 us, 88 % of the
+// SIMDs' cycles).  fp16, 144 rows with lists: 15 us, of which the CUs have waves for 11, their SIMDs busy for 73 %
+// of that: 1080 vector instructions a wave, 640 of them the mass's 20 an entry.
 template <bool kHalf>
 __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs p) {
   const int T = p.K + 1, wgs = (p.groups + 3) / 4;

@@ -52,9 +52,10 @@ __device__ __forceinline__ float row_sum8(float x) {
 
 // kRPL state rows per lane: 8 / kRPL waves per (sequence, head).  Few chains (up to two per CU) are bound by
 // the latency of one and take kRPL = 1 (one sequence of 32 heads, 5 + 5 tokens: 5.3 us against 6.7 with 2),
-// the others 2, bound by the states' traffic (128 sequences of 64 heads: 69 us, 4.65 TB/s; 83 with 1, 82 with
-// 4, 120 with 8, whose single wave has nothing beside it to cover its loads).  116 VGPRs leave four waves per
-// SIMD; held to 96 for a fifth, the spills cost more (90 us).
+// the others 2, bound by the states' traffic (128 sequences of 64 heads, 5 + 5 tokens, in a replayed graph:
+// 76 us, 4.2 TB/s; in the run that compared them 69 with 2, 83 with 1, 82 with 4, 120 with 8, whose single wave
+// has nothing beside it to cover its loads).  116 VGPRs leave four waves per SIMD; held to 96 for a fifth, the
+// spills cost more (90 us in that run).
 template <int kRPL>
 __global__ __launch_bounds__(64 * (8 / kRPL)) void wkv7_fp32_drafts_kernel(DraftArgs p) {
   constexpr int kThreads = 64 * (8 / kRPL);
