@@ -207,3 +207,22 @@ def test_looking_up_drafts_does_not_walk_the_sequence(oracle):
     for _ in range(5):
         b.step()
     assert Counted.count < 1000
+
+
+@pytest.mark.parametrize("filt", [{}, {"top_k": 5}])
+def test_the_default_type_does_not_matter(monkeypatch, filt):
+    """The uniforms are fp32, as the verification takes them, whatever torch makes by default."""
+    seen = []
+
+    def verify_drafts(logits, drafts, uniforms, tokens, accepted, **kw):
+        seen.append(uniforms.dtype)
+        tokens.fill_(3)
+        accepted.zero_()
+
+    monkeypatch.setattr(capi, "verify_drafts", verify_drafts)
+    torch.set_default_dtype(torch.float64)
+    try:
+        run(SpeculativeBatcher(Engine(), make_state(), chunk=8, **filt), PROMPTS[:2])
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert set(seen) == {torch.float32}

@@ -260,7 +260,7 @@ class SpeculativeBatcher(ContinuousBatcher):
         sizes = ((B * T, 0), (P, 0)) if self.greedy else ((B, T - 1), (P, 0))
         need = max(capi.verify_workspace_bytes(b, k, V) for b, k in sizes)
         self.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        self.zeros = torch.zeros(max(B * T, P), 1, device=self.device)
+        self.zeros = torch.zeros(max(B * T, P), 1, dtype=torch.float32, device=self.device)
         self.drafted = self.accepted = 0
         self.lookups = {}  # request id -> _Lookup
 
@@ -278,7 +278,7 @@ class SpeculativeBatcher(ContinuousBatcher):
             return self._verify_greedy(logits, drafts, n_draft)
         tokens = torch.empty(B, T, dtype=torch.int32, device=self.device)
         accepted = torch.empty(B, dtype=torch.int32, device=self.device)
-        u = torch.rand(B, T, generator=self.gen, device=self.device)
+        u = torch.rand(B, T, generator=self.gen, dtype=torch.float32, device=self.device)
         capi.verify_drafts(logits, drafts, u, tokens, accepted, n_draft=self._i32(n_draft), workspace=self.ws,
                            **self.filter)
         return tokens, accepted
