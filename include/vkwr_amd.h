@@ -641,6 +641,52 @@ VKWR_EXPORT int vkwr_frag_gemm_splitk_f16(const vkwr_frag_gemm_problem* problem,
 VKWR_EXPORT int vkwr_frag_gemm_splitk_parts_f16(const vkwr_frag_gemm_problem* problem, int splits,
                                                 void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- linear layers with 8-bit weights ----
+ *
+ * Packed 8-bit matrices [rows, k]: rows padded to a multiple of 32, k to one of 128 (the k pad is
+ * zero, pad rows are never used), in the operand order of v_mfma_i32_32x32x32_i8:
+ *   element (r, c) at byte ((r / 32) * (k_pad / 32) + c / 32) * 1024 + (((c / 16) % 2) * 32 + r % 32) * 16 + c % 16.
+ * vkwr_i8_packed_bytes: their size, or -1 for sizes that are refused (k up to 131072, so that sums of
+ * 127 * 127 stay in int32; rows up to 2^24). */
+VKWR_EXPORT int64_t vkwr_i8_packed_bytes(int64_t rows, int64_t k);
+
+/* Row-major 8-bit values src [rows, k] into a packed matrix (16-byte aligned).  Values are to be
+ * -127..127.  No counterpart in the reference. */
+VKWR_EXPORT int vkwr_i8_pack(int64_t rows, int64_t k, const int8_t* src, int8_t* dst, void* stream);
+
+/* Rounds fp16 rows x [rows, k] to 8 bits with a scale each: scale[r] = max|x_r| / 127,
+ * q = round(127 x / max|x_r|), halves to even, packed.  A row of zeros has the scale 0; a row with an
+ * infinity or a NaN has the scale NaN and zeros.  For weights (a row is an output channel); activations
+ * are rounded inside vkwr_linear_i8_f16.  No counterpart in the reference. */
+VKWR_EXPORT int vkwr_i8_quantize_rows_f16(int64_t rows, int64_t k, const uint16_t* x, int8_t* q, float* scale,
+                                          void* stream);
+
+/* One layer of a batch: y[i, j] = epilogue(s_i w_scale[j] sum_k q_ik w_jk), x [m, k] fp16 rounded to
+ * q and s row by row as vkwr_i8_quantize_rows_f16 does, w a packed matrix [n, k], y [m, n] fp16.  Sums are
+ * exact (int32), scaled in fp32 and rounded to fp16 once.  Epilogues: VKWR_GEMM_EPI_NONE, _RELU_SQUARE,
+ * _BIAS (+ bias[j] fp16), _TANH, _SIGMOID.  A row of x with an infinity or a NaN gives a row of NaN.  Any
+ * n and k, m up to 2^22; x, y contiguous, of any alignment (multiples of 8 and 16 bytes run faster). */
+typedef struct vkwr_i8_problem {
+  const uint16_t* x;
+  const int8_t* w;
+  const float* w_scale;
+  const uint16_t* bias;
+  uint16_t* y;
+  int64_t m, n, k;
+  int epilogue;
+} vkwr_i8_problem;
+
+/* Workspace of a batch (rounded activations): it grows with every problem's m, so that of the most rows
+ * serves every step; -1 on invalid arguments. */
+VKWR_EXPORT int64_t vkwr_linear_i8_workspace_bytes(int n_problems, const vkwr_i8_problem* problems);
+
+/* Runs 1..8 independent layers.  Problems that read the same x round it once.  y must not overlap what
+ * any problem reads.  workspace: 16-byte aligned, one for each of the calls that may run at the same
+ * time.  A row's bits depend on that row and the weights only, not on the batch.  No counterpart in the
+ * reference (its linear ops are fp16, csrc/v1/linear/linear_ops.cu:46-1833). */
+VKWR_EXPORT int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problems, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
 /* ---- token sampling (reference csrc/sampling/, ops vkwr_sampling::*) ----
  *
  * Per batch row b, on the logits of its last token (logits [B,T,V] fp32, row
@@ -710,6 +756,46 @@ VKWR_EXPORT int vkwr_sampling_verify_drafts(int B, int K, int V, const void* log
                                             const float* draft_probs, const float* uniforms, int32_t* tokens,
                                             int32_t* accepted, double temperature, int top_k, double top_p,
                                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- beam search ----
+ *
+ * One step over B requests of W beams (1..32): logits [B, W, V] (fp16 where logits_f16, else fp32),
+ * scores [B, W] fp32 (sums of log-probabilities), lengths [B, W] int32 (tokens generated), ended [B, W]
+ * int32 (non-zero: the beam is finished).
+ *   A live beam b offers every token v with raw = scores[b] + l_v - log sum_u exp(l_u) and the length
+ *   lengths[b] + 1; a finished one only `end`, with raw = scores[b] and its length.
+ *   The W best by raw * max(length, 1)^-length_penalty, ties to the lowest b V + v, in that order:
+ *   tokens, parents (b), scores_out (raw), lengths_out, ended_out (finished before, or token == end).
+ * A logit of -inf or NaN is never chosen, and a beam of score -inf or NaN offers nothing (all but the first
+ * of a request behind its prompt).  Logits of +inf share the whole probability.  Where fewer than W
+ * candidates are left the remaining rows are token -1, parent -1, score -inf, length 0, ended 1.
+ * end: -1 for none.  length_penalty 0..16; V up to 2^20; B W up to 65535.  Sums over the vocabulary, scores
+ * and comparisons are in 64 bits (terms and sums of 32 terms fp32).  Deterministic, and independent of the
+ * other requests.  Outputs must not overlap the inputs.  workspace: vkwr_beam_workspace_bytes(B, W, V) bytes
+ * (-1 for sizes that are refused), 16-byte aligned, one for each of the calls that may run at the same time.
+ * No counterpart in the reference. */
+VKWR_EXPORT int64_t vkwr_beam_workspace_bytes(int B, int W, int V);
+VKWR_EXPORT int vkwr_beam_select(int B, int W, int V, const void* logits, int logits_f16, const float* scores,
+                                 const int32_t* lengths, const int32_t* ended, int32_t* tokens, int32_t* parents,
+                                 float* scores_out, int32_t* lengths_out, int32_t* ended_out, int end,
+                                 float length_penalty, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A slot pool whose entries follow the beams: [layers, n_slots, slot_bytes], slot_bytes a multiple of 16. */
+typedef struct vkwr_beam_pool {
+  void* base;
+  int64_t layers, slot_bytes;
+} vkwr_beam_pool;
+
+/* Gives every new beam the state of its parent.  slots, parents, skip [B, W] int32: the slots of the old
+ * beams (distinct), each new beam's parent (0..W-1; anything else: none), and where skip is not NULL
+ * the new beams that need no state (non-zero).  slots_out [B, W]: a parent's slot goes to the first child
+ * that carries its state on; the other children take, in order, the slots that are left, and those that
+ * carry a state get a copy of it there, in all of 0..8 pools.  Nothing else in the pools changes.  A copy from or to
+ * a slot outside [0, n_slots) is left out.  slots_out must not overlap the inputs; B W up to 4096.
+ * No counterpart in the reference. */
+VKWR_EXPORT int vkwr_beam_reorder(int B, int W, int n_slots, const int32_t* slots, const int32_t* parents,
+                                  const int32_t* skip, int32_t* slots_out, int n_pools,
+                                  const vkwr_beam_pool* pools, void* stream);
 
 /* Host-side Philox4x32-10 block (the generator the sampling kernels run), for
  * checking it against published known-answer vectors.  No counterpart in the

@@ -71,6 +71,15 @@ class LoraTarget(ctypes.Structure):
     _fields_ = [("x", _p), ("a", _p), ("b", _p), ("base", _p), ("y", _p), ("n", _i64), ("k", _i64), ("epilogue", _i)]
 
 
+class I8Problem(ctypes.Structure):
+    _fields_ = [("x", _p), ("w", _p), ("w_scale", _p), ("bias", _p), ("y", _p), ("m", _i64), ("n", _i64), ("k", _i64),
+                ("epilogue", _i)]
+
+
+class BeamPool(ctypes.Structure):
+    _fields_ = [("base", _p), ("layers", _i64), ("slot_bytes", _i64)]
+
+
 def _sig(name, args, res=_i):
     fn = getattr(_LIB, name)
     fn.argtypes = args
@@ -136,6 +145,14 @@ _lora_plan_bytes = _sig("vkwr_lora_plan_bytes", [_i64, _i], _i64)
 _lora_plan = _sig("vkwr_lora_plan", [_i64, _i, _p, _p, _i64, _p])
 _lora_ws = _sig("vkwr_lora_workspace_bytes", [_i64, _i, _i, _i, ctypes.POINTER(LoraTarget)], _i64)
 _lora = _sig("vkwr_lora_f16", [_i64, _i, _i, _p, _p, _i, ctypes.POINTER(LoraTarget), _p, _i64, _p])
+_i8_packed = _sig("vkwr_i8_packed_bytes", [_i64, _i64], _i64)
+_i8_pack = _sig("vkwr_i8_pack", [_i64, _i64, _p, _p, _p])
+_i8_rows = _sig("vkwr_i8_quantize_rows_f16", [_i64, _i64, _p, _p, _p, _p])
+_linear_i8_ws = _sig("vkwr_linear_i8_workspace_bytes", [_i, ctypes.POINTER(I8Problem)], _i64)
+_linear_i8 = _sig("vkwr_linear_i8_f16", [_i, ctypes.POINTER(I8Problem), _p, _i64, _p])
+_beam_ws = _sig("vkwr_beam_workspace_bytes", [_i, _i, _i], _i64)
+_beam_select = _sig("vkwr_beam_select", [_i, _i, _i, _p, _i] + [_p] * 8 + [_i, _f, _p, _i64, _p])
+_beam_reorder = _sig("vkwr_beam_reorder", [_i, _i, _i, _p, _p, _p, _p, _i, ctypes.POINTER(BeamPool), _p])
 SAMPLING_STATE_BYTES = 32
 SAMPLING_REGISTER_VOCAB = 65536  # larger vocabularies need a B*V fp32 scratch buffer
 
@@ -633,3 +650,141 @@ def lora(plan, targets, scale=None, workspace=None):
     _check(_lora(m, G, rank, at.optional(scale, torch.float32, G, "scale"),
                  plan.on(at.dev), len(targets), arr,
                  at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()), "vkwr_lora_f16")
+
+
+I8_MAX_PROBLEMS = 8
+_I8_ARRAYS = [I8Problem * n for n in range(I8_MAX_PROBLEMS + 1)]
+_I8_EPILOGUES = (EPI_NONE, EPI_RELU_SQUARE, EPI_BIAS, EPI_TANH, EPI_SIGMOID)
+
+
+class I8Weight:
+    """8-bit weights [n, k] laid out for linear_i8, with a scale per output channel."""
+
+    def __init__(self, n, k, packed, scale):
+        self.n, self.k, self.packed, self.scale = n, k, packed, scale
+
+    @property
+    def nbytes(self):
+        return self.packed.numel() + 4 * self.n
+
+
+def _i8_empty(n, k, device):
+    nbytes = _i8_packed(n, k)
+    if nbytes <= 0:
+        raise ValueError(f"8-bit weights: bad size [{n}, {k}]")
+    return torch.empty(nbytes, dtype=torch.int8, device=device)
+
+
+def i8_weight(q, scale):
+    """Lays out weights that are 8 bits already: q [n, k] int8 of -127..127, scale [n] fp32."""
+    n, k = q.shape
+    at = _Tensors()
+    packed = _i8_empty(n, k, q.device)
+    at(scale, torch.float32, n, "scale")
+    _check(_i8_pack(n, k, at(q, torch.int8, n * k, "q"), packed.data_ptr(), at.stream()), "vkwr_i8_pack")
+    return I8Weight(n, k, packed, scale)
+
+
+def i8_quantize(w):
+    """Rounds fp16 weights w [n, k] to 8 bits with a scale per output channel (vkwr_i8_quantize_rows_f16)."""
+    n, k = w.shape
+    at = _Tensors()
+    packed, scale = _i8_empty(n, k, w.device), torch.empty(n, dtype=torch.float32, device=w.device)
+    _check(_i8_rows(n, k, at(w, torch.float16, n * k, "w"), packed.data_ptr(), scale.data_ptr(), at.stream()),
+           "vkwr_i8_quantize_rows_f16")
+    return I8Weight(n, k, packed, scale)
+
+
+def linear_i8_problem(x, w, y, epilogue=EPI_NONE, bias=None):
+    """One layer: y [m, n] = epilogue(x [m, k] w^T) with x rounded to 8 bits row by row; w an I8Weight,
+    bias [n] fp16 for EPI_BIAS."""
+    n, k = w.n, w.k
+    m = x.numel() // k
+    if x.shape[-1] != k or epilogue not in _I8_EPILOGUES or (bias is None) != (epilogue != EPI_BIAS):
+        raise ValueError(f"linear_i8_problem: x {tuple(x.shape)}, w [{n}, {k}], epilogue {epilogue}")
+    at, h = _Tensors(), torch.float16
+    p = I8Problem(at(x, h, m * k, "x"), at(w.packed, torch.int8, w.packed.numel(), "w"),
+                  at(w.scale, torch.float32, n, "w.scale"), at.optional(bias, h, n, "bias"), at(y, h, m * n, "y"), m, n, k,
+                  epilogue)
+    p.dev = at.dev
+    p.tensors = (x, w, bias, y)  # what the pointers point to
+    return p
+
+
+def _i8_problems(problems):
+    n = len(problems)
+    if not 1 <= n <= I8_MAX_PROBLEMS:
+        raise ValueError(f"linear_i8: 1 to 8 problems, got {n}")
+    return n, _I8_ARRAYS[n](*problems)
+
+
+def linear_i8_workspace_bytes(problems):
+    """Workspace of `linear_i8` for these problems at their row counts or fewer."""
+    n = _linear_i8_ws(*_i8_problems(problems))
+    if n < 0:
+        raise RuntimeError(f"vkwr_linear_i8_workspace_bytes: {_LIB.vkwr_last_error().decode()}")
+    return n
+
+
+def linear_i8(problems, workspace=None):
+    """1..8 linear layers with 8-bit weights (vkwr_linear_i8_f16).  workspace: uint8,
+    linear_i8_workspace_bytes (None: allocated)."""
+    n, arr = _i8_problems(problems)
+    at = _Tensors()
+    for p in problems:
+        if p.dev != at.dev:
+            raise ValueError(f"linear_i8: problem on cuda:{p.dev}, but the current device is cuda:{at.dev}")
+    if workspace is None:
+        workspace = torch.empty(linear_i8_workspace_bytes(problems), dtype=torch.uint8, device=problems[0].tensors[0].device)
+    nbytes = workspace.numel()
+    _check(_linear_i8(n, arr, at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()),
+           "vkwr_linear_i8_f16")
+
+
+MAX_BEAMS = 32
+
+
+def beam_workspace_bytes(B, W, V):
+    """Workspace of beam_select for up to B requests (V is the vocabulary)."""
+    n = _beam_ws(B, W, V)
+    if n < 0:
+        raise ValueError(f"beam_select: bad size B={B} W={W} V={V}")
+    return n
+
+
+def beam_select(logits, scores, lengths, ended, tokens, parents, scores_out, lengths_out, ended_out, end=-1,
+                length_penalty=0.0, workspace=None):
+    """One step of beam search (vkwr_beam_select): logits [B, W, V] fp16 or fp32; scores fp32, lengths and
+    ended int32, all [B, W]; writes tokens, parents, lengths_out and ended_out int32 and scores_out
+    fp32 [B, W], the best first.  workspace: uint8, beam_workspace_bytes (None: allocated)."""
+    B, W, V = logits.shape
+    if logits.dtype not in (torch.float16, torch.float32):
+        raise TypeError(f"logits: fp16 or fp32, got {logits.dtype}")
+    at, i32, f32, n = _Tensors(), torch.int32, torch.float32, B * W
+    if workspace is None:
+        workspace = torch.empty(beam_workspace_bytes(B, W, V), dtype=torch.uint8, device=logits.device)
+    nbytes = workspace.numel()
+    _check(_beam_select(B, W, V, at(logits, logits.dtype, n * V, "logits"), int(logits.dtype == torch.float16),
+                        at(scores, f32, n, "scores"), at(lengths, i32, n, "lengths"), at(ended, i32, n, "ended"),
+                        at(tokens, i32, n, "tokens"), at(parents, i32, n, "parents"), at(scores_out, f32, n, "scores_out"),
+                        at(lengths_out, i32, n, "lengths_out"), at(ended_out, i32, n, "ended_out"), end, length_penalty,
+                        at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()), "vkwr_beam_select")
+
+
+def beam_reorder(slots, parents, slots_out, pools, skip=None):
+    """States follow their beams (vkwr_beam_reorder): slots, parents, skip and slots_out [B, W] int32; pools:
+    up to 8 tensors [layers, n_slots, ...], whose entries for the beams' slots are copied where a beam has
+    more than one child."""
+    B, W = slots.shape
+    at, i32, n = _Tensors(), torch.int32, B * W
+    n_slots = pools[0].shape[1] if pools else 0
+    for i, t in enumerate(pools):
+        if t.dim() < 2 or t.shape[1] != n_slots:
+            raise ValueError(f"beam_reorder: pool {i} {tuple(t.shape)} is not [layers, {n_slots}, ...]")
+    arr = (BeamPool * max(len(pools), 1))()
+    for i, t in enumerate(pools):
+        size = t.numel() * t.element_size()
+        arr[i] = BeamPool(at(t, t.dtype, t.numel(), f"pool {i}"), t.shape[0], size // max(t.shape[0] * n_slots, 1))
+    _check(_beam_reorder(B, W, n_slots, at(slots, i32, n, "slots"), at(parents, i32, n, "parents"),
+                         at.optional(skip, i32, n, "skip"), at(slots_out, i32, n, "slots_out"), len(pools), arr,
+                         at.stream()), "vkwr_beam_reorder")
