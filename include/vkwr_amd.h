@@ -647,7 +647,7 @@ VKWR_EXPORT int vkwr_frag_gemm_splitk_parts_f16(const vkwr_frag_gemm_problem* pr
  * zero, pad rows are never used), in the operand order of v_mfma_i32_32x32x32_i8:
  *   element (r, c) at byte ((r / 32) * (k_pad / 32) + c / 32) * 1024 + (((c / 16) % 2) * 32 + r % 32) * 16 + c % 16.
  * vkwr_i8_packed_bytes: their size, or -1 for sizes that are refused (k up to 131072, so that sums of
- * 127 * 127 stay in int32; rows up to 2^24). */
+ * 127 * 127 stay in int32; rows up to 2^22). */
 VKWR_EXPORT int64_t vkwr_i8_packed_bytes(int64_t rows, int64_t k);
 
 /* Row-major 8-bit values src [rows, k] into a packed matrix (16-byte aligned).  Values are to be
@@ -665,7 +665,8 @@ VKWR_EXPORT int vkwr_i8_quantize_rows_f16(int64_t rows, int64_t k, const uint16_
  * q and s row by row as vkwr_i8_quantize_rows_f16 does, w a packed matrix [n, k], y [m, n] fp16.  Sums are
  * exact (int32), scaled in fp32 and rounded to fp16 once.  Epilogues: VKWR_GEMM_EPI_NONE, _RELU_SQUARE,
  * _BIAS (+ bias[j] fp16), _TANH, _SIGMOID.  A row of x with an infinity or a NaN gives a row of NaN.  Any
- * n and k, m up to 2^22; x, y contiguous, of any alignment (multiples of 8 and 16 bytes run faster). */
+ * n and k, up to 2^22 rows in a call; x, y contiguous, of any alignment (n a multiple of 8 and y on 16 bytes
+ * run faster). */
 typedef struct vkwr_i8_problem {
   const uint16_t* x;
   const int8_t* w;

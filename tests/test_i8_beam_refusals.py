@@ -29,7 +29,7 @@ def linear(*problems, workspace=at(9), nbytes=1 << 30, n=None):
 
 @pytest.mark.parametrize("change,text", [
     ({"m": -1}, "sizes"), ({"n": 0}, "sizes"), ({"k": 0}, "sizes"), ({"k": 131073}, "sizes"), ({"m": 2 ** 22 + 1}, "sizes"),
-    ({"n": 2 ** 24 + 1}, "sizes"), ({"epilogue": 2}, "epilogue"), ({"epilogue": 9}, "epilogue"), ({"x": None}, "null"),
+    ({"n": 2 ** 22 + 1}, "sizes"), ({"epilogue": 2}, "epilogue"), ({"epilogue": 9}, "epilogue"), ({"x": None}, "null"),
     ({"w": None}, "null"), ({"ws": None}, "null"), ({"y": None}, "null"), ({"epilogue": 3}, "null"),
     ({"w": at(1) + 8}, "aligned"), ({"y": at(0) + 16}, "overlaps"), ({"y": at(1)}, "overlaps"), ({"y": at(2) + 4}, "overlaps"),
     ({"y": at(9)}, "workspace"), ({"x": at(9) + 16}, "workspace"), ({"epilogue": 3, "bias": at(3) + 2}, "overlaps")])
@@ -40,6 +40,7 @@ def test_linear_refuses(change, text):
 def test_linear_refuses_batches():
     assert linear() == 1 and "1 to 8" in err()
     assert linear(*[problem()] * 9) == 1 and "1 to 8" in err()
+    assert linear(*[problem(m=2 ** 21)] * 3) == 1 and "rows together" in err()
     assert linear(problem(), workspace=None) == 1 and "workspace" in err()
     assert linear(problem(), workspace=at(9) + 4) == 1 and "workspace" in err()
     need = capi.linear_i8_workspace_bytes([problem()])
@@ -59,7 +60,7 @@ def test_linear_workspace_grows_with_rows():
 
 def test_packed_sizes():
     assert capi._i8_packed(1, 1) == 32 * 128 and capi._i8_packed(33, 129) == 64 * 256 and capi._i8_packed(0, 5) == 0
-    for bad in ((-1, 8), (8, 0), (8, 131073), (2 ** 24 + 1, 8)):
+    for bad in ((-1, 8), (8, 0), (8, 131073), (2 ** 22 + 1, 8)):
         assert capi._i8_packed(*bad) == -1
     assert capi._i8_pack(4, 4, None, at(1), None) == 1 and "null" in err()
     assert capi._i8_pack(4, 4, at(0), at(1) + 8, None) == 1 and "aligned" in err()

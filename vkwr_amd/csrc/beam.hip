@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vk_capi.h"
 #include "vk_common.cuh"
@@ -29,13 +30,15 @@ typedef uint32_t uv4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxBeams = 32;
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kRowThreads = 256, kPer = 32, kGroup = kRowThreads * kPer;  // entries of a group
-constexpr int kListCap = 512;    // entries above the bound that are ranked at once
-constexpr int kMergeKeys = 4096;  // keys that a merge pass holds: 32 beams x 128 groups
+constexpr int kRowThreads = 512, kPer = 16, kGroup = kRowThreads * kPer;  // entries of a group
+constexpr int kRowWaves = kRowThreads / 64;
+constexpr int kListCap = 512;     // entries above the bound that are ranked at once
+constexpr int kMergeKeys = 4096;  // keys that a merge pass holds (32 beams x 128 groups: one row)
+constexpr int kRankThreads = 512, kMergeThreads = kRankThreads + 64;
 
 // Entries in the order (value descending, index ascending); 0 is below every entry.
 __device__ __forceinline__ uint64_t entry_key(float v, uint32_t i) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // (-0 equals 0)
   const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
   return (uint64_t)o << 32 | (uint32_t)~i;
 }
@@ -67,14 +70,37 @@ struct BeamArgs {
   float alpha;
 };
 
+// max over the wave, in every lane: six steps from lane to lane and a broadcast
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-  return v;
+  auto step = [&](auto ctrl) __attribute__((always_inline)) {
+    const int o = __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), decltype(ctrl)::value,
+                                              0xf, 0xf, false);
+    v = fmaxf(v, __builtin_bit_cast(float, o));
+  };
+  step(std::integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2
+  step(std::integral_constant<int, 0x4E>{});   // quad_perm 2 3 0 1
+  step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  step(std::integral_constant<int, 0x140>{});  // row_mirror: every lane of a row of 16 has the row's
+  step(std::integral_constant<int, 0x142>{});  // row_bcast15
+  step(std::integral_constant<int, 0x143>{});  // row_bcast31: lane 63 has the wave's
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
+// sum over the wave, in lane 63, by the same steps
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    // lanes that the step does not reach add 0
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  using All = std::integral_constant<int, 0xf>;
+  step(std::integral_constant<int, 0xB1>{}, All{});
+  step(std::integral_constant<int, 0x4E>{}, All{});
+  step(std::integral_constant<int, 0x141>{}, All{});
+  step(std::integral_constant<int, 0x140>{}, All{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // rows 1 and 3
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // rows 2 and 3
   return v;
 }
 __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
@@ -86,54 +112,55 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
   return v;
 }
 
-// blockIdx.x: group of the row, blockIdx.y: row.  kVec: rows are 16-byte aligned; lane t then holds
-// the 16-byte pieces t, t + 256, ... of the group, else its entries t, t + 256, ...
-template <bool kHalf, bool kVec>
+// blockIdx.x: group of the row, blockIdx.y: row.  Lane t holds the pieces (8 fp16 or 4 fp32)
+// t, t + 512, ... of the group.
+template <bool kHalf>
 __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(BeamArgs a) {
-  __shared__ float wmax[4], wbound[4];
-  __shared__ double wsum[4];
-  __shared__ uint64_t list[kListCap], wkey[4];
+  constexpr int kPiece = kHalf ? 8 : 4;
+  __shared__ float wmax[kRowWaves], wbound[kRowWaves];
+  __shared__ double wsum[kRowWaves];
+  __shared__ uint64_t list[kListCap], wkey[kRowWaves];
   __shared__ int count;
   const int64_t row = blockIdx.y;
-  if (a.ended[row] || !(a.scores[row] > kNone)) return;  // (the merge leaves such rows out)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int i0 = blockIdx.x * kGroup, W = a.W;
-  constexpr int kPiece = kVec ? (kHalf ? 8 : 4) : 1;
+  const int i0 = blockIdx.x * kGroup, W = a.W, V = a.V;
+  const int over = a.ended[row];
+  const float score = a.scores[row];
   auto index_of = [&](int e) { return i0 + ((e / kPiece) * kRowThreads + tid) * kPiece + e % kPiece; };
 
-  float v[kPer];
+  typedef typename std::conditional<kHalf, hv8, fv4>::type Piece;
+  typedef typename std::conditional<kHalf, _Float16, float>::type Elem;
+  const Elem* const l = (const Elem*)a.logits + row * V;
+  constexpr Elem kLow = (Elem)kNone;
+  Piece p[kPer / kPiece];
 #pragma unroll
   for (int j = 0; j < kPer / kPiece; ++j) {
     const int i = index_of(j * kPiece);
-    if constexpr (kVec) {
-      if (i < a.V) {  // V is a multiple of a piece
-        if constexpr (kHalf) {
-          const hv8 h = *reinterpret_cast<const hv8*>((const _Float16*)a.logits + row * a.V + i);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[j * 8 + e] = (float)h[e];
-        } else {
-          const fv4 f = *reinterpret_cast<const fv4*>((const float*)a.logits + row * a.V + i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j * 4 + e] = f[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kPiece; ++e) v[j * kPiece + e] = kNone;
-      }
+    if (i + kPiece <= V) {
+      __builtin_memcpy(&p[j], l + i, 16);  // (a row need not start on 16 bytes)
     } else {
-      v[j] = kNone;
-      if (i < a.V) v[j] = kHalf ? (float)((const _Float16*)a.logits)[row * a.V + i] : ((const float*)a.logits)[row * a.V + i];
-    }
-  }
-  float top = kNone;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    v[e] = v[e] != v[e] ? kNone : v[e] + 0.0f;  // a NaN is never chosen; -0 equals 0
-    top = fmaxf(top, v[e]);
+      for (int e = 0; e < kPiece; ++e) {
+        p[j][e] = kLow;
+        if (i + e < V) p[j][e] = l[i + e];
+      }
+    }
+    if (j == 0 && (over || !(score > kNone))) return;  // (the merge leaves such rows out)
   }
-  // A bound that at least W entries reach: in each wave the q-th largest of the lanes' maxima,
-  // 4 q >= W, and the smallest of the four.
-  const int q = (W + 3) / 4;
+  Piece tops = kLow;
+#pragma unroll
+  for (int j = 0; j < kPer / kPiece; ++j) {
+    p[j] = __builtin_elementwise_max(p[j], (Piece)kLow);  // a NaN is never chosen
+    tops = __builtin_elementwise_max(tops, p[j]);
+  }
+  float top = (float)tops[0];
+#pragma unroll
+  for (int e = 1; e < kPiece; ++e) top = fmaxf(top, (float)tops[e]);
+  auto value = [&](int e) __attribute__((always_inline)) { return (float)p[e / kPiece][e % kPiece]; };
+  // A bound that at least W entries reach: in each of n waves whose lanes all hold entries (or the
+  // one there is) the q-th largest of the lanes' maxima, n q >= W, and the smallest of those.
+  const int whole = min(kRowWaves, max(1, (min(V - i0, kGroup) + kPiece - 1) / kPiece / 64));
+  const int q = (W + whole - 1) / whole;
   float left = top, bound = kNone, most = kNone;
   for (int s = 0; s < q; ++s) {
     bound = wave_max(left);
@@ -141,34 +168,44 @@ __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(BeamArgs a) {
     const uint64_t at = __ballot(left == bound);
     if (lane == __builtin_ctzll(at)) left = kNone;
   }
-  if (lane == 0) wmax[wave] = most, wbound[wave] = bound;
+  if (lane == 0) wmax[wave] = most, wbound[wave] = wave < whole ? bound : __builtin_huge_valf();
   if (tid == 0) count = 0;
   __syncthreads();
-  const float mx = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-  bound = fminf(fminf(wbound[0], wbound[1]), fminf(wbound[2], wbound[3]));
-  float sum = 0.0f;
+  float mx = wmax[0];
+  bound = wbound[0];
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    // (at an infinite maximum only the entries that are infinite themselves count)
-    const float d = v[e] - mx;
-    sum += v[e] == mx ? 1.0f : v[e] > kNone ? __expf(d) : 0.0f;
-    if (v[e] >= bound && v[e] > kNone) {
-      const int n = atomicAdd(&count, 1);
-      if (n < kListCap) list[n] = entry_key(v[e], (uint32_t)index_of(e));
+  for (int w = 1; w < kRowWaves; ++w) mx = fmaxf(mx, wmax[w]), bound = fminf(bound, wbound[w]);
+  if (top >= bound && top > kNone) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (value(e) >= bound && value(e) > kNone) {
+        const int n = atomicAdd(&count, 1);
+        if (n < kListCap) list[n] = entry_key(value(e), (uint32_t)index_of(e));
+      }
     }
   }
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e)  // (at an infinite maximum the entries that are infinite themselves count 1 each)
+    sum += __expf(fminf(value(e) - mx, 0.0f));
   if (!(mx > kNone)) sum = 0.0f;
   const double ws = wave_sum64((double)sum);
-  if (lane == 0) wsum[wave] = ws;
+  if (lane == 63) wsum[wave] = ws;
   __syncthreads();
   const int64_t g = row * a.groups + blockIdx.x;
-  if (tid == 0) a.stats[g] = RowStat{mx, 0.0f, (wsum[0] + wsum[1]) + (wsum[2] + wsum[3])};
+  if (tid == 0) {
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) all += wsum[w];
+    a.stats[g] = RowStat{mx, 0.0f, all};
+  }
   uint64_t* const out = a.keys + g * W;
   const int n = count;
   if (n <= kListCap) {
     for (int i = tid; i < n; i += kRowThreads) {
       const uint64_t k = list[i];
       int better = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) better += list[j] > k;
       if (better < W) out[better] = k;
     }
@@ -181,104 +218,188 @@ __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(BeamArgs a) {
     uint64_t best = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const uint64_t k = v[e] > kNone ? entry_key(v[e], (uint32_t)index_of(e)) : 0;
+      const uint64_t k = value(e) > kNone ? entry_key(value(e), (uint32_t)index_of(e)) : 0;
       if (k < last && k > best) best = k;
     }
     best = wave_max_key(best);
     if (lane == 0) wkey[wave] = best;
     __syncthreads();
-    const uint64_t b01 = wkey[0] > wkey[1] ? wkey[0] : wkey[1], b23 = wkey[2] > wkey[3] ? wkey[2] : wkey[3];
-    last = b01 > b23 ? b01 : b23;
+    last = wkey[0];
+#pragma unroll
+    for (int w = 1; w < kRowWaves; ++w) last = wkey[w] > last ? wkey[w] : last;
     if (tid == 0) out[s] = last;
     __syncthreads();
   }
 }
 
-// One workgroup per request.  Every list of keys is sorted, so an entry's rank among several lists is
-// its place in its own plus the heads of the others above it, counted until W are.
-__global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
+// e^x for x <= 0 in fp64: 2^n e^t with |t| <= ln(2) / 2, e^t by its series to t^11 / 11! (the rest is below
+// 7e-15).  Written out, as is the logarithm below: the merge runs once a step and waits for its own
+// instructions, of which the library's functions have three times as many.
+__device__ __forceinline__ double exp64(double x) {
+  x = x > -1100.0 ? x : -1100.0;
+  const double n = __builtin_rint(x * 1.4426950408889634);
+  const double t = __builtin_fma(n, -1.9082149292705877e-10, __builtin_fma(n, -0.693147180369123816490, x));
+  double p = 1.0;
+#pragma unroll
+  for (int k = 11; k >= 1; --k) p = __builtin_fma(t * (1.0 / k), p, 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+// log x for x >= 1: fp32's, and one step of Newton's with the next term
+__device__ __forceinline__ double log64(double x) {
+  const double y = (double)__logf((float)x);
+  const double r = __builtin_fma(x, exp64(-y), -1.0);
+  return y + (r - 0.5 * r * r);
+}
+
+// One workgroup per request.  All it reads is requested at once; then the last wave joins the groups'
+// sums while the others rank each row's keys (a key's place is the number of keys above it),
+// and all rank the W x W
+// scores.  Of a row's groups only the W with the largest first keys can hold
+// one of its W largest.
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
+  constexpr int kKeep = (kMergeKeys + kMergeThreads - 1) / kMergeThreads;  // keys per lane
   __shared__ uint64_t keys[kMergeKeys];
   __shared__ uint64_t cand[kMaxBeams * kMaxBeams];  // [beam][W], sorted
   __shared__ double rank[kMaxBeams * kMaxBeams], raw[kMaxBeams * kMaxBeams];
-  __shared__ double base[kMaxBeams], factor[kMaxBeams];
-  __shared__ float rmax[kMaxBeams];
-  __shared__ int live[kMaxBeams], valid;  // 0: offers nothing, 1: live, 2: finished
+  __shared__ double base[kMaxBeams], factor[kMaxBeams], gsum[kMergeKeys];
+  __shared__ float rmax[kMaxBeams], gmax[kMergeKeys];
+  __shared__ int before[kMaxBeams * kMaxBeams], live[kMaxBeams], len0[kMaxBeams], valid;  // live: 0 offers nothing, 1 live, 2 finished
   const int tid = threadIdx.x, W = a.W, G = a.groups;
   const int64_t r0 = (int64_t)blockIdx.x * W;
-  if (tid == 0) valid = 0;
-  if (tid < W) {
-    const float score = a.scores[r0 + tid];
-    const bool over = a.ended[r0 + tid] != 0;
-    int kind = score > kNone ? (over ? 2 : 1) : 0;
-    const int len = a.lengths[r0 + tid] + (over ? 0 : 1);
-    float mx = kNone;
-    double sum = 0.0;
-    if (kind == 1) {
-      const RowStat* const st = a.stats + (r0 + tid) * G;
-      for (int g = 0; g < G; ++g) mx = fmaxf(mx, st[g].max);
-      for (int g = 0; g < G; ++g)
-        if (st[g].max > kNone) sum += st[g].max == mx ? st[g].sum : st[g].sum * exp((double)st[g].max - (double)mx);
-      if (!(mx > kNone)) kind = 0;  // not one token is allowed
-    }
-    live[tid] = kind;
-    rmax[tid] = mx;
-    base[tid] = (double)score - (kind == 1 ? log(sum) : 0.0);
-    factor[tid] = a.alpha == 0.0f ? 1.0 : pow((double)(len > 1 ? len : 1), -(double)a.alpha);
-  }
-  for (int i = tid; i < W * W; i += 256) cand[i] = 0;
-  __syncthreads();
   const int per_row = G * W, rows = kMergeKeys / per_row > W ? W : kMergeKeys / per_row;  // rows of a pass (at least 1)
+  // all loads of the first pass before anything waits for one
+  uint64_t kr[kKeep];
+  RowStat sr{};
+  float score = kNone;
+  int over0 = 0, length = 0;
+  auto load_keys = [&](int w0, int n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u) {
+      const int i = u * kMergeThreads + tid;
+      if (i < n) kr[u] = a.keys[(r0 + w0) * per_row + i];
+    }
+  };
+  load_keys(0, rows * per_row);
+  if (tid < W * G) sr = a.stats[r0 * G + tid];
+  if (tid < W) {
+    score = a.scores[r0 + tid];
+    over0 = a.ended[r0 + tid];
+    length = a.lengths[r0 + tid];
+  }
+  for (int i = tid; i < W * W; i += kMergeThreads) cand[i] = 0;
+  for (int i = tid + kMergeThreads; i < W * G; i += kMergeThreads) {
+    const RowStat st = a.stats[r0 * G + i];
+    gmax[i] = st.max;
+    gsum[i] = st.sum;
+  }
+  if (tid < W * G) {
+    gmax[tid] = sr.max;
+    gsum[tid] = sr.sum;
+  }
+  if (tid < W) {
+    live[tid] = score > kNone ? (over0 ? 2 : 1) : 0;
+    len0[tid] = length;
+    base[tid] = (double)score;
+    if (tid == 0) valid = 0;
+  }
   for (int w0 = 0; w0 < W; w0 += rows) {
     const int n = (W - w0 < rows ? W - w0 : rows) * per_row;
-    for (int i = tid; i < n; i += 256) keys[i] = live[w0 + i / per_row] == 1 ? a.keys[(r0 + w0) * per_row + i] : 0;
+    if (w0 > 0) load_keys(w0, n);
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u)
+      if (u * kMergeThreads + tid < n) keys[u * kMergeThreads + tid] = kr[u];
     __syncthreads();
-    for (int i = tid; i < n; i += 256) {
-      const uint64_t k = keys[i];
-      if (k == 0) continue;
-      const int w = i / per_row, at = i - w * per_row, mine = at / W;
-      int better = at - mine * W;
-      for (int g = 0; g < G && better < W; ++g) {
-        if (g == mine) continue;
-        const uint64_t* const l = keys + w * per_row + g * W;
-        for (int j = 0; j < W && l[j] > k; ++j) ++better;
+    if (tid >= kRankThreads) {
+      if (w0 == 0 && tid - kRankThreads < W) {
+        const int w = tid - kRankThreads;
+        const bool over = live[w] == 2;
+        if (live[w] == 1) {
+          float mx = kNone;
+#pragma unroll 8
+          for (int g = 0; g < G; ++g) mx = fmaxf(mx, gmax[w * G + g]);
+          double sum = 0.0;
+          for (int g = 0; g < G; ++g) {
+            const float m = gmax[w * G + g];
+            if (m > kNone) sum += m == mx ? gsum[w * G + g] : gsum[w * G + g] * exp64((double)m - (double)mx);
+          }
+          rmax[w] = mx;
+          // (where not one token is allowed there are no keys either)
+          if (mx > kNone) base[w] -= log64(sum);
+        }
+        const int len = len0[w] + (over ? 0 : 1);
+        factor[w] = a.alpha == 0.0f || len <= 1 ? 1.0 : exp64(-(double)a.alpha * log64((double)len));
       }
-      if (better < W) cand[(w0 + w) * W + better] = k;
+    } else {
+      for (int i = tid; i < n; i += kRankThreads) {
+        const int wl = i / per_row, at = i - wl * per_row, mine = at / W;
+        const uint64_t* const row = keys + wl * per_row;
+        const uint64_t k = row[at];
+        if (live[w0 + wl] != 1 || k == 0) continue;
+        if (G > W) {
+          const uint64_t head = row[mine * W];
+          int before = 0;
+#pragma unroll 8
+          for (int g = 0; g < G; ++g) before += row[g * W] > head;
+          if (before >= W) continue;
+        }
+        int better = 0;
+        if (per_row <= 256) {
+#pragma unroll 8
+          for (int j = 0; j < per_row; ++j) better += row[j] > k;
+        } else {
+          better = at - mine * W;
+          for (int g = 0; g < G && better < W; ++g) {
+            if (g == mine) continue;
+            for (int j = 0; j < W && row[g * W + j] > k; ++j) ++better;
+          }
+        }
+        if (better < W) cand[(w0 + wl) * W + better] = k;
+      }
     }
     __syncthreads();
   }
   if (tid < W && live[tid] == 2) cand[tid * W] = entry_key(0.0f, (uint32_t)a.end);
   __syncthreads();
-  for (int i = tid; i < W * W; i += 256) {
+  constexpr double kBottom = -__builtin_huge_val();
+  for (int i = tid; i < W * W; i += kMergeThreads) {
     const int w = i / W;
     const uint64_t k = cand[i];
-    double r = -__builtin_huge_val();
+    double r = kBottom;
     if (k != 0) {
       const float l = key_value(k);
       r = base[w] + (live[w] == 2 || l == rmax[w] ? 0.0 : (double)l - (double)rmax[w]);
     }
     raw[i] = r;
     rank[i] = r * factor[w];
-    if (rank[i] > -__builtin_huge_val()) atomicAdd(&valid, 1);
+    before[i] = rank[i] > kBottom ? i - w * W : W;  // in its own beam's list; W: does not count
+    if (rank[i] > kBottom) atomicAdd(&valid, 1);
   }
   __syncthreads();
-  for (int i = tid; i < W * W; i += 256) {
+  // of the other beams' lists, by halving: those above, and among equals those of lower beams
+  for (int u = tid; u < W * W * W; u += kMergeThreads) {
+    const int i = u / W, o = u - i * W;
+    if (before[i] >= W || o == i / W) continue;
     const double mine = rank[i];
-    if (!(mine > -__builtin_huge_val())) continue;
-    const int w = i / W;
-    int better = i - w * W;
-    for (int o = 0; o < W && better < W; ++o) {
-      if (o == w) continue;
-      // beams before this one win ties
-      for (int j = 0; j < W && (rank[o * W + j] > mine || (o < w && rank[o * W + j] == mine)); ++j) ++better;
+    int lo = 0, hi = W;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      const double r = rank[o * W + mid];
+      if (r > mine || (r == mine && o * W < i)) lo = mid + 1;
+      else hi = mid;
     }
+    if (lo > 0) atomicAdd(&before[i], lo);
+  }
+  __syncthreads();
+  for (int i = tid; i < W * W; i += kMergeThreads) {
+    const int better = before[i];
     if (better >= W) continue;
+    const int w = i / W, token = (int)key_index(cand[i]);
     const bool over = live[w] == 2;
-    const int token = (int)key_index(cand[i]);
     const int64_t o = r0 + better;
     a.tokens[o] = token;
     a.parents[o] = w;
     a.scores_out[o] = (float)raw[i];
-    a.lengths_out[o] = a.lengths[r0 + w] + (over ? 0 : 1);
+    a.lengths_out[o] = len0[w] + (over ? 0 : 1);
     a.ended_out[o] = over || token == a.end;
   }
   if (tid < W && tid >= valid) {
@@ -453,13 +574,10 @@ extern "C" int vkwr_beam_select(int B, int W, int V, const void* logits, int log
   a.keys = reinterpret_cast<uint64_t*>(a.stats + rows * a.groups);
   const hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)a.groups, (unsigned)rows), block(kRowThreads);
-  const bool vec = (uintptr_t)logits % 16 == 0 && V % (logits_f16 ? 8 : 4) == 0;
-  if (logits_f16 && vec) hipLaunchKernelGGL((beam_rows_kernel<true, true>), grid, block, 0, s, a);
-  else if (logits_f16) hipLaunchKernelGGL((beam_rows_kernel<true, false>), grid, block, 0, s, a);
-  else if (vec) hipLaunchKernelGGL((beam_rows_kernel<false, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((beam_rows_kernel<false, false>), grid, block, 0, s, a);
+  if (logits_f16) hipLaunchKernelGGL(beam_rows_kernel<true>, grid, block, 0, s, a);
+  else hipLaunchKernelGGL(beam_rows_kernel<false>, grid, block, 0, s, a);
   if (int e = check_launch(fn)) return e;
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(kMergeThreads), 0, s, a);
   return check_launch(fn);
 }
 

@@ -14,6 +14,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <stdlib.h>
+#include <stdio.h>
 
 #include "vk_capi.h"
 #include "vk_common.cuh"
@@ -29,7 +31,8 @@ typedef uint32_t uv4 __attribute__((ext_vector_type(4)));
 constexpr int kMaxI8 = 8;          // problems per call
 constexpr int kI8Rows = 32;        // rows of a block of packed 8-bit values
 constexpr int kI8Pad = 128;        // K is padded to multiples of this, with zeros
-constexpr int64_t kI8MaxK = 131072;  // 127^2 k < 2^31
+constexpr int64_t kI8MaxK = 131072;   // 127^2 k < 2^31
+constexpr int64_t kI8MaxRows = 1 << 22;  // of a matrix, and of all the activations of a call (launch sizes)
 
 __host__ __device__ inline int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
@@ -45,7 +48,6 @@ struct QProb {
   int8_t* q;
   float* s;
   int m, k, steps;
-  int vec;       // rows of x are 16-byte aligned
   int wg_begin;  // first workgroup
 };
 struct QBatch {
@@ -74,22 +76,24 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, a), __builtin_bit_cast(u2, b)));
 }
 
-// 16 values of row x from k0, zeros past K.
-template <bool kVec>
-__device__ __forceinline__ void load16(const _Float16* x, int64_t k0, int k, uv4 (&v)[2]) {
-  if constexpr (kVec) {
-    const uv4* p = reinterpret_cast<const uv4*>(x + k0);
-    v[0] = k0 + 8 <= k ? p[0] : uv4{0, 0, 0, 0};
-    v[1] = k0 + 16 <= k ? p[1] : uv4{0, 0, 0, 0};
-  } else {
+// 8 values of a row from k0, zeros past K.  Rows that do not start on 16 bytes are loaded the same way
+// (an unaligned load: one value at a time took 13 us for 77 rows of 2501, this 4).
+__device__ __forceinline__ uv4 load8(const _Float16* x, int64_t k0, int k) {
+  uv4 v = {0, 0, 0, 0};
+  if (k0 + 8 <= k) {
+    __builtin_memcpy(&v, x + k0, 16);
+  } else if (k0 < k) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const int64_t k1 = k0 + 2 * w;
-      const uint32_t lo = k1 < k ? __builtin_bit_cast(uint16_t, x[k1]) : 0;
-      const uint32_t hi = k1 + 1 < k ? __builtin_bit_cast(uint16_t, x[k1 + 1]) : 0;
-      v[w >> 2][w & 3] = lo | hi << 16;
-    }
+    for (int e = 0; e < 8; ++e)
+      if (k0 + e < k) v[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, x[k0 + e]) << (16 * (e & 1));
   }
+  return v;
+}
+
+// 16 values of row x from k0.
+__device__ __forceinline__ void load16(const _Float16* x, int64_t k0, int k, uv4 (&v)[2]) {
+  v[0] = load8(x, k0, k);
+  v[1] = load8(x, k0 + 8, k);
 }
 
 __device__ __forceinline__ uint32_t top_bits(uint32_t top, const uv4 (&v)[2]) {
@@ -110,52 +114,63 @@ __device__ __forceinline__ iv4 quant16(const uv4 (&v)[2], float top, float inv) 
   return o;
 }
 
-// One row per wave, eight rows per workgroup: the rows of a 128-byte line of the packed matrix.
-// The row is kept in registers between its maximum and its rounding where it has at most
-// 1024 kKeep values, else read again.  |x| is compared as an integer, where an infinity or a NaN
-// exceeds every number: such a row gets the scale NaN and zeros.
-template <int kKeep, bool kVec>
-__global__ __launch_bounds__(512) void i8_rows_kernel(QBatch bt) {
+// T lanes per row, 256 / T rows per workgroup (T = 512: one row): so many that a lane holds at most 32 values
+// and a few hundred rows reach every CU (one wave per row: 433 rows of 8192 9.0 us).  The 32 rows of
+// a block go to one XCD (workgroup b runs on XCD b % 8), whose L2 joins the 16-byte pieces that they
+// write into common lines.  Rows longer than 32 T are read twice.  |x| is compared as an integer, where an
+// infinity or a NaN exceeds every number: such a row gets the scale NaN and zeros.
+template <int T>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void i8_rows_kernel(QBatch bt) {
+  constexpr int kThreads = T < 256 ? 256 : T, kRows = kThreads / T, kWaves = T / 64, kKeep = 2;
+  __shared__ uint32_t wtop[kThreads / 64];
   int pi = 0;
 #pragma unroll
   for (int i = 1; i < kMaxI8; ++i)
     if (i < bt.n && (int)blockIdx.x >= bt.p[i].wg_begin) pi = i;
   const QProb& P = bt.p[pi];
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)((int)blockIdx.x - P.wg_begin) * 8 + (threadIdx.x >> 6);
-  if (row >= P.m) return;
+  const int u = (int)blockIdx.x - P.wg_begin, per = 32 / kRows;  // workgroups of a block of rows
+  const int idx = u >> 3;
+  const int64_t row = ((int64_t)(idx / per) * 8 + (u & 7)) * 32 + idx % per * kRows + threadIdx.x / T;
+  const int t = threadIdx.x % T, wave = threadIdx.x >> 6;
+  const int k = row < P.m ? P.k : 0, chunks = row < P.m ? P.steps * 2 : 0;  // chunks of 16
   const _Float16* const x = P.x + row * P.k;
-  const int k = P.k, chunks = P.steps * 2;  // chunks of 16
   uv4 v[kKeep][2];
   uint32_t top = 0;
 #pragma unroll
-  for (int c = 0; c < kKeep; ++c) load16<kVec>(x, (int64_t)(c * 64 + lane) * 16, k, v[c]);
+  for (int c = 0; c < kKeep; ++c) load16(x, (int64_t)(c * T + t) * 16, k, v[c]);
 #pragma unroll
   for (int c = 0; c < kKeep; ++c) top = top_bits(top, v[c]);
-  for (int c = kKeep * 64 + lane; c < chunks; c += 64) {
-    uv4 u[2];
-    load16<kVec>(x, (int64_t)c * 16, k, u);
-    top = top_bits(top, u);
+  for (int c = kKeep * T + t; c < chunks; c += T) {
+    uv4 w[2];
+    load16(x, (int64_t)c * 16, k, w);
+    top = top_bits(top, w);
   }
   top = max(top & 0xffffu, top >> 16);
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+  if constexpr (kWaves > 1) {
+    if ((threadIdx.x & 63) == 0) wtop[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = max(top, wtop[wave / kWaves * kWaves + w]);
+  }
+  if (row >= P.m) return;
   const bool finite = top < 0x7c00u;
   const float a = finite ? h2f((uint16_t)top) : 0.0f;
   const float inv = a > 0.0f ? 1.0f / a : 0.0f;
-  if (lane == 0) P.s[row] = finite ? a / 127.0f : __builtin_nanf("");
+  if (t == 0) P.s[row] = finite ? a / 127.0f : __builtin_nanf("");
   int8_t* const q = P.q + i8_index(row, 0, P.steps);
-  auto put = [&](int c, const uv4(&u)[2]) __attribute__((always_inline)) {
-    const iv4 o = a > 0.0f ? quant16(u, a, inv) : iv4{0, 0, 0, 0};
+  auto put = [&](int c, const uv4(&w)[2]) __attribute__((always_inline)) {
+    const iv4 o = a > 0.0f ? quant16(w, a, inv) : iv4{0, 0, 0, 0};
     *reinterpret_cast<iv4*>(q + (int64_t)c * 512) = o;  // chunk c: 512 bytes on
   };
 #pragma unroll
   for (int c = 0; c < kKeep; ++c)
-    if (c * 64 + lane < chunks) put(c * 64 + lane, v[c]);
-  for (int c = kKeep * 64 + lane; c < chunks; c += 64) {
-    uv4 u[2];
-    load16<kVec>(x, (int64_t)c * 16, k, u);
-    put(c, u);
+    if (c * T + t < chunks) put(c * T + t, v[c]);
+  for (int c = kKeep * T + t; c < chunks; c += T) {
+    uv4 w[2];
+    load16(x, (int64_t)c * 16, k, w);
+    put(c, w);
   }
 }
 
@@ -167,9 +182,13 @@ __global__ __launch_bounds__(256) void i8_pack_kernel(int64_t rows, int64_t k, c
     const int lane = (int)(c & 63);
     const int64_t b = c >> 6, r = b / steps * 32 + (lane & 31), k0 = b % steps * 32 + (lane >> 5) * 16;
     iv4 o = {0, 0, 0, 0};
+    if (r < rows && k0 + 16 <= k) {
+      __builtin_memcpy(&o, src + r * k + k0, 16);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (r < rows && k0 + e < k) o[e >> 2] |= (int)((uint32_t)(uint8_t)src[r * k + k0 + e] << (8 * (e & 3)));
+      for (int e = 0; e < 16; ++e)
+        if (r < rows && k0 + e < k) o[e >> 2] |= (int)((uint32_t)(uint8_t)src[r * k + k0 + e] << (8 * (e & 3)));
+    }
     *reinterpret_cast<iv4*>(dst + c * 16) = o;
   }
 }
@@ -200,35 +219,38 @@ __device__ __forceinline__ float i8_act(int epi, float v) {
   return v;
 }
 
-// Eight consecutive outputs of a row: the sums scaled in fp32, the epilogue, one rounding to fp16.
+// One output: the sum scaled in fp32, the epilogue, one rounding to fp16.  Every kernel finishes its sums
+// here, so that a row's bits do not depend on which one ran.
+__device__ __forceinline__ _Float16 i8_finish(int a, float s, float t, int epi, float bias) {
+  float f = (float)a * (s * t);
+  if (epi == VKWR_GEMM_EPI_BIAS) f += bias;
+  return f16_of(i8_act(epi, f));
+}
+
+// Eight consecutive outputs of a row.
 __device__ __forceinline__ void i8_finish8(const int (&a)[8], int row, int col, int m, int n, int epi, int vec, float s,
                                            const float* t, const _Float16* bias, _Float16* y) {
   if (row >= m || col >= n) return;
-  float f[8];
+  hv8 h;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int c = col + e < n ? col + e : n - 1;
-    f[e] = (float)a[e] * (s * t[c]);
-    if (epi == VKWR_GEMM_EPI_BIAS) f[e] += (float)bias[c];
-    f[e] = i8_act(epi, f[e]);
+    h[e] = i8_finish(a[e], s, t[c], epi, epi == VKWR_GEMM_EPI_BIAS ? (float)bias[c] : 0.0f);
   }
   _Float16* const o = y + (int64_t)row * n + col;
   if (vec) {
-    hv8 h;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = f16_of(f[e]);
     *reinterpret_cast<hv8*>(o) = h;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (col + e < n) o[e] = f16_of(f[e]);
+      if (col + e < n) o[e] = h[e];
   }
 }
 
 // (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
-// KS k-steps w, w + NW, ... with the next block's loads in flight, and the NW partial
+// KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
 // tiles are added through LDS.
-template <int TM, int TN, int NW, int KS>
+template <int TM, int TN, int NW, int KS, int NB>
 __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
   constexpr int kTiles = TM * TN, kG = 65;  // 16-byte cells of a group of 4 results: 64 lanes and one of padding
   __shared__ __attribute__((aligned(16))) iv4 red[NW * kTiles * 4 * kG];
@@ -238,7 +260,9 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
     if (i < bt.n && (int)blockIdx.x >= bt.p[i].wg_begin) pi = i;
   const IProb& P = bt.p[pi];
   const int lt = (int)blockIdx.x - P.wg_begin;
-  const int mb = lt % P.nmb, cb = lt / P.nmb;
+  // the row tiles of a column tile run on one XCD, eight ids apart, and share its weights' one trip to the L2
+  const int mb = (lt >> 3) % P.nmb, cb = (lt >> 3) / P.nmb * 8 + (lt & 7);
+  if (cb >= P.ncol) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int steps = P.steps, mblk = (P.m + 31) >> 5, nblk = (P.n + 31) >> 5;
   const int8_t *xp[TM], *wp[TN];  // blocks past the last are read as the last
@@ -251,11 +275,11 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = iv16{0};
-  iv4 fx[2][KS][TM], fw[2][KS][TN];
+  iv4 fx[NB][KS][TM], fw[NB][KS][TN];
   auto load = [&](int buf, int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int64_t o = ((int64_t)b * KS + s) * 1024;
+      const int64_t o = ((int64_t)(wave + b * NW) * KS + s) * 1024;
 #pragma unroll
       for (int j = 0; j < TN; ++j) fw[buf][s][j] = *reinterpret_cast<const iv4*>(wp[j] + o);
 #pragma unroll
@@ -271,28 +295,32 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
         for (int j = 0; j < TN; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[buf][s][j], fx[buf][s][i], acc[i][j], 0, 0, 0);
   };
-  const int blocks = steps / KS;  // K is padded to 4 steps
   static_assert(kI8Pad % (32 * KS) == 0, "whole blocks");
-  int b = wave;
-  if (b < blocks) load(0, b);
-  for (; b + 2 * NW < blocks; b += 2 * NW) {
-    load(1, b + NW);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(0);
-    __builtin_amdgcn_sched_barrier(0);
-    load(0, b + 2 * NW);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(1);
+  const int blocks = steps / KS, nb = (blocks - wave + NW - 1) / NW;  // this wave's blocks
+#pragma unroll
+  for (int u = 0; u < NB; ++u)
+    if (u < nb) load(u, u);
+  __builtin_amdgcn_sched_barrier(0);
+  int b = 0;
+  // every load of the loop is unconditional, so that the waits in it are exact
+  for (; b + 2 * NB <= nb; b += NB) {
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      compute(u);
+      __builtin_amdgcn_sched_barrier(0);
+      load(u, b + NB + u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < NB; ++u) {
+    if (b + u < nb) compute(u);
+    if (b + NB + u < nb) load(u, b + NB + u);
     __builtin_amdgcn_sched_barrier(0);
   }
-  if (b + NW < blocks) {
-    load(1, b + NW);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(0);
-    compute(1);
-  } else if (b < blocks) {
-    compute(0);
-  }
+#pragma unroll
+  for (int u = 0; u < NB; ++u)
+    if (b + NB + u < nb) compute(u);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -315,6 +343,358 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
   }
 }
 
+// ---- few rows: the weights pass through once, four products an instruction
+//
+// One workgroup per 32 outputs, whose eight waves share K.  The rows (up to 4, up to 32768 values
+// together) are rounded by every workgroup itself, in LDS, while its first weights are on the way: that
+// costs less than a launch in front of this one.  A lane holds 16 k of one output, and
+// reads the row's 16 values as a broadcast.
+constexpr int kGemvKeep = 8;                      // 16-byte pieces of x per lane
+constexpr int kGemvMost = kGemvKeep * 512 * 8;    // values of all rows together
+
+struct GProb {
+  const _Float16* x;
+  const int8_t* w;
+  const float* t;
+  const _Float16* bias;
+  _Float16* y;
+  int m, n, k, steps, epi, wg_begin;
+};
+struct GBatch {
+  int n;
+  GProb p[kMaxI8];
+};
+
+template <int M>
+__global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
+  constexpr int kWaves = 8, kPer = kWaves / M, kAhead = 8;  // waves of a row; weights requested first
+  __shared__ __attribute__((aligned(16))) int8_t xq[kGemvMost + M * kI8Pad];
+  __shared__ uint32_t wtop[kWaves];
+  __shared__ int part[kWaves][M][32];
+  int pi = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxI8; ++i)
+    if (i < bt.n && (int)blockIdx.x >= bt.p[i].wg_begin) pi = i;
+  const GProb& P = bt.p[pi];
+  const int cb = (int)blockIdx.x - P.wg_begin;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int steps = P.steps, k = P.k, kpad = steps * 32;
+  const int8_t* const w = P.w + (int64_t)cb * steps * 1024 + lane * 16;
+  iv4 fw[kAhead];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    const int st = min(wave + a * kWaves, steps - 1);
+    fw[a] = *reinterpret_cast<const iv4*>(w + (int64_t)st * 1024);
+  }
+  // ---- this wave's pieces of 8 values of its row
+  const int row = min(wave / kPer, P.m - 1), w0 = wave % kPer, pieces = kpad / 8;
+  const _Float16* const x = P.x + (int64_t)row * k;
+  uv4 v[kGemvKeep];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kGemvKeep; ++i) {
+    const int c = (i * kPer + w0) * 64 + lane;
+    v[i] = load8(x, (int64_t)c * 8, k);
+  }
+#pragma unroll
+  for (int i = 0; i < kGemvKeep; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max_u16x2(top, v[i][e] & 0x7fff7fffu);
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+  if (lane == 0) wtop[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) top = max(top, wtop[wave / kPer * kPer + i]);
+  {
+    const float a = top < 0x7c00u ? h2f((uint16_t)top) : 0.0f, inv = a > 0.0f ? 1.0f / a : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kGemvKeep; ++i) {
+      const int c = (i * kPer + w0) * 64 + lane;
+      if (c < pieces) {
+        typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+        uint32_t o[2] = {0, 0};
+        if (a > 0.0f) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const h2v lo = __builtin_bit_cast(h2v, (uint32_t)v[i][2 * h]), hi = __builtin_bit_cast(h2v, (uint32_t)v[i][2 * h + 1]);
+            const float f[4] = {(float)lo.x, (float)lo.y, (float)hi.x, (float)hi.y};
+            o[h] = quant4(f, a, inv);
+          }
+        }
+        *reinterpret_cast<uint64_t*>(xq + wave / kPer * kpad + c * 8) = (uint64_t)o[1] << 32 | o[0];
+      }
+    }
+  }
+  __syncthreads();
+  int acc[M] = {};
+  const int8_t* const xl = xq + (lane >> 5) * 16;
+  auto dot = [&](const iv4& b, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+      const iv4 a = *reinterpret_cast<const iv4*>(xl + r * kpad + st * 32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[r] = __builtin_amdgcn_sdot4(a[e], b[e], acc[r], false);
+    }
+  };
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+    if (wave + a * kWaves < steps) dot(fw[a], wave + a * kWaves);
+  for (int s0 = wave + kAhead * kWaves; s0 < steps; s0 += kAhead * kWaves) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int st = min(s0 + a * kWaves, steps - 1);
+      fw[a] = *reinterpret_cast<const iv4*>(w + (int64_t)st * 1024);
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+      if (s0 + a * kWaves < steps) dot(fw[a], s0 + a * kWaves);
+  }
+#pragma unroll
+  for (int r = 0; r < M; ++r) {
+    acc[r] += __shfl_xor(acc[r], 32, 64);
+    if (lane < 32) part[wave][r][lane] = acc[r];
+  }
+  __syncthreads();
+  if (tid < 32 * M) {
+    const int r = tid >> 5, col = cb * 32 + (tid & 31);
+    if (r < P.m && col < P.n) {
+      int sum = 0;
+#pragma unroll
+      for (int q = 0; q < kWaves; ++q) sum += part[q][r][tid & 31];
+      uint32_t all = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) all = max(all, wtop[r * kPer + i]);
+      const float s = all < 0x7c00u ? h2f((uint16_t)all) / 127.0f : __builtin_nanf("");
+      P.y[(int64_t)r * P.n + col] = i8_finish(sum, s, P.t[col], P.epi, P.epi == VKWR_GEMM_EPI_BIAS ? (float)P.bias[col] : 0.0f);
+    }
+  }
+}
+
+// ---- many rows: tiles through LDS, bound by the matrix cores
+//
+// (64 TM) x (64 TN) outputs per workgroup, four waves of (32 TM) x (32 TN) in registers.  K advances
+// 128 per stage through two LDS buffers; both operands being in fragment order, a stage is a row of
+// 4 KiB pieces, copied straight to LDS, and read back lane by lane.  One barrier per stage, before the
+// last group of products, whose operands are then in registers: behind it the buffer is free and the copies of
+// the stage after next go out, one behind every other product of this and the next group, so
+// that they neither hold up the products nor arrive late.  The copies are written in assembly, as the compiler
+// would make every LDS read wait for all of them; the waits are placed here.
+template <int TM, int TN>
+struct I8Tile {
+  static constexpr int kX = 8 * TM, kW = 8 * TN, kBlocks = kX + kW;  // kilobytes of a stage
+  static constexpr int kCopies = kBlocks / 4;                        // per wave
+  static constexpr int kOutRow = 144;                                // bytes of a staged row of 64 outputs
+};
+
+__device__ __forceinline__ const void* uniform_ptr(const void* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const void*)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
+
+// 16 bytes per lane: global (base + off) -> LDS (lds + 16 lane); base and lds wave-uniform
+__device__ __forceinline__ void copy16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+
+template <int TM, int TN, int kEpi>
+__device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&acc)[TM][TN], int row0, int col0, int lane) {
+  constexpr int kRow = I8Tile<TM, TN>::kOutRow, kBuf = 32 * kRow;
+  const int lr = lane & 31, lh = lane >> 5, r8 = lane >> 3, c8 = 8 * (lane & 7);
+  typedef _Float16 __attribute__((address_space(1)))* gptr;
+  int m = P.m, n = P.n, vec = P.vec;
+  gptr y = (gptr)P.y;
+  const float *sp = P.s, *tp = P.t;
+  const _Float16* bp = P.bias;
+  asm("" : "+s"(m), "+s"(n), "+s"(vec), "+s"(y), "+s"(sp), "+s"(tp), "+s"(bp));
+  // the columns' scales (and biases) behind the two strips
+  float* const tl = reinterpret_cast<float*>(st + 2 * kBuf);
+#pragma unroll
+  for (int c = 0; c < 32 * TN; c += 64) {
+    if (c + lane < 32 * TN) {
+      const int col = min(col0 + c + lane, n - 1);
+      tl[c + lane] = tp[col];
+      if constexpr (kEpi == VKWR_GEMM_EPI_BIAS) tl[32 * TN + c + lane] = (float)bp[col];
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  float s[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) s[i] = sp[min(row0 + 32 * i + lr, m - 1)];
+  constexpr int kStrips = TM * TN / 2;
+  auto write = [&](int p) __attribute__((always_inline)) {
+    const int i = p % TM, j0 = p / TM * 2;
+    char* const o = st + (p & 1) * kBuf + lr * kRow;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = (j0 + jj) * 32 + 8 * g + 4 * lh;
+        const f4 t = *reinterpret_cast<const f4*>(tl + c);
+        f4 b = {0, 0, 0, 0};
+        if constexpr (kEpi == VKWR_GEMM_EPI_BIAS) b = *reinterpret_cast<const f4*>(tl + 32 * TN + c);
+        typedef _Float16 hv4 __attribute__((ext_vector_type(4)));
+        hv4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = i8_finish(acc[i][j0 + jj][4 * g + e], s[i], t[e], kEpi, b[e]);
+        *reinterpret_cast<hv4*>(o + (jj * 32 + 8 * g + 4 * lh) * 2) = h;
+      }
+  };
+  auto send = [&](int p) __attribute__((always_inline)) {
+    const int i = p % TM, col = col0 + p / TM * 64 + c8;
+    const char* const o = st + (p & 1) * kBuf + r8 * kRow + c8 * 2;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const hv8 v = *reinterpret_cast<const hv8*>(o + 8 * h * kRow);
+      const int row = row0 + 32 * i + 8 * h + r8;
+      if (row >= m || col >= n) continue;
+      gptr d = y + (int64_t)row * n + col;
+      if (vec) {
+        *reinterpret_cast<__attribute__((address_space(1))) hv8*>(d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < n) d[e] = v[e];
+      }
+    }
+  };
+  write(0);
+#pragma unroll
+  for (int p = 1; p < kStrips; ++p) {
+    write(p);
+    send(p - 1);
+  }
+  send(kStrips - 1);
+}
+
+template <int TM, int TN>
+__global__ __launch_bounds__(256, TM* TN > 4 ? 1 : 2) void i8_tile_kernel(IBatch bt, int tiles) {
+  using T = I8Tile<TM, TN>;
+  constexpr int ND = T::kCopies, kHalf = ND / 2;
+  constexpr int kOut = 4 * (2 * 32 * T::kOutRow + 2 * 32 * TN * 4);
+  constexpr int kRing = 2 * T::kBlocks * 1024;
+  static_assert(kOut <= kRing, "the outputs are staged where the operands were");
+  __shared__ __attribute__((aligned(1024))) char sm[kRing];
+  // workgroup b runs on XCD b % 8: each takes a contiguous range of tiles, in groups of 4 tile rows
+  int L;
+  {
+    const int b = blockIdx.x, x = b & 7, q8 = tiles >> 3, r8 = tiles & 7;
+    L = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (b >> 3);
+  }
+  int pi = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxI8; ++i)
+    if (i < bt.n && L >= bt.p[i].wg_begin) pi = i;
+  const IProb& P = bt.p[pi];
+  const int lt = L - P.wg_begin, per = 4 * P.ncol, grp = lt / per, in = lt - grp * per;
+  const int g0 = grp * 4, gs = min(4, P.nmb - g0);
+  const int mb = g0 + in % gs, cb = in / gs;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w >> 1, wn = w & 1;
+  const int steps = P.steps, ns = steps >> 2;
+  const int mlast = ((P.m + 31) >> 5) - 1 - mb * 2 * TM, nlast = ((P.n + 31) >> 5) - 1 - cb * 2 * TN;
+  // copy d of wave w: k step w of the stage, of block d of x, then of the weights
+  uint32_t off[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    const int blk = d < 2 * TM ? min(d, mlast) : min(d - 2 * TM, nlast);
+    off[d] = (uint32_t)((blk * steps + w) * 1024 + lane * 16);
+  }
+  const char* const px = (const char*)uniform_ptr(P.q + (int64_t)mb * 2 * TM * steps * 1024);
+  const char* const pw = (const char*)uniform_ptr(P.w + (int64_t)cb * 2 * TN * steps * 1024);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(VK_LDS void*)&sm[0] + w * 1024);
+  auto copies = [&](int buf, int st, int d0, int d1) __attribute__((always_inline)) {
+    const int64_t k0 = (int64_t)min(st, ns - 1) * 4096;  // past the end: the last stage once more, unused
+    const void *xb = uniform_ptr(px + k0), *wb = uniform_ptr(pw + k0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      if (d >= d0 && d < d1) copy16(d < 2 * TM ? xb : wb, off[d], lds0 + buf * T::kBlocks * 1024 + d * 4096);
+  };
+  const char* const fxp = sm + wm * TM * 4096 + lane * 16;
+  const char* const fwp = sm + (T::kX + wn * TN * 4) * 1024 + lane * 16;
+  iv4 fx[2][TM], fw[2][TN];
+  auto fread = [&](int buf, int kk, int set) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fx[set][i] = *reinterpret_cast<const iv4*>(fxp + buf * T::kBlocks * 1024 + (i * 4 + kk) * 1024);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fw[set][j] = *reinterpret_cast<const iv4*>(fwp + buf * T::kBlocks * 1024 + (j * 4 + kk) * 1024);
+  };
+  iv16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = iv16{0};
+  // the products of a group with the next group's reads between them
+  auto products = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][j], fx[set][i], acc[i][j], 0, 0, 0);
+    constexpr int kReads = TM + TN < TM * TN ? TM + TN : TM * TN;
+#pragma unroll
+    for (int q = 0; q < kReads; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, TM + TN - kReads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, TM * TN - kReads, 0);
+  };
+  // the products of a group with copies d0 .. d0 + kHalf - 1 of stage st between them
+  auto products_copies = [&](int set, int buf, int st, int d0) __attribute__((always_inline)) {
+    const int64_t k0 = (int64_t)min(st, ns - 1) * 4096;
+    const void *xb = uniform_ptr(px + k0), *wb = uniform_ptr(pw + k0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][j], fx[set][i], acc[i][j], 0, 0, 0);
+        const int p = i * TN + j;
+#pragma unroll
+        for (int q = 0; q < kHalf; ++q)
+          if (q * TM * TN / kHalf == p)
+            copy16(d0 + q < 2 * TM ? xb : wb, off[d0 + q], lds0 + buf * T::kBlocks * 1024 + (d0 + q) * 4096);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  copies(0, 0, 0, ND);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  copies(1, 1, 0, kHalf);
+  fread(0, 0, 0);
+  int cur = 0;
+  for (int s = 0; s < ns; ++s) {
+    const int nxt = cur ^ 1;
+    fread(cur, 1, 1);
+    products_copies(0, nxt, s + 1, kHalf);
+    __builtin_amdgcn_sched_barrier(0);
+    fread(cur, 2, 0);
+    products(1);
+    __builtin_amdgcn_sched_barrier(0);
+    fread(cur, 3, 1);
+    products(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // stage s + 1 has landed and this stage is read, for every wave
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fread(nxt, 0, 0);
+    products_copies(1, cur, s + 2, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    cur = nxt;
+  }
+  // the last copies have landed and every wave's reads are done
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  char* const st = sm + w * (kOut / 4);
+  const int row0 = mb * 64 * TM + wm * 32 * TM, col0 = cb * 64 * TN + wn * 32 * TN;
+  switch (P.epi) {
+    case VKWR_GEMM_EPI_RELU_SQUARE: i8_store<TM, TN, VKWR_GEMM_EPI_RELU_SQUARE>(st, P, acc, row0, col0, lane); break;
+    case VKWR_GEMM_EPI_BIAS: i8_store<TM, TN, VKWR_GEMM_EPI_BIAS>(st, P, acc, row0, col0, lane); break;
+    case VKWR_GEMM_EPI_TANH: i8_store<TM, TN, VKWR_GEMM_EPI_TANH>(st, P, acc, row0, col0, lane); break;
+    case VKWR_GEMM_EPI_SIGMOID: i8_store<TM, TN, VKWR_GEMM_EPI_SIGMOID>(st, P, acc, row0, col0, lane); break;
+    default: i8_store<TM, TN, VKWR_GEMM_EPI_NONE>(st, P, acc, row0, col0, lane); break;
+  }
+}
+
 // ---------------------------------------------------------------- host
 
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -325,16 +705,19 @@ int64_t packed_bytes(int64_t rows, int64_t k) { return up(rows, kI8Rows) * up(k,
 
 int check_problems(const char* fn, int n, const vkwr_i8_problem* p) {
   VK_REQUIRE(n >= 1 && n <= kMaxI8 && p, "%s: 1 to %d problems, got %d", fn, kMaxI8, n);
+  int64_t rows = 0;
   for (int i = 0; i < n; ++i) {
-    VK_REQUIRE(p[i].m >= 0 && p[i].m <= (1 << 22) && p[i].n >= 1 && p[i].n <= (1 << 24) && p[i].k >= 1 &&
+    VK_REQUIRE(p[i].m >= 0 && p[i].m <= kI8MaxRows && p[i].n >= 1 && p[i].n <= kI8MaxRows && p[i].k >= 1 &&
                    p[i].k <= kI8MaxK,
-               "%s: problem %d: sizes m=%lld n=%lld k=%lld (m up to 2^22, n up to 2^24, k up to %lld)", fn, i,
+               "%s: problem %d: sizes m=%lld n=%lld k=%lld (m and n up to 2^22, k up to %lld)", fn, i,
                (long long)p[i].m, (long long)p[i].n, (long long)p[i].k, (long long)kI8MaxK);
     VK_REQUIRE(p[i].epilogue == VKWR_GEMM_EPI_NONE || p[i].epilogue == VKWR_GEMM_EPI_RELU_SQUARE ||
                    p[i].epilogue == VKWR_GEMM_EPI_BIAS || p[i].epilogue == VKWR_GEMM_EPI_TANH ||
                    p[i].epilogue == VKWR_GEMM_EPI_SIGMOID,
                "%s: problem %d: unsupported epilogue %d", fn, i, p[i].epilogue);
+    rows += p[i].m;
   }
+  VK_REQUIRE(rows <= kI8MaxRows, "%s: sizes: %lld rows together, at most 2^22", fn, (long long)rows);
   return VKWR_OK;
 }
 
@@ -362,28 +745,21 @@ I8Scratch scratch_of(int n, const vkwr_i8_problem* p) {
   return c;
 }
 
-template <int kKeep>
-void launch_rows_vec(bool vec, unsigned grid, hipStream_t s, const QBatch& b) {
-  if (vec) hipLaunchKernelGGL((i8_rows_kernel<kKeep, true>), dim3(grid), dim3(512), 0, s, b);
-  else hipLaunchKernelGGL((i8_rows_kernel<kKeep, false>), dim3(grid), dim3(512), 0, s, b);
-}
-
 // Rounds the rows of every problem of `b` (wg_begin filled in here).
 void launch_rows(QBatch& b, hipStream_t s) {
-  unsigned grid = 0;
   int most = 0;
-  bool vec = true;
+  for (int i = 0; i < b.n; ++i) most = std::max(most, b.p[i].steps);
+  const int T = most <= 64 ? 64 : most <= 128 ? 128 : most <= 256 ? 256 : 512;  // lanes per row
+  unsigned grid = 0;
   for (int i = 0; i < b.n; ++i) {
     b.p[i].wg_begin = (int)grid;
-    grid += (unsigned)((b.p[i].m + 7) / 8);
-    most = std::max(most, b.p[i].steps);
-    vec = vec && b.p[i].vec;
+    grid += (unsigned)up((b.p[i].m + 31) / 32, 8) * 32 / std::max(1, 256 / T);
   }
   if (grid == 0) return;
-  if (most <= 32) launch_rows_vec<1>(vec, grid, s, b);
-  else if (most <= 64) launch_rows_vec<2>(vec, grid, s, b);
-  else if (most <= 128) launch_rows_vec<4>(vec, grid, s, b);
-  else launch_rows_vec<8>(vec, grid, s, b);
+  if (T == 64) hipLaunchKernelGGL(i8_rows_kernel<64>, dim3(grid), dim3(256), 0, s, b);
+  else if (T == 128) hipLaunchKernelGGL(i8_rows_kernel<128>, dim3(grid), dim3(256), 0, s, b);
+  else if (T == 256) hipLaunchKernelGGL(i8_rows_kernel<256>, dim3(grid), dim3(256), 0, s, b);
+  else hipLaunchKernelGGL(i8_rows_kernel<512>, dim3(grid), dim3(512), 0, s, b);
 }
 
 QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) {
@@ -394,8 +770,53 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
   p.m = (int)m;
   p.k = (int)k;
   p.steps = (int)(up(k, kI8Pad) / 32);
-  p.vec = (uintptr_t)x % 16 == 0 && k % 8 == 0;
   return p;
+}
+
+enum { kRouteGemv, kRouteStream, kRouteTile };
+struct I8Route {
+  int kind, rows, cols;  // of a workgroup's tile
+};
+
+I8Route pick_route(int n, const vkwr_i8_problem* p) {
+  bool gemv = true;
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    if (p[i].m == 0) continue;
+    gemv = gemv && p[i].m <= 4;
+    most = std::max(most, p[i].m);
+  }
+  for (int i = 0; i < n; ++i)
+    if (gemv && p[i].m > 0) gemv = (most == 1 ? 1 : most == 2 ? 2 : 4) * up(p[i].k, kI8Pad) <= kGemvMost;
+  if (gemv) return {kRouteGemv, 4, 32};
+  if (const char* e = getenv("I8R")) {
+    I8Route r;
+    sscanf(e, "%d,%d,%d", &r.kind, &r.rows, &r.cols);
+    return r;
+  }
+  if (most > 128) return {kRouteTile, 256, 256};
+  return {kRouteStream, 64, 64};
+}
+
+#define VK_I8_STREAM(tm, tn, nw, ks, nb) \
+  hipLaunchKernelGGL((i8_stream_kernel<tm, tn, nw, ks, nb>), dim3((unsigned)wgs), dim3(64 * nw), 0, s, b)
+#define VK_I8_TILE(tm, tn) hipLaunchKernelGGL((i8_tile_kernel<tm, tn>), dim3((unsigned)wgs), dim3(256), 0, s, b, wgs)
+
+void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) {
+  if (r.kind == kRouteTile) {
+    if (r.rows == 256) VK_I8_TILE(4, 4);
+    else if (r.rows == 192) VK_I8_TILE(3, 4);
+    else if (r.cols == 256) VK_I8_TILE(2, 4);
+    else VK_I8_TILE(2, 2);
+  } else if (r.rows == 32 && r.cols == 32) {
+    VK_I8_STREAM(1, 1, 8, 2, 4);
+  } else if (r.rows == 32) {
+    VK_I8_STREAM(1, 2, 8, 2, 4);
+  } else if (r.rows == 64) {
+    VK_I8_STREAM(2, 2, 8, 2, 4);
+  } else {
+    VK_I8_STREAM(4, 2, 4, 2, 3);
+  }
 }
 
 }  // namespace
@@ -404,7 +825,7 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 using namespace vk;
 
 extern "C" int64_t vkwr_i8_packed_bytes(int64_t rows, int64_t k) {
-  if (rows < 0 || rows > (1 << 24) || k < 1 || k > kI8MaxK) return -1;
+  if (rows < 0 || rows > kI8MaxRows || k < 1 || k > kI8MaxK) return -1;
   return packed_bytes(rows, k);
 }
 
@@ -478,11 +899,39 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
                  "%s: y of problem %d overlaps what problem %d reads or writes", fn, i, j);
     }
   }
+  const hipStream_t st = (hipStream_t)stream;
+  I8Route route = pick_route(n, p);
+  if (route.kind == kRouteGemv) {
+    GBatch gb{};
+    int64_t wgs = 0;
+    int most = 0;
+    for (int i = 0; i < n; ++i) {
+      if (p[i].m == 0) continue;
+      GProb& P = gb.p[gb.n++];
+      P.x = reinterpret_cast<const _Float16*>(p[i].x);
+      P.w = p[i].w;
+      P.t = p[i].w_scale;
+      P.bias = reinterpret_cast<const _Float16*>(p[i].bias);
+      P.y = reinterpret_cast<_Float16*>(p[i].y);
+      P.m = (int)p[i].m;
+      P.n = (int)p[i].n;
+      P.k = (int)p[i].k;
+      P.steps = (int)(up(p[i].k, kI8Pad) / 32);
+      P.epi = p[i].epilogue;
+      P.wg_begin = (int)wgs;
+      wgs += (p[i].n + 31) / 32;
+      most = std::max(most, P.m);
+    }
+    const dim3 grid((unsigned)wgs);
+    if (most == 1) hipLaunchKernelGGL(i8_gemv_kernel<1>, grid, dim3(512), 0, st, gb);
+    else if (most == 2) hipLaunchKernelGGL(i8_gemv_kernel<2>, grid, dim3(512), 0, st, gb);
+    else hipLaunchKernelGGL(i8_gemv_kernel<4>, grid, dim3(512), 0, st, gb);
+    return check_launch(fn);
+  }
   const I8Scratch c = scratch_of(n, p);
   char* const ws = static_cast<char*>(workspace);
   QBatch qb{};
   IBatch ib{};
-  constexpr int TM = 2, TN = 2;
   int64_t wgs = 0;
   for (int i = 0; i < n; ++i) {
     if (p[i].m == 0) continue;
@@ -501,14 +950,14 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
     P.steps = (int)(up(p[i].k, kI8Pad) / 32);
     P.epi = p[i].epilogue;
     P.vec = (uintptr_t)p[i].y % 16 == 0 && p[i].n % 8 == 0;
-    P.nmb = (P.m + 32 * TM - 1) / (32 * TM);
-    P.ncol = (P.n + 32 * TN - 1) / (32 * TN);
+    P.nmb = (P.m + route.rows - 1) / route.rows;
+    P.ncol = (P.n + route.cols - 1) / route.cols;
     P.wg_begin = (int)wgs;
-    wgs += (int64_t)P.nmb * P.ncol;
-    VK_REQUIRE(wgs < (1 << 23), "%s: too many tiles", fn);
+    wgs += (int64_t)P.nmb * (route.kind == kRouteStream ? up(P.ncol, 8) : P.ncol);
+    VK_REQUIRE(wgs < (1 << 22), "%s: too many tiles", fn);
   }
-  launch_rows(qb, (hipStream_t)stream);
+  launch_rows(qb, st);
   if (int e = check_launch(fn)) return e;
-  hipLaunchKernelGGL((i8_stream_kernel<TM, TN, 8, 2>), dim3((unsigned)wgs), dim3(512), 0, (hipStream_t)stream, ib);
+  launch_products(route, ib, (int)wgs, st);
   return check_launch(fn);
 }
