@@ -14,8 +14,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <stdlib.h>
-#include <stdio.h>
 
 #include "vk_capi.h"
 #include "vk_common.cuh"
@@ -475,11 +473,12 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
 // ---- many rows: tiles through LDS, bound by the matrix cores
 //
 // (64 TM) x (64 TN) outputs per workgroup, four waves of (32 TM) x (32 TN) in registers.  K advances
-// 128 per stage through two LDS buffers; both operands being in fragment order, a stage is a row of
+// 128 per stage through NBUF LDS buffers; both operands being in fragment order, a stage is a row of
 // 4 KiB pieces, copied straight to LDS, and read back lane by lane.  One barrier per stage, before the
 // last group of products, whose operands are then in registers: behind it the buffer is free and the copies of
-// the stage after next go out, one behind every other product of this and the next group, so
-// that they neither hold up the products nor arrive late.  The copies are written in assembly, as the compiler
+// the stage NBUF further go out, between the products of this and the next group, so
+// that they neither hold up the products nor arrive late.  NBUF: as many as fit (two 64 KiB stages of 256 x 256, four of
+// 128 x 128); two of 128 x 128 and two workgroups a CU took 46 us instead of 32 for K 8192, N 2048, m = 433.  The copies are written in assembly, as the compiler
 // would make every LDS read wait for all of them; the waits are placed here.
 template <int TM, int TN>
 struct I8Tile {
@@ -570,12 +569,12 @@ __device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&
   send(kStrips - 1);
 }
 
-template <int TM, int TN>
-__global__ __launch_bounds__(256, TM* TN > 4 ? 1 : 2) void i8_tile_kernel(IBatch bt, int tiles) {
+template <int TM, int TN, int NBUF>
+__global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
   using T = I8Tile<TM, TN>;
   constexpr int ND = T::kCopies, kHalf = ND / 2;
   constexpr int kOut = 4 * (2 * 32 * T::kOutRow + 2 * 32 * TN * 4);
-  constexpr int kRing = 2 * T::kBlocks * 1024;
+  constexpr int kBuf = T::kBlocks * 1024, kRing = NBUF * kBuf;
   static_assert(kOut <= kRing, "the outputs are staged where the operands were");
   __shared__ __attribute__((aligned(1024))) char sm[kRing];
   // workgroup b runs on XCD b % 8: each takes a contiguous range of tiles, in groups of 4 tile rows
@@ -610,16 +609,16 @@ __global__ __launch_bounds__(256, TM* TN > 4 ? 1 : 2) void i8_tile_kernel(IBatch
     const void *xb = uniform_ptr(px + k0), *wb = uniform_ptr(pw + k0);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
-      if (d >= d0 && d < d1) copy16(d < 2 * TM ? xb : wb, off[d], lds0 + buf * T::kBlocks * 1024 + d * 4096);
+      if (d >= d0 && d < d1) copy16(d < 2 * TM ? xb : wb, off[d], lds0 + buf * kBuf + d * 4096);
   };
   const char* const fxp = sm + wm * TM * 4096 + lane * 16;
   const char* const fwp = sm + (T::kX + wn * TN * 4) * 1024 + lane * 16;
   iv4 fx[2][TM], fw[2][TN];
   auto fread = [&](int buf, int kk, int set) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fx[set][i] = *reinterpret_cast<const iv4*>(fxp + buf * T::kBlocks * 1024 + (i * 4 + kk) * 1024);
+    for (int i = 0; i < TM; ++i) fx[set][i] = *reinterpret_cast<const iv4*>(fxp + buf * kBuf + (i * 4 + kk) * 1024);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fw[set][j] = *reinterpret_cast<const iv4*>(fwp + buf * T::kBlocks * 1024 + (j * 4 + kk) * 1024);
+    for (int j = 0; j < TN; ++j) fw[set][j] = *reinterpret_cast<const iv4*>(fwp + buf * kBuf + (j * 4 + kk) * 1024);
   };
   iv16 acc[TM][TN];
 #pragma unroll
@@ -655,19 +654,24 @@ __global__ __launch_bounds__(256, TM* TN > 4 ? 1 : 2) void i8_tile_kernel(IBatch
 #pragma unroll
         for (int q = 0; q < kHalf; ++q)
           if (q * TM * TN / kHalf == p)
-            copy16(d0 + q < 2 * TM ? xb : wb, off[d0 + q], lds0 + buf * T::kBlocks * 1024 + (d0 + q) * 4096);
+            copy16(d0 + q < 2 * TM ? xb : wb, off[d0 + q], lds0 + buf * kBuf + (d0 + q) * 4096);
         __builtin_amdgcn_sched_barrier(0);
       }
   };
-  copies(0, 0, 0, ND);
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  copies(1, 1, 0, kHalf);
+  // stage s + 1 has landed where all but the newest NBUF - 2 stages' copies have
+  auto landed = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * ND) : "memory");
+  };
+#pragma unroll
+  for (int u = 0; u < NBUF - 1; ++u) copies(u, u, 0, ND);
+  landed();
+  copies(NBUF - 1, NBUF - 1, 0, kHalf);
   fread(0, 0, 0);
-  int cur = 0;
+  int cur = 0, prev = NBUF - 1;
   for (int s = 0; s < ns; ++s) {
-    const int nxt = cur ^ 1;
+    const int nxt = cur + 1 == NBUF ? 0 : cur + 1;
     fread(cur, 1, 1);
-    products_copies(0, nxt, s + 1, kHalf);
+    products_copies(0, prev, s + NBUF - 1, kHalf);
     __builtin_amdgcn_sched_barrier(0);
     fread(cur, 2, 0);
     products(1);
@@ -675,11 +679,11 @@ __global__ __launch_bounds__(256, TM* TN > 4 ? 1 : 2) void i8_tile_kernel(IBatch
     fread(cur, 3, 1);
     products(0);
     __builtin_amdgcn_sched_barrier(0);
-    // stage s + 1 has landed and this stage is read, for every wave
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    landed();  // and this stage is read, for every wave
     fread(nxt, 0, 0);
-    products_copies(1, cur, s + 2, 0);
+    products_copies(1, cur, s + NBUF, 0);
     __builtin_amdgcn_sched_barrier(0);
+    prev = cur;
     cur = nxt;
   }
   // the last copies have landed and every wave's reads are done
@@ -773,49 +777,64 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
   return p;
 }
 
+// The tile that a batch runs with: the smallest whose workgroups fit the (256) CUs at once.  A second
+// round costs more than larger tiles that leave CUs idle, and larger tiles than that
+// leave bandwidth.  us of a whole call, this tile against its neighbours:
+//   32 x 32    K 8192, N 2048, m = 128   14.3; 32 x 64 16.7, 64 x 64 20.3
+//   32 x 64    K = N = 4096, m = 128     12.8; 32 x 32 13.7, 64 x 64 14.4
+//   64 x 64    K 2048, N 8192, m = 128   12.0; 32 x 64 13.5, 64 x 128 12.5
+//   64 x 128   K = N = 4096, m = 433     19.1; 64 x 64 24.3, 128 x 128 21.4
+//   128 x 128  K 8192, N 2048, m = 1100  36.0; 64 x 128 51.6, 128 x 256 51.6
+//   128 x 256  K = N = 4096, m = 1100    34.3; 128 x 128 43.4, 192 x 256 42.4
+//   192 x 256  K = N = 4096, m = 2304    51.9; 128 x 256 69.4, 256 x 256 58.3
+//   256 x 256  K = N = 4096, m = 4096    81.3; 192 x 256 98.9
+// Beyond one round of the largest: whichever of the last two takes less by its rounds, one of 192
+// rows counted as 0.77 (K 4096, N 16384, m = 2304: three rounds each, 160, 188; three of N 4096: 576 tiles
+// in three rounds 158, 432 in two 148).
+// Up to 32 rows per tile and up to 64 x 64, weights and rows go straight into registers (stream kernel).
 enum { kRouteGemv, kRouteStream, kRouteTile };
 struct I8Route {
   int kind, rows, cols;  // of a workgroup's tile
 };
+constexpr I8Route kI8Routes[] = {{kRouteStream, 32, 32}, {kRouteStream, 32, 64},  {kRouteStream, 64, 64}, {kRouteTile, 64, 128},
+                                 {kRouteTile, 128, 128}, {kRouteTile, 128, 256}, {kRouteTile, 192, 256}, {kRouteTile, 256, 256}};
 
 I8Route pick_route(int n, const vkwr_i8_problem* p) {
-  bool gemv = true;
   int64_t most = 0;
-  for (int i = 0; i < n; ++i) {
-    if (p[i].m == 0) continue;
-    gemv = gemv && p[i].m <= 4;
-    most = std::max(most, p[i].m);
-  }
+  for (int i = 0; i < n; ++i) most = std::max(most, p[i].m);
+  bool gemv = most <= 4;
   for (int i = 0; i < n; ++i)
     if (gemv && p[i].m > 0) gemv = (most == 1 ? 1 : most == 2 ? 2 : 4) * up(p[i].k, kI8Pad) <= kGemvMost;
   if (gemv) return {kRouteGemv, 4, 32};
-  if (const char* e = getenv("I8R")) {
-    I8Route r;
-    sscanf(e, "%d,%d,%d", &r.kind, &r.rows, &r.cols);
-    return r;
+  const int64_t cus = device_cus();
+  int64_t tiles[8];
+  for (int r = 0; r < 8; ++r) {
+    tiles[r] = 0;
+    for (int i = 0; i < n; ++i) tiles[r] += up(p[i].m, kI8Routes[r].rows) / kI8Routes[r].rows * (up(p[i].n, kI8Routes[r].cols) / kI8Routes[r].cols);
+    if (tiles[r] <= cus) return kI8Routes[r];
   }
-  if (most > 128) return {kRouteTile, 256, 256};
-  return {kRouteStream, 64, 64};
+  return kI8Routes[0.77 * (double)((tiles[6] + cus - 1) / cus) < (double)((tiles[7] + cus - 1) / cus) ? 6 : 7];
 }
 
-#define VK_I8_STREAM(tm, tn, nw, ks, nb) \
-  hipLaunchKernelGGL((i8_stream_kernel<tm, tn, nw, ks, nb>), dim3((unsigned)wgs), dim3(64 * nw), 0, s, b)
-#define VK_I8_TILE(tm, tn) hipLaunchKernelGGL((i8_tile_kernel<tm, tn>), dim3((unsigned)wgs), dim3(256), 0, s, b, wgs)
+#define VK_I8_STREAM(tm, tn, ks, nb) \
+  hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb>), dim3((unsigned)wgs), dim3(512), 0, s, b)
+#define VK_I8_TILE(tm, tn, nbuf) \
+  hipLaunchKernelGGL((i8_tile_kernel<tm, tn, nbuf>), dim3((unsigned)wgs), dim3(256), 0, s, b, wgs)
 
 void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) {
-  if (r.kind == kRouteTile) {
-    if (r.rows == 256) VK_I8_TILE(4, 4);
-    else if (r.rows == 192) VK_I8_TILE(3, 4);
-    else if (r.cols == 256) VK_I8_TILE(2, 4);
-    else VK_I8_TILE(2, 2);
-  } else if (r.rows == 32 && r.cols == 32) {
-    VK_I8_STREAM(1, 1, 8, 2, 4);
-  } else if (r.rows == 32) {
-    VK_I8_STREAM(1, 2, 8, 2, 4);
+  if (r.kind == kRouteStream) {
+    if (r.rows == 64) VK_I8_STREAM(2, 2, 4, 1);
+    else if (r.cols == 64) VK_I8_STREAM(1, 2, 2, 4);
+    else VK_I8_STREAM(1, 1, 2, 4);
   } else if (r.rows == 64) {
-    VK_I8_STREAM(2, 2, 8, 2, 4);
+    VK_I8_TILE(1, 2, 5);
+  } else if (r.rows == 128) {
+    if (r.cols == 128) VK_I8_TILE(2, 2, 4);
+    else VK_I8_TILE(2, 4, 3);
+  } else if (r.rows == 192) {
+    VK_I8_TILE(3, 4, 2);
   } else {
-    VK_I8_STREAM(4, 2, 4, 2, 3);
+    VK_I8_TILE(4, 4, 2);
   }
 }
 
@@ -900,7 +919,7 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
     }
   }
   const hipStream_t st = (hipStream_t)stream;
-  I8Route route = pick_route(n, p);
+  const I8Route route = pick_route(n, p);
   if (route.kind == kRouteGemv) {
     GBatch gb{};
     int64_t wgs = 0;
