@@ -9,42 +9,11 @@ import math
 import pytest
 import torch
 
+from oracle import beam_ref
 from vkwr_amd import capi
 
 pytestmark = pytest.mark.gpu
 INF = math.inf
-
-
-def ref_select(logits, scores, lengths, ended, end, alpha):
-    """The definition, beam by beam, in 64 bits."""
-    B, W, V = logits.shape
-    out = [[], [], [], [], []]
-    for b in range(B):
-        cands = []
-        for w in range(W):
-            s, n = float(scores[b, w]), int(lengths[b, w])
-            if not s > -INF:
-                continue
-            if ended[b, w]:
-                cands.append((s * max(n, 1) ** -alpha, w, end, s, n, 1))
-                continue
-            l = logits[b, w].double()
-            l = torch.where(l.isnan(), -INF, l)
-            top = float(l.max())
-            if top == -INF:
-                continue
-            d = torch.where(l == top, 0.0, l - top)
-            lp = d - torch.log(torch.exp(d).sum())
-            # the W best tokens of the beam, lowest index first among equals
-            for v in sorted(torch.topk(lp, min(V, 4 * W)).indices.tolist() + (lp == torch.sort(lp, descending=True).values[min(W, V) - 1]).nonzero()[:W, 0].tolist()):
-                x = float(lp[v])
-                if x > -INF:
-                    cands.append(((s + x) * max(n + 1, 1) ** -alpha, w, v, s + x, n + 1, int(v == end)))
-        cands = sorted(set(cands), key=lambda c: (-c[0], c[1], c[2]))[:W]
-        rows = [(c[2], c[1], c[3], c[4], c[5]) for c in cands] + [(-1, -1, -INF, 0, 1)] * (W - len(cands))
-        for o, r in zip(out, zip(*rows)):
-            o.append(list(r))
-    return [torch.tensor(o, dtype=torch.float64 if i == 2 else torch.int32) for i, o in enumerate(out)]
 
 
 def run(logits, scores, lengths, ended, end=-1, alpha=0.0, ws=None):
@@ -85,14 +54,14 @@ def inputs(B, W, V, half, seed, ended=0.0, banned=0.0):
                                    (4, 8, 5003), (2, 16, 16384), (1, 32, 40000), (5, 13, 1001), (1, 7, 131072), (17, 6, 2048)])
 def test_select(B, W, V, half):
     a = inputs(B, W, V, half, seed=B + W + V)
-    check(run(*a, end=min(2, V - 1)), ref_select(*a, min(2, V - 1), 0.0))
+    check(run(*a, end=min(2, V - 1)), beam_ref.select(*a, min(2, V - 1), 0.0))
 
 
 @pytest.mark.parametrize("alpha", [0.0, 0.6, 1.0, 2.5])
 @pytest.mark.parametrize("ended,banned", [(0.3, 0.0), (0.9, 0.5), (1.0, 0.0), (0.2, 0.999)])
 def test_finished_banned_and_length(alpha, ended, banned):
     a = inputs(6, 5, 3001, True, seed=int(10 * alpha), ended=ended, banned=banned)
-    check(run(*a, end=7, alpha=alpha), ref_select(*a, 7, alpha))
+    check(run(*a, end=7, alpha=alpha), beam_ref.select(*a, 7, alpha))
 
 
 def test_first_step_counts_one_beam():
@@ -102,7 +71,7 @@ def test_first_step_counts_one_beam():
     s[:, 0] = 0.0
     n.zero_()
     got = run(l, s, n, e)
-    check(got, ref_select(l, s, n, e, -1, 0.0))
+    check(got, beam_ref.select(l, s, n, e, -1, 0.0))
     assert (got[1] == 0).all()
 
 
@@ -116,7 +85,7 @@ def test_nothing_left():
     s[3, :] = -INF                   # dead beams
     s[4, 1] = float("nan")
     got = run(l, s, n, e)
-    check(got, ref_select(l, s, n, e, -1, 0.0))
+    check(got, beam_ref.select(l, s, n, e, -1, 0.0))
     assert (got[0][0] == -1).all() and (got[4][0] == 1).all() and (got[0][3] == -1).all()
     assert (got[1][1].cpu() == torch.tensor([0, 0, -1, -1])).all()
 
@@ -135,7 +104,7 @@ def test_ties(W, half):
     l = l.half() if half else l
     s, n, e = torch.full((4, W), -1.5), torch.full((4, W), 3, dtype=torch.int32), torch.zeros(4, W, dtype=torch.int32)
     got = run(l, s, n, e)
-    check(got, ref_select(l, s, n, e, -1, 0.0))
+    check(got, beam_ref.select(l, s, n, e, -1, 0.0))
 
 
 def test_lowest_value_and_infinities():
@@ -148,7 +117,7 @@ def test_lowest_value_and_infinities():
         l[2, 1, 77] = INF
         l[2, 1, 500] = INF
         got = run(l, s, n, e)
-        want = ref_select(l, s, n, e, -1, 0.0)
+        want = beam_ref.select(l, s, n, e, -1, 0.0)
         for i in (0, 1, 3, 4):
             assert torch.equal(got[i].cpu(), want[i])
         near = (got[2].cpu().double() - want[2]).abs() <= 2.0 ** -17 + want[2].abs() * 2.0 ** -24
@@ -168,38 +137,10 @@ def test_select_unaligned_logits():
     l, s, n, e = inputs(2, 3, 1024, True, seed=6)
     flat = torch.zeros(l.numel() + 1, dtype=torch.float16, device="cuda")
     flat[1:] = l.reshape(-1).cuda()
-    check(run(flat[1:].view(2, 3, 1024), s, n, e), ref_select(l, s, n, e, -1, 0.0))
+    check(run(flat[1:].view(2, 3, 1024), s, n, e), beam_ref.select(l, s, n, e, -1, 0.0))
 
 
 # ---------------------------------------------------------------- states
-
-def ref_reorder(slots, parents, skip, n_slots, pools):
-    pools = [p.clone() for p in pools]
-    new = []
-    moves = []
-    W = slots.shape[1]
-    for s, p, k in zip(slots.tolist(), parents.tolist(), skip.tolist()):
-        carry = [0 <= x < W and not y for x, y in zip(p, k)]
-        first = {}
-        for c in range(W):
-            if carry[c]:
-                first.setdefault(p[c], c)
-        left = [s[b] for b in range(W) if b not in first]
-        row = []
-        for c in range(W):
-            if carry[c] and first[p[c]] == c:
-                row.append(s[p[c]])
-            else:
-                row.append(left.pop(0))
-                if carry[c]:
-                    moves.append((s[p[c]], row[-1]))
-        new.append(row)
-    for pool in pools:
-        for a, b in moves:
-            if 0 <= a < n_slots and 0 <= b < n_slots:
-                pool[:, b] = pool[:, a]
-    return torch.tensor(new, dtype=torch.int32), pools
-
 
 def pools_of(layers, n_slots, C, seed, dev="cuda"):
     g = torch.Generator(device=dev).manual_seed(seed)
@@ -222,7 +163,7 @@ def test_reorder(B, W, layers, C):
             parents[-1] = torch.arange(W - 1, -1, -1, dtype=torch.int32)
         skip = (torch.rand(B, W, generator=g) < 0.3 * trial).to(torch.int32)
         pools = pools_of(layers, n_slots, C, seed=trial)
-        want, want_pools = ref_reorder(slots, parents, skip, n_slots, pools)
+        want, want_pools = beam_ref.reorder(slots, parents, skip, n_slots, pools)
         out = torch.full((B, W), -7, dtype=torch.int32, device="cuda")
         capi.beam_reorder(slots.cuda(), parents.cuda(), out, pools, skip=skip.cuda() if trial else None)
         assert torch.equal(out.cpu(), want)
@@ -236,7 +177,7 @@ def test_reorder_bad_slots_and_parents():
     pools = pools_of(2, 6, 64, seed=1)
     slots = torch.tensor([[0, 99, 2], [3, 4, -5]], dtype=torch.int32)
     parents = torch.tensor([[1, 1, 0], [0, 0, 77]], dtype=torch.int32)
-    want, want_pools = ref_reorder(slots, parents, torch.zeros_like(slots), 6, pools)
+    want, want_pools = beam_ref.reorder(slots, parents, torch.zeros_like(slots), 6, pools)
     out = torch.empty(2, 3, dtype=torch.int32, device="cuda")
     capi.beam_reorder(slots.cuda(), parents.cuda(), out, pools)
     assert torch.equal(out.cpu(), want)
@@ -285,4 +226,4 @@ def test_step_captured():
         step()
         for a, b in zip(got, (*out, new, *pools)):
             assert torch.equal(a, b)
-        check(got[:5], ref_select(l.cpu(), s.cpu(), n.cpu(), e.cpu(), 1, 0.5))
+        check(got[:5], beam_ref.select(l.cpu(), s.cpu(), n.cpu(), e.cpu(), 1, 0.5))

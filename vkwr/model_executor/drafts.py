@@ -31,9 +31,10 @@ class DraftEngine(MixedEngine):
     """Draft steps of up to `max_seqs` sequences of up to `max_draft` drafts; also a MixedEngine (prompts,
     plain decode steps) of max_seqs * (max_draft + 1) rows, or max_rows if that is more."""
 
-    def __init__(self, model, max_seqs, max_draft, max_rows=0, adapters=None):
+    def __init__(self, model, max_seqs, max_draft, max_rows=0, adapters=None, int8=None):
         self.draft_rows = max_seqs * (max_draft + 1)
-        super().__init__(model, max(max_rows, self.draft_rows), max_seqs=self.draft_rows, adapters=adapters)
+        super().__init__(model, max(max_rows, self.draft_rows), max_seqs=self.draft_rows, adapters=adapters,
+                         int8=int8)
         cfg, dev, R, C = model.cfg, model.head.device, self.draft_rows, model.cfg.n_embd
         self.max_draft, self.draft_seqs = max_draft, max_seqs
 
@@ -111,7 +112,7 @@ class DraftEngine(MixedEngine):
                 y = self.ys[0][l, :R]
                 capi.layer_norm(x, L["ln1_w"], L["ln1_b"], y, residual=res_in, x_out=None if first else res)
                 capi.token_shift(B, T, C, y, att[l], [L[k] for k in TMIX_MIX], [t[:R] for t in s.mix])
-                capi.gemm(self._proj(L, s.lw[l], R, first), ws)
+                self._run_proj(l, R)
                 if adapters is not None:
                     adapters.add(self.adapted_first[self.which ^ 1] if first else self.adapted[l]["rkv"])
                 capi.gemm(self._rank_out(L, s.lw[l], R, first), ws)
@@ -125,14 +126,14 @@ class DraftEngine(MixedEngine):
                                       pending_rows=rows)
                 capi.groupnorm_bonus_gate(R, 1, C, H, s.y[:R], s.r[:R], N["new_k"][:R], v, L["r_k"], L["lnx_w"],
                                           L["lnx_b"], s.g[:R], s.o_in[:R])
-                capi.gemm([capi.gemm_problem(s.o_in[:R], L["Wo"], s.o[:R])], ws)
+                self._linear(l, "Wo", s.o_in[:R], s.o[:R])
                 if adapters is not None:
                     adapters.add(self.adapted[l]["o"])
                 res2 = s.res[0][:R]
                 y = self.ys[1][l, :R]
                 capi.layer_norm(s.o[:R], L["ln2_w"], L["ln2_b"], y, residual=res, x_out=res2)
                 capi.token_shift(B, T, C, y, ffn[l], [L["x_k_ffn"]], [s.xk[:R]])
-                self._ffn(l, L, R, adapters)
+                self._ffn(l, R, adapters)
                 x, res_in = s.ffn[:R], res2
         finally:
             s.w, s.v_first, s.v_new = own

@@ -34,12 +34,16 @@ With `adapters` (adapters.py) each sequence of a step may have a low-rank adapte
 shared projections: x A^T B^T is added to r, k, v before the low-rank outputs, to o, to the FFN key before
 the squared ReLU (which the adapters' launch then applies) and to the FFN value.
 
+With `int8` (int8.py) the large projections named there run on 8-bit weights (vkwr_linear_i8_f16); the
+others, the low-rank projections and the head run as they do without.
+
 Every buffer is preallocated for `max_rows` rows, so a step allocates nothing.
 """
 import torch
 
 from vkwr_amd import capi
 from vkwr.model_executor.adapters import AdapterStep
+from vkwr.model_executor.int8 import Int8Step
 from vkwr.model_executor.rwkv7 import HEAD
 
 TMIX_MIX = ("x_r", "x_w", "x_k", "x_v", "x_a", "x_g")
@@ -63,7 +67,7 @@ def _pad_rank(w1, w2, r):
 class MixedEngine:
     """Forward step over up to `max_rows` rows in decode and prefill groups."""
 
-    def __init__(self, model, max_rows, max_seqs=None, adapters=None):
+    def __init__(self, model, max_rows, max_seqs=None, adapters=None, int8=None):
         cfg = model.cfg
         self.model, self.cfg, self.max_rows = model, cfg, max_rows
         self.max_seqs = max_seqs or max_rows
@@ -98,6 +102,7 @@ class MixedEngine:
         self.ffn = buf(R, C)
         self.h = buf(self.max_seqs, C)
         self.logits = buf(self.max_seqs, cfg.vocab)
+        self.int8 = None if int8 is None else Int8Step(int8, cfg, max_rows, dev)
         # GEMM workspace: the largest need of any launch at any row count a step can have
         # (the plan is not monotone in the row count, so every count is evaluated).
         need = max(capi.gemm_workspace_bytes_upto(ps) for ps in self._gemm_batches(max_rows, 1))
@@ -116,15 +121,38 @@ class MixedEngine:
             self.adapted = [self._adapted(l) for l in range(cfg.n_layer)]
 
     # -- GEMM batches (shared by planning and execution)
+    def _is_int8(self, name):
+        return self.int8 is not None and self.int8.has(name)
+
+    def _rkv(self, R, first):
+        """(name, input, output) of the time mix's large projections."""
+        s = self
+        return [("Wr", s.mix[0][:R], s.r[:R]), ("Wk", s.mix[2][:R], s.k[:R]),
+                ("Wv", s.mix[3][:R], (s.v_first if first else s.v)[:R])]
+
     def _proj(self, L, W, R, first):
+        """The fp16 projections of the time mix's inputs."""
         s, gp = self, capi.gemm_problem
-        ps = [gp(s.mix[0][:R], L["Wr"], s.r[:R]), gp(s.mix[2][:R], L["Wk"], s.k[:R]),
-              gp(s.mix[3][:R], L["Wv"], (s.v_first if first else s.v)[:R]),
-              gp(s.mix[1][:R], W["w1"], s.w1[:R], epilogue=capi.EPI_TANH), gp(s.mix[4][:R], W["a1"], s.a1[:R]),
-              gp(s.mix[5][:R], W["g1"], s.g1[:R], epilogue=capi.EPI_SIGMOID)]
+        ps = [gp(x, L[n], y) for n, x, y in self._rkv(R, first) if not self._is_int8(n)]
+        ps += [gp(s.mix[1][:R], W["w1"], s.w1[:R], epilogue=capi.EPI_TANH), gp(s.mix[4][:R], W["a1"], s.a1[:R]),
+               gp(s.mix[5][:R], W["g1"], s.g1[:R], epilogue=capi.EPI_SIGMOID)]
         if not first:
             ps.append(gp(s.mix[3][:R], W["v1"], s.v1[:R]))
         return ps
+
+    def _run_proj(self, l, R):
+        first = l == 0
+        items = [t for t in self._rkv(R, first) if self._is_int8(t[0])]
+        if items:
+            self.int8.run(l, items)
+        capi.gemm(self._proj(self.model.layers[l], self.lw[l], R, first), self.ws)
+
+    def _linear(self, l, name, x, y, epilogue=capi.EPI_NONE):
+        """One large projection, in 8 bits or in 16."""
+        if self._is_int8(name):
+            self.int8.run(l, [(name, x, y)], epilogue)
+        else:
+            capi.gemm([capi.gemm_problem(x, self.model.layers[l][name], y, epilogue=epilogue)], self.ws)
 
     def _rank_out(self, L, W, R, first):
         """The low-rank output GEMMs.  Their inputs tanh(w1) and sigmoid(g1) come activated
@@ -148,9 +176,9 @@ class MixedEngine:
         for l, L in enumerate(m.layers[:max(nl, 2)]):
             out += [self._proj(L, self.lw[l], R, l == 0), self._rank_out(L, self.lw[l], R, l == 0)]
         L = m.layers[-1]
-        out += [[gp(s.o_in[:R], L["Wo"], s.o[:R])],
-                [gp(s.xk[:R], L["key"], s.act[:R], epilogue=capi.EPI_RELU_SQUARE)],
-                [gp(s.act[:R], L["value"], s.ffn[:R])]]
+        one = {"Wo": (s.o_in, s.o, capi.EPI_NONE), "key": (s.xk, s.act, capi.EPI_RELU_SQUARE),
+               "value": (s.act, s.ffn, capi.EPI_NONE)}
+        out += [[gp(x[:R], L[n], y[:R], epilogue=e)] for n, (x, y, e) in one.items() if not self._is_int8(n)]
         return out
 
     def _wkv_gn(self, groups, pool, v, L):
@@ -205,15 +233,14 @@ class MixedEngine:
         self.adapters.begin([(B, T, r0, q0) for B, T, r0, _, q0 in groups], adapter_ids)
         return self.adapters
 
-    def _ffn(self, l, L, R, adapters):
+    def _ffn(self, l, R, adapters):
         """relu(xk K^T)^2 V^T of the rows, into ffn."""
-        s, gp = self, capi.gemm_problem
-        square = capi.EPI_RELU_SQUARE
+        s = self
         late = adapters is not None and self.adapted[l]["key"] is not None  # the square follows the adapters
-        capi.gemm([gp(s.xk[:R], L["key"], s.act[:R], epilogue=capi.EPI_NONE if late else square)], s.ws)
+        self._linear(l, "key", s.xk[:R], s.act[:R], capi.EPI_NONE if late else capi.EPI_RELU_SQUARE)
         if late:
             adapters.add(self.adapted[l]["key"])
-        capi.gemm([gp(s.act[:R], L["value"], s.ffn[:R])], s.ws)
+        self._linear(l, "value", s.act[:R], s.ffn[:R])
         if adapters is not None:
             adapters.add(self.adapted[l]["value"])
 
@@ -259,7 +286,7 @@ class MixedEngine:
             # ---- time mix: res = x + res_in, LN1 and the six lerps against the shift pool
             capi.layer_norm_shift_rows(x, L["ln1_w"], L["ln1_b"], res, [L[k] for k in TMIX_MIX],
                                        [t[:R] for t in s.mix], state.att_shift[l], shift_groups, residual=res_in)
-            capi.gemm(self._proj(L, s.lw[l], R, first), ws)
+            self._run_proj(l, R)
             if adapters is not None:
                 adapters.add(self.adapted[l]["rkv"])
             capi.gemm(self._rank_out(L, s.lw[l], R, first), ws)
@@ -267,14 +294,14 @@ class MixedEngine:
             capi.kk_a_gate(R, 1, C, H, s.k[:R], L["k_k"], L["a0"], s.a12[:R], L["k_a"], s.new_k[:R],
                            s.neg_kk[:R], s.kka[:R])
             self._wkv_gn(groups, state.wkv[l], v, L)
-            capi.gemm([capi.gemm_problem(s.o_in[:R], L["Wo"], s.o[:R])], ws)
+            self._linear(l, "Wo", s.o_in[:R], s.o[:R])
             if adapters is not None:
                 adapters.add(self.adapted[l]["o"])
             # ---- channel mix
             res2 = s.res[0][:R]
             capi.layer_norm_shift_rows(s.o[:R], L["ln2_w"], L["ln2_b"], res2, [L["x_k_ffn"]], [s.xk[:R]],
                                        state.ffn_shift[l], shift_groups, residual=res)
-            self._ffn(l, L, R, adapters)
+            self._ffn(l, R, adapters)
             x, res_in = s.ffn[:R], res2
         for B, T, r0, _, q0 in groups:
             n = B * T

@@ -726,6 +726,14 @@ def linear_i8_workspace_bytes(problems):
     return n
 
 
+def linear_i8_scratch_bytes(m, k):
+    """What one problem of m rows and K = k adds to the workspace of `linear_i8`, whatever its weights."""
+    n = _linear_i8_ws(1, _I8_ARRAYS[1](I8Problem(None, None, None, None, None, m, 1, k, EPI_NONE)))
+    if n < 0:
+        raise ValueError(f"linear_i8: bad size m={m} k={k}")
+    return n
+
+
 def linear_i8(problems, workspace=None):
     """1..8 linear layers with 8-bit weights (vkwr_linear_i8_f16).  workspace: uint8,
     linear_i8_workspace_bytes (None: allocated)."""
