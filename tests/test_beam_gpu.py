@@ -193,6 +193,15 @@ def test_reorder_without_pools():
     assert out.tolist() == [[0, 4, 1]]
 
 
+def test_reorder_refuses_pools_of_different_slots():
+    slots = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    a, b = torch.zeros(2, 3, 4, device="cuda"), torch.zeros(2, 4, 4, device="cuda")
+    with pytest.raises(ValueError, match="pool 1"):
+        capi.beam_reorder(slots, slots, slots.clone(), [a, b])
+    with pytest.raises(TypeError):
+        capi.beam_reorder(slots, slots, slots.clone(), [a.transpose(0, 2)])
+
+
 def test_step_captured():
     """Selection and reordering in one graph, replayed with eager work between: every replay as the eager calls."""
     B, W, V, n_slots = 3, 4, 9000, 14

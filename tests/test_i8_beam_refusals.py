@@ -119,8 +119,11 @@ def test_reorder_refuses(change, text):
 
 def test_reorder_sizes():
     assert reorder(B=0) == 0
-    with pytest.raises(ValueError, match="pool 1"):
-        capi.beam_reorder(torch.zeros(1, 2, dtype=torch.int32), None, None, [torch.zeros(2, 3, 4), torch.zeros(2, 4, 4)])
+    slots = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="at most"):
+        capi.beam_reorder(slots, None, None, [torch.zeros(2, 3, 4)] * 9)
+    with pytest.raises(TypeError, match="pool"):
+        capi.beam_reorder(slots, slots, slots, [torch.zeros(2, 3, 4)])
 
 
 def test_python_refuses():

@@ -779,20 +779,25 @@ def beam_select(logits, scores, lengths, ended, tokens, parents, scores_out, len
                         at(workspace, torch.uint8, nbytes, "workspace"), nbytes, at.stream()), "vkwr_beam_select")
 
 
+MAX_BEAM_POOLS = 8
+_BEAM_POOLS = [BeamPool * max(n, 1) for n in range(MAX_BEAM_POOLS + 1)]
+
+
 def beam_reorder(slots, parents, slots_out, pools, skip=None):
     """States follow their beams (vkwr_beam_reorder): slots, parents, skip and slots_out [B, W] int32; pools:
     up to 8 tensors [layers, n_slots, ...], whose entries for the beams' slots are copied where a beam has
     more than one child."""
     B, W = slots.shape
     at, i32, n = _Tensors(), torch.int32, B * W
+    if len(pools) > MAX_BEAM_POOLS:
+        raise ValueError(f"beam_reorder: {len(pools)} pools, at most {MAX_BEAM_POOLS}")
     n_slots = pools[0].shape[1] if pools else 0
-    for i, t in enumerate(pools):
-        if t.dim() < 2 or t.shape[1] != n_slots:
-            raise ValueError(f"beam_reorder: pool {i} {tuple(t.shape)} is not [layers, {n_slots}, ...]")
-    arr = (BeamPool * max(len(pools), 1))()
-    for i, t in enumerate(pools):
-        size = t.numel() * t.element_size()
-        arr[i] = BeamPool(at(t, t.dtype, t.numel(), f"pool {i}"), t.shape[0], size // max(t.shape[0] * n_slots, 1))
+    arr = []
+    for t in pools:
+        shape = t.shape
+        if len(shape) < 2 or shape[1] != n_slots:
+            raise ValueError(f"beam_reorder: pool {len(arr)} {tuple(shape)} is not [layers, {n_slots}, ...]")
+        arr.append((at(t, t.dtype, t.numel(), "pool"), shape[0], t.nbytes // max(shape[0] * n_slots, 1)))
     _check(_beam_reorder(B, W, n_slots, at(slots, i32, n, "slots"), at(parents, i32, n, "parents"),
-                         at.optional(skip, i32, n, "skip"), at(slots_out, i32, n, "slots_out"), len(pools), arr,
-                         at.stream()), "vkwr_beam_reorder")
+                         None if skip is None else at(skip, i32, n, "skip"), at(slots_out, i32, n, "slots_out"), len(arr),
+                         _BEAM_POOLS[len(arr)](*arr), at.stream()), "vkwr_beam_reorder")

@@ -310,24 +310,33 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
       if (u * kMergeThreads + tid < n) keys[u * kMergeThreads + tid] = kr[u];
     __syncthreads();
     if (tid >= kRankThreads) {
-      if (w0 == 0 && tid - kRankThreads < W) {
-        const int w = tid - kRankThreads;
-        const bool over = live[w] == 2;
-        if (live[w] == 1) {
+      if (w0 == 0) {
+        const int lane = tid - kRankThreads;
+        // a group's sum relative to the row's maximum, a lane each, then a row's, a lane each
+        for (int i = lane; i < W * G; i += 64) {
+          const int w = i / G;
           float mx = kNone;
 #pragma unroll 8
           for (int g = 0; g < G; ++g) mx = fmaxf(mx, gmax[w * G + g]);
-          double sum = 0.0;
-          for (int g = 0; g < G; ++g) {
-            const float m = gmax[w * G + g];
-            if (m > kNone) sum += m == mx ? gsum[w * G + g] : gsum[w * G + g] * exp64((double)m - (double)mx);
-          }
-          rmax[w] = mx;
-          // (where not one token is allowed there are no keys either)
-          if (mx > kNone) base[w] -= log64(sum);
+          const float m = gmax[i];
+          // (a row that offers nothing has what the workspace held: it is not used)
+          gsum[i] = m == mx ? gsum[i] : m > kNone ? gsum[i] * exp64((double)m - (double)mx) : 0.0;
+          if (i == w * G) rmax[w] = mx;
         }
-        const int len = len0[w] + (over ? 0 : 1);
-        factor[w] = a.alpha == 0.0f || len <= 1 ? 1.0 : exp64(-(double)a.alpha * log64((double)len));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (lane < W) {
+          const int w = lane;
+          const bool over = live[w] == 2;
+          if (live[w] == 1 && rmax[w] > kNone) {  // (where not one token is allowed there are no keys either)
+            double sum = 0.0;
+#pragma unroll 8
+            for (int g = 0; g < G; ++g) sum += gsum[w * G + g];
+            base[w] -= log64(sum);
+          }
+          const int len = len0[w] + (over ? 0 : 1);
+          factor[w] = a.alpha == 0.0f || len <= 1 ? 1.0 : exp64(-(double)a.alpha * log64((double)len));
+        }
       }
     } else {
       for (int i = tid; i < n; i += kRankThreads) {
