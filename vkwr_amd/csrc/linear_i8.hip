@@ -201,7 +201,7 @@ struct IProb {
   const _Float16* bias;
   _Float16* y;
   int m, n, steps;
-  int epi, vec;          // vec: rows of y are 16-byte aligned
+  int epi;
   int nmb, ncol;         // row and column tiles
   int wg_begin;
 };
@@ -225,8 +225,21 @@ __device__ __forceinline__ _Float16 i8_finish(int a, float s, float t, int epi, 
   return f16_of(i8_act(epi, f));
 }
 
+// Up to eight outputs of a row, in one store where there are eight (of any alignment).
+typedef _Float16 __attribute__((address_space(1)))* gptr;
+__device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
+  typedef hv8 __attribute__((aligned(2))) hv8u;
+  if (left >= 8) {
+    *reinterpret_cast<__attribute__((address_space(1))) hv8u*>(o) = h;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) o[e] = h[e];
+  }
+}
+
 // Eight consecutive outputs of a row.
-__device__ __forceinline__ void i8_finish8(const int (&a)[8], int row, int col, int m, int n, int epi, int vec, float s,
+__device__ __forceinline__ void i8_finish8(const int (&a)[8], int row, int col, int m, int n, int epi, float s,
                                            const float* t, const _Float16* bias, _Float16* y) {
   if (row >= m || col >= n) return;
   hv8 h;
@@ -235,14 +248,7 @@ __device__ __forceinline__ void i8_finish8(const int (&a)[8], int row, int col, 
     const int c = col + e < n ? col + e : n - 1;
     h[e] = i8_finish(a[e], s, t[c], epi, epi == VKWR_GEMM_EPI_BIAS ? (float)bias[c] : 0.0f);
   }
-  _Float16* const o = y + (int64_t)row * n + col;
-  if (vec) {
-    *reinterpret_cast<hv8*>(o) = h;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (col + e < n) o[e] = h[e];
-  }
+  store8((gptr)(y + (int64_t)row * n + col), h, n - col);
 }
 
 // (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
@@ -337,7 +343,7 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
     }
     const int row = (mb * TM + t / TN) * 32 + r, col = (cb * TN + t % TN) * 32 + 8 * g;
     const int a[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    if (row < P.m) i8_finish8(a, row, col, P.m, P.n, P.epi, P.vec, P.s[row], P.t, P.bias, P.y);
+    if (row < P.m) i8_finish8(a, row, col, P.m, P.n, P.epi, P.s[row], P.t, P.bias, P.y);
   }
 }
 
@@ -503,12 +509,13 @@ template <int TM, int TN, int kEpi>
 __device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&acc)[TM][TN], int row0, int col0, int lane) {
   constexpr int kRow = I8Tile<TM, TN>::kOutRow, kBuf = 32 * kRow;
   const int lr = lane & 31, lh = lane >> 5, r8 = lane >> 3, c8 = 8 * (lane & 7);
-  typedef _Float16 __attribute__((address_space(1)))* gptr;
-  int m = P.m, n = P.n, vec = P.vec;
+  int m = P.m, n = P.n;
   gptr y = (gptr)P.y;
-  const float *sp = P.s, *tp = P.t;
-  const _Float16* bp = P.bias;
-  asm("" : "+s"(m), "+s"(n), "+s"(vec), "+s"(y), "+s"(sp), "+s"(tp), "+s"(bp));
+  // (global address-space pointers, so that the accesses stay global, not flat, ones)
+  typedef const float __attribute__((address_space(1)))* gcf;
+  gcf sp = (gcf)P.s, tp = (gcf)P.t;
+  const _Float16 __attribute__((address_space(1)))* bp = (const _Float16 __attribute__((address_space(1)))*)P.bias;
+  asm("" : "+s"(m), "+s"(n), "+s"(y), "+s"(sp), "+s"(tp), "+s"(bp));
   // the columns' scales (and biases) behind the two strips
   float* const tl = reinterpret_cast<float*>(st + 2 * kBuf);
 #pragma unroll
@@ -550,14 +557,7 @@ __device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&
       const hv8 v = *reinterpret_cast<const hv8*>(o + 8 * h * kRow);
       const int row = row0 + 32 * i + 8 * h + r8;
       if (row >= m || col >= n) continue;
-      gptr d = y + (int64_t)row * n + col;
-      if (vec) {
-        *reinterpret_cast<__attribute__((address_space(1))) hv8*>(d) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (col + e < n) d[e] = v[e];
-      }
+      store8(y + (int64_t)row * n + col, v, n - col);
     }
   };
   write(0);
@@ -968,7 +968,6 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
     P.n = (int)p[i].n;
     P.steps = (int)(up(p[i].k, kI8Pad) / 32);
     P.epi = p[i].epilogue;
-    P.vec = (uintptr_t)p[i].y % 16 == 0 && p[i].n % 8 == 0;
     P.nmb = (P.m + route.rows - 1) / route.rows;
     P.ncol = (P.n + route.cols - 1) / route.cols;
     P.wg_begin = (int)wgs;
