@@ -112,14 +112,15 @@ __device__ __forceinline__ iv4 quant16(const uv4 (&v)[2], float top, float inv) 
   return o;
 }
 
-// T lanes per row, 256 / T rows per workgroup (T = 512: one row): so many that a lane holds at most 32 values
-// and a few hundred rows reach every CU (one wave per row: 433 rows of 8192 9.0 us).  The 32 rows of
+// T lanes per row, 256 / T rows per workgroup (T = 512: one row): so many that a lane holds 16 values, or 32 of
+// rows past 4096, and a few hundred rows reach every CU (us: 128 rows of 2048 3.1, with 32 a lane 3.3; 433 of
+// 8192 4.8, one wave per row 9.0; 2304 of 4096 9.0, of 16384 28 at 4.1 TB/s).  The 32 rows of
 // a block go to one XCD (workgroup b runs on XCD b % 8), whose L2 joins the 16-byte pieces that they
-// write into common lines.  Rows longer than 32 T are read twice.  |x| is compared as an integer, where an
+// write into common lines.  Rows longer than 16384 are read twice.  |x| is compared as an integer, where an
 // infinity or a NaN exceeds every number: such a row gets the scale NaN and zeros.
-template <int T>
+template <int T, int kKeep>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void i8_rows_kernel(QBatch bt) {
-  constexpr int kThreads = T < 256 ? 256 : T, kRows = kThreads / T, kWaves = T / 64, kKeep = 2;
+  constexpr int kThreads = T < 256 ? 256 : T, kRows = kThreads / T, kWaves = T / 64;
   __shared__ uint32_t wtop[kThreads / 64];
   int pi = 0;
 #pragma unroll
@@ -753,17 +754,18 @@ I8Scratch scratch_of(int n, const vkwr_i8_problem* p) {
 void launch_rows(QBatch& b, hipStream_t s) {
   int most = 0;
   for (int i = 0; i < b.n; ++i) most = std::max(most, b.p[i].steps);
-  const int T = most <= 64 ? 64 : most <= 128 ? 128 : most <= 256 ? 256 : 512;  // lanes per row
+  const int T = most <= 32 ? 64 : most <= 64 ? 128 : most <= 256 ? 256 : 512;  // lanes per row
   unsigned grid = 0;
   for (int i = 0; i < b.n; ++i) {
     b.p[i].wg_begin = (int)grid;
     grid += (unsigned)up((b.p[i].m + 31) / 32, 8) * 32 / std::max(1, 256 / T);
   }
   if (grid == 0) return;
-  if (T == 64) hipLaunchKernelGGL(i8_rows_kernel<64>, dim3(grid), dim3(256), 0, s, b);
-  else if (T == 128) hipLaunchKernelGGL(i8_rows_kernel<128>, dim3(grid), dim3(256), 0, s, b);
-  else if (T == 256) hipLaunchKernelGGL(i8_rows_kernel<256>, dim3(grid), dim3(256), 0, s, b);
-  else hipLaunchKernelGGL(i8_rows_kernel<512>, dim3(grid), dim3(512), 0, s, b);
+  if (T == 64) hipLaunchKernelGGL((i8_rows_kernel<64, 1>), dim3(grid), dim3(256), 0, s, b);
+  else if (T == 128) hipLaunchKernelGGL((i8_rows_kernel<128, 1>), dim3(grid), dim3(256), 0, s, b);
+  else if (most <= 128) hipLaunchKernelGGL((i8_rows_kernel<256, 1>), dim3(grid), dim3(256), 0, s, b);
+  else if (T == 256) hipLaunchKernelGGL((i8_rows_kernel<256, 2>), dim3(grid), dim3(256), 0, s, b);
+  else hipLaunchKernelGGL((i8_rows_kernel<512, 2>), dim3(grid), dim3(512), 0, s, b);
 }
 
 QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) {
