@@ -385,12 +385,6 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int steps = P.steps, k = P.k, kpad = steps * 32;
   const int8_t* const w = P.w + (int64_t)cb * steps * 1024 + lane * 16;
-  iv4 fw[kAhead];
-#pragma unroll
-  for (int a = 0; a < kAhead; ++a) {
-    const int st = min(wave + a * kWaves, steps - 1);
-    fw[a] = *reinterpret_cast<const iv4*>(w + (int64_t)st * 1024);
-  }
   // ---- this wave's pieces of 8 values of its row
   const int row = min(wave / kPer, P.m - 1), w0 = wave % kPer, pieces = kpad / 8;
   const _Float16* const x = P.x + (int64_t)row * k;
@@ -401,6 +395,15 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
     const int c = (i * kPer + w0) * 64 + lane;
     v[i] = load8(x, (int64_t)c * 8, k);
   }
+  // (behind the row, whose values are waited for first: loads come back in order)
+  __builtin_amdgcn_sched_barrier(0);
+  iv4 fw[kAhead];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    const int st = min(wave + a * kWaves, steps - 1);
+    fw[a] = *reinterpret_cast<const iv4*>(w + (int64_t)st * 1024);
+  }
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < kGemvKeep; ++i)
 #pragma unroll
