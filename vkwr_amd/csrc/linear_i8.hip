@@ -39,6 +39,20 @@ __device__ __forceinline__ int64_t i8_index(int64_t r, int64_t k, int64_t steps)
   return ((r >> 5) * steps + (k >> 5)) * 1024 + (((k >> 4) & 1) * 32 + (r & 31)) * 16 + (k & 15);
 }
 
+// The problem that workgroup b belongs to; a call of one problem is compiled without the search, and the
+// kernels that live for a few microseconds read all of its fields in one round of loads (an empty asm holds
+// them above the first branch): left alone the compiler reads each where it is used, one trip after another.
+template <bool kMulti, typename Batch>
+__device__ __forceinline__ int problem_of(const Batch& bt, int b) {
+  int pi = 0;
+  if constexpr (kMulti) {
+#pragma unroll
+    for (int i = 1; i < kMaxI8; ++i)
+      if (i < bt.n && b >= bt.p[i].wg_begin) pi = i;
+  }
+  return pi;
+}
+
 // ---------------------------------------------------------------- rounding rows to 8 bits
 
 struct QProb {
@@ -118,15 +132,12 @@ __device__ __forceinline__ iv4 quant16(const uv4 (&v)[2], float top, float inv) 
 // a block go to one XCD (workgroup b runs on XCD b % 8), whose L2 joins the 16-byte pieces that they
 // write into common lines.  Rows longer than 16384 are read twice.  |x| is compared as an integer, where an
 // infinity or a NaN exceeds every number: such a row gets the scale NaN and zeros.
-template <int T, int kKeep>
+template <int T, int kKeep, bool kMulti>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void i8_rows_kernel(QBatch bt) {
   constexpr int kThreads = T < 256 ? 256 : T, kRows = kThreads / T, kWaves = T / 64;
   __shared__ uint32_t wtop[kThreads / 64];
-  int pi = 0;
-#pragma unroll
-  for (int i = 1; i < kMaxI8; ++i)
-    if (i < bt.n && (int)blockIdx.x >= bt.p[i].wg_begin) pi = i;
-  const QProb& P = bt.p[pi];
+  const QProb P = bt.p[problem_of<kMulti>(bt, blockIdx.x)];
+  asm volatile("" ::"s"(P.x), "s"(P.q), "s"(P.s), "s"(P.m), "s"(P.k), "s"(P.steps), "s"(P.wg_begin));
   const int u = (int)blockIdx.x - P.wg_begin, per = 32 / kRows;  // workgroups of a block of rows
   const int idx = u >> 3;
   const int64_t row = ((int64_t)(idx / per) * 8 + (u & 7)) * 32 + idx % per * kRows + threadIdx.x / T;
@@ -211,19 +222,30 @@ struct IBatch {
   IProb p[kMaxI8];
 };
 
-__device__ __forceinline__ float i8_act(int epi, float v) {
-  if (epi == VKWR_GEMM_EPI_RELU_SQUARE) return v > 0.0f ? v * v : (v != v ? v : 0.0f);  // NaN stays
-  if (epi == VKWR_GEMM_EPI_TANH) return tanhf(v);
-  if (epi == VKWR_GEMM_EPI_SIGMOID) return sigmoidf(v);
-  return v;
-}
-
-// One output: the sum scaled in fp32, the epilogue, one rounding to fp16.  Every kernel finishes its sums
-// here, so that a row's bits do not depend on which one ran.
-__device__ __forceinline__ _Float16 i8_finish(int a, float s, float t, int epi, float bias) {
-  float f = (float)a * (s * t);
-  if (epi == VKWR_GEMM_EPI_BIAS) f += bias;
-  return f16_of(i8_act(epi, f));
+// N outputs: the sums scaled in fp32 (+ bias), the epilogue, one rounding to fp16.  Every kernel finishes its
+// sums here, so that a row's bits do not depend on which one ran.  One branch for all N: with one for
+// each, the code of the functions lay N times between the outputs.
+template <int N, typename H>
+__device__ __forceinline__ void i8_finish(const int (&a)[N], float s, const float (&t)[N], int epi, const float (&bias)[N],
+                                          H& h) {
+  float f[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) f[e] = (float)a[e] * (s * t[e]);
+  if (epi == VKWR_GEMM_EPI_RELU_SQUARE) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = f[e] > 0.0f ? f[e] * f[e] : (f[e] != f[e] ? f[e] : 0.0f);  // NaN stays
+  } else if (epi == VKWR_GEMM_EPI_BIAS) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] += bias[e];
+  } else if (epi == VKWR_GEMM_EPI_TANH) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = tanhf(f[e]);
+  } else if (epi == VKWR_GEMM_EPI_SIGMOID) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = sigmoidf(f[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) h[e] = f16_of(f[e]);
 }
 
 // Up to eight outputs of a row, in one store where there are eight (of any alignment).
@@ -239,37 +261,37 @@ __device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
   }
 }
 
-// Eight consecutive outputs of a row.
-__device__ __forceinline__ void i8_finish8(const int (&a)[8], int row, int col, int m, int n, int epi, float s,
-                                           const float* t, const _Float16* bias, _Float16* y) {
-  if (row >= m || col >= n) return;
-  hv8 h;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = col + e < n ? col + e : n - 1;
-    h[e] = i8_finish(a[e], s, t[c], epi, epi == VKWR_GEMM_EPI_BIAS ? (float)bias[c] : 0.0f);
-  }
-  store8((gptr)(y + (int64_t)row * n + col), h, n - col);
-}
-
 // (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
 // KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
 // tiles are added through LDS.
-template <int TM, int TN, int NW, int KS, int NB>
+template <int TM, int TN, int NW, int KS, int NB, bool kMulti>
 __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
-  constexpr int kTiles = TM * TN, kG = 65;  // 16-byte cells of a group of 4 results: 64 lanes and one of padding
+  constexpr int kTiles = TM * TN, kG = 64 + 4 / TN;  // 16-byte cells of a group of 4 results, padded: reads hit all banks
+  static_assert(kTiles * 128 <= NW * 64, "one piece of the output per thread");
   __shared__ __attribute__((aligned(16))) iv4 red[NW * kTiles * 4 * kG];
-  int pi = 0;
-#pragma unroll
-  for (int i = 1; i < kMaxI8; ++i)
-    if (i < bt.n && (int)blockIdx.x >= bt.p[i].wg_begin) pi = i;
-  const IProb& P = bt.p[pi];
+  const IProb P = bt.p[problem_of<kMulti>(bt, blockIdx.x)];
+  asm volatile("" ::"s"(P.q), "s"(P.s), "s"(P.w), "s"(P.t), "s"(P.bias), "s"(P.y), "s"(P.m), "s"(P.n), "s"(P.steps), "s"(P.epi),
+               "s"(P.nmb), "s"(P.ncol), "s"(P.wg_begin));
   const int lt = (int)blockIdx.x - P.wg_begin;
   // the row tiles of a column tile run on one XCD, eight ids apart, and share its weights' one trip to the L2
   const int mb = (lt >> 3) % P.nmb, cb = (lt >> 3) / P.nmb * 8 + (lt & 7);
   if (cb >= P.ncol) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int steps = P.steps, mblk = (P.m + 31) >> 5, nblk = (P.n + 31) >> 5;
+  // this thread's eight outputs, and their scales, requested before everything else
+  const int og = threadIdx.x & 3, ot = (threadIdx.x >> 2) % TN + threadIdx.x / (4 * TN * 32) * TN, orow = (threadIdx.x / (4 * TN)) & 31;
+  const int row = (mb * TM + ot / TN) * 32 + orow, col = (cb * TN + ot % TN) * 32 + 8 * og;
+  const bool out = threadIdx.x < kTiles * 128 && row < P.m && col < P.n;
+  float os = 0.0f, ts[8], bs[8] = {};
+  if (out) {
+    os = P.s[row];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = min(col + e, P.n - 1);
+      ts[e] = P.t[c];
+      if (P.epi == VKWR_GEMM_EPI_BIAS) bs[e] = (float)P.bias[c];
+    }
+  }
   const int8_t *xp[TM], *wp[TN];  // blocks past the last are read as the last
 #pragma unroll
   for (int i = 0; i < TM; ++i) xp[i] = P.q + (int64_t)min(mb * TM + i, mblk - 1) * steps * 1024 + lane * 16;
@@ -302,30 +324,39 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
   };
   static_assert(kI8Pad % (32 * KS) == 0, "whole blocks");
   const int blocks = steps / KS, nb = (blocks - wave + NW - 1) / NW;  // this wave's blocks
+  if (nb >= NB) {
+    // no load here or in the loop is behind a condition, so that the waits in it are exact: with the first
+    // loads under conditions the compiler waited for all that were out before every round
 #pragma unroll
-  for (int u = 0; u < NB; ++u)
-    if (u < nb) load(u, u);
-  __builtin_amdgcn_sched_barrier(0);
-  int b = 0;
-  // every load of the loop is unconditional, so that the waits in it are exact
-  for (; b + 2 * NB <= nb; b += NB) {
+    for (int u = 0; u < NB; ++u) load(u, u);
+    __builtin_amdgcn_sched_barrier(0);
+    int b = 0;
+    for (; b + 2 * NB <= nb; b += NB) {
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        compute(u);
+        __builtin_amdgcn_sched_barrier(0);
+        load(u, b + NB + u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
       compute(u);
-      __builtin_amdgcn_sched_barrier(0);
-      load(u, b + NB + u);
+      if (b + NB + u < nb) load(u, b + NB + u);
       __builtin_amdgcn_sched_barrier(0);
     }
-  }
 #pragma unroll
-  for (int u = 0; u < NB; ++u) {
-    if (b + u < nb) compute(u);
-    if (b + NB + u < nb) load(u, b + NB + u);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+    for (int u = 0; u + 1 < NB; ++u)
+      if (b + NB + u < nb) compute(u);
+  } else {
 #pragma unroll
-  for (int u = 0; u < NB; ++u)
-    if (b + NB + u < nb) compute(u);
+    for (int u = 0; u + 1 < NB; ++u)
+      if (u < nb) load(u, u);
+#pragma unroll
+    for (int u = 0; u + 1 < NB; ++u)
+      if (u < nb) compute(u);
+  }
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -334,18 +365,17 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
       red[((wave * kTiles + t) * 4 + g) * kG + lane] = iv4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
     }
   __syncthreads();
-  for (int u = threadIdx.x; u < kTiles * 128; u += NW * 64) {
-    const int g = u & 3, t = (u >> 2) % TN + (u / (4 * TN * 32)) * TN, r = (u / (4 * TN)) & 31;
-    iv4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+  if (!out) return;
+  iv4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      lo += red[((w * kTiles + t) * 4 + g) * kG + r];
-      hi += red[((w * kTiles + t) * 4 + g) * kG + r + 32];
-    }
-    const int row = (mb * TM + t / TN) * 32 + r, col = (cb * TN + t % TN) * 32 + 8 * g;
-    const int a[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    if (row < P.m) i8_finish8(a, row, col, P.m, P.n, P.epi, P.s[row], P.t, P.bias, P.y);
+  for (int w = 0; w < NW; ++w) {
+    lo += red[((w * kTiles + ot) * 4 + og) * kG + orow];
+    hi += red[((w * kTiles + ot) * 4 + og) * kG + orow + 32];
   }
+  const int sum[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  hv8 h;
+  i8_finish(sum, os, ts, P.epi, bs, h);
+  store8((gptr)(P.y + (int64_t)row * P.n + col), h, P.n - col);
 }
 
 // ---- few rows: the weights pass through once, four products an instruction
@@ -370,21 +400,26 @@ struct GBatch {
   GProb p[kMaxI8];
 };
 
-template <int M>
+template <int M, bool kMulti>
 __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
   constexpr int kWaves = 8, kPer = kWaves / M, kAhead = 8;  // waves of a row; weights requested first
   __shared__ __attribute__((aligned(16))) int8_t xq[kGemvMost + M * kI8Pad];
   __shared__ uint32_t wtop[kWaves];
   __shared__ int part[kWaves][M][32];
-  int pi = 0;
-#pragma unroll
-  for (int i = 1; i < kMaxI8; ++i)
-    if (i < bt.n && (int)blockIdx.x >= bt.p[i].wg_begin) pi = i;
-  const GProb& P = bt.p[pi];
+  const GProb P = bt.p[problem_of<kMulti>(bt, blockIdx.x)];
+  asm volatile("" ::"s"(P.x), "s"(P.w), "s"(P.t), "s"(P.bias), "s"(P.y), "s"(P.m), "s"(P.n), "s"(P.k), "s"(P.steps), "s"(P.epi),
+               "s"(P.wg_begin));
   const int cb = (int)blockIdx.x - P.wg_begin;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int steps = P.steps, k = P.k, kpad = steps * 32;
   const int8_t* const w = P.w + (int64_t)cb * steps * 1024 + lane * 16;
+  const int orow = tid >> 5, ocol = cb * 32 + (tid & 31);  // this thread's output, if it has one
+  const bool out = tid < 32 * M && orow < P.m && ocol < P.n;
+  float ts[1], bs[1] = {0.0f};
+  if (out) {
+    ts[0] = P.t[ocol];
+    if (P.epi == VKWR_GEMM_EPI_BIAS) bs[0] = (float)P.bias[ocol];
+  }
   // ---- this wave's pieces of 8 values of its row
   const int row = min(wave / kPer, P.m - 1), w0 = wave % kPer, pieces = kpad / 8;
   const _Float16* const x = P.x + (int64_t)row * k;
@@ -465,19 +500,17 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
     if (lane < 32) part[wave][r][lane] = acc[r];
   }
   __syncthreads();
-  if (tid < 32 * M) {
-    const int r = tid >> 5, col = cb * 32 + (tid & 31);
-    if (r < P.m && col < P.n) {
-      int sum = 0;
+  if (!out) return;
+  int sums[1] = {0};
 #pragma unroll
-      for (int q = 0; q < kWaves; ++q) sum += part[q][r][tid & 31];
-      uint32_t all = 0;
+  for (int q = 0; q < kWaves; ++q) sums[0] += part[q][orow][tid & 31];
+  uint32_t all = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) all = max(all, wtop[r * kPer + i]);
-      const float s = all < 0x7c00u ? h2f((uint16_t)all) / 127.0f : __builtin_nanf("");
-      P.y[(int64_t)r * P.n + col] = i8_finish(sum, s, P.t[col], P.epi, P.epi == VKWR_GEMM_EPI_BIAS ? (float)P.bias[col] : 0.0f);
-    }
-  }
+  for (int i = 0; i < kPer; ++i) all = max(all, wtop[orow * kPer + i]);
+  const float s = all < 0x7c00u ? h2f((uint16_t)all) / 127.0f : __builtin_nanf("");
+  _Float16 h[1];
+  i8_finish(sums, s, ts, P.epi, bs, h);
+  P.y[(int64_t)orow * P.n + ocol] = h[0];
 }
 
 // ---- many rows: tiles through LDS, bound by the matrix cores
@@ -548,8 +581,10 @@ __device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&
         if constexpr (kEpi == VKWR_GEMM_EPI_BIAS) b = *reinterpret_cast<const f4*>(tl + 32 * TN + c);
         typedef _Float16 hv4 __attribute__((ext_vector_type(4)));
         hv4 h;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = i8_finish(acc[i][j0 + jj][4 * g + e], s[i], t[e], kEpi, b[e]);
+        const iv16& c16 = acc[i][j0 + jj];
+        const int sums[4] = {c16[4 * g], c16[4 * g + 1], c16[4 * g + 2], c16[4 * g + 3]};
+        const float ts[4] = {t[0], t[1], t[2], t[3]}, bs[4] = {b[0], b[1], b[2], b[3]};
+        i8_finish(sums, s[i], ts, kEpi, bs, h);
         *reinterpret_cast<hv4*>(o + (jj * 32 + 8 * g + 4 * lh) * 2) = h;
       }
   };
@@ -587,11 +622,7 @@ __global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
     const int b = blockIdx.x, x = b & 7, q8 = tiles >> 3, r8 = tiles & 7;
     L = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (b >> 3);
   }
-  int pi = 0;
-#pragma unroll
-  for (int i = 1; i < kMaxI8; ++i)
-    if (i < bt.n && L >= bt.p[i].wg_begin) pi = i;
-  const IProb& P = bt.p[pi];
+  const IProb& P = bt.p[problem_of<true>(bt, L)];
   const int lt = L - P.wg_begin, per = 4 * P.ncol, grp = lt / per, in = lt - grp * per;
   const int g0 = grp * 4, gs = min(4, P.nmb - g0);
   const int mb = g0 + in % gs, cb = in / gs;
@@ -764,11 +795,17 @@ void launch_rows(QBatch& b, hipStream_t s) {
     grid += (unsigned)up((b.p[i].m + 31) / 32, 8) * 32 / std::max(1, 256 / T);
   }
   if (grid == 0) return;
-  if (T == 64) hipLaunchKernelGGL((i8_rows_kernel<64, 1>), dim3(grid), dim3(256), 0, s, b);
-  else if (T == 128) hipLaunchKernelGGL((i8_rows_kernel<128, 1>), dim3(grid), dim3(256), 0, s, b);
-  else if (most <= 128) hipLaunchKernelGGL((i8_rows_kernel<256, 1>), dim3(grid), dim3(256), 0, s, b);
-  else if (T == 256) hipLaunchKernelGGL((i8_rows_kernel<256, 2>), dim3(grid), dim3(256), 0, s, b);
-  else hipLaunchKernelGGL((i8_rows_kernel<512, 2>), dim3(grid), dim3(512), 0, s, b);
+#define VK_I8_ROWS(t, keep)                                                                                       \
+  do {                                                                                                           \
+    const dim3 th(t < 256 ? 256 : t);                                                                            \
+    if (b.n == 1) hipLaunchKernelGGL((i8_rows_kernel<t, keep, false>), dim3(grid), th, 0, s, b);                 \
+    else hipLaunchKernelGGL((i8_rows_kernel<t, keep, true>), dim3(grid), th, 0, s, b);                           \
+  } while (0)
+  if (T == 64) VK_I8_ROWS(64, 1);
+  else if (T == 128) VK_I8_ROWS(128, 1);
+  else if (most <= 128) VK_I8_ROWS(256, 1);
+  else if (T == 256) VK_I8_ROWS(256, 2);
+  else VK_I8_ROWS(512, 2);
 }
 
 QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) {
@@ -821,14 +858,18 @@ I8Route pick_route(int n, const vkwr_i8_problem* p) {
   return kI8Routes[0.77 * (double)((tiles[6] + cus - 1) / cus) < (double)((tiles[7] + cus - 1) / cus) ? 6 : 7];
 }
 
-#define VK_I8_STREAM(tm, tn, ks, nb) \
-  hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb>), dim3((unsigned)wgs), dim3(512), 0, s, b)
+#define VK_I8_STREAM(tm, tn, ks, nb)                                                                              \
+  do {                                                                                                           \
+    const dim3 grid((unsigned)wgs), th(512);                                                                     \
+    if (b.n == 1) hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, false>), grid, th, 0, s, b);           \
+    else hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, true>), grid, th, 0, s, b);                     \
+  } while (0)
 #define VK_I8_TILE(tm, tn, nbuf) \
   hipLaunchKernelGGL((i8_tile_kernel<tm, tn, nbuf>), dim3((unsigned)wgs), dim3(256), 0, s, b, wgs)
 
 void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) {
   if (r.kind == kRouteStream) {
-    if (r.rows == 64) VK_I8_STREAM(2, 2, 4, 1);
+    if (r.rows == 64) VK_I8_STREAM(2, 2, 1, 4);
     else if (r.cols == 64) VK_I8_STREAM(1, 2, 2, 4);
     else VK_I8_STREAM(1, 1, 2, 4);
   } else if (r.rows == 64) {
@@ -946,10 +987,14 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
       wgs += (p[i].n + 31) / 32;
       most = std::max(most, P.m);
     }
-    const dim3 grid((unsigned)wgs);
-    if (most == 1) hipLaunchKernelGGL(i8_gemv_kernel<1>, grid, dim3(512), 0, st, gb);
-    else if (most == 2) hipLaunchKernelGGL(i8_gemv_kernel<2>, grid, dim3(512), 0, st, gb);
-    else hipLaunchKernelGGL(i8_gemv_kernel<4>, grid, dim3(512), 0, st, gb);
+    const dim3 grid((unsigned)wgs), th(512);
+    const bool one = gb.n == 1;
+    if (most == 1 && one) hipLaunchKernelGGL((i8_gemv_kernel<1, false>), grid, th, 0, st, gb);
+    else if (most == 1) hipLaunchKernelGGL((i8_gemv_kernel<1, true>), grid, th, 0, st, gb);
+    else if (most == 2 && one) hipLaunchKernelGGL((i8_gemv_kernel<2, false>), grid, th, 0, st, gb);
+    else if (most == 2) hipLaunchKernelGGL((i8_gemv_kernel<2, true>), grid, th, 0, st, gb);
+    else if (one) hipLaunchKernelGGL((i8_gemv_kernel<4, false>), grid, th, 0, st, gb);
+    else hipLaunchKernelGGL((i8_gemv_kernel<4, true>), grid, th, 0, st, gb);
     return check_launch(fn);
   }
   const I8Scratch c = scratch_of(n, p);
