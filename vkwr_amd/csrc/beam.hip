@@ -15,6 +15,8 @@
 // never a destination, so the copies need no order and no second buffer.
 #include <hip/hip_runtime.h>
 
+#include <float.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -175,13 +177,21 @@ __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(BeamArgs a) {
   bound = wbound[0];
 #pragma unroll
   for (int w = 1; w < kRowWaves; ++w) mx = fmaxf(mx, wmax[w]), bound = fminf(bound, wbound[w]);
-  if (top >= bound && top > kNone) {
+  bound = fmaxf(bound, -FLT_MAX);  // (-inf is not an entry)
+  if (__ballot(top >= bound)) {
+    int mine = 0;  // entries of the wave
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) mine += __popcll(__ballot(value(e) >= bound));
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&count, mine);
+    at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      if (value(e) >= bound && value(e) > kNone) {
-        const int n = atomicAdd(&count, 1);
-        if (n < kListCap) list[n] = entry_key(value(e), (uint32_t)index_of(e));
-      }
+      const uint64_t b = __ballot(value(e) >= bound);
+      if (b == 0) continue;
+      const int n = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+      if (value(e) >= bound && n < kListCap) list[n] = entry_key(value(e), (uint32_t)index_of(e));
+      at += __popcll(b);
     }
   }
   float sum = 0.0f;
