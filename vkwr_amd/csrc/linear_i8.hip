@@ -39,17 +39,17 @@ __device__ __forceinline__ int64_t i8_index(int64_t r, int64_t k, int64_t steps)
   return ((r >> 5) * steps + (k >> 5)) * 1024 + (((k >> 4) & 1) * 32 + (r & 31)) * 16 + (k & 15);
 }
 
-// The problem that workgroup b belongs to; a call of one problem is compiled without the search, and the
-// kernels that live for a few microseconds read all of its fields in one round of loads (an empty asm holds
-// them above the first branch): left alone the compiler reads each where it is used, one trip after another.
-template <bool kMulti, typename Batch>
+// The problem that a workgroup belongs to: problems of equally many workgroups have a row of the grid each
+// (a call of one problem too), others are searched for by their first workgroups.  Kernels that live for a few
+// microseconds read all of its fields in one round of loads (an empty asm holds them above the
+// first branch): left alone the compiler reads each where it is used, one trip after another.
+template <bool kGridRows, typename Batch>
 __device__ __forceinline__ int problem_of(const Batch& bt, int b) {
+  if constexpr (kGridRows) return blockIdx.y;
   int pi = 0;
-  if constexpr (kMulti) {
 #pragma unroll
-    for (int i = 1; i < kMaxI8; ++i)
-      if (i < bt.n && b >= bt.p[i].wg_begin) pi = i;
-  }
+  for (int i = 1; i < kMaxI8; ++i)
+    if (i < bt.n && b >= bt.p[i].wg_begin) pi = i;
   return pi;
 }
 
@@ -132,13 +132,13 @@ __device__ __forceinline__ iv4 quant16(const uv4 (&v)[2], float top, float inv) 
 // a block go to one XCD (workgroup b runs on XCD b % 8), whose L2 joins the 16-byte pieces that they
 // write into common lines.  Rows longer than 16384 are read twice.  |x| is compared as an integer, where an
 // infinity or a NaN exceeds every number: such a row gets the scale NaN and zeros.
-template <int T, int kKeep, bool kMulti>
+template <int T, int kKeep, bool kGridRows>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void i8_rows_kernel(QBatch bt) {
   constexpr int kThreads = T < 256 ? 256 : T, kRows = kThreads / T, kWaves = T / 64;
   __shared__ uint32_t wtop[kThreads / 64];
-  const QProb P = bt.p[problem_of<kMulti>(bt, blockIdx.x)];
+  const QProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
   asm volatile("" ::"s"(P.x), "s"(P.q), "s"(P.s), "s"(P.m), "s"(P.k), "s"(P.steps), "s"(P.wg_begin));
-  const int u = (int)blockIdx.x - P.wg_begin, per = 32 / kRows;  // workgroups of a block of rows
+  const int u = (int)blockIdx.x - (kGridRows ? 0 : P.wg_begin), per = 32 / kRows;  // workgroups of a block of rows
   const int idx = u >> 3;
   const int64_t row = ((int64_t)(idx / per) * 8 + (u & 7)) * 32 + idx % per * kRows + threadIdx.x / T;
   const int t = threadIdx.x % T, wave = threadIdx.x >> 6;
@@ -264,15 +264,15 @@ __device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
 // (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
 // KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
 // tiles are added through LDS.
-template <int TM, int TN, int NW, int KS, int NB, bool kMulti>
+template <int TM, int TN, int NW, int KS, int NB, bool kGridRows>
 __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
   constexpr int kTiles = TM * TN, kG = 64 + 4 / TN;  // 16-byte cells of a group of 4 results, padded: reads hit all banks
   static_assert(kTiles * 128 <= NW * 64, "one piece of the output per thread");
   __shared__ __attribute__((aligned(16))) iv4 red[NW * kTiles * 4 * kG];
-  const IProb P = bt.p[problem_of<kMulti>(bt, blockIdx.x)];
+  const IProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
   asm volatile("" ::"s"(P.q), "s"(P.s), "s"(P.w), "s"(P.t), "s"(P.bias), "s"(P.y), "s"(P.m), "s"(P.n), "s"(P.steps), "s"(P.epi),
                "s"(P.nmb), "s"(P.ncol), "s"(P.wg_begin));
-  const int lt = (int)blockIdx.x - P.wg_begin;
+  const int lt = (int)blockIdx.x - (kGridRows ? 0 : P.wg_begin);
   // the row tiles of a column tile run on one XCD, eight ids apart, and share its weights' one trip to the L2
   const int mb = (lt >> 3) % P.nmb, cb = (lt >> 3) / P.nmb * 8 + (lt & 7);
   if (cb >= P.ncol) return;
@@ -400,16 +400,16 @@ struct GBatch {
   GProb p[kMaxI8];
 };
 
-template <int M, bool kMulti>
+template <int M, bool kGridRows>
 __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
   constexpr int kWaves = 8, kPer = kWaves / M, kAhead = 8;  // waves of a row; weights requested first
   __shared__ __attribute__((aligned(16))) int8_t xq[kGemvMost + M * kI8Pad];
   __shared__ uint32_t wtop[kWaves];
   __shared__ int part[kWaves][M][32];
-  const GProb P = bt.p[problem_of<kMulti>(bt, blockIdx.x)];
+  const GProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
   asm volatile("" ::"s"(P.x), "s"(P.w), "s"(P.t), "s"(P.bias), "s"(P.y), "s"(P.m), "s"(P.n), "s"(P.k), "s"(P.steps), "s"(P.epi),
                "s"(P.wg_begin));
-  const int cb = (int)blockIdx.x - P.wg_begin;
+  const int cb = (int)blockIdx.x - (kGridRows ? 0 : P.wg_begin);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int steps = P.steps, k = P.k, kpad = steps * 32;
   const int8_t* const w = P.w + (int64_t)cb * steps * 1024 + lane * 16;
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
     const int b = blockIdx.x, x = b & 7, q8 = tiles >> 3, r8 = tiles & 7;
     L = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (b >> 3);
   }
-  const IProb& P = bt.p[problem_of<true>(bt, L)];
+  const IProb& P = bt.p[problem_of<false>(bt, L)];
   const int lt = L - P.wg_begin, per = 4 * P.ncol, grp = lt / per, in = lt - grp * per;
   const int g0 = grp * 4, gs = min(4, P.nmb - g0);
   const int mb = g0 + in % gs, cb = in / gs;
@@ -784,6 +784,15 @@ I8Scratch scratch_of(int n, const vkwr_i8_problem* p) {
   return c;
 }
 
+// The grid of a batch whose problems begin at wg_begin, `total` workgroups in all: a row per problem where they
+// have equally many.
+template <typename Batch>
+dim3 grid_of(const Batch& b, int64_t total, bool* rows) {
+  *rows = total % b.n == 0;
+  for (int i = 0; i < b.n; ++i) *rows = *rows && b.p[i].wg_begin == i * (total / b.n);
+  return *rows ? dim3((unsigned)(total / b.n), (unsigned)b.n) : dim3((unsigned)total);
+}
+
 // Rounds the rows of every problem of `b` (wg_begin filled in here).
 void launch_rows(QBatch& b, hipStream_t s) {
   int most = 0;
@@ -795,11 +804,13 @@ void launch_rows(QBatch& b, hipStream_t s) {
     grid += (unsigned)up((b.p[i].m + 31) / 32, 8) * 32 / std::max(1, 256 / T);
   }
   if (grid == 0) return;
-#define VK_I8_ROWS(t, keep)                                                                                       \
-  do {                                                                                                           \
-    const dim3 th(t < 256 ? 256 : t);                                                                            \
-    if (b.n == 1) hipLaunchKernelGGL((i8_rows_kernel<t, keep, false>), dim3(grid), th, 0, s, b);                 \
-    else hipLaunchKernelGGL((i8_rows_kernel<t, keep, true>), dim3(grid), th, 0, s, b);                           \
+  bool by_row;
+  const dim3 g = grid_of(b, grid, &by_row);
+#define VK_I8_ROWS(t, keep)                                                                                \
+  do {                                                                                                     \
+    const dim3 th(t < 256 ? 256 : t);                                                                      \
+    if (by_row) hipLaunchKernelGGL((i8_rows_kernel<t, keep, true>), g, th, 0, s, b);                       \
+    else hipLaunchKernelGGL((i8_rows_kernel<t, keep, false>), g, th, 0, s, b);                             \
   } while (0)
   if (T == 64) VK_I8_ROWS(64, 1);
   else if (T == 128) VK_I8_ROWS(128, 1);
@@ -858,17 +869,19 @@ I8Route pick_route(int n, const vkwr_i8_problem* p) {
   return kI8Routes[0.77 * (double)((tiles[6] + cus - 1) / cus) < (double)((tiles[7] + cus - 1) / cus) ? 6 : 7];
 }
 
-#define VK_I8_STREAM(tm, tn, ks, nb)                                                                              \
-  do {                                                                                                           \
-    const dim3 grid((unsigned)wgs), th(512);                                                                     \
-    if (b.n == 1) hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, false>), grid, th, 0, s, b);           \
-    else hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, true>), grid, th, 0, s, b);                     \
+#define VK_I8_STREAM(tm, tn, ks, nb)                                                                       \
+  do {                                                                                                     \
+    const dim3 th(512);                                                                                    \
+    if (by_row) hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, true>), g, th, 0, s, b);           \
+    else hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, false>), g, th, 0, s, b);                 \
   } while (0)
 #define VK_I8_TILE(tm, tn, nbuf) \
   hipLaunchKernelGGL((i8_tile_kernel<tm, tn, nbuf>), dim3((unsigned)wgs), dim3(256), 0, s, b, wgs)
 
 void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) {
   if (r.kind == kRouteStream) {
+    bool by_row;
+    const dim3 g = grid_of(b, wgs, &by_row);
     if (r.rows == 64) VK_I8_STREAM(2, 2, 1, 4);
     else if (r.cols == 64) VK_I8_STREAM(1, 2, 2, 4);
     else VK_I8_STREAM(1, 1, 2, 4);
@@ -987,14 +1000,14 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
       wgs += (p[i].n + 31) / 32;
       most = std::max(most, P.m);
     }
-    const dim3 grid((unsigned)wgs), th(512);
-    const bool one = gb.n == 1;
-    if (most == 1 && one) hipLaunchKernelGGL((i8_gemv_kernel<1, false>), grid, th, 0, st, gb);
-    else if (most == 1) hipLaunchKernelGGL((i8_gemv_kernel<1, true>), grid, th, 0, st, gb);
-    else if (most == 2 && one) hipLaunchKernelGGL((i8_gemv_kernel<2, false>), grid, th, 0, st, gb);
-    else if (most == 2) hipLaunchKernelGGL((i8_gemv_kernel<2, true>), grid, th, 0, st, gb);
-    else if (one) hipLaunchKernelGGL((i8_gemv_kernel<4, false>), grid, th, 0, st, gb);
-    else hipLaunchKernelGGL((i8_gemv_kernel<4, true>), grid, th, 0, st, gb);
+    bool by_row;
+    const dim3 grid = grid_of(gb, wgs, &by_row), th(512);
+    if (most == 1 && by_row) hipLaunchKernelGGL((i8_gemv_kernel<1, true>), grid, th, 0, st, gb);
+    else if (most == 1) hipLaunchKernelGGL((i8_gemv_kernel<1, false>), grid, th, 0, st, gb);
+    else if (most == 2 && by_row) hipLaunchKernelGGL((i8_gemv_kernel<2, true>), grid, th, 0, st, gb);
+    else if (most == 2) hipLaunchKernelGGL((i8_gemv_kernel<2, false>), grid, th, 0, st, gb);
+    else if (by_row) hipLaunchKernelGGL((i8_gemv_kernel<4, true>), grid, th, 0, st, gb);
+    else hipLaunchKernelGGL((i8_gemv_kernel<4, false>), grid, th, 0, st, gb);
     return check_launch(fn);
   }
   const I8Scratch c = scratch_of(n, p);
