@@ -516,17 +516,19 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
 // ---- many rows: tiles through LDS, bound by the matrix cores
 //
 // (64 TM) x (64 TN) outputs per workgroup, four waves of (32 TM) x (32 TN) in registers.  K advances
-// 128 per stage through NBUF LDS buffers; both operands being in fragment order, a stage is a row of
-// 4 KiB pieces, copied straight to LDS, and read back lane by lane.  One barrier per stage, before the
-// last group of products, whose operands are then in registers: behind it the buffer is free and the copies of
-// the stage NBUF further go out, between the products of this and the next group, so
-// that they neither hold up the products nor arrive late.  NBUF: as many as fit (two 64 KiB stages of 256 x 256, four of
-// 128 x 128); two of 128 x 128 and two workgroups a CU took 46 us instead of 32 for K 8192, N 2048, m = 433.  The copies are written in assembly, as the compiler
-// would make every LDS read wait for all of them; the waits are placed here.
+// 64 per stage through a ring of NBUF LDS buffers; both operands being in fragment order, a stage is a row of
+// 2 KiB pieces, copied straight to LDS, and read back lane by lane.  One barrier per stage, before the
+// second of its two groups of products, whose operands are then in registers: behind it the buffer is free and
+// the copies of the stage NBUF further go out between the products, so that they neither hold those up
+// nor arrive late.  The copies are written in assembly, as the compiler would make every LDS read wait for all of
+// them; the waits are placed here.  (Stages of 128 k with two groups of copies each took 5 % more: 147 us instead
+// of 138 for three of K = N = 4096, m = 2304.  From three buffers on their number makes no difference.)
+// What bounds it: 2.1 POPS where every CU is busy, at 2.0 GHz (the card's power), the LDS at 75 - 85 % of its
+// rate; 2.5 where 192 CUs are (K = N = 4096, m = 2304).
 template <int TM, int TN>
 struct I8Tile {
-  static constexpr int kX = 8 * TM, kW = 8 * TN, kBlocks = kX + kW;  // kilobytes of a stage
-  static constexpr int kCopies = kBlocks / 4;                        // per wave
+  static constexpr int kX = 4 * TM, kW = 4 * TN, kBlocks = kX + kW;  // kilobytes of a stage
+  static constexpr int kCopies = TM + TN;                            // per wave
   static constexpr int kOutRow = 144;                                // bytes of a staged row of 64 outputs
 };
 
@@ -611,7 +613,7 @@ __device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&
 template <int TM, int TN, int NBUF>
 __global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
   using T = I8Tile<TM, TN>;
-  constexpr int ND = T::kCopies, kHalf = ND / 2;
+  constexpr int ND = T::kCopies;
   constexpr int kOut = 4 * (2 * 32 * T::kOutRow + 2 * 32 * TN * 4);
   constexpr int kBuf = T::kBlocks * 1024, kRing = NBUF * kBuf;
   static_assert(kOut <= kRing, "the outputs are staged where the operands were");
@@ -627,33 +629,32 @@ __global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
   const int g0 = grp * 4, gs = min(4, P.nmb - g0);
   const int mb = g0 + in % gs, cb = in / gs;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w >> 1, wn = w & 1;
-  const int steps = P.steps, ns = steps >> 2;
+  const int steps = P.steps, ns = steps >> 1;
   const int mlast = ((P.m + 31) >> 5) - 1 - mb * 2 * TM, nlast = ((P.n + 31) >> 5) - 1 - cb * 2 * TN;
-  // copy d of wave w: k step w of the stage, of block d of x, then of the weights
+  // copy d of wave w: k step w % 2 of the stage, of block 2 d + w / 2 of x, then of the weights
   uint32_t off[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    const int blk = d < 2 * TM ? min(d, mlast) : min(d - 2 * TM, nlast);
-    off[d] = (uint32_t)((blk * steps + w) * 1024 + lane * 16);
+    const int blk = d < TM ? min(2 * d + (w >> 1), mlast) : min(2 * (d - TM) + (w >> 1), nlast);
+    off[d] = (uint32_t)((blk * steps + (w & 1)) * 1024 + lane * 16);
   }
   const char* const px = (const char*)uniform_ptr(P.q + (int64_t)mb * 2 * TM * steps * 1024);
   const char* const pw = (const char*)uniform_ptr(P.w + (int64_t)cb * 2 * TN * steps * 1024);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(VK_LDS void*)&sm[0] + w * 1024);
-  auto copies = [&](int buf, int st, int d0, int d1) __attribute__((always_inline)) {
-    const int64_t k0 = (int64_t)min(st, ns - 1) * 4096;  // past the end: the last stage once more, unused
+  auto copies = [&](int buf, int st) __attribute__((always_inline)) {
+    const int64_t k0 = (int64_t)min(st, ns - 1) * 2048;  // past the end: the last stage once more, unused
     const void *xb = uniform_ptr(px + k0), *wb = uniform_ptr(pw + k0);
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-      if (d >= d0 && d < d1) copy16(d < 2 * TM ? xb : wb, off[d], lds0 + buf * kBuf + d * 4096);
+    for (int d = 0; d < ND; ++d) copy16(d < TM ? xb : wb, off[d], lds0 + buf * kBuf + d * 4096);
   };
-  const char* const fxp = sm + wm * TM * 4096 + lane * 16;
-  const char* const fwp = sm + (T::kX + wn * TN * 4) * 1024 + lane * 16;
+  const char* const fxp = sm + wm * TM * 2048 + lane * 16;
+  const char* const fwp = sm + (T::kX + wn * TN * 2) * 1024 + lane * 16;
   iv4 fx[2][TM], fw[2][TN];
   auto fread = [&](int buf, int kk, int set) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fx[set][i] = *reinterpret_cast<const iv4*>(fxp + buf * kBuf + (i * 4 + kk) * 1024);
+    for (int i = 0; i < TM; ++i) fx[set][i] = *reinterpret_cast<const iv4*>(fxp + buf * kBuf + (i * 2 + kk) * 1024);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fw[set][j] = *reinterpret_cast<const iv4*>(fwp + buf * kBuf + (j * 4 + kk) * 1024);
+    for (int j = 0; j < TN; ++j) fw[set][j] = *reinterpret_cast<const iv4*>(fwp + buf * kBuf + (j * 2 + kk) * 1024);
   };
   iv16 acc[TM][TN];
 #pragma unroll
@@ -676,9 +677,9 @@ __global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
     __builtin_amdgcn_sched_group_barrier(0x100, TM + TN - kReads, 0);
     __builtin_amdgcn_sched_group_barrier(0x008, TM * TN - kReads, 0);
   };
-  // the products of a group with copies d0 .. d0 + kHalf - 1 of stage st between them
-  auto products_copies = [&](int set, int buf, int st, int d0) __attribute__((always_inline)) {
-    const int64_t k0 = (int64_t)min(st, ns - 1) * 4096;
+  // the products of a group with the copies of stage st between them
+  auto products_copies = [&](int set, int buf, int st) __attribute__((always_inline)) {
+    const int64_t k0 = (int64_t)min(st, ns - 1) * 2048;
     const void *xb = uniform_ptr(px + k0), *wb = uniform_ptr(pw + k0);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -687,38 +688,27 @@ __global__ __launch_bounds__(256, 1) void i8_tile_kernel(IBatch bt, int tiles) {
         acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][j], fx[set][i], acc[i][j], 0, 0, 0);
         const int p = i * TN + j;
 #pragma unroll
-        for (int q = 0; q < kHalf; ++q)
-          if (q * TM * TN / kHalf == p)
-            copy16(d0 + q < 2 * TM ? xb : wb, off[d0 + q], lds0 + buf * kBuf + (d0 + q) * 4096);
+        for (int d = 0; d < ND; ++d)
+          if (d * TM * TN / ND == p) copy16(d < TM ? xb : wb, off[d], lds0 + buf * kBuf + d * 4096);
         __builtin_amdgcn_sched_barrier(0);
       }
   };
-  // stage s + 1 has landed where all but the newest NBUF - 2 stages' copies have
-  auto landed = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * ND) : "memory");
-  };
+  // all but the newest n stages' copies have landed, and this wave's reads have returned
+#define VK_I8_LANDED(n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((n) * ND) : "memory")
 #pragma unroll
-  for (int u = 0; u < NBUF - 1; ++u) copies(u, u, 0, ND);
-  landed();
-  copies(NBUF - 1, NBUF - 1, 0, kHalf);
+  for (int u = 0; u < NBUF; ++u) copies(u, u);
+  VK_I8_LANDED(NBUF - 1);
   fread(0, 0, 0);
-  int cur = 0, prev = NBUF - 1;
+  int cur = 0;
   for (int s = 0; s < ns; ++s) {
     const int nxt = cur + 1 == NBUF ? 0 : cur + 1;
     fread(cur, 1, 1);
-    products_copies(0, prev, s + NBUF - 1, kHalf);
-    __builtin_amdgcn_sched_barrier(0);
-    fread(cur, 2, 0);
-    products(1);
-    __builtin_amdgcn_sched_barrier(0);
-    fread(cur, 3, 1);
     products(0);
     __builtin_amdgcn_sched_barrier(0);
-    landed();  // and this stage is read, for every wave
+    VK_I8_LANDED(NBUF - 2);  // stage s + 1 is there, and this one is read, for every wave
     fread(nxt, 0, 0);
-    products_copies(1, cur, s + NBUF, 0);
+    products_copies(1, cur, s + NBUF);
     __builtin_amdgcn_sched_barrier(0);
-    prev = cur;
     cur = nxt;
   }
   // the last copies have landed and every wave's reads are done
@@ -886,14 +876,14 @@ void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) 
     else if (r.cols == 64) VK_I8_STREAM(1, 2, 2, 4);
     else VK_I8_STREAM(1, 1, 2, 4);
   } else if (r.rows == 64) {
-    VK_I8_TILE(1, 2, 5);
+    VK_I8_TILE(1, 2, 6);
   } else if (r.rows == 128) {
-    if (r.cols == 128) VK_I8_TILE(2, 2, 4);
-    else VK_I8_TILE(2, 4, 3);
+    if (r.cols == 128) VK_I8_TILE(2, 2, 6);
+    else VK_I8_TILE(2, 4, 4);
   } else if (r.rows == 192) {
-    VK_I8_TILE(3, 4, 2);
+    VK_I8_TILE(3, 4, 4);
   } else {
-    VK_I8_TILE(4, 4, 2);
+    VK_I8_TILE(4, 4, 4);
   }
 }
 
