@@ -233,7 +233,7 @@ __device__ __forceinline__ void i8_finish(const int (&a)[N], float s, const floa
   for (int e = 0; e < N; ++e) f[e] = (float)a[e] * (s * t[e]);
   if (epi == VKWR_GEMM_EPI_RELU_SQUARE) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = f[e] > 0.0f ? f[e] * f[e] : (f[e] != f[e] ? f[e] : 0.0f);  // NaN stays
+    for (int e = 0; e < N; ++e) f[e] = __builtin_fmaf(f[e], __builtin_fmaxf(f[e], 0.0f), 0.0f);  // (NaN stays; no -0)
   } else if (epi == VKWR_GEMM_EPI_BIAS) {
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] += bias[e];
