@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vk_capi.h"
 #include "vk_common.cuh"
@@ -39,16 +40,25 @@ __device__ __forceinline__ int64_t i8_index(int64_t r, int64_t k, int64_t steps)
   return ((r >> 5) * steps + (k >> 5)) * 1024 + (((k >> 4) & 1) * 32 + (r & 31)) * 16 + (k & 15);
 }
 
+// The problems of a launch, with room for N.  A launch of one carries that one only: the host takes 2.7 us for
+// 80 bytes of arguments and 3.4 for 700.
+template <typename Prob, int N>
+struct BatchOf {
+  int n;
+  Prob p[N];
+};
+
 // The problem that a workgroup belongs to: problems of equally many workgroups have a row of the grid each
-// (a call of one problem too), others are searched for by their first workgroups.  Kernels that live for a few
-// microseconds read all of its fields in one round of loads (an empty asm holds them above the
-// first branch): left alone the compiler reads each where it is used, one trip after another.
-template <bool kGridRows, typename Batch>
-__device__ __forceinline__ int problem_of(const Batch& bt, int b) {
+// (kGridRows; a launch of one too), others are searched for by their first workgroups.  Kernels that live for a
+// few microseconds read all of its fields in one round of loads (an empty asm holds them above
+// the first branch): left alone the compiler reads each where it is used, one trip after another.
+template <bool kGridRows, typename Prob, int N>
+__device__ __forceinline__ int problem_of(const BatchOf<Prob, N>& bt, int b) {
+  if constexpr (N == 1) return 0;
   if constexpr (kGridRows) return blockIdx.y;
   int pi = 0;
 #pragma unroll
-  for (int i = 1; i < kMaxI8; ++i)
+  for (int i = 1; i < N; ++i)
     if (i < bt.n && b >= bt.p[i].wg_begin) pi = i;
   return pi;
 }
@@ -62,10 +72,7 @@ struct QProb {
   int m, k, steps;
   int wg_begin;  // first workgroup
 };
-struct QBatch {
-  int n;
-  QProb p[kMaxI8];
-};
+typedef BatchOf<QProb, kMaxI8> QBatch;
 
 // The 8 bits of 127 x / top for 16 values, halves to even.  127 x is exact in fp32; one correction
 // of the product with 1 / top makes the quotient exact wherever it is representable, so that a
@@ -132,8 +139,8 @@ __device__ __forceinline__ iv4 quant16(const uv4 (&v)[2], float top, float inv) 
 // a block go to one XCD (workgroup b runs on XCD b % 8), whose L2 joins the 16-byte pieces that they
 // write into common lines.  Rows longer than 16384 are read twice.  |x| is compared as an integer, where an
 // infinity or a NaN exceeds every number: such a row gets the scale NaN and zeros.
-template <int T, int kKeep, bool kGridRows>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void i8_rows_kernel(QBatch bt) {
+template <int T, int kKeep, bool kGridRows, int N>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void i8_rows_kernel(BatchOf<QProb, N> bt) {
   constexpr int kThreads = T < 256 ? 256 : T, kRows = kThreads / T, kWaves = T / 64;
   __shared__ uint32_t wtop[kThreads / 64];
   const QProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
@@ -217,10 +224,7 @@ struct IProb {
   int nmb, ncol;         // row and column tiles
   int wg_begin;
 };
-struct IBatch {
-  int n;
-  IProb p[kMaxI8];
-};
+typedef BatchOf<IProb, kMaxI8> IBatch;
 
 // N outputs: the sums scaled in fp32 (+ bias), the epilogue, one rounding to fp16.  Every kernel finishes its
 // sums here, so that a row's bits do not depend on which one ran.  One branch for all N: with one for
@@ -264,8 +268,8 @@ __device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
 // (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
 // KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
 // tiles are added through LDS.
-template <int TM, int TN, int NW, int KS, int NB, bool kGridRows>
-__global__ __launch_bounds__(NW * 64) void i8_stream_kernel(IBatch bt) {
+template <int TM, int TN, int NW, int KS, int NB, bool kGridRows, int N>
+__global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt) {
   constexpr int kTiles = TM * TN, kG = 64 + 4 / TN;  // 16-byte cells of a group of 4 results, padded: reads hit all banks
   static_assert(kTiles * 128 <= NW * 64, "one piece of the output per thread");
   __shared__ __attribute__((aligned(16))) iv4 red[NW * kTiles * 4 * kG];
@@ -395,13 +399,10 @@ struct GProb {
   _Float16* y;
   int m, n, k, steps, epi, wg_begin;
 };
-struct GBatch {
-  int n;
-  GProb p[kMaxI8];
-};
+typedef BatchOf<GProb, kMaxI8> GBatch;
 
-template <int M, bool kGridRows>
-__global__ __launch_bounds__(512) void i8_gemv_kernel(GBatch bt) {
+template <int M, bool kGridRows, int N>
+__global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   constexpr int kWaves = 8, kPer = kWaves / M, kAhead = 8;  // waves of a row; weights requested first
   __shared__ __attribute__((aligned(16))) int8_t xq[kGemvMost + M * kI8Pad];
   __shared__ uint32_t wtop[kWaves];
@@ -774,8 +775,23 @@ I8Scratch scratch_of(int n, const vkwr_i8_problem* p) {
   return c;
 }
 
-// The grid of a batch whose problems begin at wg_begin, `total` workgroups in all: a row per problem where they
-// have equally many.
+// Launches `kernel` (template arguments kGridRows and N last) on batch b of `total` workgroups of `threads`: a row
+// of the grid per problem where they have equally many workgroups.
+#define VK_I8_LAUNCH(b, total, threads, stream, ...)                                                            \
+  do {                                                                                                          \
+    bool by_row;                                                                                                \
+    const dim3 g = grid_of(b, total, &by_row), th(threads);                                                     \
+    if (b.n == 1) {                                                                                             \
+      const BatchOf<std::decay_t<decltype(b.p[0])>, 1> one{1, {b.p[0]}};                                        \
+      hipLaunchKernelGGL((__VA_ARGS__, true, 1 >), g, th, 0, stream, one);                                      \
+    } else if (by_row) {                                                                                        \
+      hipLaunchKernelGGL((__VA_ARGS__, true, kMaxI8 >), g, th, 0, stream, b);                                   \
+    } else {                                                                                                    \
+      hipLaunchKernelGGL((__VA_ARGS__, false, kMaxI8 >), g, th, 0, stream, b);                                  \
+    }                                                                                                           \
+  } while (0)
+
+// That grid; problems begin at wg_begin.
 template <typename Batch>
 dim3 grid_of(const Batch& b, int64_t total, bool* rows) {
   *rows = total % b.n == 0;
@@ -794,19 +810,11 @@ void launch_rows(QBatch& b, hipStream_t s) {
     grid += (unsigned)up((b.p[i].m + 31) / 32, 8) * 32 / std::max(1, 256 / T);
   }
   if (grid == 0) return;
-  bool by_row;
-  const dim3 g = grid_of(b, grid, &by_row);
-#define VK_I8_ROWS(t, keep)                                                                                \
-  do {                                                                                                     \
-    const dim3 th(t < 256 ? 256 : t);                                                                      \
-    if (by_row) hipLaunchKernelGGL((i8_rows_kernel<t, keep, true>), g, th, 0, s, b);                       \
-    else hipLaunchKernelGGL((i8_rows_kernel<t, keep, false>), g, th, 0, s, b);                             \
-  } while (0)
-  if (T == 64) VK_I8_ROWS(64, 1);
-  else if (T == 128) VK_I8_ROWS(128, 1);
-  else if (most <= 128) VK_I8_ROWS(256, 1);
-  else if (T == 256) VK_I8_ROWS(256, 2);
-  else VK_I8_ROWS(512, 2);
+  if (T == 64) VK_I8_LAUNCH(b, grid, 256, s, i8_rows_kernel<64, 1);
+  else if (T == 128) VK_I8_LAUNCH(b, grid, 256, s, i8_rows_kernel<128, 1);
+  else if (most <= 128) VK_I8_LAUNCH(b, grid, 256, s, i8_rows_kernel<256, 1);
+  else if (T == 256) VK_I8_LAUNCH(b, grid, 256, s, i8_rows_kernel<256, 2);
+  else VK_I8_LAUNCH(b, grid, 512, s, i8_rows_kernel<512, 2);
 }
 
 QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) {
@@ -859,22 +867,14 @@ I8Route pick_route(int n, const vkwr_i8_problem* p) {
   return kI8Routes[0.77 * (double)((tiles[6] + cus - 1) / cus) < (double)((tiles[7] + cus - 1) / cus) ? 6 : 7];
 }
 
-#define VK_I8_STREAM(tm, tn, ks, nb)                                                                       \
-  do {                                                                                                     \
-    const dim3 th(512);                                                                                    \
-    if (by_row) hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, true>), g, th, 0, s, b);           \
-    else hipLaunchKernelGGL((i8_stream_kernel<tm, tn, 8, ks, nb, false>), g, th, 0, s, b);                 \
-  } while (0)
 #define VK_I8_TILE(tm, tn, nbuf) \
   hipLaunchKernelGGL((i8_tile_kernel<tm, tn, nbuf>), dim3((unsigned)wgs), dim3(256), 0, s, b, wgs)
 
 void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) {
   if (r.kind == kRouteStream) {
-    bool by_row;
-    const dim3 g = grid_of(b, wgs, &by_row);
-    if (r.rows == 64) VK_I8_STREAM(2, 2, 1, 4);
-    else if (r.cols == 64) VK_I8_STREAM(1, 2, 2, 4);
-    else VK_I8_STREAM(1, 1, 2, 4);
+    if (r.rows == 64) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<2, 2, 8, 1, 4);
+    else if (r.cols == 64) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<1, 2, 8, 2, 4);
+    else VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<1, 1, 8, 2, 4);
   } else if (r.rows == 64) {
     VK_I8_TILE(1, 2, 6);
   } else if (r.rows == 128) {
@@ -990,14 +990,9 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
       wgs += (p[i].n + 31) / 32;
       most = std::max(most, P.m);
     }
-    bool by_row;
-    const dim3 grid = grid_of(gb, wgs, &by_row), th(512);
-    if (most == 1 && by_row) hipLaunchKernelGGL((i8_gemv_kernel<1, true>), grid, th, 0, st, gb);
-    else if (most == 1) hipLaunchKernelGGL((i8_gemv_kernel<1, false>), grid, th, 0, st, gb);
-    else if (most == 2 && by_row) hipLaunchKernelGGL((i8_gemv_kernel<2, true>), grid, th, 0, st, gb);
-    else if (most == 2) hipLaunchKernelGGL((i8_gemv_kernel<2, false>), grid, th, 0, st, gb);
-    else if (by_row) hipLaunchKernelGGL((i8_gemv_kernel<4, true>), grid, th, 0, st, gb);
-    else hipLaunchKernelGGL((i8_gemv_kernel<4, false>), grid, th, 0, st, gb);
+    if (most == 1) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<1);
+    else if (most == 2) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<2);
+    else VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4);
     return check_launch(fn);
   }
   const I8Scratch c = scratch_of(n, p);
