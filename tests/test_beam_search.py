@@ -141,7 +141,7 @@ def test_refusals():
         with pytest.raises(ValueError):
             BeamSearch(e, s, **kw)
     b = BeamSearch(e, s, 2, max_new_tokens=4)
-    for args in (([[]], 2), ([[1]], 0), ([[1]], 5), ([[1]], 2, [0])):
+    for args in (([[]], 2), ([[1]], 0), ([[1]], 5), ([[1]], 2, [0]), ([[1, V]], 2), ([[0], [-1]], 2)):
         with pytest.raises(ValueError):
             b.generate(*args)
     assert b.generate([], 3) == []

@@ -32,7 +32,8 @@ def linear(*problems, workspace=at(9), nbytes=1 << 30, n=None):
     ({"n": 2 ** 22 + 1}, "sizes"), ({"epilogue": 2}, "epilogue"), ({"epilogue": 9}, "epilogue"), ({"x": None}, "null"),
     ({"w": None}, "null"), ({"ws": None}, "null"), ({"y": None}, "null"), ({"epilogue": 3}, "null"),
     ({"w": at(1) + 8}, "aligned"), ({"y": at(0) + 16}, "overlaps"), ({"y": at(1)}, "overlaps"), ({"y": at(2) + 4}, "overlaps"),
-    ({"y": at(9)}, "workspace"), ({"x": at(9) + 16}, "workspace"), ({"epilogue": 3, "bias": at(3) + 2}, "overlaps")])
+    ({"y": at(9)}, "workspace"), ({"x": at(9) + 16}, "workspace"), ({"w": at(9)}, "workspace"), ({"ws": at(9) + 4}, "workspace"),
+    ({"epilogue": 3, "bias": at(9) + 2}, "workspace"), ({"epilogue": 3, "bias": at(3) + 2}, "overlaps")])
 def test_linear_refuses(change, text):
     assert linear(problem(**change)) == 1 and text in err()
 
@@ -112,7 +113,8 @@ def reorder(B=2, W=3, n_slots=9, slots=at(0), parents=at(1), skip=None, out=at(2
     ({"pools": ((at(4), 2, 60),)}, "multiple of 16"), ({"pools": ((at(4), -1, 64),)}, "layers"),
     ({"pools": ((None, 2, 64),)}, "null"), ({"pools": ((at(4) + 4, 2, 64),)}, "aligned"),
     ({"pools": ((at(4), 2, 64), (at(4) + 64, 2, 64))}, "overlap"), ({"pools": ((at(0), 2, 64),)}, "tables"),
-    ({"pools": ((at(4), 2 ** 20, 2 ** 30), (at(4) + 2 ** 60, 2 ** 20, 2 ** 27))}, "large")])
+    ({"pools": ((at(4), 2 ** 20, 2 ** 30), (at(4) + 2 ** 60, 2 ** 20, 2 ** 27))}, "large"),
+    ({"pools": ((at(4), 2 ** 20, 2 ** 33),), "n_slots": 2 ** 31 - 1}, "large")])
 def test_reorder_refuses(change, text):
     assert reorder(**change) == 1 and text in err()
 
@@ -127,6 +129,12 @@ def test_reorder_sizes():
 
 
 def test_python_refuses():
+    for packed, scales in ((4095, 8), (4096, 7)):
+        with pytest.raises(ValueError, match="packed bytes"):
+            capi.I8Weight(8, 16, torch.zeros(packed, dtype=torch.int8), torch.zeros(scales))
+    one = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="pool 0"):
+        capi.beam_reorder(one, one, one, [torch.zeros(5)])
     w = capi.I8Weight(8, 16, torch.zeros(4096, dtype=torch.int8), torch.zeros(8))
     h = torch.zeros(2, 16, dtype=torch.float16)
     with pytest.raises(ValueError, match="linear_i8_problem"):

@@ -156,11 +156,19 @@ def test_draft_steps_on_8_bit_weights(gpu):
 
 
 def test_refusals(gpu):
-    from vkwr.model_executor import Int8Weights
+    from vkwr.model_executor import Int8Weights, MixedEngine
     cfg, model, _ = _tiny(gpu, 2)
     for names in ((), ("head",), ("key", "key")):
         with pytest.raises(ValueError):
             Int8Weights(model, names)
+    weights = Int8Weights(model)
+    whole, weights.layers = weights.layers, weights.layers[:-1]
+    with pytest.raises(ValueError, match="layers"):
+        MixedEngine(model, 4, int8=weights)
+    weights.layers = whole
+    weights.layers[1]["key"], weights.layers[1]["value"] = weights.layers[1]["value"], weights.layers[1]["key"]
+    with pytest.raises(ValueError, match="sizes"):
+        MixedEngine(model, 4, int8=weights)
 
 
 def _prompts(cfg, seed=2):

@@ -149,6 +149,9 @@ class BeamSearch:
         """prompts: lists of tokens; adapters (engines with adapters): an index per prompt, -1 for none.
         Returns a list of Hypothesis per prompt, the best first (at most `width`)."""
         prompts = [list(p) for p in prompts]
+        vocab = self.engine.cfg.vocab
+        if any(not 0 <= t < vocab for p in prompts for t in p):
+            raise ValueError(f"beam search: a token outside the vocabulary of {vocab}")
         if not all(prompts) or not 1 <= max_new_tokens <= self.max_new_tokens:
             raise ValueError(f"beam search: an empty prompt, or {max_new_tokens} new tokens (1 to {self.max_new_tokens})")
         if adapters is not None and (len(adapters) != len(prompts) or getattr(self.engine, "adapters", None) is None):

@@ -43,6 +43,10 @@ class Int8Step:
     def __init__(self, weights, cfg, max_rows, device):
         self.weights = weights
         C, F = cfg.n_embd, cfg.dim_ffn
+        shapes = {"key": (F, C), "value": (C, F)}
+        if len(weights.layers) != cfg.n_layer or any((w.n, w.k) != shapes.get(n, (C, C)) for L in weights.layers
+                                                     for n, w in L.items()):
+            raise ValueError(f"8-bit weights of {len(weights.layers)} layers, of a model of other sizes than the engine's")
         # (sizes only: a launch has at most the three projections of the time mix, or one of the channel mix)
         need = max(3 * capi.linear_i8_scratch_bytes(max_rows, C), capi.linear_i8_scratch_bytes(max_rows, F))
         self.ws = torch.empty(need, dtype=torch.uint8, device=device)

@@ -661,6 +661,8 @@ class I8Weight:
     """8-bit weights [n, k] laid out for linear_i8, with a scale per output channel."""
 
     def __init__(self, n, k, packed, scale):
+        if packed.numel() != _i8_packed(n, k) or scale.numel() != n:
+            raise ValueError(f"8-bit weights [{n}, {k}]: {packed.numel()} packed bytes, {scale.numel()} scales")
         self.n, self.k, self.packed, self.scale = n, k, packed, scale
 
     @property
@@ -791,7 +793,7 @@ def beam_reorder(slots, parents, slots_out, pools, skip=None):
     at, i32, n = _Tensors(), torch.int32, B * W
     if len(pools) > MAX_BEAM_POOLS:
         raise ValueError(f"beam_reorder: {len(pools)} pools, at most {MAX_BEAM_POOLS}")
-    n_slots = pools[0].shape[1] if pools else 0
+    n_slots = pools[0].shape[1] if pools and pools[0].dim() > 1 else 0
     arr = []
     for t in pools:
         shape = t.shape

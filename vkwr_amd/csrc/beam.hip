@@ -633,6 +633,7 @@ extern "C" int vkwr_beam_reorder(int B, int W, int n_slots, const int32_t* slots
                (long long)p.slot_bytes);
     if (p.layers == 0 || p.slot_bytes == 0 || n_slots == 0) continue;
     VK_REQUIRE(p.base && (uintptr_t)p.base % 16 == 0, "%s: pool %d: null pointer, or not 16-byte aligned", fn, i);
+    VK_REQUIRE(p.layers * p.slot_bytes <= (1ll << 48) / n_slots, "%s: slots too large", fn);  // (no such memory, and no overflow below)
     const int64_t whole = p.layers * p.slot_bytes * n_slots;
     VK_REQUIRE(!overlap(slots_out, nb, p.base, whole) && !overlap(slots, nb, p.base, whole) &&
                    !overlap(parents, nb, p.base, whole) && !(skip && overlap(skip, nb, p.base, whole)),

@@ -955,8 +955,11 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
                "%s: problem %d: null pointer", fn, i);
     VK_REQUIRE((uintptr_t)p[i].w % 16 == 0, "%s: problem %d: w must be 16-byte aligned", fn, i);
     const int64_t ny = 2 * p[i].m * p[i].n;
-    VK_REQUIRE(!overlap(p[i].y, ny, workspace, need) && !overlap(p[i].x, 2 * p[i].m * p[i].k, workspace, need),
-               "%s: problem %d: x or y overlaps the workspace", fn, i);
+    VK_REQUIRE(!overlap(p[i].y, ny, workspace, need) && !overlap(p[i].x, 2 * p[i].m * p[i].k, workspace, need) &&
+                   !overlap(p[i].w, packed_bytes(p[i].n, p[i].k), workspace, need) &&
+                   !overlap(p[i].w_scale, 4 * p[i].n, workspace, need) &&
+                   !(p[i].epilogue == VKWR_GEMM_EPI_BIAS && overlap(p[i].bias, 2 * p[i].n, workspace, need)),
+               "%s: problem %d: a tensor overlaps the workspace", fn, i);
     for (int j = 0; j < n; ++j) {
       if (p[j].m == 0) continue;
       VK_REQUIRE(!overlap(p[i].y, ny, p[j].x, 2 * p[j].m * p[j].k) &&
