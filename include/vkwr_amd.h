@@ -770,7 +770,7 @@ VKWR_EXPORT int vkwr_sampling_verify_drafts(int B, int K, int V, const void* log
  * of a request behind its prompt).  Logits of +inf share the whole probability.  Where fewer than W
  * candidates are left the remaining rows are token -1, parent -1, score -inf, length 0, ended 1.
  * end: -1 for none.  length_penalty 0..16; V up to 2^20; B W up to 65535.  Sums over the vocabulary, scores
- * and comparisons are in 64 bits (terms and sums of 32 terms fp32).  Deterministic, and independent of the
+ * and comparisons are in 64 bits (terms and sums of 16 terms fp32).  Deterministic, and independent of the
  * other requests.  Outputs must not overlap the inputs.  workspace: vkwr_beam_workspace_bytes(B, W, V) bytes
  * (-1 for sizes that are refused), 16-byte aligned, one for each of the calls that may run at the same time.
  * No counterpart in the reference. */

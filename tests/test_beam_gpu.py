@@ -2,7 +2,7 @@
 
 Whole numbers have to be equal.  Scores are rounded to fp32 once (2^-24) behind log-sums whose terms are
 fp32: an exponential is within 2^-22 + |d| 2^-23 of its value (terms with |d| > 16 weigh less than 2^-23),
-a sum of 32 terms within 31 2^-24: below 2^-17 in all.
+a lane's sum of at most 32 terms within 31 2^-24: below 2^-17 in all.
 """
 import math
 

@@ -267,7 +267,10 @@ __device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
 
 // (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
 // KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
-// tiles are added through LDS.
+// tiles are added through LDS: no operand is read twice by a workgroup, and no wave waits for another before
+// the end.  Bound by what a CU takes from its L2 (K 8192, N 2048, m = 433: 1 MiB a
+// workgroup, 16.4 us, 36 - 45 bytes a clock and CU of the 62 that a loop of nothing but loads reaches; the rounding in
+// front of it takes 5), and where K is short by the trips at its ends (K 2048, N 8192, m = 128: 8.0).
 template <int TM, int TN, int NW, int KS, int NB, bool kGridRows, int N>
 __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt) {
   constexpr int kTiles = TM * TN, kG = 64 + 4 / TN;  // 16-byte cells of a group of 4 results, padded: reads hit all banks
@@ -387,7 +390,9 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
 // One workgroup per 32 outputs, whose eight waves share K.  The rows (up to 4, up to 32768 values
 // together) are rounded by every workgroup itself, in LDS, while its first weights are on the way: that
 // costs less than a launch in front of this one.  A lane holds 16 k of one output, and
-// reads the row's 16 values as a broadcast.
+// reads the row's 16 values as a broadcast.  Bound by the weights from memory where they are large (a row of
+// K 4096, N 16384: 13.6 us, 4.9 TB/s with what the last-level cache holds), by one trip to memory and the rounding behind
+// it where they are small (three of K = N = 2048: 4.8 us, of which the bytes are 2.7).
 constexpr int kGemvKeep = 8;                      // 16-byte pieces of x per lane
 constexpr int kGemvMost = kGemvKeep * 512 * 8;    // values of all rows together
 
@@ -834,18 +839,21 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 // The tile that a batch runs with: the smallest whose workgroups fit the (256) CUs at once.  A second
 // round costs more than larger tiles that leave CUs idle, and larger tiles than that
 // leave bandwidth.  us of a whole call, this tile against its neighbours:
-//   32 x 32    K 8192, N 2048, m = 128   14.3; 32 x 64 16.7, 64 x 64 20.3
-//   32 x 64    K = N = 4096, m = 128     12.8; 32 x 32 13.7, 64 x 64 14.4
-//   64 x 64    K 2048, N 8192, m = 128   12.0; 32 x 64 13.5, 64 x 128 12.5
-//   64 x 128   K = N = 4096, m = 433     19.1; 64 x 64 24.3, 128 x 128 21.4
-//   128 x 128  K 8192, N 2048, m = 1100  36.0; 64 x 128 51.6, 128 x 256 51.6
-//   128 x 256  K = N = 4096, m = 1100    34.3; 128 x 128 43.4, 192 x 256 42.4
-//   192 x 256  K = N = 4096, m = 2304    51.9; 128 x 256 69.4, 256 x 256 58.3
-//   256 x 256  K = N = 4096, m = 4096    81.3; 192 x 256 98.9
+//   32 x 32    K 8192, N 2048, m = 128   12.6; 32 x 64 14.9, 64 x 64 18.3
+//   32 x 64    K = N = 4096, m = 128     10.6; 32 x 32 11.6, 64 x 64 12.6
+//   64 x 64    K 2048, N 8192, m = 128   10.2; 32 x 64 11.2, 64 x 128 11.8
+//              K 8192, N 2048, m = 433   20.7; 64 x 128 25.3, 128 x 128 34.0
+//   64 x 128   K = N = 4096, m = 433     17.2; 64 x 64 21.0, 128 x 128 21.6
+//   128 x 128  K 8192, N 2048, m = 1100  36.2; 64 x 128 44.0, 128 x 256 49.1
+//   128 x 256  K = N = 4096, m = 1100    31.3; 128 x 128 41.3, 192 x 256 41.0
+//   192 x 256  K = N = 4096, m = 2304    48.7; 128 x 256 63.2, 256 x 256 58.6
+//   256 x 256  K = N = 4096, m = 4096    76.8; 192 x 256 88.6
 // Beyond one round of the largest: whichever of the last two takes less by its rounds, one of 192
-// rows counted as 0.77 (K 4096, N 16384, m = 2304: three rounds each, 160, 188; three of N 4096: 576 tiles
-// in three rounds 158, 432 in two 148).
-// Up to 32 rows per tile and up to 64 x 64, weights and rows go straight into registers (stream kernel).
+// rows counted as 0.77 (K 4096, N 16384, m = 2304: three rounds each, 145, 179; three of N 4096: 576 tiles
+// in three rounds 142, 432 in two 135).
+// Up to 4 rows the weights pass through the vector units: a row of K = N = 2048, three of them, 4.8 us, on 32 x 32
+// tiles 7.1; 4 rows of K 2048, N 8192 6.3 and 7.6; 4 of K 8192, N 2048 9.0 and 10.9.
+// Up to 64 x 64, weights and rows go straight into registers (stream kernel).
 enum { kRouteGemv, kRouteStream, kRouteTile };
 struct I8Route {
   int kind, rows, cols;  // of a workgroup's tile
