@@ -393,8 +393,8 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
 // reads the row's 16 values as a broadcast.  Bound by the weights from memory where they are large (a row of
 // K 4096, N 16384: 13.6 us, 4.9 TB/s with what the last-level cache holds), by one trip to memory and the rounding behind
 // it where they are small (three of K = N = 2048: 4.8 us, of which the bytes are 2.7).
-constexpr int kGemvKeep = 8;                      // 16-byte pieces of x per lane
-constexpr int kGemvMost = kGemvKeep * 512 * 8;    // values of all rows together
+constexpr int kGemvRows = 8;
+constexpr int gemv_most(int keep) { return keep * 512 * 8; }  // values of all rows at `keep` 16-byte pieces a lane
 
 struct GProb {
   const _Float16* x;
@@ -406,12 +406,13 @@ struct GProb {
 };
 typedef BatchOf<GProb, kMaxI8> GBatch;
 
-template <int M, bool kGridRows, int N>
+template <int M, int kKeep, bool kGridRows, int N>
 __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   constexpr int kWaves = 8, kPer = kWaves / M, kAhead = 8;  // waves of a row; blocks of weights in flight
-  __shared__ __attribute__((aligned(16))) int8_t xq[kGemvMost + M * kI8Pad];
+  constexpr int kSkew = 32;  // bytes between rows, so that a read of a block's 32 k of 8 rows hits all banks
+  __shared__ __attribute__((aligned(16))) int8_t xq[gemv_most(kKeep) + M * (kI8Pad + kSkew)];
   __shared__ uint32_t wtop[kWaves];
-  __shared__ int part[kWaves][M][32];
+  __shared__ __attribute__((aligned(16))) int part[kWaves][M][32];
   const GProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
   asm volatile("" ::"s"(P.x), "s"(P.w), "s"(P.t), "s"(P.bias), "s"(P.y), "s"(P.m), "s"(P.n), "s"(P.k), "s"(P.steps), "s"(P.epi),
                "s"(P.wg_begin));
@@ -429,10 +430,10 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   // ---- this wave's pieces of 8 values of its row
   const int row = min(wave / kPer, P.m - 1), w0 = wave % kPer, pieces = kpad / 8;
   const _Float16* const x = P.x + (int64_t)row * k;
-  uv4 v[kGemvKeep];
+  uv4 v[kKeep];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kGemvKeep; ++i) {
+  for (int i = 0; i < kKeep; ++i) {
     const int c = (i * kPer + w0) * 64 + lane;
     v[i] = load8(x, (int64_t)c * 8, k);
   }
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int i = 0; i < kGemvKeep; ++i)
+  for (int i = 0; i < kKeep; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = max_u16x2(top, v[i][e] & 0x7fff7fffu);
   top = max(top & 0xffffu, top >> 16);
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   {
     const float a = top < 0x7c00u ? h2f((uint16_t)top) : 0.0f, inv = a > 0.0f ? 1.0f / a : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kGemvKeep; ++i) {
+    for (int i = 0; i < kKeep; ++i) {
       const int c = (i * kPer + w0) * 64 + lane;
       if (c < pieces) {
         typedef _Float16 h2v __attribute__((ext_vector_type(2)));
@@ -472,19 +473,20 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
             o[h] = quant4(f, a, inv);
           }
         }
-        *reinterpret_cast<uint64_t*>(xq + wave / kPer * kpad + c * 8) = (uint64_t)o[1] << 32 | o[0];
+        *reinterpret_cast<uint64_t*>(xq + wave / kPer * (kpad + kSkew) + c * 8) = (uint64_t)o[1] << 32 | o[0];
       }
     }
   }
   __syncthreads();
-  int acc[M] = {};
-  const int8_t* const xl = xq + (lane >> 5) * 16;
+  typename std::conditional<M == 1, int, iv16>::type acc = {0};
+  const int8_t* const xl = xq + min(lane & 31, M - 1) * (kpad + kSkew) + (lane >> 5) * 16;
   auto dot = [&](const iv4& b, int st) __attribute__((always_inline)) {
+    const iv4 a = *reinterpret_cast<const iv4*>(xl + st * 32);
+    if constexpr (M == 1) {
 #pragma unroll
-    for (int r = 0; r < M; ++r) {
-      const iv4 a = *reinterpret_cast<const iv4*>(xl + r * kpad + st * 32);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[r] = __builtin_amdgcn_sdot4(a[e], b[e], acc[r], false);
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_sdot4(a[e], b[e], acc, false);
+    } else {
+      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(b, a, acc, 0, 0, 0);
     }
   };
   // a block's registers take the block kAhead rounds further as soon as it is done (a row of K 16384, N 4096: 16.1 us;
@@ -503,10 +505,14 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
 #pragma unroll
   for (int a = 0; a < kAhead; ++a)
     if (s0 + a * kWaves < steps) dot(fw[a], s0 + a * kWaves);
+  if constexpr (M == 1) {
+    acc += __shfl_xor(acc, 32, 64);
+    if (lane < 32) part[wave][0][lane] = acc;
+  } else if ((lane & 31) < M) {
 #pragma unroll
-  for (int r = 0; r < M; ++r) {
-    acc[r] += __shfl_xor(acc[r], 32, 64);
-    if (lane < 32) part[wave][r][lane] = acc[r];
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<iv4*>(&part[wave][lane & 31][8 * g + 4 * (lane >> 5)]) =
+          iv4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
   }
   __syncthreads();
   if (!out) return;
@@ -864,10 +870,13 @@ constexpr I8Route kI8Routes[] = {{kRouteStream, 32, 32}, {kRouteStream, 32, 64},
 I8Route pick_route(int n, const vkwr_i8_problem* p) {
   int64_t most = 0;
   for (int i = 0; i < n; ++i) most = std::max(most, p[i].m);
-  bool gemv = most <= 4;
-  for (int i = 0; i < n; ++i)
-    if (gemv && p[i].m > 0) gemv = (most == 1 ? 1 : most == 2 ? 2 : 4) * up(p[i].k, kI8Pad) <= kGemvMost;
-  if (gemv) return {kRouteGemv, 4, 32};
+  if (most <= kGemvRows) {
+    int64_t values = 0;
+    for (int i = 0; i < n; ++i)
+      if (p[i].m > 0) values = std::max(values, (most <= 2 ? most : most <= 4 ? 4 : 8) * up(p[i].k, kI8Pad));
+    if (values <= gemv_most(8)) return {kRouteGemv, (int)most, 8};
+    if (values <= gemv_most(16) && most > 2) return {kRouteGemv, (int)most, 16};
+  }
   const int64_t cus = device_cus();
   int64_t tiles[8];
   for (int r = 0; r < 8; ++r) {
@@ -1004,9 +1013,12 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
       wgs += (p[i].n + 31) / 32;
       most = std::max(most, P.m);
     }
-    if (most == 1) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<1);
-    else if (most == 2) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<2);
-    else VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4);
+    if (most == 1) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<1, 8);
+    else if (most == 2) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<2, 8);
+    else if (most <= 4 && route.cols == 8) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4, 8);
+    else if (most <= 4) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4, 16);
+    else if (route.cols == 8) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<8, 8);
+    else VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<8, 16);
     return check_launch(fn);
   }
   const I8Scratch c = scratch_of(n, p);
