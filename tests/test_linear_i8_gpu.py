@@ -69,6 +69,24 @@ def test_matches_formula(m, n, k):
     close(y, *expected(x, wq, t, "none", None), f"{m}x{n}x{k}")
 
 
+# one size for each tile on 256 CUs, from 16 x 16 to 256 x 256, with an odd last row and column tile each, and
+# the largest rows that are rounded by the kernel that multiplies them
+TILES = [(9, 501, 200), (20, 2101, 140), (40, 3005, 200), (70, 3001, 330), (130, 5003, 260), (250, 5003, 200), (500, 5001, 136),
+         (1000, 5001, 130), (2050, 5001, 72), (2400, 5001, 72), (4100, 5001, 64), (8, 77, 4096), (5, 77, 4097), (4, 45, 8192),
+         (3, 45, 8193), (2, 33, 16384), (1, 33, 32768), (6, 90, 640)]
+
+
+@pytest.mark.parametrize("m,n,k", TILES)
+def test_every_tile(m, n, k):
+    x, (wq, t) = rand(m, k, seed=m).half(), weights(n, k, seed=n)
+    bias = rand(n, seed=3).half()
+    out = torch.full((m * n + 64,), 5.0, dtype=torch.float16, device="cuda")
+    y = out[:m * n].view(m, n)
+    capi.linear_i8([capi.linear_i8_problem(x.cuda(), capi.i8_weight(wq.cuda(), t.cuda()), y, capi.EPI_BIAS, bias.cuda())])
+    close(y, *expected(x, wq, t, "bias", bias), f"{m}x{n}x{k}")
+    assert (out[m * n:] == 5).all()
+
+
 @pytest.mark.parametrize("epi", sorted(EPI))
 @pytest.mark.parametrize("m,n,k", [(1, 2048, 512), (3, 37, 100), (40, 200, 384), (150, 1001, 260), (300, 640, 512)])
 def test_epilogues(m, n, k, epi):

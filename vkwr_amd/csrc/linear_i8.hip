@@ -265,17 +265,20 @@ __device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
   }
 }
 
-// (32 TM) rows x (32 TN) outputs per workgroup over the whole of K: the NW waves take the blocks of
-// KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
+// (S TM) rows x (S TN) outputs per workgroup, S = 16 or 32 (the matrix instruction's), over the whole of K: the NW
+// waves take the blocks of KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
 // tiles are added through LDS: no operand is read twice by a workgroup, and no wave waits for another before
 // the end.  Bound by what a CU takes from its L2 (K 8192, N 2048, m = 433: 1 MiB a
 // workgroup, 16.4 us, 36 - 45 bytes a clock and CU of the 62 that a loop of nothing but loads reaches; the rounding in
 // front of it takes 5), and where K is short by the trips at its ends (K 2048, N 8192, m = 128: 8.0).
-template <int TM, int TN, int NW, int KS, int NB, bool kGridRows, int N>
+template <int S, int TM, int TN, int NW, int KS, int NB, bool kGridRows, int N>
 __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt) {
   constexpr int kTiles = TM * TN, kG = 64 + 4 / TN;  // 16-byte cells of a group of 4 results, padded: reads hit all banks
-  static_assert(kTiles * 128 <= NW * 64, "one piece of the output per thread");
-  __shared__ __attribute__((aligned(16))) iv4 red[NW * kTiles * 4 * kG];
+  constexpr int kRegs = S * S / 64, kGroups = kRegs / 4, kOuts = S / 8;  // of a tile: a lane's results, groups; a row's eights
+  constexpr int kStep = 1024 / S;                                        // k of an instruction
+  static_assert(kTiles * S * kOuts <= NW * 64, "one piece of the output per thread");
+  typedef int Acc __attribute__((ext_vector_type(kRegs)));
+  __shared__ __attribute__((aligned(16))) iv4 red[NW * kTiles * kGroups * kG];
   const IProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
   asm volatile("" ::"s"(P.q), "s"(P.s), "s"(P.w), "s"(P.t), "s"(P.bias), "s"(P.y), "s"(P.m), "s"(P.n), "s"(P.steps), "s"(P.epi),
                "s"(P.nmb), "s"(P.ncol), "s"(P.wg_begin));
@@ -284,11 +287,12 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
   const int mb = (lt >> 3) % P.nmb, cb = (lt >> 3) / P.nmb * 8 + (lt & 7);
   if (cb >= P.ncol) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int steps = P.steps, mblk = (P.m + 31) >> 5, nblk = (P.n + 31) >> 5;
+  const int steps = P.steps * 32 / kStep, mblk = (P.m + S - 1) / S, nblk = (P.n + S - 1) / S;
   // this thread's eight outputs, and their scales, requested before everything else
-  const int og = threadIdx.x & 3, ot = (threadIdx.x >> 2) % TN + threadIdx.x / (4 * TN * 32) * TN, orow = (threadIdx.x / (4 * TN)) & 31;
-  const int row = (mb * TM + ot / TN) * 32 + orow, col = (cb * TN + ot % TN) * 32 + 8 * og;
-  const bool out = threadIdx.x < kTiles * 128 && row < P.m && col < P.n;
+  const int og = threadIdx.x % kOuts, ot = threadIdx.x / kOuts % TN + threadIdx.x / (kOuts * TN * S) * TN;
+  const int orow = threadIdx.x / (kOuts * TN) % S;
+  const int row = (mb * TM + ot / TN) * S + orow, col = (cb * TN + ot % TN) * S + 8 * og;
+  const bool out = threadIdx.x < kTiles * S * kOuts && row < P.m && col < P.n;
   float os = 0.0f, ts[8], bs[8] = {};
   if (out) {
     os = P.s[row];
@@ -299,21 +303,27 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
       if (P.epi == VKWR_GEMM_EPI_BIAS) bs[e] = (float)P.bias[c];
     }
   }
-  const int8_t *xp[TM], *wp[TN];  // blocks past the last are read as the last
+  // block u's first operand (S = 16: lane l holds row l % 16, k 16 (l / 16) .. + 15, of two packed blocks); blocks
+  // past the last are read as the last
+  auto operand = [&](const int8_t* q, int u) __attribute__((always_inline)) {
+    if constexpr (S == 32) return q + (int64_t)u * P.steps * 1024 + lane * 16;
+    else return q + (int64_t)(u >> 1) * P.steps * 1024 + (lane >> 4) * 512 + ((u & 1) * 16 + (lane & 15)) * 16;
+  };
+  const int8_t *xp[TM], *wp[TN];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) xp[i] = P.q + (int64_t)min(mb * TM + i, mblk - 1) * steps * 1024 + lane * 16;
+  for (int i = 0; i < TM; ++i) xp[i] = operand(P.q, min(mb * TM + i, mblk - 1));
 #pragma unroll
-  for (int j = 0; j < TN; ++j) wp[j] = P.w + (int64_t)min(cb * TN + j, nblk - 1) * steps * 1024 + lane * 16;
-  iv16 acc[TM][TN];
+  for (int j = 0; j < TN; ++j) wp[j] = operand(P.w, min(cb * TN + j, nblk - 1));
+  Acc acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = iv16{0};
+    for (int j = 0; j < TN; ++j) acc[i][j] = Acc{0};
   iv4 fx[NB][KS][TM], fw[NB][KS][TN];
   auto load = [&](int buf, int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int64_t o = ((int64_t)(wave + b * NW) * KS + s) * 1024;
+      const int64_t o = ((int64_t)(wave + b * NW) * KS + s) * (kStep * 32);
 #pragma unroll
       for (int j = 0; j < TN; ++j) fw[buf][s][j] = *reinterpret_cast<const iv4*>(wp[j] + o);
 #pragma unroll
@@ -326,10 +336,12 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[buf][s][j], fx[buf][s][i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < TN; ++j) {
+          if constexpr (S == 32) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[buf][s][j], fx[buf][s][i], acc[i][j], 0, 0, 0);
+          else acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[buf][s][j], fx[buf][s][i], acc[i][j], 0, 0, 0);
+        }
   };
-  static_assert(kI8Pad % (32 * KS) == 0, "whole blocks");
+  static_assert(kI8Pad % (kStep * KS) == 0, "whole blocks");
   const int blocks = steps / KS, nb = (blocks - wave + NW - 1) / NW;  // this wave's blocks
   if (nb >= NB) {
     // no load here or in the loop is behind a condition, so that the waits in it are exact: with the first
@@ -367,17 +379,19 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const iv16& a = acc[t / TN][t % TN];
-      red[((wave * kTiles + t) * 4 + g) * kG + lane] = iv4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+    for (int g = 0; g < kGroups; ++g) {
+      const Acc& a = acc[t / TN][t % TN];
+      red[((wave * kTiles + t) * kGroups + g) * kG + lane] = iv4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
     }
   __syncthreads();
   if (!out) return;
+  // eight outputs are two cells: S lanes apart in group og, or in the one group there is
   iv4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    lo += red[((w * kTiles + ot) * 4 + og) * kG + orow];
-    hi += red[((w * kTiles + ot) * 4 + og) * kG + orow + 32];
+    const int at = (w * kTiles + ot) * kGroups * kG + (S == 32 ? og * kG : 2 * og * S) + orow;
+    lo += red[at];
+    hi += red[at + S];
   }
   const int sum[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   hv8 h;
@@ -385,16 +399,19 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
   store8((gptr)(P.y + (int64_t)row * P.n + col), h, P.n - col);
 }
 
-// ---- few rows: the weights pass through once, four products an instruction
+// ---- few rows: rounded by the kernel that multiplies them
 //
-// One workgroup per 32 outputs, whose eight waves share K.  The rows (up to 4, up to 32768 values
+// One workgroup per 32 outputs, whose eight waves share K.  The rows (up to 8, up to 32768 values
 // together) are rounded by every workgroup itself, in LDS, while its first weights are on the way: that
-// costs less than a launch in front of this one.  A lane holds 16 k of one output, and
-// reads the row's 16 values as a broadcast.  Bound by the weights from memory where they are large (a row of
-// K 4096, N 16384: 13.6 us, 4.9 TB/s with what the last-level cache holds), by one trip to memory and the rounding behind
-// it where they are small (three of K = N = 2048: 4.8 us, of which the bytes are 2.7).
+// costs less than a launch in front of this one.  One row is multiplied four k an instruction, a lane holding 16 k of one
+// output and reading the row's 16 values as a broadcast; more by the matrix cores, most of whose columns repeat the
+// last row (with four k an instruction 4 rows of K 8192, N 2048 took 9.0 us, so 7.8).  Bound by the weights from
+// memory where they are large (a row of K 4096, N 16384: 13.6 us, 4.9 TB/s with what the last-level cache holds), by one
+// trip to memory and the rounding behind it where they are small (three of K = N = 2048: 4.8 us, of which
+// the bytes are 2.7).
 constexpr int kGemvRows = 8;
-constexpr int gemv_most(int keep) { return keep * 512 * 8; }  // values of all rows at `keep` 16-byte pieces a lane
+constexpr int kGemvKeep = 8;                    // 16-byte pieces of x per lane
+constexpr int kGemvMost = kGemvKeep * 512 * 8;  // values of all rows together
 
 struct GProb {
   const _Float16* x;
@@ -406,11 +423,11 @@ struct GProb {
 };
 typedef BatchOf<GProb, kMaxI8> GBatch;
 
-template <int M, int kKeep, bool kGridRows, int N>
+template <int M, bool kGridRows, int N>
 __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   constexpr int kWaves = 8, kPer = kWaves / M, kAhead = 8;  // waves of a row; blocks of weights in flight
   constexpr int kSkew = 32;  // bytes between rows, so that a read of a block's 32 k of 8 rows hits all banks
-  __shared__ __attribute__((aligned(16))) int8_t xq[gemv_most(kKeep) + M * (kI8Pad + kSkew)];
+  __shared__ __attribute__((aligned(16))) int8_t xq[kGemvMost + M * (kI8Pad + kSkew)];
   __shared__ uint32_t wtop[kWaves];
   __shared__ __attribute__((aligned(16))) int part[kWaves][M][32];
   const GProb P = bt.p[problem_of<kGridRows>(bt, blockIdx.x)];
@@ -430,10 +447,10 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   // ---- this wave's pieces of 8 values of its row
   const int row = min(wave / kPer, P.m - 1), w0 = wave % kPer, pieces = kpad / 8;
   const _Float16* const x = P.x + (int64_t)row * k;
-  uv4 v[kKeep];
+  uv4 v[kGemvKeep];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
+  for (int i = 0; i < kGemvKeep; ++i) {
     const int c = (i * kPer + w0) * 64 + lane;
     v[i] = load8(x, (int64_t)c * 8, k);
   }
@@ -447,7 +464,7 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i)
+  for (int i = 0; i < kGemvKeep; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = max_u16x2(top, v[i][e] & 0x7fff7fffu);
   top = max(top & 0xffffu, top >> 16);
@@ -460,7 +477,7 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
   {
     const float a = top < 0x7c00u ? h2f((uint16_t)top) : 0.0f, inv = a > 0.0f ? 1.0f / a : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
+    for (int i = 0; i < kGemvKeep; ++i) {
       const int c = (i * kPer + w0) * 64 + lane;
       if (c < pieces) {
         typedef _Float16 h2v __attribute__((ext_vector_type(2)));
@@ -845,6 +862,9 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 // The tile that a batch runs with: the smallest whose workgroups fit the (256) CUs at once.  A second
 // round costs more than larger tiles that leave CUs idle, and larger tiles than that
 // leave bandwidth.  us of a whole call, this tile against its neighbours:
+//   16 x 16    K 8192, N 2048, m = 9     8.7; 16 x 32 9.7, 32 x 32 10.7
+//              K 16384, N 4096, m = 9    17.7; 16 x 32 19.9, 32 x 32 23.9
+//   16 x 32    K 16384, N 4096, m = 32   20.8; 16 x 16 22.6, 32 x 32 25.6
 //   32 x 32    K 8192, N 2048, m = 128   12.6; 32 x 64 14.9, 64 x 64 18.3
 //   32 x 64    K = N = 4096, m = 128     10.6; 32 x 32 11.6, 64 x 64 12.6
 //   64 x 64    K 2048, N 8192, m = 128   10.2; 32 x 64 11.2, 64 x 128 11.8
@@ -857,15 +877,18 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 // Beyond one round of the largest: whichever of the last two takes less by its rounds, one of 192
 // rows counted as 0.77 (K 4096, N 16384, m = 2304: three rounds each, 145, 179; three of N 4096: 576 tiles
 // in three rounds 142, 432 in two 135).
-// Up to 4 rows the weights pass through the vector units: a row of K = N = 2048, three of them, 4.8 us, on 32 x 32
-// tiles 7.1; 4 rows of K 2048, N 8192 6.3 and 7.6; 4 of K 8192, N 2048 9.0 and 10.9.
+// Up to 8 rows of 32768 values together are rounded by the kernel that multiplies them: three of K = N = 2048, 1 row
+// 4.8 us, on tiles 7.1; 8 rows 6.0 and 7.4; 5 of K = N = 4096 7.1 and 7.8; 4 of K 8192, N 2048 7.8 and 8.5.  With
+// twice as many values (8 rows of K 8192: 10.1 and 8.7) the rounding costs more than its launch.
 // Up to 64 x 64, weights and rows go straight into registers (stream kernel).
 enum { kRouteGemv, kRouteStream, kRouteTile };
 struct I8Route {
   int kind, rows, cols;  // of a workgroup's tile
 };
-constexpr I8Route kI8Routes[] = {{kRouteStream, 32, 32}, {kRouteStream, 32, 64},  {kRouteStream, 64, 64}, {kRouteTile, 64, 128},
-                                 {kRouteTile, 128, 128}, {kRouteTile, 128, 256}, {kRouteTile, 192, 256}, {kRouteTile, 256, 256}};
+constexpr I8Route kI8Routes[] = {{kRouteStream, 16, 16}, {kRouteStream, 16, 32}, {kRouteStream, 32, 32}, {kRouteStream, 32, 64},
+                                 {kRouteStream, 64, 64}, {kRouteTile, 64, 128},  {kRouteTile, 128, 128}, {kRouteTile, 128, 256},
+                                 {kRouteTile, 192, 256}, {kRouteTile, 256, 256}};
+constexpr int kI8RouteCount = sizeof(kI8Routes) / sizeof(kI8Routes[0]);
 
 I8Route pick_route(int n, const vkwr_i8_problem* p) {
   int64_t most = 0;
@@ -874,17 +897,17 @@ I8Route pick_route(int n, const vkwr_i8_problem* p) {
     int64_t values = 0;
     for (int i = 0; i < n; ++i)
       if (p[i].m > 0) values = std::max(values, (most <= 2 ? most : most <= 4 ? 4 : 8) * up(p[i].k, kI8Pad));
-    if (values <= gemv_most(8)) return {kRouteGemv, (int)most, 8};
-    if (values <= gemv_most(16) && most > 2) return {kRouteGemv, (int)most, 16};
+    if (values <= kGemvMost) return {kRouteGemv, kGemvRows, 32};
   }
   const int64_t cus = device_cus();
-  int64_t tiles[8];
-  for (int r = 0; r < 8; ++r) {
+  int64_t tiles[kI8RouteCount];
+  for (int r = 0; r < kI8RouteCount; ++r) {
     tiles[r] = 0;
     for (int i = 0; i < n; ++i) tiles[r] += up(p[i].m, kI8Routes[r].rows) / kI8Routes[r].rows * (up(p[i].n, kI8Routes[r].cols) / kI8Routes[r].cols);
     if (tiles[r] <= cus) return kI8Routes[r];
   }
-  return kI8Routes[0.77 * (double)((tiles[6] + cus - 1) / cus) < (double)((tiles[7] + cus - 1) / cus) ? 6 : 7];
+  constexpr int a = kI8RouteCount - 2, b = kI8RouteCount - 1;
+  return kI8Routes[0.77 * (double)((tiles[a] + cus - 1) / cus) < (double)((tiles[b] + cus - 1) / cus) ? a : b];
 }
 
 #define VK_I8_TILE(tm, tn, nbuf) \
@@ -892,9 +915,11 @@ I8Route pick_route(int n, const vkwr_i8_problem* p) {
 
 void launch_products(const I8Route& r, const IBatch& b, int wgs, hipStream_t s) {
   if (r.kind == kRouteStream) {
-    if (r.rows == 64) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<2, 2, 8, 1, 4);
-    else if (r.cols == 64) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<1, 2, 8, 2, 4);
-    else VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<1, 1, 8, 2, 4);
+    if (r.rows == 64) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<32, 2, 2, 8, 1, 4);
+    else if (r.cols == 64) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<32, 1, 2, 8, 2, 4);
+    else if (r.rows == 32) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<32, 1, 1, 8, 2, 4);
+    else if (r.cols == 32) VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<16, 1, 2, 8, 2, 4);
+    else VK_I8_LAUNCH(b, wgs, 512, s, i8_stream_kernel<16, 1, 1, 8, 2, 4);
   } else if (r.rows == 64) {
     VK_I8_TILE(1, 2, 6);
   } else if (r.rows == 128) {
@@ -1013,12 +1038,10 @@ extern "C" int vkwr_linear_i8_f16(int n_problems, const vkwr_i8_problem* problem
       wgs += (p[i].n + 31) / 32;
       most = std::max(most, P.m);
     }
-    if (most == 1) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<1, 8);
-    else if (most == 2) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<2, 8);
-    else if (most <= 4 && route.cols == 8) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4, 8);
-    else if (most <= 4) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4, 16);
-    else if (route.cols == 8) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<8, 8);
-    else VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<8, 16);
+    if (most == 1) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<1);
+    else if (most == 2) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<2);
+    else if (most <= 4) VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<4);
+    else VK_I8_LAUNCH(gb, wgs, 512, st, i8_gemv_kernel<8);
     return check_launch(fn);
   }
   const I8Scratch c = scratch_of(n, p);
