@@ -269,8 +269,8 @@ __device__ __forceinline__ void store8(gptr o, const hv8& h, int left) {
 // waves take the blocks of KS k-steps w, w + NW, ... with NB blocks' loads in flight, straight into registers, and the NW partial
 // tiles are added through LDS: no operand is read twice by a workgroup, and no wave waits for another before
 // the end.  Bound by what a CU takes from its L2 (K 8192, N 2048, m = 433: 1 MiB a
-// workgroup, 16.4 us, 36 - 45 bytes a clock and CU of the 62 that a loop of nothing but loads reaches; the rounding in
-// front of it takes 5), and where K is short by the trips at its ends (K 2048, N 8192, m = 128: 8.0).
+// workgroup, 15.4 us, 36 - 45 bytes a clock and CU of the 62 that a loop of nothing but loads reaches; the rounding in
+// front of it takes 5), and where K is short by the trips at its ends (K 2048, N 8192, m = 128: 7.9).
 template <int S, int TM, int TN, int NW, int KS, int NB, bool kGridRows, int N>
 __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt) {
   constexpr int kTiles = TM * TN, kG = 64 + 4 / TN;  // 16-byte cells of a group of 4 results, padded: reads hit all banks
