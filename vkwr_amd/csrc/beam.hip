@@ -436,7 +436,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
 
 // ---------------------------------------------------------------- states behind the beams
 
-constexpr int kMaxPools = 8;
+constexpr int kMaxPools = 8, kFewPools = 3;
 constexpr int kCopyThreads = 256;
 constexpr int kCopyBytes = 16384;  // of a work item: one 64 x 64 fp32 block
 constexpr int kMaxChildren = 4096;
@@ -446,18 +446,21 @@ struct RPool {
   int64_t layer_stride, slot_bytes;  // slot_bytes: of one layer; slots are that far apart
   int layers, pieces;                // work items of a layer's slot
 };
+// Room for N pools: the host takes longer for more bytes of arguments (3 pools 2.9 us, 8 pools 3.2).
+template <int N>
 struct RArgs {
-  int W, children, n_pools, n_slots;
+  int W, children, n_slots;
   const int32_t *slots, *parents, *skip;
   int32_t* slots_out;
   int items;  // work items of a slot: all pools, all layers
-  RPool p[kMaxPools];
+  RPool p[N];
 };
 
 // Every workgroup works the copies out by itself (up to 4096 children, in LDS: a launch of its own for that
 // would cost more), then they share the work items out evenly.  Bound by memory: 16 x 8 beams of a 24-layer state, 1.1 GB
 // moved, 246 us at 4.5 TB/s, which is what a large copy reaches; a small one by its launch (4.7 us).
-__global__ __launch_bounds__(kCopyThreads) void beam_reorder_kernel(RArgs a) {
+template <int N>
+__global__ __launch_bounds__(kCopyThreads) void beam_reorder_kernel(RArgs<N> a) {
   extern __shared__ __attribute__((aligned(16))) int lds[];
   int* const par = lds;                   // [children]: parent, or -1 where no state goes along
   int2* const moves = reinterpret_cast<int2*>(lds + ((a.children + 1) & ~1));  // [children]: from slot, to slot
@@ -619,10 +622,9 @@ extern "C" int vkwr_beam_reorder(int B, int W, int n_slots, const int32_t* slots
   VK_REQUIRE(!overlap(slots_out, nb, slots, nb) && !overlap(slots_out, nb, parents, nb) &&
                  !(skip && overlap(slots_out, nb, skip, nb)),
              "%s: slots_out overlaps an input", fn);
-  RArgs a{};
+  RArgs<kMaxPools> a{};
   a.W = W;
   a.children = B * W;
-  a.n_pools = n_pools;
   a.n_slots = n_slots;
   a.slots = slots;
   a.parents = parents;
@@ -658,6 +660,12 @@ extern "C" int vkwr_beam_reorder(int B, int W, int n_slots, const int32_t* slots
   const int64_t most = items * (int64_t)B * std::max(0, W - 1);
   const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, 8 * device_cus()));
   const size_t lds = (size_t)((a.children + 1) & ~1) * 4 + (size_t)a.children * 8;
-  hipLaunchKernelGGL(beam_reorder_kernel, dim3(grid), dim3(kCopyThreads), lds, (hipStream_t)stream, a);
+  if (n_pools <= kFewPools) {
+    RArgs<kFewPools> few{a.W, a.children, a.n_slots, slots, parents, skip, slots_out, a.items, {}};
+    std::copy(a.p, a.p + kFewPools, few.p);
+    hipLaunchKernelGGL(beam_reorder_kernel<kFewPools>, dim3(grid), dim3(kCopyThreads), lds, (hipStream_t)stream, few);
+  } else {
+    hipLaunchKernelGGL(beam_reorder_kernel<kMaxPools>, dim3(grid), dim3(kCopyThreads), lds, (hipStream_t)stream, a);
+  }
   return check_launch(fn);
 }
