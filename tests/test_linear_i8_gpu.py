@@ -73,7 +73,8 @@ def test_matches_formula(m, n, k):
 # the largest rows that are rounded by the kernel that multiplies them
 TILES = [(9, 501, 200), (20, 2101, 140), (40, 3005, 200), (70, 3001, 330), (130, 5003, 260), (250, 5003, 200), (500, 5001, 136),
          (1000, 5001, 130), (2050, 5001, 72), (2400, 5001, 72), (4100, 5001, 64), (8, 77, 4096), (5, 77, 4097), (4, 45, 8192),
-         (3, 45, 8193), (2, 33, 16384), (1, 33, 32768), (6, 90, 640)]
+         (3, 45, 8193), (2, 33, 16384), (1, 33, 32768), (6, 90, 640),
+         (16, 77, 2048), (11, 45, 2040), (13, 100, 2049), (9, 2101, 140)]
 
 
 @pytest.mark.parametrize("m,n,k", TILES)
