@@ -664,8 +664,10 @@ VKWR_EXPORT int vkwr_i8_quantize_rows_f16(int64_t rows, int64_t k, const uint16_
 /* One layer of a batch: y[i, j] = epilogue(s_i w_scale[j] sum_k q_ik w_jk), x [m, k] fp16 rounded to
  * q and s row by row as vkwr_i8_quantize_rows_f16 does, w a packed matrix [n, k], y [m, n] fp16.  Sums are
  * exact (int32), scaled in fp32 and rounded to fp16 once.  Epilogues: VKWR_GEMM_EPI_NONE, _RELU_SQUARE,
- * _BIAS (+ bias[j] fp16), _TANH, _SIGMOID.  A row of x with an infinity or a NaN gives a row of NaN.  Any
- * n and k, up to 2^22 rows in a call; x, y contiguous, of any alignment. */
+ * _BIAS (+ bias[j] fp16), _TANH, _SIGMOID.  A row of x with an infinity or a NaN gives a row of NaN.
+ * w_scale of either sign and any finite size (results beyond fp16's range are infinities; a NaN in it makes its
+ * column NaN, an infinity there counts as 2^86).  Any n and k, up to 2^22 rows in a call; x, y contiguous,
+ * of any alignment. */
 typedef struct vkwr_i8_problem {
   const uint16_t* x;
   const int8_t* w;

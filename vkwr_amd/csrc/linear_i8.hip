@@ -226,6 +226,14 @@ struct IProb {
 };
 typedef BatchOf<IProb, kMaxI8> IBatch;
 
+// A weight scale as the products use it: within 2^86, so that s t and the scaled sum stay finite (s < 2^10,
+// |sum| < 2^31), and neither a sum of 0 nor a negative one under the square meets an infinity.  No output
+// changes: from a scale of 2^86 on every other sum (s >= 2^-31) scales to 2^55 and more, which each epilogue takes
+// to the end of its range.  (Two instructions; NaN stays.)
+__device__ __forceinline__ float column_scale(float t) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_minimum(t, 0x1p86f), -0x1p86f);
+}
+
 // N outputs: the sums scaled in fp32 (+ bias), the epilogue, one rounding to fp16.  Every kernel finishes its
 // sums here, so that a row's bits do not depend on which one ran.  One branch for all N: with one for
 // each, the code of the functions lay N times between the outputs.
@@ -393,6 +401,8 @@ __global__ __launch_bounds__(NW * 64) void i8_stream_kernel(BatchOf<IProb, N> bt
     lo += red[at];
     hi += red[at + S];
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ts[e] = column_scale(ts[e]);
   const int sum[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   hv8 h;
   i8_finish(sum, os, ts, P.epi, bs, h);
@@ -540,6 +550,7 @@ __global__ __launch_bounds__(512) void i8_gemv_kernel(BatchOf<GProb, N> bt) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) all = max(all, wtop[orow * kPer + i]);
   const float s = all < 0x7c00u ? h2f((uint16_t)all) / 127.0f : __builtin_nanf("");
+  ts[0] = column_scale(ts[0]);
   _Float16 h[1];
   i8_finish(sums, s, ts, P.epi, bs, h);
   P.y[(int64_t)orow * P.n + ocol] = h[0];
@@ -593,7 +604,7 @@ __device__ __forceinline__ void i8_store(char* st, const IProb& P, const iv16 (&
   for (int c = 0; c < 32 * TN; c += 64) {
     if (c + lane < 32 * TN) {
       const int col = min(col0 + c + lane, n - 1);
-      tl[c + lane] = tp[col];
+      tl[c + lane] = column_scale(tp[col]);
       if constexpr (kEpi == VKWR_GEMM_EPI_BIAS) tl[32 * TN + c + lane] = (float)bp[col];
     }
   }
