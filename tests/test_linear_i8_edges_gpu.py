@@ -1,4 +1,5 @@
-"""Linear layers with 8-bit weights where the other tests do not go: scales near the end of fp32's range.
+"""Linear layers with 8-bit weights where the other tests do not go: scales near the end of fp32's range, rows up to the
+largest K, and on the tile kernel many stages, every epilogue, several problems, and rows of zeros, infinities and NaN.
 
 Tolerances as in test_linear_i8_gpu, whose formula in 64 bits is used here; results beyond fp16's range are infinities.
 tanh and the sigmoid move by at most 0.45 of their argument's relative error (x / cosh(x)^2 <= 0.45), however large it is.
@@ -52,3 +53,151 @@ def test_large_weight_scales(m, n, epi):
     ref, tol = (v.cpu() for v in expected(x, wq, t, epi, bias))
     assert ref.isfinite().all() and (ref == 0).any() | (epi in ("bias", "sigmoid"))
     close16(y, ref, tol, epi)
+
+
+# ---------------------------------------------------------------- the tile kernel's other uses
+
+@pytest.mark.parametrize("epi", sorted(EPI))
+@pytest.mark.parametrize("m,n", TILE_ROUTES)
+def test_many_stages_and_every_epilogue(m, n, epi):
+    """22 stages of 64 k, more than three times round a ring of 4 or 6 buffers and no multiple of either."""
+    k = 1300
+    x, (wq, t) = rand(m, k, seed=m).half().cuda(), weights(n, k, seed=n)
+    wq, t = wq.cuda(), t.cuda()
+    bias = rand(n, seed=3).half().cuda() if epi == "bias" else None
+    out = torch.full((m * n + 64,), 5.0, dtype=torch.float16, device="cuda")
+    y = out[:m * n].view(m, n)
+    capi.linear_i8([capi.linear_i8_problem(x, capi.i8_weight(wq, t), y, EPI[epi], bias)])
+    close(y, *(v.cpu() for v in expected(x, wq, t, epi, bias)), f"{m}x{n} {epi}")
+    assert (out[m * n:] == 5).all()
+
+
+def run_batch(sizes, shared=(0, 0)):
+    """One call of problems (m, n, k, epilogue), the two of `shared` on the same activations."""
+    ps, want = [], []
+    xs = [rand(m, k, seed=i).half().cuda() for i, (m, n, k, epi) in enumerate(sizes)]
+    xs[shared[1]] = xs[shared[0]]
+    for i, (m, n, k, epi) in enumerate(sizes):
+        wq, t = (v.cuda() for v in weights(n, k, seed=50 + i))
+        bias = rand(n, seed=90 + i).half().cuda() if epi == "bias" else None
+        y = torch.full((m, n), 7.0, dtype=torch.float16, device="cuda")
+        ps.append(capi.linear_i8_problem(xs[i], capi.i8_weight(wq, t), y, EPI[epi], bias))
+        if m:
+            want.append((y, xs[i], wq, t, epi, bias))
+    ws = torch.empty(capi.linear_i8_workspace_bytes(ps), dtype=torch.uint8, device="cuda")
+    capi.linear_i8(ps, ws)
+    for i, (y, *args) in enumerate(want):
+        close(y, *(v.cpu() for v in expected(*args)), f"problem {i} of {sizes}")
+
+
+@pytest.mark.parametrize("m", [300, 700, 1500, 2304])
+def test_equal_problems_on_tiles(m):
+    """r, k, v of a large step: tiles of 64 x 128, 128 x 256, 192 x 256 and 256 x 256 over three problems."""
+    n = {300: 2048, 700: 2100, 1500: 2048, 2304: 4096}[m]
+    run_batch([(m, n, 328, "none"), (m, n, 328, "relu2"), (m, n, 328, "sigmoid")])
+
+
+@pytest.mark.parametrize("rows", [(500, 130, 900), (1000, 1500, 77), (2304, 2304, 2304)])
+def test_different_problems_on_tiles(rows):
+    """Problems of other sizes and epilogues, one of no rows and two on the same activations."""
+    a, b, c = rows
+    run_batch([(a, 2051, 200, "none"), (0, 64, 64, "tanh"), (b, 3000, 640, "relu2"), (1, 8, 40, "bias"),
+               (a, 1030, 200, "tanh"), (c, 517, 1100, "bias")], shared=(0, 4))
+
+
+@pytest.mark.parametrize("epi", ["none", "relu2", "bias"])
+@pytest.mark.parametrize("m,n", TILE_ROUTES)
+def test_zero_and_nonfinite_rows_on_tiles(m, n, epi):
+    k = 200
+    x, (wq, t) = rand(m, k, seed=4).half(), weights(n, k, seed=5)
+    bias = rand(n, seed=6).half().cuda() if epi == "bias" else None
+    bad = {1: math.inf, m // 2: math.nan, m - 1: -math.inf}
+    x[[0, 33]] = 0.0
+    for i, v in bad.items():
+        x[i, i % k] = v
+    y = torch.empty(m, n, dtype=torch.float16, device="cuda")
+    wq, t = wq.cuda(), t.cuda()
+    capi.linear_i8([capi.linear_i8_problem(x.cuda(), capi.i8_weight(wq, t), y, EPI[epi], bias)])
+    rows = sorted(bad)
+    assert y[rows].isnan().all()
+    x[rows] = 0.0
+    ref, tol = (v.cpu() for v in expected(x.cuda(), wq, t, epi, bias))
+    keep = [i for i in range(m) if i not in bad]
+    close(y.cpu()[keep], ref[keep], tol[keep], epi)
+
+
+@pytest.mark.parametrize("m,n", TILE_ROUTES)
+def test_largest_values_on_tiles(m, n):
+    """All values at 127 over 22 stages: sums that fp32 does not hold exactly."""
+    k = 1300
+    x = torch.ones(m, k, dtype=torch.float16, device="cuda")
+    x[:, 1::2] = -1.0
+    x[m // 3] *= -1.0
+    wq = torch.full((n, k), 127, dtype=torch.int8, device="cuda")
+    wq[:, 1::2] = -127
+    wq[5::7, 0] = 126
+    t = torch.full((n,), 1.0 / 127 / k, device="cuda")
+    y = torch.empty(m, n, dtype=torch.float16, device="cuda")
+    capi.linear_i8([capi.linear_i8_problem(x, capi.i8_weight(wq, t), y)])
+    close(y, *(v.cpu() for v in expected(x, wq, t, "none", None)), f"{m}")
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 131072), (1, 40, 32769), (3, 40, 131071), (8, 100, 65536), (20, 2101, 131072),
+                                   (40, 3005, 40000), (70, 3001, 33000), (130, 5003, 33000), (250, 5003, 33000), (9, 33, 131072)])
+def test_longest_rows(m, n, k):
+    """K up to 131072, the sums up to 127^2 K = 2^31 - 2^25, and among them ones of ordinary values."""
+    x = rand(m, k, seed=1).half()
+    x[0] = 1.0
+    g = torch.Generator(device="cuda").manual_seed(2)
+    wq = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    wq[0] = 127
+    wq[1] = -127
+    x, t = x.cuda(), 2e-5 * (1.0 + torch.rand(n, generator=g, device="cuda"))
+    y = torch.empty(m, n, dtype=torch.float16, device="cuda")
+    capi.linear_i8([capi.linear_i8_problem(x, capi.i8_weight(wq, t), y)])
+    close(y, *(v.cpu() for v in expected(x, wq, t, "none", None)), f"{m}x{n}x{k}")
+
+
+@pytest.mark.parametrize("m,n", TILE_ROUTES)
+def test_row_bits_on_tiles(m, n):
+    """Rows among many have the bits that they have alone, among a few and on streams."""
+    k = 1300
+    x = rand(m, k, seed=7).half().cuda()
+    wq, t = weights(n, k, seed=8)
+    w, bias = capi.i8_weight(wq.cuda(), t.cuda()), rand(n, seed=9).half().cuda()
+    for epi in sorted(EPI):
+        def run(rows, y):
+            capi.linear_i8([capi.linear_i8_problem(rows, w, y, EPI[epi], bias if epi == "bias" else None)])
+            return y
+        whole = run(x, torch.empty(m, n, dtype=torch.float16, device="cuda"))
+        for a, b in [(m - 1, m), (3, 9), (100, 120), (63, 129), (7, 137)]:
+            assert torch.equal(run(x[a:b].contiguous(), torch.empty(b - a, n, dtype=torch.float16, device="cuda")),
+                               whole[a:b]), (epi, a, b)
+
+
+@pytest.mark.parametrize("m,n", [(250, 5003), (1000, 5001), (2400, 5001)])
+def test_captured_on_tiles(m, n):
+    """Three problems, replayed three times with new inputs and eager work between."""
+    k = 330
+    xs = [rand(m, k, seed=i).half().cuda() for i in range(3)]
+    ws8 = [tuple(v.cuda() for v in weights(n // 3, k, seed=10 + i)) for i in range(3)]
+    ys = [torch.empty(m, n // 3, dtype=torch.float16, device="cuda") for _ in range(3)]
+    ps = [capi.linear_i8_problem(x, capi.i8_weight(*w), y, capi.EPI_RELU_SQUARE) for x, w, y in zip(xs, ws8, ys)]
+    ws = torch.empty(capi.linear_i8_workspace_bytes(ps), dtype=torch.uint8, device="cuda")
+    capi.linear_i8(ps, ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        capi.linear_i8(ps, ws)
+    for seed in (20, 30, 40):
+        for i, x in enumerate(xs):
+            x.copy_(rand(m, k, seed=seed + i).half())
+            ys[i].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = [y.clone() for y in ys]
+        for x, w, y in zip(xs, ws8, got):
+            close(y, *(v.cpu() for v in expected(x, *w, "relu2", None)), f"replay {seed}")
+        capi.linear_i8(ps, ws)
+        for a, b in zip(got, ys):
+            assert torch.equal(a, b)
