@@ -773,8 +773,9 @@ VKWR_EXPORT int vkwr_sampling_verify_drafts(int B, int K, int V, const void* log
  * candidates are left the remaining rows are token -1, parent -1, score -inf, length 0, ended 1.
  * end: -1 for none.  length_penalty 0..16; V up to 2^20; B W up to 65535.  Sums over the vocabulary, scores
  * and comparisons are in 64 bits (terms and sums of 16 terms fp32).  Deterministic, and independent of the
- * other requests.  Outputs must not overlap the inputs.  workspace: vkwr_beam_workspace_bytes(B, W, V) bytes
- * (-1 for sizes that are refused), 16-byte aligned, one for each of the calls that may run at the same time.
+ * other requests.  Outputs must not overlap the inputs, nor the workspace any of them.
+ * workspace: vkwr_beam_workspace_bytes(B, W, V) bytes (-1 for sizes that are refused), 16-byte aligned, one for each
+ * of the calls that may run at the same time.
  * No counterpart in the reference. */
 VKWR_EXPORT int64_t vkwr_beam_workspace_bytes(int B, int W, int V);
 VKWR_EXPORT int vkwr_beam_select(int B, int W, int V, const void* logits, int logits_f16, const float* scores,

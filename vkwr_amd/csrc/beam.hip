@@ -575,10 +575,13 @@ extern "C" int vkwr_beam_select(int B, int W, int V, const void* logits, int log
              (long long)workspace_bytes);
   const void* const ins[] = {scores, lengths, ended};
   void* const outs[] = {tokens, parents, scores_out, lengths_out, ended_out};
+  const int64_t logits_bytes = rows * V * (logits_f16 ? 2 : 4);
+  for (const void* in : ins) VK_REQUIRE(!overlap(in, 4 * rows, workspace, need), "%s: an input overlaps the workspace", fn);
+  VK_REQUIRE(!overlap(logits, logits_bytes, workspace, need), "%s: the logits overlap the workspace", fn);
   for (int i = 0; i < 5; ++i) {
     for (const void* in : ins) VK_REQUIRE(!overlap(outs[i], 4 * rows, in, 4 * rows), "%s: an output overlaps an input", fn);
     for (int j = 0; j < i; ++j) VK_REQUIRE(!overlap(outs[i], 4 * rows, outs[j], 4 * rows), "%s: outputs overlap", fn);
-    VK_REQUIRE(!overlap(outs[i], 4 * rows, workspace, need) && !overlap(outs[i], 4 * rows, logits, rows * V * (logits_f16 ? 2 : 4)),
+    VK_REQUIRE(!overlap(outs[i], 4 * rows, workspace, need) && !overlap(outs[i], 4 * rows, logits, logits_bytes),
                "%s: an output overlaps the workspace or the logits", fn);
   }
   BeamArgs a{};
