@@ -1,0 +1,41 @@
+"""Calls that the beam search refuses, on the CPU: what it refuses is left as it was."""
+import types
+
+import pytest
+import torch
+
+from tests.test_beam_search import PROMPTS, Engine, make_state, oracle  # noqa: F401  (the fixture replaces the kernels)
+from vkwr.model_executor import BeamSearch
+
+
+class Drafts(Engine):
+    """An engine that keeps drafts of `state` between two of its calls, as DraftEngine does."""
+
+    def __init__(self, state):
+        super().__init__()
+        self.open = (state, [0])
+
+    def drop(self, slots, state=None):
+        if self.open is not None and self.open[0].wkv is state.wkv:
+            raise RuntimeError("drop: the last step's drafts are not accepted yet")
+
+    def step(self, *args, **kw):
+        if self.open is not None:
+            raise RuntimeError("step: the last step's drafts are not accepted yet")
+        return super().step(*args, **kw)
+
+
+@pytest.mark.parametrize("same", [True, False])
+def test_between_a_draft_step_and_its_accept(same):
+    """Refused before any state is reset, whichever state the drafts are of."""
+    state = make_state(6)
+    engine = Drafts(state if same else make_state(6))
+    search = BeamSearch(engine, state, 2, max_requests=2, max_new_tokens=3)
+    before = [t.clone() for t in (state.wkv, state.att_shift, state.ffn_shift)]
+    with pytest.raises(RuntimeError, match="accepted"):
+        search.generate(PROMPTS[:2], 3)
+    for a, b in zip(before, (state.wkv, state.att_shift, state.ffn_shift)):
+        assert torch.equal(a, b)
+    engine.open = None
+    want = BeamSearch(Engine(), make_state(6), 2, max_requests=2, max_new_tokens=3).generate(PROMPTS[:2], 3)
+    assert search.generate(PROMPTS[:2], 3) == want
