@@ -156,6 +156,9 @@ class BeamSearch:
             raise ValueError(f"beam search: an empty prompt, or {max_new_tokens} new tokens (1 to {self.max_new_tokens})")
         if adapters is not None and (len(adapters) != len(prompts) or getattr(self.engine, "adapters", None) is None):
             raise ValueError(f"beam search: {len(adapters)} adapters for {len(prompts)} prompts, or an engine without")
+        pool = getattr(getattr(self.engine, "adapters", None), "pool", None)
+        if adapters is not None and pool is not None and not all(-1 <= a < pool.n_adapters for a in adapters):
+            raise ValueError(f"beam search: adapters {list(adapters)} of {pool.n_adapters}")
         if getattr(self.engine, "open", None) is not None:  # a DraftEngine, whose step would refuse it when states are reset
             raise RuntimeError("beam search: the engine's last drafts are not accepted yet")
         out = []
