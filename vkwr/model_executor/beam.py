@@ -157,7 +157,7 @@ class BeamSearch:
         if adapters is not None and (len(adapters) != len(prompts) or getattr(self.engine, "adapters", None) is None):
             raise ValueError(f"beam search: {len(adapters)} adapters for {len(prompts)} prompts, or an engine without")
         pool = getattr(getattr(self.engine, "adapters", None), "pool", None)
-        if adapters is not None and pool is not None and not all(-1 <= a < pool.n_adapters for a in adapters):
+        if adapters is not None and pool is not None and any(a >= pool.n_adapters for a in adapters):
             raise ValueError(f"beam search: adapters {list(adapters)} of {pool.n_adapters}")
         if getattr(self.engine, "open", None) is not None:  # a DraftEngine, whose step would refuse it when states are reset
             raise RuntimeError("beam search: the engine's last drafts are not accepted yet")
