@@ -130,10 +130,10 @@ class MixedEngine:
         return [("Wr", s.mix[0][:R], s.r[:R]), ("Wk", s.mix[2][:R], s.k[:R]),
                 ("Wv", s.mix[3][:R], (s.v_first if first else s.v)[:R])]
 
-    def _proj(self, L, W, R, first):
-        """The fp16 projections of the time mix's inputs."""
+    def _proj(self, L, W, R, first, rkv=None):
+        """The fp16 projections of the time mix's inputs (rkv: what _rkv gave, for the caller that has it)."""
         s, gp = self, capi.gemm_problem
-        ps = [gp(x, L[n], y) for n, x, y in self._rkv(R, first) if not self._is_int8(n)]
+        ps = [gp(x, L[n], y) for n, x, y in rkv or self._rkv(R, first) if not self._is_int8(n)]
         ps += [gp(s.mix[1][:R], W["w1"], s.w1[:R], epilogue=capi.EPI_TANH), gp(s.mix[4][:R], W["a1"], s.a1[:R]),
                gp(s.mix[5][:R], W["g1"], s.g1[:R], epilogue=capi.EPI_SIGMOID)]
         if not first:
@@ -142,10 +142,11 @@ class MixedEngine:
 
     def _run_proj(self, l, R):
         first = l == 0
-        items = [t for t in self._rkv(R, first) if self._is_int8(t[0])]
+        rkv = self._rkv(R, first)
+        items = [t for t in rkv if self._is_int8(t[0])]
         if items:
             self.int8.run(l, items)
-        capi.gemm(self._proj(self.model.layers[l], self.lw[l], R, first), self.ws)
+        capi.gemm(self._proj(self.model.layers[l], self.lw[l], R, first, rkv), self.ws)
 
     def _linear(self, l, name, x, y, epilogue=capi.EPI_NONE):
         """One large projection, in 8 bits or in 16."""
