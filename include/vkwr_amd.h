@@ -766,8 +766,10 @@ VKWR_EXPORT int vkwr_sampling_verify_drafts(int B, int K, int V, const void* log
  * int32 (non-zero: the beam is finished).
  *   A live beam b offers every token v with raw = scores[b] + l_v - log sum_u exp(l_u) and the length
  *   lengths[b] + 1; a finished one only `end`, with raw = scores[b] and its length.
- *   The W best by raw * max(length, 1)^-length_penalty, ties to the lowest b V + v, in that order:
+ *   The W best by raw * max(length, 1)^-length_penalty, in that order; within a beam that is the order of the
+ * logits, ties to the lowest v, and scores of different beams that are equal in 64 bits go to the lower b:
  *   tokens, parents (b), scores_out (raw), lengths_out, ended_out (finished before, or token == end).
+ * Scores are finite, or -inf or NaN; lengths up to 2^31 - 2.
  * A logit of -inf or NaN is never chosen, and a beam of score -inf or NaN offers nothing (all but the first
  * of a request behind its prompt).  Logits of +inf share the whole probability.  Where fewer than W
  * candidates are left the remaining rows are token -1, parent -1, score -inf, length 0, ended 1.
