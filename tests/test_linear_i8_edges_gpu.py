@@ -201,3 +201,55 @@ def test_captured_on_tiles(m, n):
         capi.linear_i8(ps, ws)
         for a, b in zip(got, ys):
             assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+
+def part(w, a, b):
+    """Outputs a..b of weights w (a a multiple of 32): their blocks of the packed matrix."""
+    row = w.packed.numel() // (-(-w.n // 32))
+    return capi.I8Weight(b - a, w.k, w.packed[a // 32 * row:-(-b // 32) * row], w.scale[a:b])
+
+
+@pytest.mark.parametrize("m", [1, 5, 20, 130, 700])
+def test_weights_past_32_bits(m):
+    """70016 outputs of K 32768, 2.3 GB: the last outputs are those of their own block of the weights alone."""
+    n, k = 70001, 32768
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = capi.I8Weight(n, k, torch.randint(-127, 128, (70016 * k,), generator=g, dtype=torch.int8, device="cuda"),
+                      1e-5 * torch.rand(n, generator=g, device="cuda"))
+    x = torch.randn(m, k, generator=g, device="cuda").half()
+    y, tail = (torch.empty(m, c, dtype=torch.float16, device="cuda") for c in (n, n - 69600))
+    capi.linear_i8([capi.linear_i8_problem(x, w, y)])
+    capi.linear_i8([capi.linear_i8_problem(x, part(w, 69600, n), tail)])
+    assert torch.equal(y[:, 69600:], tail) and (tail != 0).any()
+
+
+@pytest.mark.parametrize("m,n,k", [(70001, 300, 32768), (131072, 16500, 40)])
+def test_rows_past_32_bits(m, n, k):
+    """Activations of 4.6 GB (2.3 GB in 8 bits), outputs of 4.3 GB: the last rows are those they give alone."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = capi.i8_weight(torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8, device="cuda"),
+                       1e-5 * torch.rand(n, generator=g, device="cuda"))
+    x = torch.empty(m, k, dtype=torch.float16, device="cuda")
+    x[:] = torch.randn(k, generator=g, device="cuda").half()
+    x[-150:] = torch.randn(150, k, generator=g, device="cuda").half()
+    y, tail = (torch.empty(r, n, dtype=torch.float16, device="cuda") for r in (m, 150))
+    capi.linear_i8([capi.linear_i8_problem(x, w, y)])
+    capi.linear_i8([capi.linear_i8_problem(x[-150:].contiguous(), w, tail)])
+    assert torch.equal(y[-150:], tail) and (tail != 0).any() and torch.equal(y[0], y[m // 2])
+
+
+def test_packing_past_32_bits():
+    """Weights of 2.3 GB packed from 8-bit and from fp16 values: the last rows' blocks are those they give alone."""
+    n, k = 70001, 32768
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    tail = q[69984:].contiguous()
+    whole, alone = capi.i8_weight(q, torch.ones(n, device="cuda")), capi.i8_weight(tail, torch.ones(17, device="cuda"))
+    assert torch.equal(whole.packed[69984 * k:], alone.packed)
+    whole = capi.i8_quantize(q.half())
+    alone = capi.i8_quantize(tail.half())
+    used = lambda p: p.view(-1, 2, 32, 16)[:, :, :17]  # noqa: E731  (the block's pad rows are never used)
+    assert torch.equal(used(whole.packed[69984 * k:]), used(alone.packed))
+    assert torch.equal(whole.scale[69984:], alone.scale)
