@@ -253,3 +253,31 @@ def test_packing_past_32_bits():
     used = lambda p: p.view(-1, 2, 32, 16)[:, :, :17]  # noqa: E731  (the block's pad rows are never used)
     assert torch.equal(used(whole.packed[69984 * k:]), used(alone.packed))
     assert torch.equal(whole.scale[69984:], alone.scale)
+
+
+# ---------------------------------------------------------------- what 8 bits cost
+
+@pytest.mark.parametrize("kind", ["normal", "channels", "relu2"])
+def test_error_against_fp16_weights(kind):
+    """Against the product of unrounded rows and weights: every output within the bound of its roundings, half a step
+    of each factor.  Errors spread evenly over a step of max / 127 give a root mean square of sqrt(c_x^2 + c_w^2) /
+    (127 sqrt 12) of the output's, c = max / rms of a row (zeros and values below half a step err less: at most that):
+    2^-6.4 of normal rows, 2^-5.6 and 2^-5.9 of the others.  The sums have 2048 terms over 256 rows and 512 columns;
+    a tenth leaves room for the statistics."""
+    m, n, k = 256, 512, 2048
+    x = rand(m, k, seed=1)
+    x = {"normal": x, "channels": x * torch.exp(0.6 * rand(k, seed=2)), "relu2": torch.relu(x).square()}[kind].half()
+    w = (0.02 * rand(n, k, seed=3) * torch.exp(0.3 * rand(n, 1, seed=4))).half()
+    y = torch.empty(m, n, dtype=torch.float16, device="cuda")
+    capi.linear_i8([capi.linear_i8_problem(x.cuda(), capi.i8_quantize(w.cuda()), y)])
+    xd, wd = x.double(), w.double()
+    ref = torch.matmul(xd, wd.t())
+    err = y.cpu().double() - ref
+    sx, sw = (v.abs().amax(1, keepdim=True) / 127.0 for v in (xd, wd))
+    bound = sx / 2 * wd.abs().sum(1) + xd.abs().sum(1, keepdim=True) * sw.t() / 2 + sx * sw.t() * k / 4
+    assert (err.abs() <= bound + y.cpu().double().abs() * 2.0 ** -10 + 2.0 ** -24).all()
+    c2 = [((v.abs().amax(1) / v.square().mean(1).sqrt()) ** 2).mean() for v in (xd, wd)]
+    want = float(((c2[0] + c2[1]) / 12).sqrt() / 127)
+    got = float((err.square().mean(1) / ref.square().mean(1)).mean().sqrt())
+    assert got < 1.1 * want and (kind == "relu2" or got > 0.9 * want)
+    assert 2.0 ** -6.6 < got < 2.0 ** -5.4

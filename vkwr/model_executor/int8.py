@@ -3,9 +3,10 @@
 `Int8Weights` holds the projections named (r, k, v, o of the time mix, key and value of the channel mix)
 in 8 bits with a scale per output channel, laid out for vkwr_linear_i8_f16; the engine rounds each row
 of activations to 8 bits as it multiplies.  The low-rank projections, which make the decay, the gates and
-the learning rates, and the head stay fp16.  Half the weight bytes of a step and twice the matrix rate, at
-an error of about 2^-8 of each product's typical size; the model's fp16 matrices of these names are not
-read by such an engine and may be freed.
+the learning rates, and the head stay fp16.  Half the weight bytes of a step and twice the matrix rate; the
+error of a product has a root mean square of sqrt(c_x^2 + c_w^2) / 440 of the output's, with c = max / rms of a row
+of activations and of weights: 2^-6.4 for normally distributed ones of 2048, 2^-5.5 where some channels are much larger than
+others.  The model's fp16 matrices of these names are not read by such an engine and may be freed.
 """
 import torch
 
