@@ -871,7 +871,7 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 }
 
 // The tile that a batch runs with: the smallest whose workgroups fit the (256) CUs at once.  A second
-// round costs more than larger tiles that leave CUs idle, and larger tiles than that
+// round mostly costs more than larger tiles that leave CUs idle, and larger tiles than that
 // leave bandwidth.  us of a whole call, this tile against its neighbours:
 //   16 x 16    K 8192, N 2048, m = 9     8.7; 16 x 32 9.7, 32 x 32 10.7
 //              K 16384, N 4096, m = 9    17.7; 16 x 32 19.9, 32 x 32 23.9
@@ -885,6 +885,12 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 //   128 x 256  K = N = 4096, m = 1100    31.3; 128 x 128 41.3, 192 x 256 41.0
 //   192 x 256  K = N = 4096, m = 2304    48.7; 128 x 256 63.2, 256 x 256 58.6
 //   256 x 256  K = N = 4096, m = 4096    76.8; 192 x 256 88.6
+// Where it loses, up to an eighth: few rows of many outputs, whose smaller tiles take two to five rounds
+// (K 4096, the rule's / the best of 16 x 16 to 128 x 128):
+//   16 rows    N 12288  32 x 64 13.2 / 16 x 16 12.5; N 16384 15.6 / 14.7; N 16448 64 x 128 16.5 / 16 x 16 15.6; N 20480 19.4 / 17.0
+//   32 rows    N 16448  64 x 128 17.1 (64 x 64 20.9); N 20480 21.1 / 32 x 32 20.0
+//   64 rows    N 12288  64 x 64 15.8 / 32 x 32 14.6; N 16384 19.2 / 32 x 64 17.2; N 16448 64 x 128 17.3 (64 x 64 24.1)
+//              three of N 4096  64 x 64 16.6 / 32 x 32 15.6 (48 rows 15.9 / 15.2)
 // Beyond one round of the largest: whichever of the last two takes less by its rounds, one of 192
 // rows counted as 0.77 (K 4096, N 16384, m = 2304: three rounds each, 145, 179; three of N 4096: 576 tiles
 // in three rounds 142, 432 in two 135).
