@@ -116,7 +116,7 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 
 // blockIdx.x: group of the row, blockIdx.y: row.  Lane t holds the pieces (8 fp16 or 4 fp32)
 // t, t + 512, ... of the group.  Bound by memory where the logits are many (64 x 8 beams of 65536 fp32: 29.5 us,
-// 4.6 TB/s); at 16 x 8 of fp16 (10.5 us; the bytes are 3.5) by its own instructions, an exponential of each
+// 4.6 TB/s; reads alone have reached 6.1); at 16 x 8 of fp16 (10.5 us; the bytes are 3.5) by its own instructions, an exponential of each
 // entry above all, behind one load per lane; at 1 x 4 (4.9 us) by that trip and four barriers.  Groups of 8192
 // (us of a whole step at 1 x 4, 16 x 8, 64 x 8: 9.3, 14.8, 33.1): of 4096 9.2, 18.5, 44.3, of 16384 10.3, 14.2, 35.1.
 template <bool kHalf>
@@ -457,8 +457,8 @@ struct RArgs {
 };
 
 // Every workgroup works the copies out by itself (up to 4096 children, in LDS: a launch of its own for that
-// would cost more), then they share the work items out evenly.  Bound by memory: 16 x 8 beams of a 24-layer state, 1.1 GB
-// moved, 246 us at 4.5 TB/s, which is what a large copy reaches; a small one by its launch (4.7 us).
+// would cost more), then they share the work items out evenly.  Bound by memory: 16 x 8 beams of a 24-layer state, 1.13 GB
+// moved, 237 us at 4.77 TB/s, which is what a large copy reaches; a small one by its launch (4.7 - 6 us).
 template <int N>
 __global__ __launch_bounds__(kCopyThreads) void beam_reorder_kernel(RArgs<N> a) {
   extern __shared__ __attribute__((aligned(16))) int lds[];
