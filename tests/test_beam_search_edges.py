@@ -51,3 +51,25 @@ def test_adapters_outside_the_pool(adapters):
         search.generate(PROMPTS[:2], 3, adapters=adapters)
     assert engine.calls == []
     assert [len(h) for h in search.generate(PROMPTS[:2], 3, adapters=[1, -7])] == [2, 2]
+
+
+def test_more_beams_than_a_call_reorders(monkeypatch):
+    """129 requests of 32 beams: run in parts of at most 4096 beams, which is what the reordering takes."""
+    from vkwr_amd import capi
+    seen = []
+    inner = capi.beam_reorder
+
+    def reorder(slots, *args, **kw):
+        seen.append(slots.numel())
+        assert slots.numel() <= 4096
+        inner(slots, *args, **kw)
+
+    monkeypatch.setattr(capi, "beam_reorder", reorder)
+    engine = Engine(max_rows=5000, max_seqs=5000)
+    search = BeamSearch(engine, make_state(129 * 32), 32, max_requests=129, max_new_tokens=1, max_prefill_chunks=129)
+    prompts = [[i % 12, i // 12] for i in range(129)]
+    got = search.generate(prompts, 1)
+    assert seen == [4096, 32] and len(got) == 129
+    for i in (0, 127, 128):
+        alone = BeamSearch(Engine(), make_state(32), 32, max_new_tokens=1).generate([prompts[i]], 1)
+        assert got[i] == alone[0]

@@ -162,8 +162,9 @@ class BeamSearch:
         if getattr(self.engine, "open", None) is not None:  # a DraftEngine, whose step would refuse it when states are reset
             raise RuntimeError("beam search: the engine's last drafts are not accepted yet")
         out = []
-        for i in range(0, len(prompts), self.max_requests):
-            part = slice(i, i + self.max_requests)
+        at_once = min(self.max_requests, capi.MAX_BEAM_ROWS // self.width)
+        for i in range(0, len(prompts), at_once):
+            part = slice(i, i + at_once)
             out += self._generate(prompts[part], max_new_tokens, None if adapters is None else list(adapters[part]))
         return out
 

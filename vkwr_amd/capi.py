@@ -752,6 +752,7 @@ def linear_i8(problems, workspace=None):
 
 
 MAX_BEAMS = 32
+MAX_BEAM_ROWS = 4096  # of one beam_reorder
 
 
 def beam_workspace_bytes(B, W, V):
