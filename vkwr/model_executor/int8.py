@@ -27,8 +27,9 @@ class Int8Weights:
         """Replaces one projection by weights that are 8 bits already: q [N, K] int8 of -127..127, scale [N]
         fp32 (of a quantised checkpoint).  In place: captured steps see it."""
         w = self.layers[layer][name]
-        if tuple(q.shape) != (w.n, w.k):
-            raise ValueError(f"layer {layer}, {name}: q {tuple(q.shape)}, expected [{w.n}, {w.k}]")
+        if tuple(q.shape) != (w.n, w.k) or tuple(scale.shape) != (w.n,):
+            raise ValueError(f"layer {layer}, {name}: q {tuple(q.shape)}, scale {tuple(scale.shape)}, expected [{w.n}, {w.k}] "
+                             f"and [{w.n}]")
         new = capi.i8_weight(q, scale)
         w.packed.copy_(new.packed)
         w.scale.copy_(new.scale)
