@@ -116,9 +116,10 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 
 // blockIdx.x: group of the row, blockIdx.y: row.  Lane t holds the pieces (8 fp16 or 4 fp32)
 // t, t + 512, ... of the group.  Bound by memory where the logits are many (64 x 8 beams of 65536 fp32: 29.5 us,
-// 4.6 TB/s; reads alone have reached 6.1); at 16 x 8 of fp16 (10.5 us; the bytes are 3.5) by its own instructions, an exponential of each
-// entry above all, behind one load per lane; at 1 x 4 (4.9 us) by that trip and four barriers.  Groups of 8192
-// (us of a whole step at 1 x 4, 16 x 8, 64 x 8: 9.3, 14.8, 33.1): of 4096 9.2, 18.5, 44.3, of 16384 10.3, 14.2, 35.1.
+// 4.6 TB/s; reads alone have reached 6.1); at 16 x 8 of fp16 (10.5 us; the bytes are 3.5) by its own instructions,
+// an exponential of each entry above all, behind one load per lane; at 1 x 4 (4.9 us) by that trip and four
+// barriers.  Groups of 8192 (us of a whole step at 1 x 4, 16 x 8, 64 x 8: 9.3, 14.8, 33.1): of 4096 9.2, 18.5, 44.3,
+// of 16384 10.3, 14.2, 35.1.
 template <bool kHalf>
 __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(BeamArgs a) {
   constexpr int kPiece = kHalf ? 8 : 4;

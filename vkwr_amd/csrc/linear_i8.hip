@@ -885,7 +885,7 @@ QProb row_problem(const uint16_t* x, int64_t m, int64_t k, int8_t* q, float* s) 
 //   128 x 256  K = N = 4096, m = 1100    31.3; 128 x 128 41.3, 192 x 256 41.0
 //   192 x 256  K = N = 4096, m = 2304    48.7; 128 x 256 63.2, 256 x 256 58.6
 //   256 x 256  K = N = 4096, m = 4096    76.8; 192 x 256 88.6
-// Where it loses, up to an eighth: few rows of many outputs, whose smaller tiles take two to five rounds
+// Where it loses, up to a seventh: few rows of many outputs, whose smaller tiles take two to five rounds
 // (K 4096, the rule's / the best of 16 x 16 to 128 x 128):
 //   16 rows    N 12288  32 x 64 13.2 / 16 x 16 12.5; N 16384 15.6 / 14.7; N 16448 64 x 128 16.5 / 16 x 16 15.6; N 20480 19.4 / 17.0
 //   32 rows    N 16448  64 x 128 17.1 (64 x 64 20.9); N 20480 21.1 / 32 x 32 20.0
